@@ -579,6 +579,52 @@ int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step_args* a,
                          kad_stream_t stream);
 
 /* --------------------------------------------------------------------------
+ * The 8-bit prefix cache (no reference counterpart: the reference keeps its
+ * prefix in the model's type, src/kadllm/adapters/qwen3_5.py:106-133).
+ *
+ * A pool of pages per layer: codes [pages, HK, block, D] e4m3 and scales
+ * [pages, HK] e8m0 (2^(byte - 127)); a value is code * scale.  tables [B,
+ * width] int32 name a request's pages in order; entries outside [0, pages)
+ * name none.  Supported: D in {64, 128, 256}, block in {32, 64, 128, 256}.
+ *
+ * kad_prefix_block_tables: request b needs ceil(lengths[b] / block) -
+ * ceil(starts[b] / block) pages more (starts may be null: none held), taken in
+ * request order from the front of free_blocks; tables gets the held entries of
+ * old_tables [B, old_width], then the new pages, then -1, and *used the pages
+ * needed in all (above num_free: the entries past the list are -1).  Lengths
+ * above max_length <= width * block are cut there. */
+int kad_prefix_block_tables(const int32_t* lengths, const int32_t* starts,
+                            const int32_t* old_tables, int old_width, const int32_t* free_blocks,
+                            int num_free, int32_t* tables, int width, int32_t* used, int B,
+                            int block, int max_length, kad_stream_t stream);
+/* Token i of request b (k, v at [b*s_b + i*s_t + h*s_h + d], bf16, fp16 or
+ * fp32) to position starts[b] + i (starts may be null: 0) while that is below
+ * lengths[b].  A page's scale is the smallest power of two s >= 2^-100 with
+ * amax <= 448 s over the finite values written, or the page's own where that
+ * is larger and the page holds earlier tokens (whose codes are rounded again
+ * when the scale grows).  Tokens without a page are left out. */
+int kad_write_prefix_blocks(const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h,
+                            const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int dtype,
+                            const int32_t* tables, int width, const int32_t* lengths,
+                            const int32_t* starts, void* k_codes, void* v_codes, void* k_scale,
+                            void* v_scale, int pages, int B, int N, int HK, int D, int block,
+                            kad_stream_t stream);
+/* kad_prefix_attention_decode_ex's attention over such a prefix: query rows
+ * (n, t, h) see the first lengths[b] cached tokens of their request b = n / W
+ * and the suffix keys j <= Tk - T + t of their beam (Tk = 0: no suffix).  bf16
+ * or fp16 queries, suffixes, gate (may be null) and out; last dimensions
+ * contiguous.  A row that sees no key gives zeros. */
+int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_t sq_h,
+                               const void* k_codes, const void* v_codes, const void* k_scale,
+                               const void* v_scale, int pages, const int32_t* tables, int width,
+                               const int32_t* lengths, const void* suffix_k, int64_t ssk_n,
+                               int64_t ssk_t, int64_t ssk_h, const void* suffix_v, int64_t ssv_n,
+                               int64_t ssv_t, int64_t ssv_h, const void* gate, int64_t sg_n,
+                               int64_t sg_t, int64_t sg_h, void* out, int64_t so_n, int64_t so_t,
+                               int64_t so_h, int B, int W, int T, int Tk, int H, int HK, int D,
+                               int block, int dtype, float scale, kad_stream_t stream);
+
+/* --------------------------------------------------------------------------
  * MFMA lane-layout self-test (no reference counterpart): C[16x16] = A[16x32]
  * B[32x16] (bf16 in, fp32 out, all row-major) computed by one wave with the
  * operand layout the kernels above assume for v_mfma_f32_16x16x32_bf16, and

@@ -9,9 +9,10 @@ in libkadllm_hip.so).  WideTuning (``GatedMLPSpec``, ``WideTuningMLP``,
 not provided.
 """
 
-from kadllm_amd import (Constraint, GRBeamAdapter, GRBeamResult, PrefillResult,
-                        causal_conv1d, conditional_search, gated_delta, grbeam_search,
-                        merge_attention, prefix_attention)
+from kadllm_amd import (Constraint, GRBeamAdapter, GRBeamResult, PrefillResult, PrefixBlocks,
+                        block_prefix_attention, causal_conv1d, conditional_search, gated_delta,
+                        grbeam_search, merge_attention, prefix_attention, prefix_block_tables,
+                        write_prefix_blocks)
 
 from . import adapters, grbeam, ops  # noqa: E402  (the reference's submodules)
 
@@ -26,4 +27,8 @@ __all__ = [
     "gated_delta",
     "prefix_attention",
     "merge_attention",
+    "PrefixBlocks",
+    "prefix_block_tables",
+    "write_prefix_blocks",
+    "block_prefix_attention",
 ]

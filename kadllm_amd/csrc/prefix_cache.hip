@@ -1,0 +1,187 @@
+// The 8-bit prefix cache: pages of a batch's requests, and keys and values into them.
+//
+// A cache is a pool of pages.  A page holds `block` tokens of one layer:
+// codes [HK, block, D] in e4m3 (OCP) and one scale per KV head in e8m0, the
+// power of two 2^(byte - 127).  A token's value is code * scale.  Powers of
+// two cost an e4m3 value no precision (its significand is untouched) and make
+// both a change of scale and the product in the attention's scaled MFMAs
+// exact.  The pool's codes are [pages, HK, block, D], so that the rows of a
+// page and head are one contiguous piece.
+
+#include "kad_common.h"
+
+// ---------------------------------------------------------------------------
+// Block tables.  Request b has `starts[b]` tokens in pages that it holds
+// already and `lengths[b]` after this call; it gets
+//   need[b] = ceil(lengths / block) - ceil(starts / block)
+// pages, taken from `free` in request order: entry j of its row is
+//   old[b][j]                              j <  ceil(starts / block)
+//   free[sum of need before b + j - held]  j <  ceil(lengths / block)
+//   -1                                     otherwise, or when `free` is used up.
+
+__device__ __forceinline__ int pages_of(int tokens, int block) {
+  return (int)(((int64_t)max(tokens, 0) + block - 1) / block);
+}
+
+__global__ __launch_bounds__(256) void block_tables_kernel(
+    const int* __restrict__ lengths, const int* __restrict__ starts, const int* __restrict__ old,
+    int old_width, const int* __restrict__ free_blocks, int num_free, int* __restrict__ tables,
+    int width, int* __restrict__ used, int B, int block, int max_length) {
+  __shared__ int part[256];
+  const int tid = threadIdx.x, b = blockIdx.x;
+  // pages the requests before b need; the last workgroup adds its own
+  int before = 0;
+  for (int i = tid; i < b; i += 256) {
+    const int held = starts ? pages_of(min(starts[i], max_length), block) : 0;
+    before += max(pages_of(min(lengths[i], max_length), block) - held, 0);
+  }
+  part[tid] = before;
+  __syncthreads();
+  for (int s = 128; s > 0; s >>= 1) {
+    if (tid < s) part[tid] += part[tid + s];
+    __syncthreads();
+  }
+  before = part[0];
+  const int held = starts ? pages_of(min(starts[b], max_length), block) : 0;
+  const int total = max(pages_of(min(lengths[b], max_length), block), held);
+  for (int j = tid; j < width; j += 256) {
+    int page = -1;
+    if (j < held) {
+      if (old && j < old_width) page = old[(int64_t)b * old_width + j];
+    } else if (j < total && before + (j - held) < num_free) {
+      page = free_blocks[before + (j - held)];
+    }
+    tables[(int64_t)b * width + j] = page;
+  }
+  if (b == B - 1 && tid == 0) *used = before + total - held;
+}
+
+extern "C" int kad_prefix_block_tables(const int32_t* lengths, const int32_t* starts,
+                                       const int32_t* old_tables, int old_width,
+                                       const int32_t* free_blocks, int num_free, int32_t* tables,
+                                       int width, int32_t* used, int B, int block, int max_length,
+                                       kad_stream_t stream) {
+  KAD_REQUIRE(B > 0 && width > 0 && old_width >= 0 && num_free >= 0,
+              "block tables need requests and columns");
+  KAD_REQUIRE(block > 0 && max_length > 0 && kad_cdiv(max_length, block) <= width,
+              "tables of %d columns of %d tokens do not hold %d", width, block, max_length);
+  KAD_REQUIRE(lengths && tables && used && (free_blocks || num_free == 0),
+              "null pointer argument");
+  KAD_REQUIRE(!old_tables || starts, "held tables need the tokens held");
+  hipLaunchKernelGGL(block_tables_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream,
+                     lengths, starts, old_tables, old_width, free_blocks, num_free, tables, width,
+                     used, B, block, max_length);
+  return kad_launch_status("block_tables_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// Writing.  Token i of request b goes to position starts[b] + i while that is
+// below lengths[b].  A workgroup owns one touched page of one request and
+// head, so the page's scale has one writer:
+//   e_need = the smallest e >= -100 with amax <= 448 * 2^e over the finite new values
+//   e      = e_need, or max(e_need, the page's) when it holds earlier tokens
+//   code   = e4m3(x * 2^-e), to nearest even; infinities and NaN become NaN
+// and the earlier tokens' codes are rounded again when the scale has grown.
+// Rows past lengths[b] are left as they were.
+constexpr int kMinExp = -100;
+
+__device__ __forceinline__ int scale_exp(float amax) {
+  // amax = 1.m * 2^x; 448 = 1.75 * 2^8
+  const uint32_t bits = __float_as_uint(amax);
+  const int x = (int)(bits >> 23) - 127;
+  const int e = x - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, kMinExp);  // zeros and subnormals of fp32 give x = -127
+}
+__device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+__device__ __forceinline__ uint8_t to_e4m3(float x) {
+  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff);
+}
+__device__ __forceinline__ float from_e4m3(uint8_t c) {
+  return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
+}
+
+struct WriteArgs {
+  const void* x[2];       // k, v
+  int64_t s_b[2], s_t[2], s_h[2];
+  const int* tables;
+  const int* lengths;
+  const int* starts;
+  uint8_t* codes[2];
+  uint8_t* scale[2];
+  int width, pages, B, N, HK, D, block, touched;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void write_blocks_kernel(WriteArgs a) {
+  __shared__ float part[4];
+  const int tid = threadIdx.x;
+  const int u = blockIdx.x % a.touched, b = blockIdx.x / a.touched;
+  const int h = blockIdx.y, kv = blockIdx.z;
+  const int start = a.starts ? max(a.starts[b], 0) : 0;
+  const int64_t stop64 = min((int64_t)start + a.N, (int64_t)a.width * a.block);
+  const int stop = min(a.lengths[b], (int)stop64);   // one past the last new position
+  const int blk = start / a.block + u;
+  const int lo = max(start - blk * a.block, 0), hi = min(stop - blk * a.block, a.block);
+  if (blk >= a.width || hi <= lo) return;             // rows [lo, hi) of the page are new
+  const int page = a.tables[(int64_t)b * a.width + blk];
+  if (page < 0 || page >= a.pages) return;
+  const T* x = (const T*)a.x[kv] + (int64_t)b * a.s_b[kv] + (int64_t)h * a.s_h[kv] +
+               ((int64_t)blk * a.block - start) * a.s_t[kv];
+  uint8_t* codes = a.codes[kv] + ((int64_t)page * a.HK + h) * a.block * a.D;
+  uint8_t* scale = a.scale[kv] + (int64_t)page * a.HK + h;
+  float amax = 0.f;
+  for (int i = lo * a.D + tid; i < hi * a.D; i += 256) {
+    const float f = fabsf(Elem<T>::to_f(x[(int64_t)(i / a.D) * a.s_t[kv] + i % a.D]));
+    if (f < INFINITY) amax = fmaxf(amax, f);
+  }
+  amax = wave_max(amax);
+  if ((tid & 63) == 0) part[tid >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  int e = scale_exp(amax);
+  if (lo > 0) {
+    const int before = (int)*scale - 127;
+    if (e > before) {
+      const float f = pow2f(max(before - e, -126));
+      for (int i = tid; i < lo * a.D; i += 256) codes[i] = to_e4m3(from_e4m3(codes[i]) * f);
+    }
+    e = max(e, before);
+  }
+  const float inv = pow2f(-e);
+  for (int i = lo * a.D + tid; i < hi * a.D; i += 256)
+    codes[i] = to_e4m3(Elem<T>::to_f(x[(int64_t)(i / a.D) * a.s_t[kv] + i % a.D]) * inv);
+  __syncthreads();
+  if (tid == 0) *scale = (uint8_t)(e + 127);
+}
+
+extern "C" int kad_write_prefix_blocks(
+    const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b,
+    int64_t sv_t, int64_t sv_h, int dtype, const int32_t* tables, int width,
+    const int32_t* lengths, const int32_t* starts, void* k_codes, void* v_codes, void* k_scale,
+    void* v_scale, int pages, int B, int N, int HK, int D, int block, kad_stream_t stream) {
+  KAD_REQUIRE(B > 0 && N > 0 && HK > 0 && width > 0 && pages > 0, "empty dimensions");
+  KAD_REQUIRE(k && v && tables && lengths && k_codes && v_codes && k_scale && v_scale,
+              "null pointer argument");
+  KAD_REQUIRE(D == 64 || D == 128 || D == 256, "head dim %d is not 64, 128 or 256", D);
+  KAD_REQUIRE(block == 32 || block == 64 || block == 128 || block == 256,
+              "block size %d is not 32, 64, 128 or 256", block);
+  WriteArgs a = {{k, v}, {sk_b, sv_b}, {sk_t, sv_t}, {sk_h, sv_h}, tables, lengths, starts,
+                 {(uint8_t*)k_codes, (uint8_t*)v_codes}, {(uint8_t*)k_scale, (uint8_t*)v_scale},
+                 width, pages, B, N, HK, D, block, 0};
+  // N tokens reach into at most this many pages of a request
+  a.touched = (int)(starts ? ((int64_t)N + block - 2) / block + 1 : kad_cdiv(N, block));
+  if (a.touched > width) a.touched = width;
+  KAD_REQUIRE((int64_t)a.touched * B <= 0x7fffffff && HK <= 65535, "too many pages for a launch");
+  const dim3 grid((unsigned)(a.touched * B), (unsigned)HK, 2);
+  if (dtype == KAD_DTYPE_BF16)
+    hipLaunchKernelGGL(write_blocks_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (dtype == KAD_DTYPE_F16)
+    hipLaunchKernelGGL(write_blocks_kernel<_Float16>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else if (dtype == KAD_DTYPE_F32)
+    hipLaunchKernelGGL(write_blocks_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  else
+    KAD_UNSUPPORTED("dtype code %d", dtype);
+  return kad_launch_status("write_blocks_kernel");
+}

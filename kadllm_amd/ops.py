@@ -18,6 +18,8 @@ import math
 import torch
 
 from . import _lib
+from .prefix_cache import (PrefixBlocks, block_prefix_attention,  # noqa: F401
+                           prefix_block_tables, write_prefix_blocks)
 
 
 def _backend(name, tensors):

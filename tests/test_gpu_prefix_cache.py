@@ -1,0 +1,579 @@
+"""The 8-bit prefix cache's operators on the GPU against the oracle in 64 bits.
+
+Block tables and writes are compared exactly.  Attention is held to a bound
+for each output that counts the roundings (u = half a step of the type: 2^-8
+for bf16, 2^-11 for fp16; e4m3's is 2^-4):
+  - the output's own rounding: u |out|, and half of fp16's subnormal step;
+  - the softmax weights' rounding before the second product: two e4m3 pieces
+    for bf16 (2^-8), three for fp16 (2^-12), or the suffix's weights in the
+    queries' own type (u): u sum_j p_j |v_j|;
+  - pieces below e4m3's range: a piece's subnormal step is 2^-9, half of it
+    2^-10, and the last piece carries at least another 2^-4 while 32 weights
+    share a scale that puts their largest, at most 1, above 2^7: 2^-21 |v_j|
+    for each cached key's weight before the division by l;
+  - the scores: an fp32 sum of D products, (D + 4) 2^-24 sum_d |q_d k_d|, and
+    a query element's piece, 2^-21 max|q| sum_d |k_d| for the row; twice the
+    largest such error, relative, on all weights (weights and their sum), plus
+    2^-19 for exponentials, sums and the division in fp32.
+"""
+
+import pytest
+import torch
+
+from kadllm_amd.ops import (PrefixBlocks, block_prefix_attention, prefix_attention,
+                            prefix_block_tables, write_prefix_blocks)
+from oracle import prefix_cache_ref as ref
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def _ints(values, device):
+    return torch.tensor(values, dtype=I32, device=device)
+
+
+# ----------------------------------------------------------------------------
+# block tables
+
+@pytest.mark.parametrize("B, most, block, seed", [
+    (1, 1, 64, 0), (1, 64, 64, 1), (1, 65, 64, 2), (3, 31, 32, 3), (32, 1024, 64, 4),
+    (257, 700, 128, 5), (1000, 90, 32, 6), (5, 70000, 32, 7), (2, 300, 256, 8)])
+@pytest.mark.parametrize("mode", ["fresh", "grow", "grow_fresh_columns", "short"])
+def test_tables_match_the_oracle(device, B, most, block, seed, mode):
+    gen = torch.Generator().manual_seed(seed)
+    lengths = torch.randint(0, most + 1, (B,), generator=gen)
+    lengths[0] = most
+    if B > 2:
+        lengths[1], lengths[2] = 0, most + 5   # cut at max_length
+    width = -(-most // block)
+    free = torch.randperm(B * width + 3, generator=gen)
+    starts = tables = None
+    if mode.startswith("grow"):
+        starts = (lengths * torch.rand(B, generator=gen)).long()
+        cols = width if mode == "grow" else max(1, width // 2)
+        tables = torch.randint(0, 10**6, (B, cols), generator=gen)
+    if mode == "short":
+        free = free[:max(1, B * width // 3)]
+    want, used = ref.block_tables(lengths.tolist(), free.tolist(), block, most,
+                                  None if starts is None else starts.tolist(),
+                                  None if tables is None else tables.tolist())
+    on = lambda x: None if x is None else x.int().to(device)  # noqa: E731
+    got, n = prefix_block_tables(on(lengths), on(free), block_size=block, max_length=most,
+                                 starts=on(starts), tables=on(tables))
+    assert got.dtype == n.dtype == I32
+    assert got.cpu().tolist() == want and n.cpu().tolist() == [used]
+
+
+def test_tables_take_views_and_an_empty_list(device):
+    lengths = _ints([[70, 1], [64, 2], [0, 3]], device)[:, 0]
+    got, used = prefix_block_tables(lengths, _ints([], device), block_size=64, max_length=70)
+    assert got.tolist() == [[-1, -1]] * 3 and used.item() == 3
+    # requests that shrink keep their pages
+    got, used = prefix_block_tables(_ints([1], device), _ints([9], device), block_size=32,
+                                    max_length=64, starts=_ints([64], device),
+                                    tables=_ints([[4, 5]], device))
+    assert got.tolist() == [[4, 5]] and used.item() == 0
+
+
+# ----------------------------------------------------------------------------
+# writing
+
+def _pool(device, pages, HK, block, D, seed):
+    """A pool whose every byte is set: codes without NaN, scales around 1."""
+    gen = torch.Generator().manual_seed(seed)
+    codes = [torch.randint(0, 256, (pages, HK, block, D), generator=gen, dtype=torch.uint8)
+             for _ in range(2)]
+    for c in codes:
+        c[(c & 127) == 127] = 0
+    scales = [torch.randint(117, 130, (pages, HK), generator=gen, dtype=torch.uint8)
+              for _ in range(2)]
+    return PrefixBlocks(*(c.to(device).view(torch.float8_e4m3fn) for c in codes),
+                        *(s.to(device).view(torch.float8_e8m0fnu) for s in scales))
+
+
+def _check_write(blocks, before, k, v, tables, lengths, starts):
+    block = blocks.k.shape[2]
+    for x, now, was in ((k, (blocks.k, blocks.k_scale), (before.k, before.k_scale)),
+                        (v, (blocks.v, blocks.v_scale), (before.v, before.v_scale))):
+        codes, scales = ref.decode(*was)
+        ref.write(codes, scales, x.double().cpu(), tables, lengths, starts, block)
+        got_codes, got_scales = ref.decode(*now)
+        assert torch.equal(got_scales, scales)
+        assert torch.equal(got_codes.isnan(), codes.isnan())
+        assert torch.equal(got_codes.nan_to_num(0), codes.nan_to_num(0))
+
+
+def _clone(blocks):
+    return PrefixBlocks(*(t.view(torch.uint8).clone().view(t.dtype) for t in blocks))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("HK, D, block", [(2, 256, 64), (1, 64, 32), (3, 128, 128), (1, 256, 256),
+                                          (8, 64, 64), (2, 128, 32)])
+def test_write_matches_the_oracle(device, dtype, HK, D, block):
+    """Whole prompts of unequal length: none, one token, a page's end and
+    beside it, more tokens than given, a missing page and one out of range."""
+    gen = torch.Generator().manual_seed(D + block)
+    N = 2 * block + 3
+    lengths = [0, 1, block - 1, block, block + 1, 2 * block, N, N + 9, -4]
+    B, width = len(lengths), 3
+    order = torch.randperm(B * width, generator=gen).view(B, width)
+    order[6, 1], order[7, 0] = -1, 10**6
+    blocks = _pool(device, B * width + 1, HK, block, D, 1)
+    before = _clone(blocks)
+    magnitudes = torch.randn(B, N, HK, 1, generator=gen).mul(3).exp()
+    k, v = (torch.randn(B, N, HK, D, generator=gen).mul(magnitudes).to(dtype) for _ in range(2))
+    k[3, :, 0] = 0                            # a page and head of zeros
+    if dtype != torch.float16:
+        v[5] *= 1e-36 if dtype == torch.float32 else 1e-20
+    got = write_prefix_blocks(blocks, k.to(device), v.to(device), order.int().to(device),
+                              _ints(lengths, device))
+    assert got is blocks
+    _check_write(blocks, before, k, v, order.tolist(), lengths, [0] * B)
+
+
+def test_write_takes_infinities_nan_and_extremes(device):
+    blocks = _pool(device, 4, 1, 32, 64, 2)
+    before = _clone(blocks)
+    k = torch.randn(4, 32, 1, 64, generator=torch.Generator().manual_seed(3))
+    v = k.clone()
+    k[0, 3, 0, 5], k[0, 4, 0, 6], k[0, 5, 0, 7] = torch.inf, -torch.inf, torch.nan
+    k[1] = torch.nan                          # nothing finite
+    k[2] *= torch.finfo(torch.float32).max / k[2].abs().max()
+    v[2] = torch.finfo(torch.float32).smallest_normal / 4
+    v[3, 0, 0, 0] = 448.0 * 2.0 ** 5          # a border of the scale, and just past it
+    k[3, 0, 0, 0] = 448.0 * 2.0 ** 5 * (1 + 2.0 ** -23)
+    write_prefix_blocks(blocks, k.to(device), v.to(device), _ints([[0], [1], [2], [3]], device),
+                        _ints([32] * 4, device))
+    _check_write(blocks, before, k, v, [[0], [1], [2], [3]], [32] * 4, [0] * 4)
+
+
+@pytest.mark.parametrize("layout", ["heads_first", "projection", "every_other", "broadcast",
+                                    "odd_offset", "columns"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_write_takes_strides(device, layout, dtype):
+    B, N, HK, D, block = 2, 70, 2, 64, 32
+    gen = torch.Generator(device=device).manual_seed(4)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=device).to(dtype)  # noqa: E731
+    if layout == "heads_first":
+        k, v = (rand(B, HK, N, D).transpose(1, 2) for _ in range(2))
+    elif layout == "projection":
+        rows = rand(B, N, 3 * HK * D + 8)
+        k, v = (rows[..., i * HK * D:(i + 1) * HK * D].unflatten(2, (HK, D)) for i in (1, 2))
+    elif layout == "every_other":
+        k, v = (rand(B, 2 * N, HK, D)[:, ::2] for _ in range(2))
+    elif layout == "broadcast":
+        k, v = rand(1, N, 1, D).expand(B, N, HK, D), rand(B, 1, HK, D).expand(B, N, HK, D)
+    elif layout == "odd_offset":              # rows that start at any element
+        k, v = (rand(B * N * HK * (D + 1) + 1)[1:].view(B, N, HK, D + 1)[..., :D]
+                for _ in range(2))
+    else:                                     # a last dimension that is not contiguous
+        k, v = (rand(B, N, D, HK).transpose(2, 3) for _ in range(2))
+    blocks = _pool(device, 6, HK, block, D, 5)
+    before = _clone(blocks)
+    tables, lengths = [[3, 1, 5], [0, 2, 4]], [70, 41]
+    write_prefix_blocks(blocks, k, v, _ints(tables, device), _ints(lengths, device))
+    _check_write(blocks, before, k, v, tables, lengths, [0, 0])
+
+
+@pytest.mark.parametrize("HK, D, block", [(2, 256, 64), (1, 64, 32), (2, 128, 256)])
+def test_single_tokens_and_chunks_extend_pages(device, HK, D, block):
+    """Appends of one token, then of chunks, with magnitudes that grow, shrink
+    and grow, so that scales stay, rise and make earlier codes round again."""
+    gen = torch.Generator().manual_seed(6)
+    B, width = 3, 3
+    tables = torch.randperm(B * width, generator=gen).view(B, width)
+    blocks = _pool(device, B * width, HK, block, D, 6)
+    starts = [0, block - 2, 5]
+    steps = [(1, 1.0), (1, 0.1), (1, 30.0), (1, 2.0), (block // 2 + 1, 1e-3), (3, 500.0),
+             (block, 40.0)]
+    for n, magnitude in steps:
+        k, v = (torch.randn(B, n, HK, D, generator=gen).mul(magnitude).bfloat16()
+                for _ in range(2))
+        lengths = [s + n for s in starts]
+        lengths[1] -= n // 2                  # one request takes fewer tokens than given
+        before = _clone(blocks)
+        write_prefix_blocks(blocks, k.to(device), v.to(device), tables.int().to(device),
+                            _ints(lengths, device), starts=_ints(starts, device))
+        _check_write(blocks, before, k, v, tables.tolist(), lengths, starts)
+        starts = lengths
+
+
+# ----------------------------------------------------------------------------
+# attention
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _attention_bound(q, pool_k, y, weight, slack, suffix_k, scale):
+    """The module docstring's bound for each output."""
+    dtype, D = q.dtype, q.shape[3]
+    codes, scales = pool_k
+    keys = (codes.nan_to_num(0) * scales[..., None, None]).abs()
+    rows = keys.flatten(0, 2)
+    if suffix_k is not None:
+        rows = torch.cat((rows, suffix_k.double().cpu().nan_to_num(0, 0, 0).abs().flatten(0, 2)))
+    qa = q.double().cpu().abs().flatten(0, 2)
+    product = (qa @ rows.T).max(1).values                      # largest sum_d |q_d k_d| of a row
+    piece = qa.max(1).values * rows.sum(1).max() * 2.0 ** -21
+    score = (abs(scale) * (product * (D + 4) * 2.0 ** -24 + piece)).view(q.shape[:3] + (1,))
+    p = max(_u(dtype), 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -12)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    return (_u(dtype) * y.abs() + (p + 2 * score + 2.0 ** -19) * (1 + _u(dtype)) * weight
+            + 2.0 ** -21 * slack + tiny)
+
+
+def _check_attention(out, q, blocks, tables, lengths, sk, sv, W, gate=None, scale=None):
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    pool_k = ref.decode(blocks.k, blocks.k_scale)
+    pool_v = ref.decode(blocks.v, blocks.v_scale)
+    y, weight, slack = ref.attention(q, pool_k, pool_v, tables, lengths, sk, sv, W, scale, gate)
+    assert out.dtype == q.dtype and out.shape == q.shape
+    got = out.double().cpu()
+    assert torch.equal(got.isnan(), y.isnan())
+    bound = _attention_bound(q, pool_k, y, weight, slack, sk, scale)
+    off = (got - y).abs() - bound
+    off = off[~y.isnan()]
+    assert off.numel() == 0 or off.max() <= 0, f"over the bound by {off.max():.3g}"
+
+
+def _quiet_pool(device, pages, HK, block, D, seed):
+    """A pool of normal keys and values."""
+    gen = torch.Generator().manual_seed(seed)
+    blocks = _pool(device, pages, HK, block, D, seed)
+    x = [torch.randn(pages, block, HK, D, generator=gen).to(device) for _ in range(2)]
+    ids = torch.arange(pages, dtype=I32, device=device).view(pages, 1)
+    return write_prefix_blocks(blocks, *x, ids, _ints([block] * pages, device))
+
+
+def _problem(device, lengths, W, T, Tk, H, HK, D, block, dtype, gated=False, seed=0, spread=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    B = len(lengths)
+    width = max(1, -(-max(lengths) // block))
+    blocks = _quiet_pool(device, B * width + 1, HK, block, D, seed)
+    tables = torch.randperm(B * width + 1, generator=gen)[:B * width].view(B, width)
+    held = torch.tensor([[j * block < n for j in range(width)] for n in lengths])
+    tables = torch.where(held, tables, -1).int()
+    rand = lambda *s: torch.randn(*s, generator=gen).to(dtype).to(device)  # noqa: E731
+    q = rand(B * W, T, H, D) * spread
+    sk, sv = (rand(B * W, Tk, HK, D) if Tk else None for _ in range(2))
+    gate = rand(B * W, T, H * D) if gated else None
+    return q, blocks, tables.to(device), _ints(lengths, device), sk, sv, gate
+
+
+def _run_and_check(device, lengths, W, T, Tk, H, HK, D, block, dtype, **more):
+    q, blocks, tables, lens, sk, sv, gate = _problem(device, lengths, W, T, Tk, H, HK, D, block,
+                                                     dtype, **more)
+    before = _clone(blocks)
+    out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W, gate=gate)
+    _check_attention(out, q, blocks, tables.tolist(), lengths, sk, sv, W, gate)
+    for now, was in zip(blocks, before):      # the cache is only read
+        assert torch.equal(now.view(torch.uint8), was.view(torch.uint8))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H, HK, D, block", [(8, 2, 256, 64), (4, 1, 64, 32), (6, 2, 128, 128),
+                                             (2, 2, 64, 64), (5, 1, 256, 256), (16, 1, 128, 32)])
+@pytest.mark.parametrize("W, T, Tk", [(1, 1, 0), (1, 1, 1), (3, 1, 2), (2, 3, 3), (2, 2, 5),
+                                      (9, 1, 1)])
+def test_attention_matches_the_oracle(device, dtype, H, HK, D, block, W, T, Tk):
+    """Requests without a prefix, of one token, ending at and beside a page."""
+    _run_and_check(device, [0, 1, block - 1, 2 * block + 1], W, T, Tk, H, HK, D, block, dtype,
+                   gated=Tk == 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths, W, T, Tk, H, HK, D, block", [
+    ([1500], 1, 1, 1, 2, 1, 256, 64),
+    ([1023, 65], 40, 1, 2, 2, 1, 128, 64),
+    ([700, 0, 33], 33, 2, 2, 4, 1, 64, 32),
+    ([300], 70, 3, 4, 2, 1, 256, 64),
+    ([257, 256, 255], 5, 1, 8, 3, 1, 128, 256),
+    ([4100], 2, 1, 0, 1, 1, 64, 128),
+])
+def test_attention_over_longer_prefixes(device, dtype, lengths, W, T, Tk, H, HK, D, block):
+    _run_and_check(device, lengths, W, T, Tk, H, HK, D, block, dtype, seed=1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T, Tk, W, H, HK, D", [(9, 9, 2, 2, 1, 64), (40, 40, 1, 4, 2, 64),
+                                                (1, 33, 3, 2, 1, 128), (37, 70, 1, 3, 1, 256)])
+def test_attention_takes_long_suffixes(device, dtype, T, Tk, W, H, HK, D):
+    """A chunk of a prompt against what is cached, and long replays."""
+    _run_and_check(device, [70], W, T, Tk, H, HK, D, 32, dtype, seed=2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("spread", [0.0, 30.0])
+def test_attention_flat_and_peaked_softmax(device, dtype, spread):
+    _run_and_check(device, [333, 90], 3, 1, 1, 4, 2, 128, 64, dtype, spread=spread, seed=3)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_attention_scores_far_apart(device, D):
+    """Scores that climb by hundreds from page to page, and an outlier that
+    comes last: the running maximum has to follow."""
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, [320, 320], 9, 1, 1, 4, 1, D, 32,
+                                                  torch.bfloat16, seed=4)
+    scales = blocks.k_scale.view(torch.uint8)
+    for j in range(tables.shape[1]):          # each page's keys four times the one before
+        scales[tables[0, j].long()] = 122 + 2 * j
+        scales[tables[1, j].long()] = 140 - 2 * j
+    out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=9)
+    assert out.isfinite().all()
+    # scores of 2^18: an fp32 sum of D products is off by up to 2^18 D 2^-24, so
+    # only rows whose two best keys lie further apart than that have a value
+    y, _, _ = ref.attention(q, ref.decode(blocks.k, blocks.k_scale),
+                            ref.decode(blocks.v, blocks.v_scale), tables.tolist(), [320, 320],
+                            sk, sv, 9, D ** -0.5)
+    near = (out.double().cpu() - y).abs().amax(3) <= 2.0 ** -7 * y.abs().amax(3) + 2.0 ** -8
+    assert near.float().mean() > 0.9
+
+
+def test_attention_ignores_what_lies_behind_the_lengths(device):
+    """NaN codes behind a request's end, in pages that it does not hold and in
+    the suffixes of other beams, and pages out of range."""
+    lengths, W, T, Tk, H, HK, D, block = [70, 33, 0], 5, 2, 2, 4, 2, 64, 32
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, lengths, W, T, Tk, H, HK, D, block,
+                                                  torch.bfloat16, seed=5)
+    want = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W)
+    used = set()
+    raw = [blocks.k.view(torch.uint8), blocks.v.view(torch.uint8)]
+    for b, n in enumerate(lengths):
+        for j, page in enumerate(tables[b].tolist()):
+            if page >= 0:
+                used.add(page)
+                for x in raw:
+                    x[page, :, max(0, n - j * block):] = 0x7f
+    for page in set(range(blocks.k.shape[0])) - used:
+        for x in raw:
+            x[page] = 0xff
+        blocks.k_scale.view(torch.uint8)[page] = 255
+        blocks.v_scale.view(torch.uint8)[page] = 255
+    tables = torch.where(tables < 0, 10**9, tables)
+    got = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W)
+    assert torch.equal(got, want)
+    # one beam's suffix holds NaN and infinities: the others' outputs stay, and
+    # its own first token does not see the second one's
+    for bad in (torch.nan, torch.inf):
+        ks, vs = sk.clone(), sv.clone()
+        ks[6, 1], vs[6, 1] = bad, bad
+        got = block_prefix_attention(q, blocks, tables, lens, ks, vs, beam_width=W)
+        others = [n for n in range(3 * W) if n != 6]
+        assert torch.equal(got[others], want[others])
+        assert torch.equal(got[6, 0], want[6, 0])
+        assert not got[6, 1].isfinite().all()
+
+
+def test_attention_leaves_out_tokens_without_a_page(device):
+    lengths, W, H, HK, D, block = [150, 64], 2, 2, 1, 64, 32
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, lengths, W, 1, 1, H, HK, D, block,
+                                                  torch.bfloat16, seed=6)
+    tables[0, 1], tables[0, 4], tables[1, :] = -1, blocks.k.shape[0], -7
+    out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W)
+    _check_attention(out, q, blocks, tables.tolist(), lengths, sk, sv, W)
+    out = block_prefix_attention(q, blocks, tables, lens, beam_width=W)
+    _check_attention(out, q, blocks, tables.tolist(), lengths, None, None, W)
+    assert (out[W:] == 0).all()               # nothing to see at all
+
+
+def test_attention_nan_in_a_visible_key(device):
+    """A NaN that a query sees makes its row NaN, and no other request's."""
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, [40, 40], 3, 1, 1, 2, 1, 64, 32,
+                                                  torch.bfloat16, seed=7)
+    want = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=3)
+    blocks.k.view(torch.uint8)[tables[0, 1].item(), 0, 3, 9] = 0x7f
+    got = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=3)
+    assert got[:3].isnan().all() and torch.equal(got[3:], want[3:])
+    q[4, 0, 1, 7] = torch.nan
+    got = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=3)
+    assert got[4, 0, 1].isnan().all() and torch.equal(got[4, 0, 0], want[4, 0, 0])
+    assert torch.equal(got[[3, 5]], want[[3, 5]])
+
+
+def test_attention_takes_strides(device):
+    lengths, W, T, Tk, H, HK, D, block = [50, 90], 3, 2, 3, 4, 2, 64, 32
+    q, blocks, tables, lens, sk, sv, gate = _problem(device, lengths, W, T, Tk, H, HK, D, block,
+                                                     torch.bfloat16, gated=True, seed=8)
+    want = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W, gate=gate)
+
+    def spread(x, pad):                       # rows that start at odd elements
+        y = torch.zeros(*x.shape[:-1], x.shape[-1] + pad, dtype=x.dtype, device=device)
+        y[..., 1:1 + x.shape[-1]] = x
+        return y[..., 1:1 + x.shape[-1]]
+
+    wide = torch.full((2, 2 * tables.shape[1]), -1, dtype=I32, device=device)
+    wide[:, ::2] = tables
+    got = block_prefix_attention(spread(q, 5), blocks, wide[:, ::2], lens, spread(sk, 3),
+                                 spread(sv, 7), beam_width=W, gate=spread(gate, 9))
+    assert torch.equal(got, want)
+    turned = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    across = lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)  # noqa: E731
+    got = block_prefix_attention(turned(q), blocks, tables, lens, turned(sk), across(sv),
+                                 beam_width=W, gate=gate)
+    assert torch.equal(got, want)
+    one = sk[:1].expand(2 * W, Tk, HK, D)     # every beam the same suffix
+    got = block_prefix_attention(q, blocks, tables, lens, one, one, beam_width=W)
+    _check_attention(got, q, blocks, tables.tolist(), lengths, one, one, W)
+
+
+def test_requests_share_pages(device):
+    """Two requests whose tables name the same pages, one shorter."""
+    q, blocks, tables, _, sk, sv, _ = _problem(device, [96, 96], 2, 1, 1, 2, 1, 64, 32,
+                                               torch.bfloat16, seed=9)
+    tables[1, :2] = tables[0, :2]
+    lengths = [96, 41]
+    out = block_prefix_attention(q, blocks, tables, _ints(lengths, device), sk, sv, beam_width=2)
+    _check_attention(out, q, blocks, tables.tolist(), lengths, sk, sv, 2)
+
+
+def test_scale_and_its_sign(device):
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, [77], 2, 1, 1, 2, 1, 128, 32,
+                                                  torch.bfloat16, seed=10)
+    for scale in (0.3, -0.2, 0.0):
+        out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=2, scale=scale)
+        _check_attention(out, q, blocks, tables.tolist(), [77], sk, sv, 2, scale=scale)
+
+
+def test_rows_do_not_depend_on_what_comes_with_them(device):
+    """The same request alone, twice, and among others gives the same bits
+    within one launch shape; calls repeat bit for bit."""
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, [200, 500, 200], 4, 1, 2, 8, 2, 256, 64,
+                                                  torch.bfloat16, seed=11)
+    tables[2], q[8:], sk[8:], sv[8:] = tables[0], q[:4], sk[:4], sv[:4]
+    out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=4)
+    assert torch.equal(out[8:], out[:4])
+    for _ in range(3):
+        assert torch.equal(block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=4),
+                           out)
+
+
+def test_pool_past_32_bits(device):
+    """Pages whose bytes lie more than 2^31 (and 2^32) into the pool."""
+    HK, D, block = 2, 256, 64
+    pages = 2**32 // (HK * D * block) + 9
+    codes = [torch.empty(pages, HK, block, D, dtype=torch.uint8, device=device)
+             .view(torch.float8_e4m3fn) for _ in range(2)]
+    scales = [torch.empty(pages, HK, dtype=torch.uint8, device=device)
+              .view(torch.float8_e8m0fnu) for _ in range(2)]
+    blocks = PrefixBlocks(*codes, *scales)
+    ids = [pages - 1, pages // 2 + 1, 3]
+    gen = torch.Generator(device=device).manual_seed(12)
+    k, v = (torch.randn(1, 150, HK, D, generator=gen, device=device).bfloat16()
+            for _ in range(2))
+    small = PrefixBlocks.empty(3, HK, D, block_size=block, device=device)
+    q = torch.randn(3, 1, 8, D, generator=gen, device=device).bfloat16()
+    got = []
+    for b, table in ((blocks, ids), (small, [0, 1, 2])):
+        table = _ints([table], device)
+        write_prefix_blocks(b, k, v, table, _ints([150], device))
+        got.append(block_prefix_attention(q, b, table, _ints([150], device), beam_width=3))
+    assert torch.equal(*got)
+    for j, page in enumerate(ids):
+        rows = min(block, 150 - j * block)
+        assert torch.equal(blocks.v.view(torch.uint8)[page, :, :rows],
+                           small.v.view(torch.uint8)[j, :, :rows])
+        assert torch.equal(blocks.k_scale.view(torch.uint8)[page],
+                           small.k_scale.view(torch.uint8)[j])
+
+
+# ----------------------------------------------------------------------------
+# the operators together
+
+def _serve(blocks, free, k, v, k1, v1, q, sk, sv, lengths, W):
+    """Pages for the prompts, their keys and values, one token more for each
+    request, and the beams' attention: what a serving step calls."""
+    L = k.shape[1] + 1
+    tables, used = prefix_block_tables(lengths, free, block_size=32, max_length=L)
+    write_prefix_blocks(blocks, k, v, tables, lengths)
+    longer = lengths + 1
+    tables, more = prefix_block_tables(longer, free[6:], block_size=32, max_length=L,
+                                       starts=lengths, tables=tables)
+    write_prefix_blocks(blocks, k1, v1, tables, longer, starts=lengths)
+    return block_prefix_attention(q, blocks, tables, longer, sk, sv, beam_width=W), tables, \
+        used, more
+
+
+def _serving_inputs(device, seed):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, generator=gen, device=device).bfloat16()  # noqa: E731
+    B, L, W, H, HK, D = 3, 95, 4, 4, 2, 64
+    free = torch.randperm(12, generator=gen, device=device).int()
+    return (free, rand(B, HK, L, D).transpose(1, 2), rand(B, HK, L, D).transpose(1, 2),
+            rand(B, 1, HK, D) * 3, rand(B, 1, HK, D) * 3, rand(B * W, 2, H, D),
+            rand(B * W, 2, HK, D), rand(B * W, 2, HK, D), _ints([95, 64, 31], device))
+
+
+def test_tables_writes_and_attention_together(device):
+    args = _serving_inputs(device, 13)
+    free, k, v, k1, v1, q, sk, sv, lengths = args
+    blocks = _pool(device, 12, 2, 32, 64, 13)
+    codes = [ref.decode(blocks.k, blocks.k_scale), ref.decode(blocks.v, blocks.v_scale)]
+    out, tables, used, more = _serve(blocks, *args, W=4)
+    assert used.item() == 3 + 2 + 1 and more.item() == 1
+    longer = (lengths + 1).tolist()
+    want, _ = ref.block_tables(lengths.tolist(), free.tolist(), 32, 96)
+    want, _ = ref.block_tables(longer, free.tolist()[6:], 32, 96, lengths.tolist(), want)
+    assert tables.tolist() == want
+    for (c, s), first, second in zip(codes, (k, v), (k1, v1)):
+        ref.write(c, s, first.double().cpu(), want, lengths.tolist(), [0] * 3, 32)
+        ref.write(c, s, second.double().cpu(), want, longer, lengths.tolist(), 32)
+    for (c, s), now in zip(codes, ((blocks.k, blocks.k_scale), (blocks.v, blocks.v_scale))):
+        got = ref.decode(*now)
+        assert torch.equal(got[0], c) and torch.equal(got[1], s)
+    _check_attention(out, q, blocks, want, longer, sk, sv, 4)
+    # near the operator that keeps the prefix in bf16: 8 bits cost up to half a
+    # step (2^-4) of every key and value, at random over 64 dims and ~90 keys
+    dense = prefix_attention(q[:4], torch.cat((k, k1), 1)[:1], torch.cat((v, v1), 1)[:1], sk[:4],
+                             sv[:4], beam_width=4)
+    assert (out[:4].float() - dense.float()).norm() < 2 * 2.0 ** -4 * dense.float().norm()
+
+
+def test_a_captured_step_replays(device):
+    """The whole step in a graph, replayed over changing inputs with eager work
+    between the replays, and a second graph beside it."""
+    runs = []
+    for seed in (14, 15):
+        args = [x.clone() for x in _serving_inputs(device, seed)]
+        blocks = _pool(device, 12, 2, 32, 64, seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _serve(blocks, *args, W=4)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _serve(blocks, *args, W=4)
+        runs.append((args, blocks, graph, got))
+    for turn in range(3):
+        for seed, (args, blocks, graph, got) in enumerate(runs):
+            fresh = _serving_inputs(device, 20 + 2 * turn + seed)
+            for dst, src in zip(args, fresh):
+                dst.copy_(src)
+            base = _pool(device, 12, 2, 32, 64, turn)
+            for dst, src in zip(blocks, base):
+                dst.view(torch.uint8).copy_(src.view(torch.uint8))
+            graph.replay()
+            torch.cuda.synchronize()
+            want = _serve(base, *fresh, W=4)
+            for x, y in zip(got, want):
+                assert torch.equal(x, y)
+            for x, y in zip(blocks, base):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def test_two_streams_at_once(device):
+    args = [_serving_inputs(device, s) for s in (30, 31)]
+    want = [_serve(_pool(device, 12, 2, 32, 64, 3), *a, W=4)[0] for a in args]
+    pools = [_pool(device, 12, 2, 32, 64, 3) for _ in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = _serve(pools[i], *args[i], W=4)[0]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
