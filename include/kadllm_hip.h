@@ -613,7 +613,12 @@ int kad_write_prefix_blocks(const void* k, int64_t sk_b, int64_t sk_t, int64_t s
  * (n, t, h) see the first lengths[b] cached tokens of their request b = n / W
  * and the suffix keys j <= Tk - T + t of their beam (Tk = 0: no suffix).  bf16
  * or fp16 queries, suffixes, gate (may be null) and out; last dimensions
- * contiguous.  A row that sees no key gives zeros. */
+ * contiguous; query and suffix K rows 16-byte, suffix V rows 8-byte aligned.  A
+ * row that sees no key gives zeros.  The workspace (its size from
+ * kad_block_prefix_attention_workspace_bytes, 0 where none is needed) holds
+ * the partial results of a prefix that is split over workgroups. */
+int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, int H, int HK, int D,
+                                               int width, int block, int64_t* bytes);
 int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_t sq_h,
                                const void* k_codes, const void* v_codes, const void* k_scale,
                                const void* v_scale, int pages, const int32_t* tables, int width,
@@ -621,8 +626,9 @@ int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_
                                int64_t ssk_t, int64_t ssk_h, const void* suffix_v, int64_t ssv_n,
                                int64_t ssv_t, int64_t ssv_h, const void* gate, int64_t sg_n,
                                int64_t sg_t, int64_t sg_h, void* out, int64_t so_n, int64_t so_t,
-                               int64_t so_h, int B, int W, int T, int Tk, int H, int HK, int D,
-                               int block, int dtype, float scale, kad_stream_t stream);
+                               int64_t so_h, void* workspace, int64_t workspace_bytes, int B,
+                               int W, int T, int Tk, int H, int HK, int D, int block, int dtype,
+                               float scale, kad_stream_t stream);
 
 /* --------------------------------------------------------------------------
  * MFMA lane-layout self-test (no reference counterpart): C[16x16] = A[16x32]

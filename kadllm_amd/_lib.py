@@ -73,8 +73,9 @@ SIGNATURES = {
     "kad_qwen_decode_step": "pps",
     "kad_prefix_block_tables": "pppipipipiiis",
     "kad_write_prefix_blocks": "plll" "plll" "i" "pipp" "pppp" "iiiiii" "s",
-    "kad_block_prefix_attention": "plll" "ppppi" "pip" "plll" "plll" "plll" "plll" "iiiiiiiii"
-                                  "f" "s",
+    "kad_block_prefix_attention_workspace_bytes": "iiiiiiiip",
+    "kad_block_prefix_attention": "plll" "ppppi" "pip" "plll" "plll" "plll" "plll" "pl"
+                                  "iiiiiiiii" "f" "s",
     "kad_selftest_mfma_f32": "ppps",
     "kad_selftest_mfma16": "ppps",
     "kad_selftest_mfma32": "ppps",

@@ -6,8 +6,26 @@
 //   out = sum_j softmax(s)_j v_j, times sigmoid(gate) where one is given
 // with k_j, v_j = code * scale of the page and KV head that holds token j.  A
 // row that sees no key gives zeros.
+//
+// Both products over the cache run on v_mfma_scale_f32_32x32x64_f8f6f4, which
+// reads the cache's e4m3 codes as they are and applies the page's power of two
+// itself.  The other operand is split into e4m3 pieces: x = 2^E (y0 + y1 / 16
+// + y2 / 256), each y the e4m3 rounding of 16 times what the pieces before it
+// left.  A piece keeps 4 significant bits, so two hold a bf16 value exactly
+// (8 bits) and three an fp16 one (11 bits), as far down as 2^-10 of the row's
+// largest element; below that the error is at most 2^-22 of the largest.  Two
+// pieces cost what one bf16 product would (e4m3 runs at twice the rate), and
+// the cache is neither widened in registers nor stored wide in LDS.
+//
+// The softmax weights of 32 keys are split the same way against the block's own
+// power of two, which the second product's scale operand restores: 2^-8
+// relative per weight with two pieces (bf16), 2^-12 with three (fp16).
+
+#include <type_traits>
 
 #include "kad_common.h"
+
+namespace {
 
 struct BlockAttnArgs {
   const void* q;
@@ -23,78 +41,671 @@ struct BlockAttnArgs {
   int64_t sg_n, sg_t, sg_h;
   void* out;
   int64_t so_n, so_t, so_h;
-  int pages, width, W, T, Tk, H, HK, block;
-  int64_t rows;
-  float scale;
+  float* part_o;    // splits > 1: [split][B*HK][R][D] unnormalised outputs
+  float* part_ml;   // and [split][B*HK][R][2]: the exponent they are relative to, the sum
+  int pages, width, B, W, T, Tk, H, HK, lblock;
+  int splits, nqblk;
+  int R;            // query rows of a request and KV head, W * T * (H / HK)
+  float qmul, sl2;  // sign of the scale (0 for none), |scale| in log2 units
 };
 
-// One wave per query row, lane l holding D / 64 of its elements; the softmax
-// runs over the keys one at a time.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void block_attn_row_kernel(BlockAttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  const int h = (int)(row % a.H), t = (int)(row / a.H % a.T);
-  const int64_t n = row / a.H / a.T;
-  const int b = (int)(n / a.W), kh = h / (a.H / a.HK);
-  float q[E], o[E];
-  for (int i = 0; i < E; ++i) {
-    q[i] = a.scale * Elem<T>::to_f(
-        ((const T*)a.q)[n * a.sq_n + t * a.sq_t + h * a.sq_h + lane * E + i]);
-    o[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  auto take = [&](const float* k, const float* v) {
-    float s = 0.f;
-    for (int i = 0; i < E; ++i) s = fmaf(q[i], k[i], s);
-    s = wave_sum(s);
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : expf(m - top), p = expf(s - top);
-    for (int i = 0; i < E; ++i) o[i] = fmaf(p, v[i], o[i] * keep);
-    l = l * keep + p;
-    m = top;
-  };
-  const int len = min(a.lengths[b], a.width * a.block);
-  for (int j = 0; j < len; ++j) {
-    const int page = a.tables[(int64_t)b * a.width + j / a.block];
-    if (page < 0 || page >= a.pages) continue;
-    const int64_t ph = (int64_t)page * a.HK + kh;
-    const int64_t at = (ph * a.block + j % a.block) * D + lane * E;
-    const float ks = ldexpf(1.f, (int)a.ksc[ph] - 127), vs = ldexpf(1.f, (int)a.vsc[ph] - 127);
-    float k[E], v[E];
-    for (int i = 0; i < E; ++i) {
-      k[i] = __builtin_amdgcn_cvt_f32_fp8((int)a.kc[at + i], 0) * ks;
-      v[i] = __builtin_amdgcn_cvt_f32_fp8((int)a.vc[at + i], 0) * vs;
-    }
-    take(k, v);
-  }
-  for (int j = 0; j <= a.Tk - a.T + t && j < a.Tk; ++j) {
-    float k[E], v[E];
-    for (int i = 0; i < E; ++i) {
-      const int d = lane * E + i;
-      k[i] = Elem<T>::to_f(((const T*)a.sk)[n * a.ssk_n + j * a.ssk_t + kh * a.ssk_h + d]);
-      v[i] = Elem<T>::to_f(((const T*)a.sv)[n * a.ssv_n + j * a.ssv_t + kh * a.ssv_h + d]);
-    }
-    take(k, v);
-  }
-  for (int i = 0; i < E; ++i) {
-    float y = l > 0.f || l != l ? o[i] / l : 0.f;
-    if (a.gate)
-      y *= sigmoid_f(Elem<T>::to_f(
-          ((const T*)a.gate)[n * a.sg_n + t * a.sg_t + h * a.sg_h + lane * E + i]));
-    ((T*)a.out)[n * a.so_n + t * a.so_t + h * a.so_h + lane * E + i] = Elem<T>::from_f(y);
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) void lds_t;
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    static_for<N, I + 1>(f);
   }
 }
 
+__device__ __forceinline__ float max_xor32_f(float x) { return max_xor32(x); }
+
+// A wave's fragment layout of v_mfma_scale_f32_32x32x64 for 8-bit operands:
+// lane l holds row (column for B) l % 32; its bytes 0-15 are k = 16 (l / 32) +
+// 0..15 and its bytes 16-31 k = 32 + 16 (l / 32) + 0..15; the scale byte of
+// lanes 0-31 serves k < 32 and that of lanes 32-63 k >= 32.
+__device__ __forceinline__ f32x16 mfma_scaled(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
+}
+
+// 4 floats to a dword of e4m3 codes, and what they leave, times 16
+__device__ __forceinline__ int piece4(const float* y, float* rest) {
+  int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
+  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+  rest[0] = (y[0] - lo[0]) * 16.f;
+  rest[1] = (y[1] - lo[1]) * 16.f;
+  rest[2] = (y[2] - hi[0]) * 16.f;
+  rest[3] = (y[3] - hi[1]) * 16.f;
+  return c;
+}
+__device__ __forceinline__ float pow2i(int e) {  // 2^e, -126 <= e <= 127
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+template <typename T> struct Pieces;
+template <> struct Pieces<bf16_t> { static constexpr int n = 2; };
+template <> struct Pieces<_Float16> { static constexpr int n = 3; };
+
+// 8 elements at a 16-byte aligned address as floats
+__device__ __forceinline__ void load8(const bf16_t* p, float* f) {
+  const u32x4 v = *(const u32x4*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(v[i] << 16);
+    f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const _Float16* p, float* f) {
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  const f16x8 v = *(const f16x8*)p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
+}
+// 4 elements at an 8-byte aligned address
+__device__ __forceinline__ void load4(const bf16_t* p, float* f) {
+  const u32x2 v = *(const u32x2*)p;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[2 * i] = __uint_as_float(v[i] << 16);
+    f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load4(const _Float16* p, float* f) {
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  const f16x4 v = *(const f16x4*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = (float)v[i];
+}
+
+constexpr int kKeys = 64;       // keys per tile: two halves of 32, each within a page
+constexpr int kMaxUp = 60;      // a tile may exceed the row's reference by 2^60 before it moves
+
+template <int D>
+struct Shape {
+  static constexpr int KS = D / 64, DT = D / 32;   // k-steps of q . k, 32-wide tiles of the output
+  static constexpr int CPR = D / 16;               // 16-byte chunks per key
+  static constexpr int RPI = 64 / CPR;             // keys per 1 KB load instruction
+  static constexpr int tile = kKeys * D;           // bytes of a K (or V) tile
+  static constexpr int slot = 2 * tile;
+  static constexpr int LT = tile / 1024;           // load instructions per K (or V) tile
+  static constexpr int stages = 4;
+  static constexpr int EpiLd = D + 4;              // fp32 row stride of the output transpose
+  static constexpr int epi = 4 * 32 * EpiLd * 4;
+  static constexpr int lds = stages * slot > epi ? stages * slot : epi;
+  // physical 16-byte chunk of logical chunk c in key row r is c ^ sw(r): the 8
+  // rows that one fragment read serves together then lie in 8 different bank
+  // groups.  K fragments take rows 0-7 of 8; V's transpose reads rows {0-3,
+  // 8-11} + 4 (l / 32).
+  __device__ static __forceinline__ int swk(int r) {
+    return D == 256 ? r & 15 : D == 128 ? r & 7 : (r >> 1) & 3;
+  }
+  __device__ static __forceinline__ int swv(int r) {
+    const int b0 = r & 1, b1 = r >> 1 & 1, b2 = r >> 2 & 1, b3 = r >> 3 & 1;
+    return D == 256 ? b0 | b1 << 1 | b3 << 2 | b2 << 3 : D == 128 ? b0 | b1 << 1 | b3 << 2
+                                                                  : b1 | b3 << 1;
+  }
+};
+
+// the V^T fragments of two 32-wide output tiles: for each, 4 transpose reads of
+// 8 keys (within 16 lanes, lane i receives byte i % 8 of the 8-byte pieces that
+// lanes 2e + i / 8 address, e < 8), waited for inside
+template <int D>
+__device__ __forceinline__ void read_v2(uint32_t p0, uint32_t p1, i32x8& f0, i32x8& f1) {
+  u32x2 a0, a1, a2, a3, b0, b1, b2, b3;
+  asm volatile(
+      "ds_read_b64_tr_b8 %0, %8\n\t"
+      "ds_read_b64_tr_b8 %1, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b8 %2, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b8 %3, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b8 %4, %9\n\t"
+      "ds_read_b64_tr_b8 %5, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b8 %6, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b8 %7, %9 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3), "=&v"(b0), "=&v"(b1), "=&v"(b2), "=&v"(b3)
+      : "v"(p0), "v"(p1), "i"(16 * D), "i"(32 * D), "i"(48 * D)
+      : "memory");
+  f0 = i32x8{(int)a0[0], (int)a0[1], (int)a1[0], (int)a1[1],
+             (int)a2[0], (int)a2[1], (int)a3[0], (int)a3[1]};
+  f1 = i32x8{(int)b0[0], (int)b0[1], (int)b1[0], (int)b1[1],
+             (int)b2[0], (int)b2[1], (int)b3[0], (int)b3[1]};
+}
+
+__device__ __forceinline__ void wait_vm(int n) {
+  // vmcnt(n), lgkmcnt and expcnt left alone; n a constant after inlining
+  switch (n) {
+#define KAD_W(N) case N: __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14)); break;
+    KAD_W(0) KAD_W(1) KAD_W(2) KAD_W(3) KAD_W(4) KAD_W(6) KAD_W(8) KAD_W(12) KAD_W(16)
+    KAD_W(24) KAD_W(32)
+#undef KAD_W
+    default: __builtin_amdgcn_s_waitcnt(0x0f70);
+  }
+}
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A workgroup of 4 waves takes a request, a KV head, a range of the prefix
+// (one of `splits`) and query rows, ordered (beam, head in the group, token).
+// A wave holds 32 rows: Q's pieces, the output O^T and the softmax state stay
+// in its registers.  S^T = K Q^T gives a lane the scores of one row (16 of a
+// half tile's 32 keys, the other 16 in lane l ^ 32), and the bytes of its
+// weights are the second product's operand O^T += V^T P^T as they stand.
+//   SHARED: the waves hold 128 rows and walk the same tiles, which arrive in a
+//     ring of 4 LDS stages, three tiles ahead of their use.
+//   otherwise: the waves hold the same 32 rows and take every fourth tile, each
+//     through an LDS slot of its own, K refilled while V is used and V refilled
+//     while the next K is, so no wave waits for another; their states are
+//     joined at the end.
+template <typename T, int D, bool SHARED>
+__global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
+  using S = Shape<D>;
+  constexpr int NP = Pieces<T>::n, KS = S::KS, DT = S::DT;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  __shared__ float sm_m[4][32], sm_l[4][32];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hi = lane >> 5, col = lane & 31;
+  const int lid = xcd_logical_id(blockIdx.x, gridDim.x);
+  const int qb = lid % a.nqblk, split = lid / a.nqblk % a.splits;
+  const int bk = lid / a.nqblk / a.splits;
+  const int kh = bk % a.HK, b = bk / a.HK;
+  const int G = a.H / a.HK;
+
+  // this lane's row (rows past the end repeat the last one and are not stored)
+  const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
+  const int r = min(row0 + col, a.R - 1);
+  const int t = r % a.T, g = r / a.T % G, w = r / a.T / G;
+  const int64_t n = (int64_t)b * a.W + w;
+  const int h = kh * G + g;
+
+  // ---- Q in e4m3 pieces against the row's power of two
+  i32x8 qf[NP][KS];
+  int qs[NP];
+  {
+    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h;
+    float amax = 0.f;
+    float qv[32];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        load8(qrow + 64 * s + 32 * (c >> 1) + 16 * hi + 8 * (c & 1), qv);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(qv[i]));
+      }
+    amax = max_xor32_f(amax);
+    const int E = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -100);
+    const float inv = pow2i(-E) * a.qmul;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        load8(qrow + 64 * s + 32 * (c >> 1) + 16 * hi + 8 * (c & 1), qv + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) qv[i] *= inv;
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[p][s][i] = piece4(qv + 4 * i, qv + 4 * i);
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) qs[p] = E - 4 * p + 127;
+  }
+
+  // ---- softmax state: weights are 2^(s - m) for a reference m that moves only
+  // when a score exceeds it by 2^kMaxUp
+  float m = -INFINITY, l = 0.f;
+  f32x16 O[DT];
+#pragma unroll
+  for (int i = 0; i < DT; ++i) O[i] = f32x16{};
+  auto raise = [&](float top) {   // m up to the row's `top` (where that is far above it)
+    const float to = top > m + kMaxUp ? top : m;
+    const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) O[i][j] *= f;
+  };
+
+  // ---- the beam's own suffix, in fp32, by the first range's first wave
+  if (a.Tk > 0 && split == 0 && (SHARED || wave == 0)) {
+    const int last = a.Tk - a.T + t;             // the row sees suffix keys 0..last
+    int most = last;                             // (all rows of the wave: 0..most)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h;
+    const T* krow = (const T*)a.sk + n * a.ssk_n + kh * a.ssk_h;
+    const T* vrow = (const T*)a.sv + n * a.ssv_n + kh * a.ssv_h;
+    for (int j = 0; j <= most; ++j) {
+      const int jj = min(j, last);
+      const T* kr = krow + (int64_t)jj * a.ssk_t;
+      const T* vr = vrow + (int64_t)jj * a.ssv_t;
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) {
+        float x[8], y[8];
+        load8(qrow + 16 * c + 8 * hi, x);
+        load8(kr + 16 * c + 8 * hi, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+      }
+      s = add_xor32(s) * a.qmul * a.sl2;
+      if (j <= last) {
+        if (m == -INFINITY) m = s;
+      } else {
+        s = -INFINITY;
+      }
+      if (__ballot(s > m + kMaxUp) != 0) raise(s);
+      if (j <= last) {
+        const float p = __builtin_amdgcn_exp2f(s - m);
+        l += p;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            float y[4];
+            load4(vr + 32 * dt + 8 * q4 + 4 * hi, y);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[dt][4 * q4 + i] = fmaf(p, y[i], O[dt][4 * q4 + i]);
+          }
+      }
+    }
+  }
+
+  // ---- this wave's tiles of the prefix: first + stride * k, k < count
+  const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
+  const int tiles = (len + kKeys - 1) / kKeys;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int begin = min(split * per, tiles), end = min(begin + per, tiles);
+  const int first = begin + (SHARED ? 0 : wave), stride = SHARED ? 1 : 4;
+  const int count = __builtin_amdgcn_readfirstlane(
+      SHARED ? end - begin : max((end - first + stride - 1) / stride, 0));
+
+  // Pages: lane i of a chunk of 32 tiles describes half tile i: its page
+  // (-1: none) and keys held | K's scale byte << 8 | V's << 16
+  int pg = -1, meta = 0;
+  auto describe = [&](int chunk) {
+    const int k = 32 * chunk + (lane >> 1);
+    const int pos = (first + stride * k) * kKeys + (lane & 1) * 32;
+    pg = -1;
+    meta = 127 << 8 | 127 << 16;
+    if (k < count && pos < len) {
+      const int id = a.tables[(int64_t)b * a.width + (pos >> a.lblock)];
+      if (id >= 0 && id < a.pages) {
+        const int64_t ph = (int64_t)id * a.HK + kh;
+        pg = id;
+        meta = min(len - pos, 32) | (int)a.ksc[ph] << 8 | (int)a.vsc[ph] << 16;
+      }
+    }
+  };
+  // per-lane source offsets of load instruction i of a tile: key i * RPI +
+  // lane / CPR, the chunk that the swizzle puts at place lane % CPR
+  const int d_row = lane / S::CPR, d_pc = lane % S::CPR;
+  // instruction i of half-tile data `kv` (0 K, 1 V) of the wave's tile k into dst
+  auto load1 = [&](int kv, int k, int i, uint8_t* dst) {
+    const int at = 2 * (k & 31) + i * S::RPI / 32;       // the lane that describes the half
+    const int page = __builtin_amdgcn_readlane(pg, at);
+    const int held = __builtin_amdgcn_readlane(meta, at) & 0xff;
+    const int pos = (first + stride * k) * kKeys + i * S::RPI / 32 * 32;
+    const int64_t key = (((int64_t)max(page, 0) * a.HK + kh) << a.lblock) +
+                        (pos & ((1 << a.lblock) - 1));
+    const uint8_t* base = (kv ? a.vc : a.kc) + key * D;
+    const int row = i * S::RPI + d_row;
+    const int off = (row & 31) * D + (d_pc ^ (kv ? S::swv(row) : S::swk(row))) * 16;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base), 0, held * D, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t*)(dst + i * 1024), 16, off, 0, 0, 0);
+  };
+
+  // LDS offsets of the fragments
+  // V: key 8 (e / 4) + 4 hi + e % 4, e = (lane % 16) / 2; d = 32 dt + 16 (lane / 16 % 2) +
+  // 8 (lane % 2)
+  const int v_e = (lane & 15) >> 1;
+  const int v_row = 8 * (v_e >> 2) + 4 * hi + (v_e & 3);
+  const int v_chunk = lane >> 4 & 1, v_sw = S::swv(v_row);
+
+  // ---- one tile in LDS: scores, weights, output
+  int m0 = 0, m1 = 0;   // meta of the tile's halves
+  auto scores = [&](const uint8_t* ks, f32x16* st) {
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      st[hf] = f32x16{};
+      const int sk = (hf ? m1 : m0) >> 8 & 0xff;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        // chunk 4s + 2c + hi: the XOR touches the low bits only where 4s does not
+        const uint8_t* row = ks + hf * 32 * D + col * D;
+        const i32x4 x = *(const i32x4*)(row + ((4 * s + hi) ^ S::swk(col)) * 16);
+        const i32x4 y = *(const i32x4*)(row + ((4 * s + 2 + hi) ^ S::swk(col)) * 16);
+        const i32x8 kf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+        for (int p = 0; p < NP; ++p) st[hf] = mfma_scaled(kf, qf[p][s], st[hf], sk, qs[p]);
+      }
+    }
+  };
+  i32x8 pf[NP];
+  int ps[NP];
+  auto weights = [&](f32x16* st) {
+    const int held[2] = {m0 & 0xff, m1 & 0xff};
+    float top[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      if (held[hf] < 32) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          st[hf][j] = 8 * (j >> 2) + 4 * hi + (j & 3) < held[hf] ? st[hf][j] : -INFINITY;
+      }
+      float x = st[hf][0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) x = fmaxf(x, st[hf][j]);
+      top[hf] = max_xor32_f(x) * a.sl2;
+    }
+    const float both = fmaxf(top[0], top[1]);
+    if (m == -INFINITY) m = both;
+    if (__ballot(both > m + kMaxUp) != 0) raise(both);
+    const float ref = m == -INFINITY ? 0.f : m;
+    int e[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      e[hf] = (int)fmaxf(ceilf(top[hf] - ref), -100.f);
+      const float nm = (float)(8 - e[hf]) - ref;
+      float sum = 0.f;
+#pragma unroll
+      for (int j4 = 0; j4 < 4; ++j4) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[i] = __builtin_amdgcn_exp2f(fmaf(st[hf][4 * j4 + i], a.sl2, nm));
+          sum += y[i];
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) pf[p][4 * hf + j4] = piece4(y, y);
+      }
+      l = fmaf(add_xor32(sum), pow2i(e[hf] - 8), l);
+    }
+    const int own = hi ? e[1] : e[0];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) ps[p] = own - 8 - 4 * p + 127;
+  };
+  auto outputs = [&](const uint8_t* vs) {
+    const int sv = (hi ? m1 : m0) >> 16 & 0xff;
+    const uint32_t base = (uint32_t)(uintptr_t)(vs + v_row * D + (lane & 1) * 8);
+#pragma unroll
+    for (int d2 = 0; d2 < DT / 2; ++d2) {
+      i32x8 f0, f1;
+      read_v2<D>(base + (((4 * d2 + v_chunk) ^ v_sw) * 16),
+                 base + (((4 * d2 + 2 + v_chunk) ^ v_sw) * 16), f0, f1);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        O[2 * d2] = mfma_scaled(f0, pf[p], O[2 * d2], sv, ps[p]);
+        O[2 * d2 + 1] = mfma_scaled(f1, pf[p], O[2 * d2 + 1], sv, ps[p]);
+      }
+    }
+  };
+  auto take_meta = [&](int k) {
+    m0 = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
+    m1 = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
+  };
+
+  if constexpr (SHARED) {
+    // wave w loads LT / 4 instructions of K and of V of every tile; the chunk
+    // of page descriptions changes with the tile that is loaded, three ahead of
+    // the one in use, whose own are kept in a ring of registers
+    constexpr int LW = S::LT / 4;
+    int ring0[4], ring1[4];
+    auto issue = [&](int k) {
+      if ((k & 31) == 0) describe(k >> 5);
+      uint8_t* dst = smem + (k & 3) * S::slot;
+#pragma unroll
+      for (int i = 0; i < LW; ++i) load1(0, k, wave * LW + i, dst);
+#pragma unroll
+      for (int i = 0; i < LW; ++i) load1(1, k, wave * LW + i, dst + S::tile);
+    };
+    auto push = [&](int k) {
+      ring0[0] = ring0[1]; ring0[1] = ring0[2]; ring0[2] = ring0[3];
+      ring1[0] = ring1[1]; ring1[1] = ring1[2]; ring1[2] = ring1[3];
+      ring0[3] = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
+      ring1[3] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
+    };
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (k < count) issue(k);
+      push(k);
+    }
+    for (int k = 0; k < count; ++k) {
+      // tile k has landed when at most those of k + 1 and k + 2 are in flight
+      if (k + 2 < count) wait_vm(4 * LW);
+      else if (k + 1 < count) wait_vm(2 * LW);
+      else wait_vm(0);
+      tile_barrier();
+      // every wave is done with tile k - 1, whose stage tile k + 3 takes
+      if (k + 3 < count) issue(k + 3);
+      push(k + 3);
+      m0 = ring0[0];
+      m1 = ring1[0];
+      const uint8_t* stage = smem + (k & 3) * S::slot;
+      f32x16 st[2];
+      scores(stage, st);
+      weights(st);
+      outputs(stage + S::tile);
+    }
+  } else {
+    uint8_t* mine = smem + wave * S::slot;
+    auto issue = [&](int kv, int k) {
+#pragma unroll
+      for (int i = 0; i < S::LT; ++i) load1(kv, k, i, mine + kv * S::tile);
+    };
+    if (count > 0) {
+      describe(0);
+      issue(0, 0);
+      issue(1, 0);
+    }
+    for (int k = 0; k < count; ++k) {
+      take_meta(k);
+      wait_vm(S::LT);              // K of tile k is there, V may be on its way
+      f32x16 st[2];
+      scores(mine, st);
+      // the next tile's K goes where this one's was, once its reads are done
+      // (the products above have taken them)
+      if (k + 1 < count) {
+        if ((k + 1 & 31) == 0) describe((k + 1) >> 5);
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+        issue(0, k + 1);
+      }
+      weights(st);
+      if (k + 1 < count) wait_vm(S::LT);
+      else wait_vm(0);
+      outputs(mine + S::tile);
+      if (k + 1 < count) issue(1, k + 1);     // outputs() waits for its own reads
+    }
+  }
+
+  // ---- the rows, one at a time over a wave: O^T through LDS, joined over the
+  // waves that hold the same rows, then stored whole (or as a partial result)
+  wait_vm(0);
+  __syncthreads();
+  float* ep = (float*)smem + wave * 32 * S::EpiLd;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *(f32x4*)(ep + col * S::EpiLd + 32 * dt + 8 * q4 + 4 * hi) =
+          f32x4{O[dt][4 * q4], O[dt][4 * q4 + 1], O[dt][4 * q4 + 2], O[dt][4 * q4 + 3]};
+  if (hi == 0) {
+    sm_m[wave][col] = m;
+    sm_l[wave][col] = l;
+  }
+  __syncthreads();
+  constexpr int E = D / 64;       // elements of a row per lane
+  for (int i = SHARED ? 0 : wave; i < 32; i += SHARED ? 1 : 4) {
+    const int rr = row0 + i;
+    if (rr >= a.R) break;
+    float o[E], ll, mm;
+    if constexpr (SHARED) {
+      mm = sm_m[wave][i];
+      ll = sm_l[wave][i];
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = ep[i * S::EpiLd + lane * E + e];
+    } else {
+      mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
+      ll = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float f = sm_m[x][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[x][i] - mm);
+        ll = fmaf(f, sm_l[x][i], ll);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          o[e] = fmaf(f, ((float*)smem)[(x * 32 + i) * S::EpiLd + lane * E + e], o[e]);
+      }
+    }
+    if (a.splits > 1) {
+      const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + rr;
+#pragma unroll
+      for (int e = 0; e < E; ++e) a.part_o[at * D + lane * E + e] = o[e];
+      if (lane == 0) {
+        a.part_ml[2 * at] = mm;
+        a.part_ml[2 * at + 1] = ll;
+      }
+      continue;
+    }
+    const int t2 = rr % a.T, g2 = rr / a.T % G, w2 = rr / a.T / G;
+    const int64_t n2 = (int64_t)b * a.W + w2;
+    const int h2 = kh * G + g2;
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    const T* gate = (const T*)a.gate + n2 * a.sg_n + t2 * a.sg_t + h2 * a.sg_h + lane * E;
+    T* out = (T*)a.out + n2 * a.so_n + t2 * a.so_t + h2 * a.so_h + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float y = o[e] * inv;
+      if (a.gate) y *= sigmoid_f(Elem<T>::to_f(gate[e]));
+      out[e] = Elem<T>::from_f(y);
+    }
+  }
+}
+
+// Joins the ranges of a split prefix: one wave per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
+  constexpr int E = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.B * a.HK * a.R;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  float mm = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (s * rows + row)]);
+  float o[E], ll = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float ms = a.part_ml[2 * (s * rows + row)];
+    if (ms == -INFINITY) continue;
+    const float f = __builtin_amdgcn_exp2f(ms - mm);
+    ll = fmaf(f, a.part_ml[2 * (s * rows + row) + 1], ll);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      o[e] = fmaf(f, a.part_o[(s * rows + row) * D + lane * E + e], o[e]);
+  }
+  const int G = a.H / a.HK;
+  const int rr = (int)(row % a.R), bk = (int)(row / a.R);
+  const int t = rr % a.T, g = rr / a.T % G, w = rr / a.T / G;
+  const int64_t n = (int64_t)(bk / a.HK) * a.W + w;
+  const int h = bk % a.HK * G + g;
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const T* gate = (const T*)a.gate + n * a.sg_n + t * a.sg_t + h * a.sg_h + lane * E;
+  T* out = (T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    float y = o[e] * inv;
+    if (a.gate) y *= sigmoid_f(Elem<T>::to_f(gate[e]));
+    out[e] = Elem<T>::from_f(y);
+  }
+}
+
+// The launch of a call: whether the waves share tiles, and the ranges the
+// prefix is split into.
+struct Plan {
+  bool shared;
+  int nqblk, splits;
+};
+
+Plan plan_of(int B, int HK, int R, int keys) {
+  Plan p;
+  p.shared = R > 64;
+  p.nqblk = (int)kad_cdiv(R, p.shared ? 128 : 32);
+  const int64_t blocks = (int64_t)B * HK * p.nqblk;
+  const int tiles = (int)kad_cdiv(keys, kKeys);
+  const int least = 4;
+  int64_t s = kad_cdiv(256, blocks);
+  const int64_t cap = kad_cdiv(tiles, least);
+  if (s > cap) s = cap;
+  p.splits = (int)(s < 1 ? 1 : s);
+  return p;
+}
+
+template <typename T, int D>
+int launch(const BlockAttnArgs& a, bool shared, hipStream_t stream) {
+  constexpr int lds = Shape<D>::lds;
+  const void* f = shared ? (const void*)block_attn_kernel<T, D, true>
+                         : (const void*)block_attn_kernel<T, D, false>;
+  if (lds > 64 * 1024 &&
+      hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    kad_set_error("block_attn_kernel: %d bytes of LDS refused", lds);
+    return KAD_ERR_HIP;
+  }
+  const dim3 grid((unsigned)((int64_t)a.B * a.HK * a.splits * a.nqblk));
+  if (shared)
+    hipLaunchKernelGGL((block_attn_kernel<T, D, true>), grid, dim3(256), lds, stream, a);
+  else
+    hipLaunchKernelGGL((block_attn_kernel<T, D, false>), grid, dim3(256), lds, stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((block_attn_join_kernel<T, D>),
+                       dim3((unsigned)kad_cdiv((int64_t)a.B * a.HK * a.R, 4)), dim3(256), 0,
+                       stream, a);
+  return kad_launch_status("block_attn_kernel");
+}
+
 template <typename T>
-static void launch_rows(const BlockAttnArgs& a, int D, hipStream_t stream) {
-  const dim3 grid((unsigned)kad_cdiv(a.rows, 4));
-  if (D == 64) hipLaunchKernelGGL((block_attn_row_kernel<T, 64>), grid, dim3(256), 0, stream, a);
-  else if (D == 128)
-    hipLaunchKernelGGL((block_attn_row_kernel<T, 128>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((block_attn_row_kernel<T, 256>), grid, dim3(256), 0, stream, a);
+int launch_d(const BlockAttnArgs& a, int D, bool shared, hipStream_t stream) {
+  if (D == 64) return launch<T, 64>(a, shared, stream);
+  if (D == 128) return launch<T, 128>(a, shared, stream);
+  return launch<T, 256>(a, shared, stream);
+}
+
+bool aligned(const void* p, int64_t s0, int64_t s1, int64_t s2, int elements) {
+  return ((uintptr_t)p % (2 * elements)) == 0 && s0 % elements == 0 && s1 % elements == 0 &&
+         s2 % elements == 0;
+}
+
+}  // namespace
+
+extern "C" int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, int H, int HK,
+                                                          int D, int width, int block,
+                                                          int64_t* bytes) {
+  KAD_REQUIRE(bytes, "null pointer argument");
+  KAD_REQUIRE(B > 0 && W > 0 && T > 0 && H > 0 && HK > 0 && H % HK == 0 && width > 0,
+              "empty dimensions");
+  KAD_REQUIRE((int64_t)width * block <= 0x7fffffff - 256, "tables of %d columns", width);
+  const int64_t R = (int64_t)W * T * (H / HK);
+  KAD_REQUIRE(R <= 0x7fffffff - 256, "%lld rows for a KV head", (long long)R);
+  const Plan p = plan_of(B, HK, (int)R, width * block);
+  *bytes = p.splits > 1 ? (int64_t)p.splits * B * HK * R * (D + 2) * 4 : 0;
+  return KAD_OK;
 }
 
 extern "C" int kad_block_prefix_attention(
@@ -103,8 +714,9 @@ extern "C" int kad_block_prefix_attention(
     const int32_t* tables, int width, const int32_t* lengths, const void* suffix_k,
     int64_t ssk_n, int64_t ssk_t, int64_t ssk_h, const void* suffix_v, int64_t ssv_n,
     int64_t ssv_t, int64_t ssv_h, const void* gate, int64_t sg_n, int64_t sg_t, int64_t sg_h,
-    void* out, int64_t so_n, int64_t so_t, int64_t so_h, int B, int W, int T, int Tk, int H,
-    int HK, int D, int block, int dtype, float scale, kad_stream_t stream) {
+    void* out, int64_t so_n, int64_t so_t, int64_t so_h, void* workspace,
+    int64_t workspace_bytes, int B, int W, int T, int Tk, int H, int HK, int D, int block,
+    int dtype, float scale, kad_stream_t stream) {
   KAD_REQUIRE(B > 0 && W > 0 && T > 0 && H > 0 && HK > 0 && width > 0 && pages > 0,
               "empty dimensions");
   KAD_REQUIRE(H % HK == 0, "%d heads over %d KV heads", H, HK);
@@ -115,15 +727,41 @@ extern "C" int kad_block_prefix_attention(
   KAD_REQUIRE(D == 64 || D == 128 || D == 256, "head dim %d is not 64, 128 or 256", D);
   KAD_REQUIRE(block == 32 || block == 64 || block == 128 || block == 256,
               "block size %d is not 32, 64, 128 or 256", block);
-  KAD_REQUIRE((int64_t)width * block <= 0x7fffffff, "tables of %d columns", width);
-  BlockAttnArgs a = {q, sq_n, sq_t, sq_h, (const uint8_t*)k_codes, (const uint8_t*)v_codes,
-                     (const uint8_t*)k_scale, (const uint8_t*)v_scale, tables, lengths, suffix_k,
-                     ssk_n, ssk_t, ssk_h, suffix_v, ssv_n, ssv_t, ssv_h, gate, sg_n, sg_t, sg_h,
-                     out, so_n, so_t, so_h, pages, width, W, T, Tk, H, HK, block,
-                     (int64_t)B * W * T * H, scale};
-  KAD_REQUIRE(kad_cdiv(a.rows, 4) <= 0x7fffffff, "too many rows for a launch");
-  if (dtype == KAD_DTYPE_BF16) launch_rows<bf16_t>(a, D, (hipStream_t)stream);
-  else if (dtype == KAD_DTYPE_F16) launch_rows<_Float16>(a, D, (hipStream_t)stream);
-  else KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
-  return kad_launch_status("block_attn_row_kernel");
+  KAD_REQUIRE(aligned(k_codes, 0, 0, 0, 8) && aligned(v_codes, 0, 0, 0, 8) &&
+                  aligned(q, sq_n, sq_t, sq_h, 8),
+              "codes and query rows must be 16-byte aligned");
+  KAD_REQUIRE(Tk == 0 || (aligned(suffix_k, ssk_n, ssk_t, ssk_h, 8) &&
+                          aligned(suffix_v, ssv_n, ssv_t, ssv_h, 4)),
+              "suffix rows must be 16-byte (K) and 8-byte (V) aligned");
+  if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
+    KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
+  int64_t need = 0;
+  const int rc = kad_block_prefix_attention_workspace_bytes(B, W, T, H, HK, D, width, block, &need);
+  if (rc != KAD_OK) return rc;
+  KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "a workspace of %lld bytes is needed", (long long)need);
+  const int R = W * T * (H / HK);
+  const Plan p = plan_of(B, HK, R, width * block);
+  KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff &&
+                  kad_cdiv((int64_t)B * HK * R, 4) <= 0x7fffffff,
+              "too many rows for a launch");
+  BlockAttnArgs a = {};
+  a.q = q; a.sq_n = sq_n; a.sq_t = sq_t; a.sq_h = sq_h;
+  a.kc = (const uint8_t*)k_codes; a.vc = (const uint8_t*)v_codes;
+  a.ksc = (const uint8_t*)k_scale; a.vsc = (const uint8_t*)v_scale;
+  a.tables = tables; a.lengths = lengths;
+  a.sk = suffix_k; a.ssk_n = ssk_n; a.ssk_t = ssk_t; a.ssk_h = ssk_h;
+  a.sv = suffix_v; a.ssv_n = ssv_n; a.ssv_t = ssv_t; a.ssv_h = ssv_h;
+  a.gate = gate; a.sg_n = sg_n; a.sg_t = sg_t; a.sg_h = sg_h;
+  a.out = out; a.so_n = so_n; a.so_t = so_t; a.so_h = so_h;
+  a.part_o = (float*)workspace;
+  a.part_ml = a.part_o + (int64_t)p.splits * B * HK * R * D;
+  a.pages = pages; a.width = width; a.B = B; a.W = W; a.T = T; a.Tk = Tk; a.H = H; a.HK = HK;
+  a.lblock = block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : 8;
+  a.splits = p.splits; a.nqblk = p.nqblk; a.R = R;
+  const float log2e = 1.4426950408889634f;
+  a.qmul = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale == 0.f ? 0.f : scale;
+  a.sl2 = scale == 0.f ? log2e : fabsf(scale) * log2e;
+  return dtype == KAD_DTYPE_BF16 ? launch_d<bf16_t>(a, D, p.shared, (hipStream_t)stream)
+                                 : launch_d<_Float16>(a, D, p.shared, (hipStream_t)stream);
 }

@@ -18,6 +18,7 @@ the reference, whose prefix stays in the model's type
 """
 
 import contextlib
+import ctypes
 import math
 from typing import NamedTuple
 
@@ -244,8 +245,13 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
                             gate, gate_strides)
 
 
-def _rows(t):
-    return t if t.stride(3) == 1 else t.contiguous()
+def _rows(t, elements):
+    """t, or a copy whose rows start at multiples of ``elements`` elements."""
+    if t.stride(3) == 1 and not any(s % elements for s in t.stride()[:3]) and \
+            t.data_ptr() % (2 * elements) == 0:
+        return t
+    return t.contiguous(memory_format=torch.contiguous_format) if not t.is_contiguous() \
+        else t.clone()
 
 
 def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale, gate=None,
@@ -255,23 +261,27 @@ def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
     (beam, token, head)."""
     BW, T, H, D = q.shape
     pages, HK, block, _ = blocks.k.shape
-    q = _rows(q)
+    q = _rows(q, 8)
     tables, lengths = tables.contiguous(), lengths.contiguous()
     none = (None, 0, 0, 0)
     sk = sv = g = none
     Tk = 0
     if suffix_k is not None:
-        suffix_k, suffix_v = _rows(suffix_k), _rows(suffix_v)
+        suffix_k, suffix_v = _rows(suffix_k, 8), _rows(suffix_v, 4)
         Tk = suffix_k.shape[1]
         sk = (_lib.ptr(suffix_k), *suffix_k.stride()[:3])
         sv = (_lib.ptr(suffix_v), *suffix_v.stride()[:3])
     if gate is not None:
         g = (_lib.ptr(gate), *gate_strides)
     out = torch.empty(BW, T, H, D, dtype=q.dtype, device=q.device)
+    need = ctypes.c_int64(0)
+    _lib.call("kad_block_prefix_attention_workspace_bytes", BW // beam_width, beam_width, T, H, HK,
+              D, tables.shape[1], block, ctypes.byref(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     with _on_device(q):
         _lib.call("kad_block_prefix_attention", _lib.ptr(q), *q.stride()[:3],
                   *map(_lib.ptr, blocks), pages, _lib.ptr(tables), tables.shape[1],
                   _lib.ptr(lengths), *sk, *sv, *g, _lib.ptr(out), *out.stride()[:3],
-                  BW // beam_width, beam_width, T, Tk, H, HK, D, block,
+                  _lib.ptr(ws), need.value, BW // beam_width, beam_width, T, Tk, H, HK, D, block,
                   _lib.dtype_code(q.dtype), float(scale), _lib.stream_of(q))
     return out

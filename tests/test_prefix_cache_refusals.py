@@ -136,11 +136,19 @@ def test_entry_points_refuse_before_any_launch():
     assert write(k=None) == write(B=0) == write(D=96) == write(block=48) == -1
     assert write(dtype=7) == -2
     attend = lambda **k: lib.kad_block_prefix_attention(  # noqa: E731
-        k.get("q", p), 0, 0, 0, p, p, p, p, 1, p, 1, p, k.get("sk", None), 0, 0, 0, None, 0, 0, 0,
-        None, 0, 0, 0, p, 0, 0, 0, 1, 1, 1, k.get("Tk", 0), k.get("H", 2), 2, k.get("D", 64),
+        k.get("q", p), 0, 0, k.get("sq", 0), p, p, p, p, 1, p, k.get("width", 1), p, k.get("sk", None), 0, 0, 0, None, 0, 0, 0,
+        None, 0, 0, 0, p, 0, 0, 0, None, 0, k.get("B", 1), 1, 1, k.get("Tk", 0), k.get("H", 2), 2, k.get("D", 64),
         k.get("block", 64), k.get("dtype", 0), 1.0, None)
     assert attend(q=None) == attend(Tk=1) == attend(H=3) == attend(D=32) == attend(block=16) == -1
+    assert attend(sq=4) == attend(q=ctypes.c_void_p(264)) == attend(width=2**30) == -1
+    assert attend(width=64) == -1 and b"workspace" in lib.kad_last_error()
     assert attend(dtype=2) == -2
+    need = ctypes.c_int64(-1)
+    size = lib.kad_block_prefix_attention_workspace_bytes
+    assert size(1, 1, 1, 2, 2, 64, 1, 64, ctypes.byref(need)) == 0 and need.value == 0
+    assert size(1, 1, 1, 2, 2, 64, 64, 64, ctypes.byref(need)) == 0 and need.value > 0
+    assert size(1, 1, 1, 3, 2, 64, 1, 64, ctypes.byref(need)) == -1
+    assert size(1, 1, 1, 2, 2, 64, 1, 64, None) == -1
 
 
 def test_oracle_codes_agree_with_torch():
