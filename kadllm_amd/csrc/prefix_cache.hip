@@ -95,12 +95,6 @@ __device__ __forceinline__ int scale_exp(float amax) {
 __device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
-__device__ __forceinline__ uint8_t to_e4m3(float x) {
-  return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xff);
-}
-__device__ __forceinline__ float from_e4m3(uint8_t c) {
-  return __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
-}
 
 struct WriteArgs {
   const void* x[2];       // k, v
@@ -113,47 +107,146 @@ struct WriteArgs {
   int width, pages, B, N, HK, D, block, touched;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void write_blocks_kernel(WriteArgs a) {
-  __shared__ float part[4];
-  const int tid = threadIdx.x;
+// 16 elements of a row as floats
+__device__ __forceinline__ void load16(const bf16_t* p, float* f) {
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const u32x4 x = *(const u32x4*)(p + 8 * v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[8 * v + 2 * i] = __uint_as_float(x[i] << 16);
+      f[8 * v + 2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+    }
+  }
+}
+__device__ __forceinline__ void load16(const _Float16* p, float* f) {
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const f16x8 x = *(const f16x8*)(p + 8 * v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[8 * v + i] = (float)x[i];
+  }
+}
+__device__ __forceinline__ void load16(const float* p, float* f) {
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const f32x4 x = *(const f32x4*)(p + 4 * v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[4 * v + i] = x[i];
+  }
+}
+__device__ __forceinline__ void store16(uint8_t* p, const float* f, float scale) {
+  u32x4 c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i] * scale, f[4 * i + 1] * scale, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2] * scale, f[4 * i + 3] * scale, w, true);
+    c[i] = (uint32_t)w;
+  }
+  *(u32x4*)p = c;
+}
+
+// A page and head is block * D / 16 pieces of 16 elements.  Each of up to 1024
+// threads keeps 4 of them in registers between the maximum and the rounding, so
+// the input is read once and the codes are written once, 16 bytes a lane.
+// VEC: rows of the input start at 16-byte boundaries.
+constexpr int kPieces = 4;
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(1024) void write_blocks_kernel(WriteArgs a) {
+  __shared__ float part[16];
+  const int tid = threadIdx.x, threads = blockDim.x;
   const int u = blockIdx.x % a.touched, b = blockIdx.x / a.touched;
   const int h = blockIdx.y, kv = blockIdx.z;
   const int start = a.starts ? max(a.starts[b], 0) : 0;
   const int64_t stop64 = min((int64_t)start + a.N, (int64_t)a.width * a.block);
   const int stop = min(a.lengths[b], (int)stop64);   // one past the last new position
   const int blk = start / a.block + u;
+  if (blk >= a.width) return;
   const int lo = max(start - blk * a.block, 0), hi = min(stop - blk * a.block, a.block);
-  if (blk >= a.width || hi <= lo) return;             // rows [lo, hi) of the page are new
+  if (hi <= lo) return;                               // rows [lo, hi) of the page are new
   const int page = a.tables[(int64_t)b * a.width + blk];
   if (page < 0 || page >= a.pages) return;
   const T* x = (const T*)a.x[kv] + (int64_t)b * a.s_b[kv] + (int64_t)h * a.s_h[kv] +
                ((int64_t)blk * a.block - start) * a.s_t[kv];
   uint8_t* codes = a.codes[kv] + ((int64_t)page * a.HK + h) * a.block * a.D;
   uint8_t* scale = a.scale[kv] + (int64_t)page * a.HK + h;
+  const int ppr = a.D / 16;                           // pieces per row
+  float f[kPieces][16];
   float amax = 0.f;
-  for (int i = lo * a.D + tid; i < hi * a.D; i += 256) {
-    const float f = fabsf(Elem<T>::to_f(x[(int64_t)(i / a.D) * a.s_t[kv] + i % a.D]));
-    if (f < INFINITY) amax = fmaxf(amax, f);
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = tid + p * threads, row = i / ppr, d = i % ppr * 16;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) f[p][e] = 0.f;
+    if (row >= lo && row < hi) {
+      const T* src = x + row * a.s_t[kv] + d;
+      if constexpr (VEC) {
+        load16(src, f[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[p][e] = Elem<T>::to_f(src[e]);
+      }
+    }
+  }
+  // (fmaxf leaves NaN out; an infinity, seen by one compare, is left out in a
+  // second pass over the registers)
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(f[p][e]));
+  if (amax == INFINITY) {
+    amax = 0.f;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (fabsf(f[p][e]) < INFINITY) amax = fmaxf(amax, fabsf(f[p][e]));
   }
   amax = wave_max(amax);
   if ((tid & 63) == 0) part[tid >> 6] = amax;
   __syncthreads();
-  amax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  for (int i = 0; i < threads / 64; ++i) amax = fmaxf(amax, part[i]);
   int e = scale_exp(amax);
   if (lo > 0) {
-    const int before = (int)*scale - 127;
-    if (e > before) {
-      const float f = pow2f(max(before - e, -126));
-      for (int i = tid; i < lo * a.D; i += 256) codes[i] = to_e4m3(from_e4m3(codes[i]) * f);
+    const int before = min((int)*scale - 127, 127);
+    if (e > before) {                                 // the earlier rows to the new scale
+      const float m = pow2f(max(before - e, -126));
+      for (int i = tid; i < lo * ppr; i += threads) {
+        const u32x4 c = *(const u32x4*)(codes + 16 * i);
+        float g[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          g[4 * j] = __builtin_amdgcn_cvt_f32_fp8((int)c[j], 0);
+          g[4 * j + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[j], 1);
+          g[4 * j + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[j], 2);
+          g[4 * j + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[j], 3);
+        }
+        store16(codes + 16 * i, g, m);
+      }
     }
     e = max(e, before);
   }
   const float inv = pow2f(-e);
-  for (int i = lo * a.D + tid; i < hi * a.D; i += 256)
-    codes[i] = to_e4m3(Elem<T>::to_f(x[(int64_t)(i / a.D) * a.s_t[kv] + i % a.D]) * inv);
-  __syncthreads();
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = tid + p * threads, row = i / ppr;
+    if (row >= lo && row < hi) store16(codes + 16 * i, f[p], inv);
+  }
+  __syncthreads();                                    // every thread has read the old scale
   if (tid == 0) *scale = (uint8_t)(e + 127);
+}
+
+template <typename T>
+static void launch_write(const WriteArgs& a, bool vec, hipStream_t stream) {
+  const dim3 grid((unsigned)(a.touched * a.B), (unsigned)a.HK, 2);
+  // 4 pieces a thread, whole waves
+  const int threads = max(64, a.block * a.D / (16 * kPieces));
+  if (vec)
+    hipLaunchKernelGGL((write_blocks_kernel<T, true>), grid, dim3(threads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((write_blocks_kernel<T, false>), grid, dim3(threads), 0, stream, a);
 }
 
 extern "C" int kad_write_prefix_blocks(
@@ -174,14 +267,17 @@ extern "C" int kad_write_prefix_blocks(
   a.touched = (int)(starts ? ((int64_t)N + block - 2) / block + 1 : kad_cdiv(N, block));
   if (a.touched > width) a.touched = width;
   KAD_REQUIRE((int64_t)a.touched * B <= 0x7fffffff && HK <= 65535, "too many pages for a launch");
-  const dim3 grid((unsigned)(a.touched * B), (unsigned)HK, 2);
-  if (dtype == KAD_DTYPE_BF16)
-    hipLaunchKernelGGL(write_blocks_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else if (dtype == KAD_DTYPE_F16)
-    hipLaunchKernelGGL(write_blocks_kernel<_Float16>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else if (dtype == KAD_DTYPE_F32)
-    hipLaunchKernelGGL(write_blocks_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else
-    KAD_UNSUPPORTED("dtype code %d", dtype);
+  KAD_REQUIRE(((uintptr_t)k_codes % 16) == 0 && ((uintptr_t)v_codes % 16) == 0,
+              "codes must be 16-byte aligned");
+  const int item = dtype == KAD_DTYPE_F32 ? 4 : 2;
+  auto rows16 = [&](const void* p, int64_t b, int64_t t, int64_t h) {
+    return (uintptr_t)p % 16 == 0 && b * item % 16 == 0 && t * item % 16 == 0 &&
+           h * item % 16 == 0;
+  };
+  const bool vec = rows16(k, sk_b, sk_t, sk_h) && rows16(v, sv_b, sv_t, sv_h);
+  if (dtype == KAD_DTYPE_BF16) launch_write<bf16_t>(a, vec, (hipStream_t)stream);
+  else if (dtype == KAD_DTYPE_F16) launch_write<_Float16>(a, vec, (hipStream_t)stream);
+  else if (dtype == KAD_DTYPE_F32) launch_write<float>(a, vec, (hipStream_t)stream);
+  else KAD_UNSUPPORTED("dtype code %d", dtype);
   return kad_launch_status("write_blocks_kernel");
 }
