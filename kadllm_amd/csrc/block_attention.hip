@@ -52,6 +52,8 @@ struct BlockAttnArgs {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(1))) const void global_t;
 typedef __attribute__((address_space(3))) void lds_t;
 
 // f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
@@ -62,8 +64,6 @@ __device__ __forceinline__ void static_for(F&& f) {
     static_for<N, I + 1>(f);
   }
 }
-
-__device__ __forceinline__ float max_xor32_f(float x) { return max_xor32(x); }
 
 // A wave's fragment layout of v_mfma_scale_f32_32x32x64 for 8-bit operands:
 // lane l holds row (column for B) l % 32; its bytes 0-15 are k = 16 (l / 32) +
@@ -93,35 +93,41 @@ template <typename T> struct Pieces;
 template <> struct Pieces<bf16_t> { static constexpr int n = 2; };
 template <> struct Pieces<_Float16> { static constexpr int n = 3; };
 
-// 8 elements at a 16-byte aligned address as floats
-__device__ __forceinline__ void load8(const bf16_t* p, float* f) {
-  const u32x4 v = *(const u32x4*)p;
+// 8 elements as floats
+__device__ __forceinline__ void widen8(const bf16_t*, u32x4 v, float* f) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[2 * i] = __uint_as_float(v[i] << 16);
     f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ void load8(const _Float16* p, float* f) {
-  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-  const f16x8 v = *(const f16x8*)p;
+__device__ __forceinline__ void widen8(const _Float16*, u32x4 x, float* f) {
+  const f16x8 v = __builtin_bit_cast(f16x8, x);
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = (float)v[i];
 }
-// 4 elements at an 8-byte aligned address
-__device__ __forceinline__ void load4(const bf16_t* p, float* f) {
-  const u32x2 v = *(const u32x2*)p;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    f[2 * i] = __uint_as_float(v[i] << 16);
-    f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-  }
+// the products of the suffix, in the queries' type
+__device__ __forceinline__ f32x16 mfma_wide(const bf16_t*, u32x4 a, u32x4 b, f32x16 c) {
+  return mfma32x32x16(as_bf16x8(a), as_bf16x8(b), c);
 }
-__device__ __forceinline__ void load4(const _Float16* p, float* f) {
-  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-  const f16x4 v = *(const f16x4*)p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = (float)v[i];
+__device__ __forceinline__ f32x16 mfma_wide(const _Float16*, u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack2(const bf16_t*, float a, float b) {
+  return pack_bf16x2(a, b);
+}
+__device__ __forceinline__ uint32_t pack2(const _Float16*, float a, float b) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+}
+// the exponent bits of a pair of elements: all set in an infinity or NaN
+template <typename T>
+constexpr uint32_t kExponents = std::is_same<T, bf16_t>::value ? 0x7f807f80u : 0x7c007c00u;
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
 }
 
 constexpr int kKeys = 64;       // keys per tile: two halves of 32, each within a page
@@ -178,6 +184,25 @@ __device__ __forceinline__ void read_v2(uint32_t p0, uint32_t p1, i32x8& f0, i32
              (int)b2[0], (int)b2[1], (int)b3[0], (int)b3[1]};
 }
 
+// the same for two output tiles of 16-bit rows (the suffix): 16 keys, 2 reads of
+// 4 keys each (lane i of 16 receives element i % 4 of the 8-byte pieces that
+// lanes 4e + i / 4 address, e < 4)
+template <int D>
+__device__ __forceinline__ void read_wide2(uint32_t p0, uint32_t p1, u32x4& f0, u32x4& f1) {
+  u32x2 a0, a1, b0, b1;
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4\n\t"
+      "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+      "ds_read_b64_tr_b16 %2, %5\n\t"
+      "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(a0), "=&v"(a1), "=&v"(b0), "=&v"(b1)
+      : "v"(p0), "v"(p1), "i"(16 * D)
+      : "memory");
+  f0 = u32x4{a0[0], a0[1], a1[0], a1[1]};
+  f1 = u32x4{b0[0], b0[1], b1[0], b1[1]};
+}
+
 __device__ __forceinline__ void wait_vm(int n) {
   // vmcnt(n), lgkmcnt and expcnt left alone; n a constant after inlining
   switch (n) {
@@ -187,6 +212,7 @@ __device__ __forceinline__ void wait_vm(int n) {
 #undef KAD_W
     default: __builtin_amdgcn_s_waitcnt(0x0f70);
   }
+  asm volatile("" ::: "memory");   // (reads of what has landed stay behind the wait)
 }
 __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
@@ -212,6 +238,7 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   constexpr int NP = Pieces<T>::n, KS = S::KS, DT = S::DT;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   __shared__ float sm_m[4][32], sm_l[4][32];
+  __shared__ int sm_spoilt[4];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -229,39 +256,44 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   const int64_t n = (int64_t)b * a.W + w;
   const int h = kh * G + g;
 
-  // ---- Q in e4m3 pieces against the row's power of two
+  // ---- Q: the row's elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7 as they
+  // are, and in e4m3 pieces against the row's power of two
+  const T* const kind = nullptr;
+  u32x4 qr[4 * KS];
+  {
+    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h + 16 * hi;
+#pragma unroll
+    for (int c = 0; c < 4 * KS; ++c) qr[c] = *(const u32x4*)(qrow + 32 * (c >> 1) + 8 * (c & 1));
+  }
   i32x8 qf[NP][KS];
   int qs[NP];
-  {
-    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h;
+  auto split_q = [&]() {
     float amax = 0.f;
-    float qv[32];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+    for (int c = 0; c < 4 * KS; ++c) {
+      float x[8];
+      widen8(kind, qr[c], x);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        load8(qrow + 64 * s + 32 * (c >> 1) + 16 * hi + 8 * (c & 1), qv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(qv[i]));
-      }
-    amax = max_xor32_f(amax);
+      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
+    }
+    amax = max_xor32(amax);
     const int E = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -100);
     const float inv = pow2i(-E) * a.qmul;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
+    for (int c = 0; c < 4 * KS; ++c) {
+      float x[8];
+      widen8(kind, qr[c], x);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        load8(qrow + 64 * s + 32 * (c >> 1) + 16 * hi + 8 * (c & 1), qv + 8 * c);
+      for (int i = 0; i < 8; ++i) x[i] *= inv;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) qv[i] *= inv;
-#pragma unroll
-      for (int p = 0; p < NP; ++p)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[p][s][i] = piece4(qv + 4 * i, qv + 4 * i);
+      for (int p = 0; p < NP; ++p) {
+        qf[p][c >> 2][2 * (c & 3)] = piece4(x, x);
+        qf[p][c >> 2][2 * (c & 3) + 1] = piece4(x + 4, x + 4);
+      }
     }
 #pragma unroll
     for (int p = 0; p < NP; ++p) qs[p] = E - 4 * p + 127;
-  }
+  };
 
   // ---- softmax state: weights are 2^(s - m) for a reference m that moves only
   // when a score exceeds it by 2^kMaxUp
@@ -269,8 +301,8 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   f32x16 O[DT];
 #pragma unroll
   for (int i = 0; i < DT; ++i) O[i] = f32x16{};
-  auto raise = [&](float top) {   // m up to the row's `top` (where that is far above it)
-    const float to = top > m + kMaxUp ? top : m;
+  auto raise = [&](float top, float slack) {   // m up to the row's `top` where that is far above
+    const float to = top > m + slack ? top : m;
     const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
     m = to;
     l *= f;
@@ -280,50 +312,101 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       for (int j = 0; j < 16; ++j) O[i][j] *= f;
   };
 
-  // ---- the beam's own suffix, in fp32, by the first range's first wave
-  if (a.Tk > 0 && split == 0 && (SHARED || wave == 0)) {
-    const int last = a.Tk - a.T + t;             // the row sees suffix keys 0..last
-    int most = last;                             // (all rows of the wave: 0..most)
+  // ---- the beams' own suffixes.  The suffix keys of the wave's beams, in order,
+  // are its key rows: of group after group of 32, S^T = K Q^T over all of them,
+  // masked to each row's beam and to the tokens before its own, then O^T += V^T
+  // P^T from LDS (area: 64 * D bytes of the wave's own).  A value that is not
+  // finite would reach the rows that do not see it as 0 * inf, so a group that
+  // holds one is multiplied without it, and the rows that do see it add it when
+  // they are stored.
+  bool spoilt = false;
+  auto suffix = [&](uint8_t* area) {
+    const int w0 = row0 / a.T / G, w1 = min(row0 + 31, a.R - 1) / a.T / G;
+    const int vlo = (w - w0) * a.Tk, vhi = vlo + a.Tk - a.T + t;   // keys the row sees
+    int keys = vhi + 1;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
-    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h;
-    const T* krow = (const T*)a.sk + n * a.ssk_n + kh * a.ssk_h;
-    const T* vrow = (const T*)a.sv + n * a.ssv_n + kh * a.ssv_h;
-    for (int j = 0; j <= most; ++j) {
-      const int jj = min(j, last);
-      const T* kr = krow + (int64_t)jj * a.ssk_t;
-      const T* vr = vrow + (int64_t)jj * a.ssv_t;
-      float s = 0.f;
+    for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o, 64));
+    keys = min(__builtin_amdgcn_readfirstlane(keys), (w1 - w0 + 1) * a.Tk);
+    const int64_t n0 = (int64_t)b * a.W + w0;
+    constexpr int CPV = D / 8, RPV = 512 / D;        // chunks per V row, rows per load
+    for (int f0 = 0; f0 < keys; f0 += 32) {
+      const bool both = keys - f0 > 16;              // 16 or 32 rows of V
+      const int fk = min(f0 + col, keys - 1);
+      const T* krow = (const T*)a.sk + (n0 + fk / a.Tk) * a.ssk_n +
+                      (int64_t)(fk % a.Tk) * a.ssk_t + kh * a.ssk_h + 16 * hi;
+      u32x4 kr[4 * KS];
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        float x[8], y[8];
-        load8(qrow + 16 * c + 8 * hi, x);
-        load8(kr + 16 * c + 8 * hi, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+      for (int c = 0; c < 4 * KS; ++c)
+        kr[c] = *(const u32x4*)(krow + 32 * (c >> 1) + 8 * (c & 1));
+      for (int i = 0; i < (both ? 32 : 16) / RPV; ++i) {
+        const int row = i * RPV + lane / CPV;
+        const int fv = min(f0 + row, keys - 1);
+        const int chunk = (lane % CPV) ^ (D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
+        const T* src = (const T*)a.sv + (n0 + fv / a.Tk) * a.ssv_n +
+                       (int64_t)(fv % a.Tk) * a.ssv_t + kh * a.ssv_h + chunk * 8;
+        __builtin_amdgcn_global_load_lds((global_t*)src, (lds_t*)(area + i * 1024), 16, 0, 0);
       }
-      s = add_xor32(s) * a.qmul * a.sl2;
-      if (j <= last) {
-        if (m == -INFINITY) m = s;
-      } else {
-        s = -INFINITY;
+      f32x16 st = f32x16{};
+#pragma unroll
+      for (int c = 0; c < 4 * KS; ++c) st = mfma_wide(kind, kr[c], qr[c], st);
+      const float mul = a.qmul * a.sl2;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int f = f0 + 8 * (j >> 2) + 4 * hi + (j & 3);
+        st[j] = f >= vlo && f <= vhi ? st[j] * mul : -INFINITY;
+        top = fmaxf(top, st[j]);
       }
-      if (__ballot(s > m + kMaxUp) != 0) raise(s);
-      if (j <= last) {
-        const float p = __builtin_amdgcn_exp2f(s - m);
-        l += p;
+      top = max_xor32(top);
+      if (__ballot(top > m) != 0) raise(top, 0.f);   // (so weights are at most 1)
+      const float ref = m == -INFINITY ? 0.f : m;
+      u32x4 pk[2];
+      float sum = 0.f;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            float y[4];
-            load4(vr + 32 * dt + 8 * q4 + 4 * hi, y);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) O[dt][4 * q4 + i] = fmaf(p, y[i], O[dt][4 * q4 + i]);
-          }
+      for (int j = 0; j < 16; j += 2) {
+        const float x = __builtin_amdgcn_exp2f(st[j] - ref);
+        const float y = __builtin_amdgcn_exp2f(st[j + 1] - ref);
+        sum += x + y;
+        pk[j >> 3][j >> 1 & 3] = pack2(kind, x, y);
       }
+      l += add_xor32(sum);
+      wait_vm(0);
+      // (each lane looks at what its own loads brought)
+      uint32_t top_exp = 0;
+      const int pieces = (both ? 32 : 16) / RPV;
+      for (int i = 0; i < pieces; ++i) {
+        const u32x4 x = *(const u32x4*)(area + i * 1024 + lane * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top_exp = max_u16x2(top_exp, x[e] & kExponents<T>);
+      }
+      const uint32_t full = kExponents<T> & 0xffffu;
+      const bool bad = __ballot((top_exp & 0xffffu) == full || top_exp >> 16 == full) != 0;
+      if (bad) {
+        for (int i = 0; i < pieces; ++i) {
+          uint16_t* x = (uint16_t*)(area + i * 1024 + lane * 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((x[e] & full) == full) x[e] = 0;
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+      }
+      const int gi = lane & 15, v_row = 4 * hi + (gi >> 2);
+      const int v_d = (lane >> 4 & 1) * 16 + (gi & 3) * 4;
+      const int v_sw = D == 64 ? (v_row >> 1 & 1) * 4 : (v_row & 3) * 4;
+      for (int ks = 0; ks < (both ? 2 : 1); ++ks) {
+        const uint32_t base = (uint32_t)(uintptr_t)(area + (16 * ks + v_row) * D * 2 + (v_d & 7) * 2);
+#pragma unroll
+        for (int d2 = 0; d2 < DT / 2; ++d2) {
+          u32x4 x, y;
+          read_wide2<D>(base + ((((64 * d2 + v_d) >> 3) ^ v_sw) * 16),
+                        base + ((((64 * d2 + 32 + v_d) >> 3) ^ v_sw) * 16), x, y);
+          O[2 * d2] = mfma_wide(kind, x, ks ? pk[1] : pk[0], O[2 * d2]);
+          O[2 * d2 + 1] = mfma_wide(kind, y, ks ? pk[1] : pk[0], O[2 * d2 + 1]);
+        }
+      }
+      spoilt |= bad;
     }
-  }
+  };
 
   // ---- this wave's tiles of the prefix: first + stride * k, k < count
   const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
@@ -411,11 +494,11 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       float x = st[hf][0];
 #pragma unroll
       for (int j = 1; j < 16; ++j) x = fmaxf(x, st[hf][j]);
-      top[hf] = max_xor32_f(x) * a.sl2;
+      top[hf] = max_xor32(x) * a.sl2;
     }
     const float both = fmaxf(top[0], top[1]);
     if (m == -INFINITY) m = both;
-    if (__ballot(both > m + kMaxUp) != 0) raise(both);
+    if (__ballot(both > m + kMaxUp) != 0) raise(both, kMaxUp);
     const float ref = m == -INFINITY ? 0.f : m;
     int e[2];
 #pragma unroll
@@ -481,10 +564,17 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       ring1[3] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
     };
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < 2; ++k) {
       if (k < count) issue(k);
       push(k);
     }
+    if (a.Tk > 0 && split == 0) {   // in stages 2 and 3
+      suffix(smem + 2 * S::slot + wave * S::tile);
+      tile_barrier();
+    }
+    if (2 < count) issue(2);
+    push(2);
+    split_q();
     for (int k = 0; k < count; ++k) {
       // tile k has landed when at most those of k + 1 and k + 2 are in flight
       if (k + 2 < count) wait_vm(4 * LW);
@@ -511,8 +601,10 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     if (count > 0) {
       describe(0);
       issue(0, 0);
-      issue(1, 0);
     }
+    if (a.Tk > 0 && split == 0 && wave == 0) suffix(mine + S::tile);   // where V goes
+    if (count > 0) issue(1, 0);
+    split_q();
     for (int k = 0; k < count; ++k) {
       take_meta(k);
       wait_vm(S::LT);              // K of tile k is there, V may be on its way
@@ -549,6 +641,7 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     sm_m[wave][col] = m;
     sm_l[wave][col] = l;
   }
+  if (lane == 0) sm_spoilt[wave] = spoilt;
   __syncthreads();
   constexpr int E = D / 64;       // elements of a row per lane
   for (int i = SHARED ? 0 : wave; i < 32; i += SHARED ? 1 : 4) {
@@ -574,6 +667,17 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
           o[e] = fmaf(f, ((float*)smem)[(x * 32 + i) * S::EpiLd + lane * E + e], o[e]);
       }
     }
+    const int t2 = rr % a.T, g2 = rr / a.T % G, w2 = rr / a.T / G;
+    const int64_t n2 = (int64_t)b * a.W + w2;
+    if (sm_spoilt[SHARED ? wave : 0]) {
+      const T* vr = (const T*)a.sv + n2 * a.ssv_n + kh * a.ssv_h + lane * E;
+      for (int j = 0; j <= a.Tk - a.T + t2; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + e]);
+          if (!(fabsf(x) < INFINITY)) o[e] += x;
+        }
+    }
     if (a.splits > 1) {
       const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + rr;
 #pragma unroll
@@ -584,8 +688,6 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       }
       continue;
     }
-    const int t2 = rr % a.T, g2 = rr / a.T % G, w2 = rr / a.T / G;
-    const int64_t n2 = (int64_t)b * a.W + w2;
     const int h2 = kh * G + g2;
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
     const T* gate = (const T*)a.gate + n2 * a.sg_n + t2 * a.sg_t + h2 * a.sg_h + lane * E;
@@ -731,8 +833,8 @@ extern "C" int kad_block_prefix_attention(
                   aligned(q, sq_n, sq_t, sq_h, 8),
               "codes and query rows must be 16-byte aligned");
   KAD_REQUIRE(Tk == 0 || (aligned(suffix_k, ssk_n, ssk_t, ssk_h, 8) &&
-                          aligned(suffix_v, ssv_n, ssv_t, ssv_h, 4)),
-              "suffix rows must be 16-byte (K) and 8-byte (V) aligned");
+                          aligned(suffix_v, ssv_n, ssv_t, ssv_h, 8)),
+              "suffix rows must be 16-byte aligned");
   if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
     KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
   int64_t need = 0;

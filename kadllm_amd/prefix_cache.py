@@ -267,7 +267,7 @@ def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
     sk = sv = g = none
     Tk = 0
     if suffix_k is not None:
-        suffix_k, suffix_v = _rows(suffix_k, 8), _rows(suffix_v, 4)
+        suffix_k, suffix_v = _rows(suffix_k, 8), _rows(suffix_v, 8)
         Tk = suffix_k.shape[1]
         sk = (_lib.ptr(suffix_k), *suffix_k.stride()[:3])
         sv = (_lib.ptr(suffix_v), *suffix_v.stride()[:3])
