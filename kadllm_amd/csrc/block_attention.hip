@@ -220,6 +220,54 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// o *= f on accumulation registers.  Left to the compiler, this rare branch would
+// keep O in ordinary registers and copy all of it to and fro around the products
+// of every tile.  (The first nops cover a product still writing o, the last ones
+// the next product's read.)
+__device__ __forceinline__ void scale_acc(f32x16& o, float f) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 4) {
+    float x0 = o[j], x1 = o[j + 1], x2 = o[j + 2], x3 = o[j + 3], t0, t1, t2, t3;
+    asm volatile(
+        "s_nop 15\n\ts_nop 15\n\t"
+        "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+        "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
+        "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
+        "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\ts_nop 1\n\t"
+        "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+        "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 4"
+        : "+a"(x0), "+a"(x1), "+a"(x2), "+a"(x3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+        : "v"(f));
+    o[j] = x0;
+    o[j + 1] = x1;
+    o[j + 2] = x2;
+    o[j + 3] = x3;
+  }
+}
+
+// 4 elements of an output row: normalised, gated, rounded once (the gate's
+// sigmoid by the hardware's reciprocal, 1 ulp)
+template <typename T>
+__device__ __forceinline__ void store_row4(T* out, const float* o, float l, bool gated,
+                                           u32x2 gate) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float y[4];
+  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+  const f16x4 gh = __builtin_bit_cast(f16x4, gate);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = o[e] * inv;
+    if (gated) {
+      const float g = std::is_same<T, bf16_t>::value
+                          ? __uint_as_float(e & 1 ? gate[e >> 1] & 0xffff0000u : gate[e >> 1] << 16)
+                          : (float)gh[e];
+      y[e] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+    }
+  }
+  const T* const kind = nullptr;
+  *(u32x2*)out = u32x2{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3])};
+}
+
 // A workgroup of 4 waves takes a request, a KV head, a range of the prefix
 // (one of `splits`) and query rows, ordered (beam, head in the group, token).
 // A wave holds 32 rows: Q's pieces, the output O^T and the softmax state stay
@@ -307,9 +355,7 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     m = to;
     l *= f;
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) O[i][j] *= f;
+    for (int i = 0; i < DT; ++i) scale_acc(O[i], f);
   };
 
   // ---- the beams' own suffixes.  The suffix keys of the wave's beams, in order,
@@ -394,7 +440,8 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       const int v_d = (lane >> 4 & 1) * 16 + (gi & 3) * 4;
       const int v_sw = D == 64 ? (v_row >> 1 & 1) * 4 : (v_row & 3) * 4;
       for (int ks = 0; ks < (both ? 2 : 1); ++ks) {
-        const uint32_t base = (uint32_t)(uintptr_t)(area + (16 * ks + v_row) * D * 2 + (v_d & 7) * 2);
+        const uint32_t base =
+            (uint32_t)(uintptr_t)(area + (16 * ks + v_row) * D * 2 + (v_d & 7) * 2);
 #pragma unroll
         for (int d2 = 0; d2 < DT / 2; ++d2) {
           u32x4 x, y;
@@ -454,11 +501,20 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   };
 
   // LDS offsets of the fragments
+  uint32_t k_off[KS][2];   // K: key col of a half, chunks 4 s + hi and 4 s + 2 + hi
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      k_off[s][c] = col * D + ((4 * s + 2 * c + hi) ^ S::swk(col)) * 16;
   // V: key 8 (e / 4) + 4 hi + e % 4, e = (lane % 16) / 2; d = 32 dt + 16 (lane / 16 % 2) +
   // 8 (lane % 2)
   const int v_e = (lane & 15) >> 1;
   const int v_row = 8 * (v_e >> 2) + 4 * hi + (v_e & 3);
-  const int v_chunk = lane >> 4 & 1, v_sw = S::swv(v_row);
+  uint32_t v_off[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    v_off[dt] = v_row * D + (lane & 1) * 8 + (((2 * dt + (lane >> 4 & 1)) ^ S::swv(v_row)) * 16);
 
   // ---- one tile in LDS: scores, weights, output
   int m0 = 0, m1 = 0;   // meta of the tile's halves
@@ -469,10 +525,8 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       const int sk = (hf ? m1 : m0) >> 8 & 0xff;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        // chunk 4s + 2c + hi: the XOR touches the low bits only where 4s does not
-        const uint8_t* row = ks + hf * 32 * D + col * D;
-        const i32x4 x = *(const i32x4*)(row + ((4 * s + hi) ^ S::swk(col)) * 16);
-        const i32x4 y = *(const i32x4*)(row + ((4 * s + 2 + hi) ^ S::swk(col)) * 16);
+        const i32x4 x = *(const i32x4*)(ks + k_off[s][0] + hf * 32 * D);
+        const i32x4 y = *(const i32x4*)(ks + k_off[s][1] + hf * 32 * D);
         const i32x8 kf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
         for (int p = 0; p < NP; ++p) st[hf] = mfma_scaled(kf, qf[p][s], st[hf], sk, qs[p]);
@@ -525,12 +579,11 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   };
   auto outputs = [&](const uint8_t* vs) {
     const int sv = (hi ? m1 : m0) >> 16 & 0xff;
-    const uint32_t base = (uint32_t)(uintptr_t)(vs + v_row * D + (lane & 1) * 8);
+    const uint32_t base = (uint32_t)(uintptr_t)vs;
 #pragma unroll
     for (int d2 = 0; d2 < DT / 2; ++d2) {
       i32x8 f0, f1;
-      read_v2<D>(base + (((4 * d2 + v_chunk) ^ v_sw) * 16),
-                 base + (((4 * d2 + 2 + v_chunk) ^ v_sw) * 16), f0, f1);
+      read_v2<D>(base + v_off[2 * d2], base + v_off[2 * d2 + 1], f0, f1);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         O[2 * d2] = mfma_scaled(f0, pf[p], O[2 * d2], sv, ps[p]);
@@ -626,8 +679,9 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     }
   }
 
-  // ---- the rows, one at a time over a wave: O^T through LDS, joined over the
-  // waves that hold the same rows, then stored whole (or as a partial result)
+  // ---- the rows: O^T through LDS, joined over the waves that hold the same
+  // rows, then stored whole (or as a partial result).  A wave takes 256 / D rows
+  // at a time, 4 elements a lane, and 8 such steps' gates at once.
   wait_vm(0);
   __syncthreads();
   float* ep = (float*)smem + wave * 32 * S::EpiLd;
@@ -643,100 +697,112 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   }
   if (lane == 0) sm_spoilt[wave] = spoilt;
   __syncthreads();
-  constexpr int E = D / 64;       // elements of a row per lane
-  for (int i = SHARED ? 0 : wave; i < 32; i += SHARED ? 1 : 4) {
-    const int rr = row0 + i;
-    if (rr >= a.R) break;
-    float o[E], ll, mm;
-    if constexpr (SHARED) {
-      mm = sm_m[wave][i];
-      ll = sm_l[wave][i];
+  constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
+  constexpr int STEPS = SHARED ? 32 / RPS : (32 / RPS + 3) / 4, AT_ONCE = STEPS < 8 ? STEPS : 8;
+  const int sub = lane / LPR, d0 = lane % LPR * 4;
+  const bool spoilt_rows = sm_spoilt[SHARED ? wave : 0];
+  const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
+  const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
+  auto of_lane = [](int64_t v, int from) {
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
+                     (uint64_t)(uint32_t)__shfl((int)(v >> 32), from, 64) << 32);
+  };
+  const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
+#pragma unroll 1
+  for (int s0 = 0; s0 < STEPS; s0 += AT_ONCE) {
+    if ((SHARED ? s0 : 4 * s0 + wave) * RPS >= rows) break;
+    u32x2 gv[AT_ONCE];
+    int64_t at[AT_ONCE];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = ep[i * S::EpiLd + lane * E + e];
-    } else {
-      mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
-      ll = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float f = sm_m[x][i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm_m[x][i] - mm);
-        ll = fmaf(f, sm_l[x][i], ll);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          o[e] = fmaf(f, ((float*)smem)[(x * 32 + i) * S::EpiLd + lane * E + e], o[e]);
-      }
+    for (int s = 0; s < AT_ONCE; ++s) {
+      const int i = min((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub, 31);
+      at[s] = of_lane(out_at, i);
+      gv[s] = u32x2{};
+      if (a.gate) gv[s] = *(const u32x2*)((const T*)a.gate + of_lane(gate_at, i) + d0);
     }
-    const int t2 = rr % a.T, g2 = rr / a.T % G, w2 = rr / a.T / G;
-    const int64_t n2 = (int64_t)b * a.W + w2;
-    if (sm_spoilt[SHARED ? wave : 0]) {
-      const T* vr = (const T*)a.sv + n2 * a.ssv_n + kh * a.ssv_h + lane * E;
-      for (int j = 0; j <= a.Tk - a.T + t2; ++j)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + e]);
-          if (!(fabsf(x) < INFINITY)) o[e] += x;
+    for (int s = 0; s < AT_ONCE; ++s) {
+      const int i = min((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub, 31);
+      float o[4], ll, mm;
+      if constexpr (SHARED) {
+        mm = sm_m[wave][i];
+        ll = sm_l[wave][i];
+        const f32x4 x = *(const f32x4*)(ep + i * S::EpiLd + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = x[e];
+      } else {
+        mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
+        ll = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float mx = sm_m[x][i];
+          const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mm);
+          ll = fmaf(f, sm_l[x][i], ll);
+          const f32x4 y = *(const f32x4*)((float*)smem + (x * 32 + i) * S::EpiLd + d0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
         }
-    }
-    if (a.splits > 1) {
-      const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + rr;
-#pragma unroll
-      for (int e = 0; e < E; ++e) a.part_o[at * D + lane * E + e] = o[e];
-      if (lane == 0) {
-        a.part_ml[2 * at] = mm;
-        a.part_ml[2 * at + 1] = ll;
       }
-      continue;
-    }
-    const int h2 = kh * G + g2;
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    const T* gate = (const T*)a.gate + n2 * a.sg_n + t2 * a.sg_t + h2 * a.sg_h + lane * E;
-    T* out = (T*)a.out + n2 * a.so_n + t2 * a.so_t + h2 * a.so_h + lane * E;
+      if ((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub >= rows) continue;
+      const int rr = row0 + i;
+      if (spoilt_rows) {
+        const int t2 = rr % a.T, w2 = rr / a.T / G;
+        const T* vr = (const T*)a.sv + ((int64_t)b * a.W + w2) * a.ssv_n + kh * a.ssv_h + d0;
+        for (int j = 0; j <= a.Tk - a.T + t2; ++j)
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float y = o[e] * inv;
-      if (a.gate) y *= sigmoid_f(Elem<T>::to_f(gate[e]));
-      out[e] = Elem<T>::from_f(y);
+          for (int e = 0; e < 4; ++e) {
+            const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + e]);
+            if (!(fabsf(x) < INFINITY)) o[e] += x;
+          }
+      }
+      if (a.splits > 1) {
+        const int64_t to = ((int64_t)split * a.B * a.HK + bk) * a.R + rr;
+        *(f32x4*)(a.part_o + to * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
+        if (d0 == 0) {
+          a.part_ml[2 * to] = mm;
+          a.part_ml[2 * to + 1] = ll;
+        }
+      } else {
+        store_row4<T>((T*)a.out + at[s] + d0, o, ll, a.gate != nullptr, gv[s]);
+      }
     }
   }
 }
 
-// Joins the ranges of a split prefix: one wave per row.
+// Joins the ranges of a split prefix: a wave takes 256 / D rows, 4 elements a
+// lane.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
+  constexpr int LPR = D / 4, RPB = 256 / LPR;
   const int64_t rows = (int64_t)a.B * a.HK * a.R;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+  const int d0 = threadIdx.x % LPR * 4;
   if (row >= rows) return;
-  float mm = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (s * rows + row)]);
-  float o[E], ll = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float ms = a.part_ml[2 * (s * rows + row)];
-    if (ms == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(ms - mm);
-    ll = fmaf(f, a.part_ml[2 * (s * rows + row) + 1], ll);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      o[e] = fmaf(f, a.part_o[(s * rows + row) * D + lane * E + e], o[e]);
-  }
   const int G = a.H / a.HK;
   const int rr = (int)(row % a.R), bk = (int)(row / a.R);
   const int t = rr % a.T, g = rr / a.T % G, w = rr / a.T / G;
   const int64_t n = (int64_t)(bk / a.HK) * a.W + w;
   const int h = bk % a.HK * G + g;
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  const T* gate = (const T*)a.gate + n * a.sg_n + t * a.sg_t + h * a.sg_h + lane * E;
-  T* out = (T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + lane * E;
+  u32x2 gate = u32x2{};
+  if (a.gate)
+    gate = *(const u32x2*)((const T*)a.gate + n * a.sg_n + t * a.sg_t + h * a.sg_h + d0);
+  float mm = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (s * rows + row)]);
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = s * rows + row;
+    const float ms = a.part_ml[2 * at], ls = a.part_ml[2 * at + 1];
+    const f32x4 x = *(const f32x4*)(a.part_o + at * D + d0);
+    const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mm);
+    ll = fmaf(f, ls, ll);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float y = o[e] * inv;
-    if (a.gate) y *= sigmoid_f(Elem<T>::to_f(gate[e]));
-    out[e] = Elem<T>::from_f(y);
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
   }
+  store_row4<T>((T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + d0, o, ll, a.gate != nullptr,
+                gate);
 }
 
 // The launch of a call: whether the waves share tiles, and the ranges the
@@ -777,8 +843,8 @@ int launch(const BlockAttnArgs& a, bool shared, hipStream_t stream) {
     hipLaunchKernelGGL((block_attn_kernel<T, D, false>), grid, dim3(256), lds, stream, a);
   if (a.splits > 1)
     hipLaunchKernelGGL((block_attn_join_kernel<T, D>),
-                       dim3((unsigned)kad_cdiv((int64_t)a.B * a.HK * a.R, 4)), dim3(256), 0,
-                       stream, a);
+                       dim3((unsigned)kad_cdiv((int64_t)a.B * a.HK * a.R, 1024 / D)), dim3(256),
+                       0, stream, a);
   return kad_launch_status("block_attn_kernel");
 }
 
@@ -835,6 +901,8 @@ extern "C" int kad_block_prefix_attention(
   KAD_REQUIRE(Tk == 0 || (aligned(suffix_k, ssk_n, ssk_t, ssk_h, 8) &&
                           aligned(suffix_v, ssv_n, ssv_t, ssv_h, 8)),
               "suffix rows must be 16-byte aligned");
+  KAD_REQUIRE(aligned(out, so_n, so_t, so_h, 4) && (!gate || aligned(gate, sg_n, sg_t, sg_h, 4)),
+              "gate and output rows must be 8-byte aligned");
   if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
     KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
   int64_t need = 0;

@@ -237,9 +237,9 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
         raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
     _check_devices(q, tables, lengths, suffix_k, suffix_v, gate, *blocks)
     scale = 1 / math.sqrt(D) if scale is None else scale
-    gate_strides = None if gate is None else (gate.stride(0), gate.stride(1), D)
-    if gate is not None and gate.stride(2) != 1:
-        gate = gate.contiguous()
+    gate_strides = None
+    if gate is not None:
+        gate = _rows(gate, 4)
         gate_strides = (gate.stride(0), gate.stride(1), D)
     return _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale,
                             gate, gate_strides)
@@ -247,11 +247,11 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
 
 def _rows(t, elements):
     """t, or a copy whose rows start at multiples of ``elements`` elements."""
-    if t.stride(3) == 1 and not any(s % elements for s in t.stride()[:3]) and \
+    strides = t.stride()
+    if strides[-1] == 1 and not any(s % elements for s in strides[:-1]) and \
             t.data_ptr() % (2 * elements) == 0:
         return t
-    return t.contiguous(memory_format=torch.contiguous_format) if not t.is_contiguous() \
-        else t.clone()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale, gate=None,
