@@ -128,6 +128,13 @@ def stream_of(t):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def stream_of_index(device):
+    """Raw hipStream_t of torch's current stream on a device given by its index."""
+    if _raw_stream is not None:
+        return _raw_stream(device)
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 _call_hook = None
 
 

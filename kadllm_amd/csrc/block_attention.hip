@@ -51,9 +51,9 @@ struct BlockAttnArgs {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(1))) const void global_t;
 typedef __attribute__((address_space(3))) void lds_t;
 
 // f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>)
@@ -245,12 +245,40 @@ __device__ __forceinline__ void scale_acc(f32x16& o, float f) {
   }
 }
 
-// 4 elements of an output row: normalised, gated, rounded once (the gate's
+// 16 bytes a lane from base + off (zeros from nbytes on) into LDS at lds + 16 *
+// lane; base, nbytes and lds wave-uniform.  In assembly so that the compiler does
+// not make the next transpose read wait for every such load in flight: waits are
+// the callers' (wait_vm).  (No register is written; the nops cover scalar
+// operands that a vector instruction has just written, and m0.)
+__device__ __forceinline__ void load_lds16(const uint8_t* base, int nbytes, uint32_t off,
+                                           uint32_t lds) {
+  const uint64_t p = (uint64_t)(uintptr_t)base;
+  const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)nbytes, 0x00020000u};
+  asm volatile(
+      "s_mov_b32 m0, %2\n\t"
+      "s_nop 4\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(off), "s"(rsrc), "s"(lds)
+      : "memory", "m0");
+}
+
+// the same from an address of each lane's own
+__device__ __forceinline__ void load_lds16(const void* src, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %0, off"
+      :
+      : "v"(src), "s"(lds)
+      : "memory", "m0");
+}
+
+// 4 elements of an output row: times inv, gated, rounded once (the gate's
 // sigmoid by the hardware's reciprocal, 1 ulp)
 template <typename T>
-__device__ __forceinline__ void store_row4(T* out, const float* o, float l, bool gated,
+__device__ __forceinline__ void store_row4(T* out, const float* o, float inv, bool gated,
                                            u32x2 gate) {
-  const float inv = l == 0.f ? 0.f : 1.f / l;
   float y[4];
   typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
   const f16x4 gh = __builtin_bit_cast(f16x4, gate);
@@ -281,12 +309,12 @@ __device__ __forceinline__ void store_row4(T* out, const float* o, float l, bool
 //     while the next K is, so no wave waits for another; their states are
 //     joined at the end.
 template <typename T, int D, bool SHARED>
-__global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
+__global__ __launch_bounds__(256, D == 256 || (SHARED && D == 128) ? 1 : 2) void
+block_attn_kernel(BlockAttnArgs a) {
   using S = Shape<D>;
   constexpr int NP = Pieces<T>::n, KS = S::KS, DT = S::DT;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   __shared__ float sm_m[4][32], sm_l[4][32];
-  __shared__ int sm_spoilt[4];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -303,6 +331,37 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   const int t = r % a.T, g = r / a.T % G, w = r / a.T / G;
   const int64_t n = (int64_t)b * a.W + w;
   const int h = kh * G + g;
+
+  // ---- this wave's tiles of the prefix: first + stride * k, k < count.  (With one
+  // range the first pages do not wait for the length.)
+  const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
+  const int tiles = (len + kKeys - 1) / kKeys;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int begin = split == 0 ? 0 : min(split * per, tiles), end = min(begin + per, tiles);
+  const int first = begin + (SHARED ? 0 : wave), stride = SHARED ? 1 : 4;
+  const int count = __builtin_amdgcn_readfirstlane(
+      SHARED ? end - begin : max((end - first + stride - 1) / stride, 0));
+
+  // Pages: lane i of a chunk of 32 tiles describes half tile i: its page
+  // (-1: none) and keys held | K's scale byte << 8 | V's << 16
+  int pg = -1, meta = 0;
+  auto half_at = [&](int chunk) {
+    return (first + stride * (32 * chunk + (lane >> 1))) * kKeys + (lane & 1) * 32;
+  };
+  auto page_at = [&](int chunk) {
+    return a.tables[(int64_t)b * a.width + min(half_at(chunk) >> a.lblock, a.width - 1)];
+  };
+  auto describe = [&](int chunk, int id) {
+    const int pos = half_at(chunk);
+    pg = -1;
+    meta = 127 << 8 | 127 << 16;
+    if (32 * chunk + (lane >> 1) < count && pos < len && id >= 0 && id < a.pages) {
+      const int64_t ph = (int64_t)id * a.HK + kh;
+      pg = id;
+      meta = min(len - pos, 32) | (int)a.ksc[ph] << 8 | (int)a.vsc[ph] << 16;
+    }
+  };
+  const int first_page = page_at(0);
 
   // ---- Q: the row's elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7 as they
   // are, and in e4m3 pieces against the row's power of two
@@ -363,34 +422,53 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   // masked to each row's beam and to the tokens before its own, then O^T += V^T
   // P^T from LDS (area: 64 * D bytes of the wave's own).  A value that is not
   // finite would reach the rows that do not see it as 0 * inf, so a group that
-  // holds one is multiplied without it, and the rows that do see it add it when
-  // they are stored.
+  // holds one is multiplied without it, and the rows that do see it add it at the
+  // end.
   bool spoilt = false;
-  auto suffix = [&](uint8_t* area) {
-    const int w0 = row0 / a.T / G, w1 = min(row0 + 31, a.R - 1) / a.T / G;
-    const int vlo = (w - w0) * a.Tk, vhi = vlo + a.Tk - a.T + t;   // keys the row sees
-    int keys = vhi + 1;
+  const bool has_suffix = a.Tk > 0 && split == 0 && (SHARED || wave == 0);
+  int vlo = 0, vhi = -1, keys = 0;                   // keys the row sees, keys of the wave
+  const int w0 = row0 / a.T / G;
+  const int64_t n0 = (int64_t)b * a.W + w0;
+  constexpr int CPV = D / 8, RPV = 512 / D;          // chunks per V row, rows per load
+  u32x4 kr[4 * KS];
+  if (has_suffix) {
+    const int w1 = min(row0 + 31, a.R - 1) / a.T / G;
+    vlo = (w - w0) * a.Tk;
+    vhi = vlo + a.Tk - a.T + t;
+    keys = vhi + 1;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o, 64));
-    keys = min(__builtin_amdgcn_readfirstlane(keys), (w1 - w0 + 1) * a.Tk);
-    const int64_t n0 = (int64_t)b * a.W + w0;
-    constexpr int CPV = D / 8, RPV = 512 / D;        // chunks per V row, rows per load
-    for (int f0 = 0; f0 < keys; f0 += 32) {
-      const bool both = keys - f0 > 16;              // 16 or 32 rows of V
-      const int fk = min(f0 + col, keys - 1);
-      const T* krow = (const T*)a.sk + (n0 + fk / a.Tk) * a.ssk_n +
-                      (int64_t)(fk % a.Tk) * a.ssk_t + kh * a.ssk_h + 16 * hi;
-      u32x4 kr[4 * KS];
+    keys = max(min(__builtin_amdgcn_readfirstlane(keys), (w1 - w0 + 1) * a.Tk), 1);
+  }
+  auto of_lane = [](int64_t v, int from) {
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
+                     (uint64_t)(uint32_t)__shfl((int)(v >> 32), from, 64) << 32);
+  };
+  auto suffix_load = [&](uint8_t* area, int f0) {
+    const uint32_t area_at = (uint32_t)(uintptr_t)(lds_t*)area;
+    const int f = min(f0 + col, keys - 1), beam = f / a.Tk, token = f - beam * a.Tk;
+    const T* krow = (const T*)a.sk + (n0 + beam) * a.ssk_n + (int64_t)token * a.ssk_t +
+                    kh * a.ssk_h + 16 * hi;
 #pragma unroll
-      for (int c = 0; c < 4 * KS; ++c)
-        kr[c] = *(const u32x4*)(krow + 32 * (c >> 1) + 8 * (c & 1));
-      for (int i = 0; i < (both ? 32 : 16) / RPV; ++i) {
-        const int row = i * RPV + lane / CPV;
-        const int fv = min(f0 + row, keys - 1);
-        const int chunk = (lane % CPV) ^ (D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
-        const T* src = (const T*)a.sv + (n0 + fv / a.Tk) * a.ssv_n +
-                       (int64_t)(fv % a.Tk) * a.ssv_t + kh * a.ssv_h + chunk * 8;
-        __builtin_amdgcn_global_load_lds((global_t*)src, (lds_t*)(area + i * 1024), 16, 0, 0);
+    for (int c = 0; c < 4 * KS; ++c)
+      kr[c] = *(const u32x4*)(krow + 32 * (c >> 1) + 8 * (c & 1));
+    const int64_t v_at = (n0 + beam) * a.ssv_n + (int64_t)token * a.ssv_t + kh * a.ssv_h;
+    const int pieces = (keys - f0 > 16 ? 32 : 16) / RPV;   // 16 or 32 rows of V
+#pragma unroll 4
+    for (int i = 0; i < pieces; ++i) {
+      const int row = i * RPV + lane / CPV;
+      const int chunk = (lane % CPV) ^ (D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
+      const T* src = (const T*)a.sv + of_lane(v_at, row) + chunk * 8;
+      load_lds16(src, area_at + i * 1024);
+    }
+  };
+  // in_flight: loads issued after the first group's
+  auto suffix = [&](uint8_t* area, int in_flight) {
+    for (int f0 = 0; f0 < keys; f0 += 32) {
+      const bool both = keys - f0 > 16;
+      if (f0 > 0) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        suffix_load(area, f0);
       }
       f32x16 st = f32x16{};
 #pragma unroll
@@ -404,6 +482,7 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
         top = fmaxf(top, st[j]);
       }
       top = max_xor32(top);
+      if (m == -INFINITY) m = top;
       if (__ballot(top > m) != 0) raise(top, 0.f);   // (so weights are at most 1)
       const float ref = m == -INFINITY ? 0.f : m;
       u32x4 pk[2];
@@ -416,7 +495,8 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
         pk[j >> 3][j >> 1 & 3] = pack2(kind, x, y);
       }
       l += add_xor32(sum);
-      wait_vm(0);
+      if (f0 == 0 && in_flight) wait_vm(in_flight);
+      else wait_vm(0);
       // (each lane looks at what its own loads brought)
       uint32_t top_exp = 0;
       const int pieces = (both ? 32 : 16) / RPV;
@@ -455,50 +535,18 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     }
   };
 
-  // ---- this wave's tiles of the prefix: first + stride * k, k < count
-  const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
-  const int tiles = (len + kKeys - 1) / kKeys;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int begin = min(split * per, tiles), end = min(begin + per, tiles);
-  const int first = begin + (SHARED ? 0 : wave), stride = SHARED ? 1 : 4;
-  const int count = __builtin_amdgcn_readfirstlane(
-      SHARED ? end - begin : max((end - first + stride - 1) / stride, 0));
-
-  // Pages: lane i of a chunk of 32 tiles describes half tile i: its page
-  // (-1: none) and keys held | K's scale byte << 8 | V's << 16
-  int pg = -1, meta = 0;
-  auto describe = [&](int chunk) {
-    const int k = 32 * chunk + (lane >> 1);
-    const int pos = (first + stride * k) * kKeys + (lane & 1) * 32;
-    pg = -1;
-    meta = 127 << 8 | 127 << 16;
-    if (k < count && pos < len) {
-      const int id = a.tables[(int64_t)b * a.width + (pos >> a.lblock)];
-      if (id >= 0 && id < a.pages) {
-        const int64_t ph = (int64_t)id * a.HK + kh;
-        pg = id;
-        meta = min(len - pos, 32) | (int)a.ksc[ph] << 8 | (int)a.vsc[ph] << 16;
-      }
-    }
-  };
-  // per-lane source offsets of load instruction i of a tile: key i * RPI +
-  // lane / CPR, the chunk that the swizzle puts at place lane % CPR
+  // load instruction i of a K (kv 0) or V tile: key i * RPI + lane / CPR, at place
+  // lane % CPR the chunk that the swizzle puts there; page and meta describe
+  // the half tile it lies in, pos is the tile's first key
   const int d_row = lane / S::CPR, d_pc = lane % S::CPR;
-  // instruction i of half-tile data `kv` (0 K, 1 V) of the wave's tile k into dst
-  auto load1 = [&](int kv, int k, int i, uint8_t* dst) {
-    const int at = 2 * (k & 31) + i * S::RPI / 32;       // the lane that describes the half
-    const int page = __builtin_amdgcn_readlane(pg, at);
-    const int held = __builtin_amdgcn_readlane(meta, at) & 0xff;
-    const int pos = (first + stride * k) * kKeys + i * S::RPI / 32 * 32;
-    const int64_t key = (((int64_t)max(page, 0) * a.HK + kh) << a.lblock) +
-                        (pos & ((1 << a.lblock) - 1));
-    const uint8_t* base = (kv ? a.vc : a.kc) + key * D;
+  auto load1 = [&](int kv, int page, int meta_of, int pos, int i, uint32_t dst) {
     const int row = i * S::RPI + d_row;
+    const int64_t key = (((int64_t)max(page, 0) * a.HK + kh) << a.lblock) +
+                        ((pos + i * S::RPI / 32 * 32) & ((1 << a.lblock) - 1));
     const int off = (row & 31) * D + (d_pc ^ (kv ? S::swv(row) : S::swk(row))) * 16;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(base), 0, held * D, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t*)(dst + i * 1024), 16, off, 0, 0, 0);
+    load_lds16((kv ? a.vc : a.kc) + key * D, (meta_of & 0xff) * D, off, dst + i * 1024);
   };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
 
   // LDS offsets of the fragments
   uint32_t k_off[KS][2];   // K: key col of a half, chunks 4 s + hi and 4 s + 2 + hi
@@ -597,65 +645,231 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
   };
 
   if constexpr (SHARED) {
-    // wave w loads LT / 4 instructions of K and of V of every tile; the chunk
-    // of page descriptions changes with the tile that is loaded, three ahead of
-    // the one in use, whose own are kept in a ring of registers
+    // Two rings of 4 tiles, K's and then V's.  Step k forms the scores of tile
+    // k + 1 and adds tile k - 1 to the output while the vector unit turns tile k's
+    // scores into weights: the three are independent, so the products run
+    // without a pause (a step's vector work takes about 3/4 of their time at D =
+    // 256).  K(k) and V(k - 2) have been used by then, and K(k + 4) and V(k + 2)
+    // are loaded into their places, three steps before their use; wave w loads
+    // the w-th quarter of each.  Tiles past the last are loaded as zeros, which
+    // keeps the counts of loads in flight the same.
     constexpr int LW = S::LT / 4;
-    int ring0[4], ring1[4];
-    auto issue = [&](int k) {
-      if ((k & 31) == 0) describe(k >> 5);
-      uint8_t* dst = smem + (k & 3) * S::slot;
+    int ring_pg[6][2], ring_meta[6][2];     // halves of the tiles k - 1 .. k + 4 (-1: none)
+    auto read_ring = [&](int x, int k) {
 #pragma unroll
-      for (int i = 0; i < LW; ++i) load1(0, k, wave * LW + i, dst);
-#pragma unroll
-      for (int i = 0; i < LW; ++i) load1(1, k, wave * LW + i, dst + S::tile);
+      for (int hf = 0; hf < 2; ++hf) {
+        ring_pg[x][hf] = __builtin_amdgcn_readlane(pg, 2 * (k & 31) + hf);
+        ring_meta[x][hf] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + hf);
+      }
     };
-    auto push = [&](int k) {
-      ring0[0] = ring0[1]; ring0[1] = ring0[2]; ring0[2] = ring0[3];
-      ring1[0] = ring1[1]; ring1[1] = ring1[2]; ring1[2] = ring1[3];
-      ring0[3] = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
-      ring1[3] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
-    };
+    auto issue = [&](int kv, int x, int k) {  // tile k, described in ring[x]
+      const uint32_t dst = lds0 + (4 * kv + (k & 3)) * S::tile;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (k < count) issue(k);
-      push(k);
+      for (int i = 0; i < LW; ++i) {
+        const int at = wave * LW + i, hf = at * S::RPI / 32;
+        load1(kv, hf ? ring_pg[x][1] : ring_pg[x][0], hf ? ring_meta[x][1] : ring_meta[x][0],
+              (first + k) * kKeys, at, dst);
+      }
+    };
+    uint8_t* area = smem + (4 + wave) * S::tile;   // the suffix: where V's tiles go
+    if (has_suffix) suffix_load(area, 0);
+    describe(0, first_page);
+    ring_pg[0][0] = ring_pg[0][1] = -1;
+    ring_meta[0][0] = ring_meta[0][1] = 127 << 8 | 127 << 16;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      read_ring(k + 1, k);
+      issue(0, k + 1, k);
     }
-    if (a.Tk > 0 && split == 0) {   // in stages 2 and 3
-      suffix(smem + 2 * S::slot + wave * S::tile);
+    if (has_suffix) {
+      suffix(area, 4 * LW);
       tile_barrier();
     }
-    if (2 < count) issue(2);
-    push(2);
+    issue(1, 0, -1);
+    issue(1, 1, 0);
+    issue(1, 2, 1);
+    ring_pg[5][0] = ring_pg[5][1] = ring_meta[5][0] = ring_meta[5][1] = 0;
     split_q();
+    f32x16 st[2];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      pf[p] = i32x8{};
+      ps[p] = 127;
+    }
+    wait_vm(6 * LW);                        // K(0)
+    tile_barrier();
+    m0 = ring_meta[1][0];
+    m1 = ring_meta[1][1];
+    scores(smem, st);
+
+    auto read_v = [&](const uint8_t* vs, int dt) {
+      typedef __attribute__((address_space(3))) i32x2* piece_t;
+      const uint32_t at = (uint32_t)(uintptr_t)(lds_t*)vs + v_off[dt];
+      i32x8 f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((piece_t)(at + 16 * c * D));
+        f[2 * c] = x[0];
+        f[2 * c + 1] = x[1];
+      }
+      return f;
+    };
+#pragma unroll 1
     for (int k = 0; k < count; ++k) {
-      // tile k has landed when at most those of k + 1 and k + 2 are in flight
-      if (k + 2 < count) wait_vm(4 * LW);
-      else if (k + 1 < count) wait_vm(2 * LW);
-      else wait_vm(0);
+      f32x16 cur[2] = {st[0], st[1]};
+      i32x8 pc[NP];
+      int pcs[NP];
+      if (k >= 2) wait_vm(4 * LW);          // K(k + 1) and V(k - 1)
+      else wait_vm(2 * LW);
       tile_barrier();
-      // every wave is done with tile k - 1, whose stage tile k + 3 takes
-      if (k + 3 < count) issue(k + 3);
-      push(k + 3);
-      m0 = ring0[0];
-      m1 = ring1[0];
-      const uint8_t* stage = smem + (k & 3) * S::slot;
-      f32x16 st[2];
-      scores(stage, st);
-      weights(st);
-      outputs(stage + S::tile);
+#pragma unroll
+      for (int x = 0; x < 5; ++x)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          if (k > 0) ring_pg[x][hf] = ring_pg[x + 1][hf];
+          if (k > 0) ring_meta[x][hf] = ring_meta[x + 1][hf];
+        }
+      if ((k + 4 & 31) == 0) describe((k + 4) >> 5, page_at((k + 4) >> 5));
+      read_ring(5, k + 4);
+      issue(0, 5, k + 4);
+      issue(1, 3, k + 2);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int held = ring_meta[1][hf] & 0xff;
+        if (held < 32) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            cur[hf][j] = 8 * (j >> 2) + 4 * hi + (j & 3) < held ? cur[hf][j] : -INFINITY;
+        }
+      }
+      const uint8_t* ks = smem + (k + 1 & 3) * S::tile;
+      const uint8_t* vs = smem + (4 + (k - 1 & 3)) * S::tile;
+      const int sk[2] = {ring_meta[2][0] >> 8 & 0xff, ring_meta[2][1] >> 8 & 0xff};
+      const int sv = (hi ? ring_meta[0][1] : ring_meta[0][0]) >> 16 & 0xff;
+      // the vector work in slices: 8 of maxima, 1 of references, 24 of weights
+      float top[2] = {-INFINITY, -INFINITY}, nm[2], sum[2] = {0.f, 0.f}, y[4], fac = 1.f;
+      int e[2];
+      bool moved = false;
+      auto slice = [&](auto c_c) {
+        constexpr int c = decltype(c_c)::value;
+        if constexpr (c < 8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top[c / 4] = fmaxf(top[c / 4], cur[c / 4][4 * (c % 4) + j]);
+        } else if constexpr (c == 8) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) top[hf] = max_xor32(top[hf]) * a.sl2;
+          const float both = fmaxf(top[0], top[1]);
+          moved = both > m + kMaxUp && m != -INFINITY;
+          const float to = m == -INFINITY || moved ? both : m;
+          fac = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
+          m = to;
+          const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            e[hf] = (int)fmaxf(ceilf(top[hf] - ref), -100.f);
+            nm[hf] = (float)(8 - e[hf]) - ref;
+          }
+          const int own = hi ? e[1] : e[0];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) pcs[p] = own - 8 - 4 * p + 127;
+        } else {
+          constexpr int g = (c - 9) / 3, part = (c - 9) % 3, hf = g / 4, j4 = g % 4;
+          if constexpr (part < 2) {
+#pragma unroll
+            for (int i = 2 * part; i < 2 * part + 2; ++i) {
+              y[i] = __builtin_amdgcn_exp2f(fmaf(cur[hf][4 * j4 + i], a.sl2, nm[hf]));
+              sum[hf] += y[i];
+            }
+            asm volatile("" ::"v"(sum[hf]));   // (here, not where it is used)
+          } else {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+              const int word = piece4(y, y);
+              asm volatile("" ::"v"(word));
+              pc[p][4 * hf + j4] = word;
+            }
+          }
+        }
+      };
+      constexpr int NF = 4 * KS, MF = NF * NP, SL = 33;
+      i32x8 fr[3];
+      auto fetch = [&](auto f_c) {
+        constexpr int f = decltype(f_c)::value;
+        if constexpr (f < 2 * KS) {
+          constexpr int hf = f / KS, s = f % KS;
+          const i32x4 x = *(const i32x4*)(ks + k_off[s][0] + hf * 32 * D);
+          const i32x4 z = *(const i32x4*)(ks + k_off[s][1] + hf * 32 * D);
+          fr[f % 3] = i32x8{x[0], x[1], x[2], x[3], z[0], z[1], z[2], z[3]};
+        } else if constexpr (f < NF) {
+          fr[f % 3] = read_v(vs, f - 2 * KS);
+        }
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(std::integral_constant<int, 0>{});
+      fetch(std::integral_constant<int, 1>{});
+      static_for<MF>([&](auto i_c) {
+        constexpr int i = decltype(i_c)::value, f = i / NP, p = i % NP;
+        if constexpr (p == 0) fetch(std::integral_constant<int, f + 2>{});
+        if constexpr (f < 2 * KS) {
+          constexpr int hf = f / KS, s = f % KS;
+          if constexpr (s == 0 && p == 0)
+            st[hf] = mfma_scaled(fr[f % 3], qf[p][s], f32x16{}, sk[hf], qs[p]);
+          else
+            st[hf] = mfma_scaled(fr[f % 3], qf[p][s], st[hf], sk[hf], qs[p]);
+        } else {
+          constexpr int dt = f - 2 * KS;
+          O[dt] = mfma_scaled(fr[f % 3], pf[p], O[dt], sv, ps[p]);
+        }
+        constexpr int c0 = i * SL / MF, c1 = (i + 1) * SL / MF;
+        static_for<c1 - c0>([&](auto x_c) {
+          slice(std::integral_constant<int, c0 + decltype(x_c)::value>{});
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      // (the products above stay here, not where their results are used)
+      asm volatile("" ::"a"(st[0]), "a"(st[1]));
+      l = l * fac + add_xor32(sum[0]) * pow2i(e[0] - 8) + add_xor32(sum[1]) * pow2i(e[1] - 8);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        pf[p] = pc[p];
+        ps[p] = pcs[p];
+      }
+      if (__ballot(moved) != 0) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) scale_acc(O[i], fac);
+      }
+    }
+    // the last tile's output
+    wait_vm(0);
+    tile_barrier();
+    if (count > 0) {
+      const uint8_t* vs = smem + (4 + (count - 1 & 3)) * S::tile;
+      const int sv = (hi ? ring_meta[1][1] : ring_meta[1][0]) >> 16 & 0xff;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const i32x8 f = read_v(vs, dt);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[p], O[dt], sv, ps[p]);
+      }
     }
   } else {
     uint8_t* mine = smem + wave * S::slot;
+    const uint32_t mine_at = lds0 + wave * S::slot;
     auto issue = [&](int kv, int k) {
 #pragma unroll
-      for (int i = 0; i < S::LT; ++i) load1(kv, k, i, mine + kv * S::tile);
+      for (int i = 0; i < S::LT; ++i) {
+        const int at = 2 * (k & 31) + i * S::RPI / 32;       // the lane that describes the half
+        load1(kv, __builtin_amdgcn_readlane(pg, at), __builtin_amdgcn_readlane(meta, at),
+              (first + stride * k) * kKeys, i, mine_at + kv * S::tile);
+      }
     };
-    if (count > 0) {
-      describe(0);
-      issue(0, 0);
+    if (has_suffix) suffix_load(mine + S::tile, 0);   // where V goes
+    describe(0, first_page);
+    if (count > 0) issue(0, 0);
+    if (has_suffix) {
+      if (count > 0) suffix(mine + S::tile, S::LT);
+      else suffix(mine + S::tile, 0);
     }
-    if (a.Tk > 0 && split == 0 && wave == 0) suffix(mine + S::tile);   // where V goes
     if (count > 0) issue(1, 0);
     split_q();
     for (int k = 0; k < count; ++k) {
@@ -666,7 +880,7 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
       // the next tile's K goes where this one's was, once its reads are done
       // (the products above have taken them)
       if (k + 1 < count) {
-        if ((k + 1 & 31) == 0) describe((k + 1) >> 5);
+        if ((k + 1 & 31) == 0) describe((k + 1) >> 5, page_at((k + 1) >> 5));
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
         __builtin_amdgcn_sched_barrier(0);
         issue(0, k + 1);
@@ -681,7 +895,35 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
 
   // ---- the rows: O^T through LDS, joined over the waves that hold the same
   // rows, then stored whole (or as a partial result).  A wave takes 256 / D rows
-  // at a time, 4 elements a lane, and 8 such steps' gates at once.
+  // at a time, 4 elements a lane; the gates of 8 such steps are loaded while the
+  // 8 before them are stored.
+  constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
+  constexpr int STEPS = SHARED ? 32 / RPS : (32 / RPS + 3) / 4, BATCH = STEPS < 8 ? STEPS : 8;
+  const int sub = lane / LPR, d0 = lane % LPR * 4;
+  const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
+  const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
+  const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
+  auto first_row = [&](int s) { return (SHARED ? s : 4 * s + wave) * RPS; };
+  // the value of the row that this lane stores in step s
+  auto of_row = [&](int64_t v, int s) {
+    if constexpr (RPS == 1) {
+      const int i = first_row(s);
+      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, i) |
+                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32);
+    } else {
+      return of_lane(v, first_row(s) + sub);
+    }
+  };
+  const bool gated = a.gate != nullptr && a.splits == 1;
+  u32x2 gv[BATCH];
+  auto load_gates = [&](int s0) {
+#pragma unroll
+    for (int s = 0; s < BATCH; ++s) {
+      gv[s] = u32x2{};
+      if (gated) gv[s] = *(const u32x2*)((const T*)a.gate + of_row(gate_at, s0 + s) + d0);
+    }
+  };
+  load_gates(0);
   wait_vm(0);
   __syncthreads();
   float* ep = (float*)smem + wave * 32 * S::EpiLd;
@@ -691,38 +933,35 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
     for (int q4 = 0; q4 < 4; ++q4)
       *(f32x4*)(ep + col * S::EpiLd + 32 * dt + 8 * q4 + 4 * hi) =
           f32x4{O[dt][4 * q4], O[dt][4 * q4 + 1], O[dt][4 * q4 + 2], O[dt][4 * q4 + 3]};
+  if (spoilt) {   // values that are not finite to the rows that see them
+    const int64_t v_at = n * a.ssv_n + kh * a.ssv_h;
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) {
+      const T* vr = (const T*)a.sv + of_lane(v_at, i);
+      const int last = a.Tk - a.T + __shfl(t, i, 64);
+#pragma unroll 1
+      for (int e = lane; e < (last + 1) * D; e += 64) {
+        const float x = Elem<T>::to_f(vr[(int64_t)(e / D) * a.ssv_t + e % D]);
+        if (!(fabsf(x) < INFINITY)) ep[i * S::EpiLd + e % D] += x;
+      }
+    }
+  }
   if (hi == 0) {
     sm_m[wave][col] = m;
-    sm_l[wave][col] = l;
+    sm_l[wave][col] = SHARED && a.splits == 1 ? (l == 0.f ? 0.f : 1.f / l) : l;
   }
-  if (lane == 0) sm_spoilt[wave] = spoilt;
   __syncthreads();
-  constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
-  constexpr int STEPS = SHARED ? 32 / RPS : (32 / RPS + 3) / 4, AT_ONCE = STEPS < 8 ? STEPS : 8;
-  const int sub = lane / LPR, d0 = lane % LPR * 4;
-  const bool spoilt_rows = sm_spoilt[SHARED ? wave : 0];
-  const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
-  const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
-  auto of_lane = [](int64_t v, int from) {
-    return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
-                     (uint64_t)(uint32_t)__shfl((int)(v >> 32), from, 64) << 32);
-  };
-  const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
 #pragma unroll 1
-  for (int s0 = 0; s0 < STEPS; s0 += AT_ONCE) {
-    if ((SHARED ? s0 : 4 * s0 + wave) * RPS >= rows) break;
-    u32x2 gv[AT_ONCE];
-    int64_t at[AT_ONCE];
+  for (int s0 = 0; s0 < STEPS && first_row(s0) < rows; s0 += BATCH) {
+    u32x2 gate[BATCH];
 #pragma unroll
-    for (int s = 0; s < AT_ONCE; ++s) {
-      const int i = min((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub, 31);
-      at[s] = of_lane(out_at, i);
-      gv[s] = u32x2{};
-      if (a.gate) gv[s] = *(const u32x2*)((const T*)a.gate + of_lane(gate_at, i) + d0);
-    }
+    for (int s = 0; s < BATCH; ++s) gate[s] = gv[s];
+    if (s0 + BATCH < STEPS && first_row(s0 + BATCH) < rows) load_gates(s0 + BATCH);
 #pragma unroll
-    for (int s = 0; s < AT_ONCE; ++s) {
-      const int i = min((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub, 31);
+    for (int s = 0; s < BATCH; ++s) {
+      const int i = first_row(s0 + s) + sub;
+      const int64_t to = of_row(out_at, s0 + s);
+      if (first_row(s0 + s) >= rows) break;
       float o[4], ll, mm;
       if constexpr (SHARED) {
         mm = sm_m[wave][i];
@@ -744,28 +983,19 @@ __global__ __launch_bounds__(256, 1) void block_attn_kernel(BlockAttnArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
         }
+        if (a.splits == 1) ll = ll == 0.f ? 0.f : 1.f / ll;
       }
-      if ((SHARED ? s0 + s : 4 * (s0 + s) + wave) * RPS + sub >= rows) continue;
-      const int rr = row0 + i;
-      if (spoilt_rows) {
-        const int t2 = rr % a.T, w2 = rr / a.T / G;
-        const T* vr = (const T*)a.sv + ((int64_t)b * a.W + w2) * a.ssv_n + kh * a.ssv_h + d0;
-        for (int j = 0; j <= a.Tk - a.T + t2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + e]);
-            if (!(fabsf(x) < INFINITY)) o[e] += x;
+      if (i < rows) {
+        if (a.splits > 1) {
+          const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + i;
+          *(f32x4*)(a.part_o + at * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
+          if (d0 == 0) {
+            a.part_ml[2 * at] = mm;
+            a.part_ml[2 * at + 1] = ll;
           }
-      }
-      if (a.splits > 1) {
-        const int64_t to = ((int64_t)split * a.B * a.HK + bk) * a.R + rr;
-        *(f32x4*)(a.part_o + to * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
-        if (d0 == 0) {
-          a.part_ml[2 * to] = mm;
-          a.part_ml[2 * to + 1] = ll;
+        } else {
+          store_row4<T>((T*)a.out + to + d0, o, ll, gated, gate[s]);
         }
-      } else {
-        store_row4<T>((T*)a.out + at[s] + d0, o, ll, a.gate != nullptr, gv[s]);
       }
     }
   }
@@ -801,28 +1031,39 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
   }
-  store_row4<T>((T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + d0, o, ll, a.gate != nullptr,
-                gate);
+  store_row4<T>((T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + d0, o,
+                ll == 0.f ? 0.f : 1.f / ll, a.gate != nullptr, gate);
 }
 
 // The launch of a call: whether the waves share tiles, and the ranges the
-// prefix is split into.
+// prefix is split into.  More ranges fill the GPU and shorten each workgroup's
+// walk, but every workgroup starts and ends at a cost of about kStart tiles, and
+// the second kernel costs about kJoin of them; the cheapest number of ranges
+// by that count is taken.
 struct Plan {
   bool shared;
   int nqblk, splits;
 };
+constexpr int kStart = 6, kJoin = 6;
 
-Plan plan_of(int B, int HK, int R, int keys) {
+Plan plan_of(int B, int HK, int R, int D, int keys) {
   Plan p;
   p.shared = R > 64;
   p.nqblk = (int)kad_cdiv(R, p.shared ? 128 : 32);
   const int64_t blocks = (int64_t)B * HK * p.nqblk;
-  const int tiles = (int)kad_cdiv(keys, kKeys);
-  const int least = 4;
-  int64_t s = kad_cdiv(256, blocks);
-  const int64_t cap = kad_cdiv(tiles, least);
-  if (s > cap) s = cap;
-  p.splits = (int)(s < 1 ? 1 : s);
+  const int64_t slots = D == 256 ? 256 : 512;      // workgroups that run at once
+  const int step = p.shared ? 1 : 4;               // tiles a workgroup takes side by side
+  const int64_t tiles = kad_cdiv(keys, kKeys);
+  p.splits = 1;
+  int64_t best = INT64_MAX;
+  for (int s = 1; s <= 64 && (s == 1 || tiles >= (int64_t)s * step); ++s) {
+    const int64_t walk = kad_cdiv(kad_cdiv(tiles, s), step) + kStart;
+    const int64_t cost = kad_cdiv(blocks * s, slots) * walk + (s > 1 ? kJoin : 0);
+    if (cost < best) {
+      best = cost;
+      p.splits = s;
+    }
+  }
   return p;
 }
 
@@ -868,10 +1109,10 @@ extern "C" int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, i
   KAD_REQUIRE(bytes, "null pointer argument");
   KAD_REQUIRE(B > 0 && W > 0 && T > 0 && H > 0 && HK > 0 && H % HK == 0 && width > 0,
               "empty dimensions");
-  KAD_REQUIRE((int64_t)width * block <= 0x7fffffff - 256, "tables of %d columns", width);
+  KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
   const int64_t R = (int64_t)W * T * (H / HK);
   KAD_REQUIRE(R <= 0x7fffffff - 256, "%lld rows for a KV head", (long long)R);
-  const Plan p = plan_of(B, HK, (int)R, width * block);
+  const Plan p = plan_of(B, HK, (int)R, D, width * block);
   *bytes = p.splits > 1 ? (int64_t)p.splits * B * HK * R * (D + 2) * 4 : 0;
   return KAD_OK;
 }
@@ -911,7 +1152,7 @@ extern "C" int kad_block_prefix_attention(
   KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "a workspace of %lld bytes is needed", (long long)need);
   const int R = W * T * (H / HK);
-  const Plan p = plan_of(B, HK, R, width * block);
+  const Plan p = plan_of(B, HK, R, D, width * block);
   KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff &&
                   kad_cdiv((int64_t)B * HK * R, 4) <= 0x7fffffff,
               "too many rows for a launch");

@@ -17,9 +17,8 @@ the reference, whose prefix stays in the model's type
 (src/kadllm/adapters/qwen3_5.py:106-133).
 """
 
-import contextlib
 import ctypes
-import math
+import functools
 from typing import NamedTuple
 
 import torch
@@ -28,6 +27,7 @@ from . import _lib
 
 BLOCK_SIZES = (32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
+MAX_LENGTH = 2**30          # tokens of a request
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -56,28 +56,36 @@ class PrefixBlocks(NamedTuple):
         return cls(*codes, *scales)
 
 
-def _on_device(t):
-    """A context in which ``t``'s device is the current one."""
-    if t.get_device() == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(device, name, *args):
+    """An entry point on the current stream of ``device`` (an index), which
+    need not be the current device."""
+    if device == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_of_index(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream_of_index(device))
 
 
-def _check_devices(first, *others):
+def _device_of(first, *others):
+    """The index of the ROCm device that all the tensors are on."""
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise ValueError("all tensors must be on the same device")
-    if not first.is_cuda:
+    if index < 0 or not first.is_cuda:
         raise RuntimeError(
             "kadllm_amd operators run on ROCm devices only; move tensors to the GPU")
+    return index
 
 
-def _check_int32(name, t, shape):
-    if t.dtype != torch.int32:
+def _check_int32(name, t, ndim, rows=None):
+    """t is int32 with ``ndim`` dimensions, the first of ``rows``; contiguous."""
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32")
-    if t.ndim != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
-        want = ", ".join("*" if w is None else str(w) for w in shape)
-        raise ValueError(f"{name} must have shape [{want}]")
+    if t.ndim != ndim or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} must have {ndim} dimension(s)"
+                         + ("" if rows is None else f", the first of {rows}"))
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_blocks(blocks):
@@ -85,21 +93,23 @@ def _check_blocks(blocks):
     if not isinstance(blocks, PrefixBlocks):
         raise TypeError("blocks must be a PrefixBlocks")
     k, v, k_scale, v_scale = blocks
-    if k.dtype != _CODES or v.dtype != _CODES:
+    if k.dtype is not _CODES or v.dtype is not _CODES:
         raise TypeError("the codes of a prefix cache are torch.float8_e4m3fn")
-    if k_scale.dtype != _SCALES or v_scale.dtype != _SCALES:
+    if k_scale.dtype is not _SCALES or v_scale.dtype is not _SCALES:
         raise TypeError("the scales of a prefix cache are torch.float8_e8m0fnu")
-    if k.ndim != 4 or v.shape != k.shape or min(k.shape) < 1:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or 0 in shape:
         raise ValueError("codes must be [pages, HK, block_size, D]")
-    if k_scale.shape != k.shape[:2] or v_scale.shape != k.shape[:2]:
+    if k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
         raise ValueError("scales must be [pages, HK]")
-    if k.shape[2] not in BLOCK_SIZES:
+    if shape[2] not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
-    if k.shape[3] not in HEAD_DIMS:
+    if shape[3] not in HEAD_DIMS:
         raise ValueError(f"head_dim must be one of {HEAD_DIMS}")
-    if not all(t.is_contiguous() for t in blocks):
+    if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
         raise ValueError("the tensors of a prefix cache must be contiguous")
-    return k.shape
+    return shape
 
 
 def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=None, tables=None):
@@ -118,31 +128,27 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
     if not isinstance(block_size, int) or block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
     if not isinstance(max_length, int) or isinstance(max_length, bool) or \
-            not 0 < max_length < 2**31 - 256:
-        raise ValueError("max_length must be a positive integer below 2**31 - 256")
-    _check_int32("lengths", lengths, (None,))
-    _check_int32("free_blocks", free_blocks, (None,))
+            not 0 < max_length <= MAX_LENGTH:
+        raise ValueError(f"max_length must be a positive integer of at most {MAX_LENGTH}")
+    lengths = _check_int32("lengths", lengths, 1)
+    free_blocks = _check_int32("free_blocks", free_blocks, 1)
     B = lengths.shape[0]
     if B < 1:
         raise ValueError("lengths must not be empty")
     if starts is not None:
-        _check_int32("starts", starts, (B,))
+        starts = _check_int32("starts", starts, 1, B)
     if tables is not None:
         if starts is None:
             raise ValueError("earlier tables need the tokens held (starts)")
-        _check_int32("tables", tables, (B, None))
-    _check_devices(lengths, free_blocks, starts, tables)
-    lengths, free_blocks = lengths.contiguous(), free_blocks.contiguous()
-    starts = None if starts is None else starts.contiguous()
-    tables = None if tables is None else tables.contiguous()
+        tables = _check_int32("tables", tables, 2, B)
+    device = _device_of(lengths, free_blocks, starts, tables)
     width = -(-max_length // block_size)
-    out = torch.empty(B, width, dtype=torch.int32, device=lengths.device)
+    out = torch.empty((B, width), dtype=torch.int32, device=lengths.device)
     used = torch.empty(1, dtype=torch.int32, device=lengths.device)
-    with _on_device(lengths):
-        _lib.call("kad_prefix_block_tables", _lib.ptr(lengths), _lib.ptr(starts),
-                  _lib.ptr(tables), 0 if tables is None else tables.shape[1],
-                  _lib.ptr(free_blocks), free_blocks.shape[0], _lib.ptr(out), width,
-                  _lib.ptr(used), B, block_size, max_length, _lib.stream_of(lengths))
+    _launch(device, "kad_prefix_block_tables", lengths.data_ptr(), _lib.ptr(starts),
+            _lib.ptr(tables), 0 if tables is None else tables.shape[1], free_blocks.data_ptr(),
+            free_blocks.shape[0], out.data_ptr(), width, used.data_ptr(), B, block_size,
+            max_length)
     return out, used
 
 
@@ -164,31 +170,29 @@ def write_prefix_blocks(blocks, k, v, tables, lengths, *, starts=None):
     must not write to the same page.  Returns ``blocks``.
     """
     pages, HK, block, D = _check_blocks(blocks)
-    if k.ndim != 4 or v.shape != k.shape:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("k and v must be [B, N, HK, D]")
-    if k.dtype != v.dtype:
+    if k.dtype is not v.dtype:
         raise ValueError("k and v must have the same dtype")
     if k.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError("k and v must be bf16, fp16 or fp32")
-    B, N = k.shape[:2]
-    if min(B, N) < 1 or k.shape[2:] != (HK, D):
+    B, N, heads, dim = shape
+    if 0 in shape or heads != HK or dim != D:
         raise ValueError("k and v do not fit the cache's heads")
-    _check_int32("tables", tables, (B, None))
-    _check_int32("lengths", lengths, (B,))
+    tables = _check_int32("tables", tables, 2, B)
+    lengths = _check_int32("lengths", lengths, 1, B)
     if starts is not None:
-        _check_int32("starts", starts, (B,))
+        starts = _check_int32("starts", starts, 1, B)
     if tables.shape[1] < 1:
         raise ValueError("tables must have columns")
-    _check_devices(k, v, tables, lengths, starts, *blocks)
+    device = _device_of(k, v, tables, lengths, starts, *blocks)
     k = k if k.stride(3) == 1 else k.contiguous()
     v = v if v.stride(3) == 1 else v.contiguous()
-    tables, lengths = tables.contiguous(), lengths.contiguous()
-    starts = None if starts is None else starts.contiguous()
-    with _on_device(k):
-        _lib.call("kad_write_prefix_blocks", _lib.ptr(k), *k.stride()[:3], _lib.ptr(v),
-                  *v.stride()[:3], _lib.dtype_code(k.dtype), _lib.ptr(tables), tables.shape[1],
-                  _lib.ptr(lengths), _lib.ptr(starts), *map(_lib.ptr, blocks), pages, B, N, HK, D,
-                  block, _lib.stream_of(k))
+    _launch(device, "kad_write_prefix_blocks", k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+            *v.stride()[:3], _lib.dtype_code(k.dtype), tables.data_ptr(), tables.shape[1],
+            lengths.data_ptr(), _lib.ptr(starts), *[x.data_ptr() for x in blocks], pages, B, N,
+            HK, D, block)
     return blocks
 
 
@@ -209,49 +213,69 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
 
     _width(beam_width)
     pages, HK, block, D = _check_blocks(blocks)
-    if q.ndim != 4 or q.shape[3] != D:
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != D:
         raise ValueError("q must be [B*W, T, H, D] with the cache's head dim")
-    BW, T, H, _ = q.shape
-    if min(BW, T, H) < 1 or BW % beam_width or H % HK:
+    BW, T, H, _ = shape
+    if 0 in shape or BW % beam_width or H % HK:
         raise ValueError("empty dimensions or incompatible beam/head counts")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    dtype = q.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise TypeError("queries over the 8-bit cache must be bf16 or fp16")
     B = BW // beam_width
-    _check_int32("tables", tables, (B, None))
-    _check_int32("lengths", lengths, (B,))
-    if tables.shape[1] < 1:
-        raise ValueError("tables must have columns")
+    tables = _check_int32("tables", tables, 2, B)
+    lengths = _check_int32("lengths", lengths, 1, B)
+    if not 0 < tables.shape[1] * block <= MAX_LENGTH:
+        raise ValueError(f"tables must have columns, for at most {MAX_LENGTH} tokens")
     if (suffix_k is None) != (suffix_v is None):
         raise ValueError("give both suffix_k and suffix_v or neither")
-    Tk = 0
     if suffix_k is not None:
-        Tk = suffix_k.shape[1] if suffix_k.ndim == 4 else -1
-        if Tk < T or suffix_k.shape != (BW, Tk, HK, D) or suffix_v.shape != suffix_k.shape:
+        s = suffix_k.shape
+        if len(s) != 4 or s[0] != BW or s[1] < T or s[2] != HK or s[3] != D or \
+                suffix_v.shape != s:
             raise ValueError("suffix_k and suffix_v must be [B*W, Tk, HK, D] with Tk >= T")
-        if suffix_k.dtype != q.dtype or suffix_v.dtype != q.dtype:
+        if suffix_k.dtype is not dtype or suffix_v.dtype is not dtype:
             raise ValueError("attention inputs must have the same dtype")
-    if gate is not None and (gate.shape != (BW, T, H * D) or gate.dtype != q.dtype):
+    if gate is not None and (gate.shape != (BW, T, H * D) or gate.dtype is not dtype):
         raise ValueError("gate must be [B*W, T, H*D] in the query dtype")
-    given = [t for t in (q, suffix_k, suffix_v, gate) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    if torch.is_grad_enabled() and (
+            q.requires_grad or (suffix_k is not None and (suffix_k.requires_grad
+                                                          or suffix_v.requires_grad))
+            or (gate is not None and gate.requires_grad)):
         raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
-    _check_devices(q, tables, lengths, suffix_k, suffix_v, gate, *blocks)
-    scale = 1 / math.sqrt(D) if scale is None else scale
+    _device_of(q, tables, lengths, suffix_k, suffix_v, gate, *blocks)
     gate_strides = None
     if gate is not None:
         gate = _rows(gate, 4)
         gate_strides = (gate.stride(0), gate.stride(1), D)
-    return _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale,
-                            gate, gate_strides)
+    return _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
+                            D ** -0.5 if scale is None else scale, gate, gate_strides)
 
 
 def _rows(t, elements):
-    """t, or a copy whose rows start at multiples of ``elements`` elements."""
-    strides = t.stride()
-    if strides[-1] == 1 and not any(s % elements for s in strides[:-1]) and \
-            t.data_ptr() % (2 * elements) == 0:
+    """t, or a copy whose rows start at multiples of ``elements`` (a power of
+    two) 16-bit elements."""
+    *outer, inner = t.stride()
+    bits = 0
+    for s in outer:
+        bits |= s
+    if inner == 1 and not bits % elements and not t.data_ptr() % (2 * elements):
         return t
     return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes):
+    need = ctypes.c_int64(0)
+    _lib.call("kad_block_prefix_attention_workspace_bytes", *sizes, ctypes.byref(need))
+    return need.value
+
+
+_NONE = (None, 0, 0, 0)
+
+
+def _strided(t):
+    return (t.data_ptr(), *t.stride()[:3])
 
 
 def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale, gate=None,
@@ -261,27 +285,19 @@ def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
     (beam, token, head)."""
     BW, T, H, D = q.shape
     pages, HK, block, _ = blocks.k.shape
+    B, width = BW // beam_width, tables.shape[1]
     q = _rows(q, 8)
-    tables, lengths = tables.contiguous(), lengths.contiguous()
-    none = (None, 0, 0, 0)
-    sk = sv = g = none
-    Tk = 0
+    Tk, sk, sv, g = 0, _NONE, _NONE, _NONE
     if suffix_k is not None:
         suffix_k, suffix_v = _rows(suffix_k, 8), _rows(suffix_v, 8)
-        Tk = suffix_k.shape[1]
-        sk = (_lib.ptr(suffix_k), *suffix_k.stride()[:3])
-        sv = (_lib.ptr(suffix_v), *suffix_v.stride()[:3])
+        Tk, sk, sv = suffix_k.shape[1], _strided(suffix_k), _strided(suffix_v)
     if gate is not None:
-        g = (_lib.ptr(gate), *gate_strides)
-    out = torch.empty(BW, T, H, D, dtype=q.dtype, device=q.device)
-    need = ctypes.c_int64(0)
-    _lib.call("kad_block_prefix_attention_workspace_bytes", BW // beam_width, beam_width, T, H, HK,
-              D, tables.shape[1], block, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    with _on_device(q):
-        _lib.call("kad_block_prefix_attention", _lib.ptr(q), *q.stride()[:3],
-                  *map(_lib.ptr, blocks), pages, _lib.ptr(tables), tables.shape[1],
-                  _lib.ptr(lengths), *sk, *sv, *g, _lib.ptr(out), *out.stride()[:3],
-                  _lib.ptr(ws), need.value, BW // beam_width, beam_width, T, Tk, H, HK, D, block,
-                  _lib.dtype_code(q.dtype), float(scale), _lib.stream_of(q))
+        g = (gate.data_ptr(), *gate_strides)
+    out = torch.empty((BW, T, H, D), dtype=q.dtype, device=q.device)
+    need = _workspace_bytes(B, beam_width, T, H, HK, D, width, block)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch(q.get_device(), "kad_block_prefix_attention", *_strided(q),
+            *[x.data_ptr() for x in blocks], pages, tables.data_ptr(), width, lengths.data_ptr(),
+            *sk, *sv, *g, out.data_ptr(), T * H * D, H * D, D, _lib.ptr(ws), need, B, beam_width,
+            T, Tk, H, HK, D, block, _lib.DTYPE_CODES[q.dtype], float(scale))
     return out
