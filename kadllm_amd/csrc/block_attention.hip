@@ -73,20 +73,25 @@ __device__ __forceinline__ f32x16 mfma_scaled(i32x8 a, i32x8 b, f32x16 c, int sa
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, sa, 0, sb);
 }
 
-// 4 floats to a dword of e4m3 codes, and what they leave, times 16
+// 4 floats to a dword of e4m3 codes, and what they leave
 __device__ __forceinline__ int piece4(const float* y, float* rest) {
   int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   c = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
   const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-  rest[0] = (y[0] - lo[0]) * 16.f;
-  rest[1] = (y[1] - lo[1]) * 16.f;
-  rest[2] = (y[2] - hi[0]) * 16.f;
-  rest[3] = (y[3] - hi[1]) * 16.f;
+  rest[0] = y[0] - lo[0];
+  rest[1] = y[1] - lo[1];
+  rest[2] = y[2] - hi[0];
+  rest[3] = y[3] - hi[1];
   return c;
 }
 __device__ __forceinline__ float pow2i(int e) {  // 2^e, -126 <= e <= 127
   return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// the largest of three, NaN where one is (fmaxf would first quiet each operand)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
 template <typename T> struct Pieces;
@@ -159,34 +164,9 @@ struct Shape {
   }
 };
 
-// the V^T fragments of two 32-wide output tiles: for each, 4 transpose reads of
-// 8 keys (within 16 lanes, lane i receives byte i % 8 of the 8-byte pieces that
-// lanes 2e + i / 8 address, e < 8), waited for inside
-template <int D>
-__device__ __forceinline__ void read_v2(uint32_t p0, uint32_t p1, i32x8& f0, i32x8& f1) {
-  u32x2 a0, a1, a2, a3, b0, b1, b2, b3;
-  asm volatile(
-      "ds_read_b64_tr_b8 %0, %8\n\t"
-      "ds_read_b64_tr_b8 %1, %8 offset:%10\n\t"
-      "ds_read_b64_tr_b8 %2, %8 offset:%11\n\t"
-      "ds_read_b64_tr_b8 %3, %8 offset:%12\n\t"
-      "ds_read_b64_tr_b8 %4, %9\n\t"
-      "ds_read_b64_tr_b8 %5, %9 offset:%10\n\t"
-      "ds_read_b64_tr_b8 %6, %9 offset:%11\n\t"
-      "ds_read_b64_tr_b8 %7, %9 offset:%12\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(a0), "=&v"(a1), "=&v"(a2), "=&v"(a3), "=&v"(b0), "=&v"(b1), "=&v"(b2), "=&v"(b3)
-      : "v"(p0), "v"(p1), "i"(16 * D), "i"(32 * D), "i"(48 * D)
-      : "memory");
-  f0 = i32x8{(int)a0[0], (int)a0[1], (int)a1[0], (int)a1[1],
-             (int)a2[0], (int)a2[1], (int)a3[0], (int)a3[1]};
-  f1 = i32x8{(int)b0[0], (int)b0[1], (int)b1[0], (int)b1[1],
-             (int)b2[0], (int)b2[1], (int)b3[0], (int)b3[1]};
-}
-
-// the same for two output tiles of 16-bit rows (the suffix): 16 keys, 2 reads of
-// 4 keys each (lane i of 16 receives element i % 4 of the 8-byte pieces that
-// lanes 4e + i / 4 address, e < 4)
+// V^T fragments of two 32-wide output tiles of 16-bit rows (the suffix): for each,
+// 16 keys, 2 transpose reads of 4 keys (lane i of 16 receives element i % 4 of
+// the 8-byte pieces that lanes 4e + i / 4 address, e < 4), waited for inside
 template <int D>
 __device__ __forceinline__ void read_wide2(uint32_t p0, uint32_t p1, u32x4& f0, u32x4& f1) {
   u32x2 a0, a1, b0, b1;
@@ -220,47 +200,21 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// o *= f on accumulation registers.  Left to the compiler, this rare branch would
-// keep O in ordinary registers and copy all of it to and fro around the products
-// of every tile.  (The first nops cover a product still writing o, the last ones
-// the next product's read.)
-__device__ __forceinline__ void scale_acc(f32x16& o, float f) {
-#pragma unroll
-  for (int j = 0; j < 16; j += 4) {
-    float x0 = o[j], x1 = o[j + 1], x2 = o[j + 2], x3 = o[j + 3], t0, t1, t2, t3;
-    asm volatile(
-        "s_nop 15\n\ts_nop 15\n\t"
-        "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
-        "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
-        "v_mul_f32 %4, %4, %8\n\tv_mul_f32 %5, %5, %8\n\t"
-        "v_mul_f32 %6, %6, %8\n\tv_mul_f32 %7, %7, %8\n\ts_nop 1\n\t"
-        "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
-        "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 4"
-        : "+a"(x0), "+a"(x1), "+a"(x2), "+a"(x3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
-        : "v"(f));
-    o[j] = x0;
-    o[j + 1] = x1;
-    o[j + 2] = x2;
-    o[j + 3] = x3;
-  }
-}
-
 // 16 bytes a lane from base + off (zeros from nbytes on) into LDS at lds + 16 *
 // lane; base, nbytes and lds wave-uniform.  In assembly so that the compiler does
 // not make the next transpose read wait for every such load in flight: waits are
 // the callers' (wait_vm).  (No register is written; the nops cover scalar
 // operands that a vector instruction has just written, and m0.)
-__device__ __forceinline__ void load_lds16(const uint8_t* base, int nbytes, uint32_t off,
-                                           uint32_t lds) {
-  const uint64_t p = (uint64_t)(uintptr_t)base;
-  const u32x4 rsrc = {(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)nbytes, 0x00020000u};
+// AT goes to both addresses (as the instruction's offset field does).
+template <int AT>
+__device__ __forceinline__ void load_lds16(u32x4 rsrc, uint32_t off, uint32_t lds) {
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
       "s_nop 4\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      "buffer_load_dwordx4 %0, %1, 0 offen offset:%3 lds"
       :
-      : "v"(off), "s"(rsrc), "s"(lds)
-      : "memory", "m0");
+      : "v"(off), "s"(rsrc), "s"(lds), "n"(AT)
+      : "memory");
 }
 
 // the same from an address of each lane's own
@@ -271,7 +225,7 @@ __device__ __forceinline__ void load_lds16(const void* src, uint32_t lds) {
       "global_load_lds_dwordx4 %0, off"
       :
       : "v"(src), "s"(lds)
-      : "memory", "m0");
+      : "memory");
 }
 
 // 4 elements of an output row: times inv, gated, rounded once (the gate's
@@ -302,19 +256,24 @@ __device__ __forceinline__ void store_row4(T* out, const float* o, float inv, bo
 // in its registers.  S^T = K Q^T gives a lane the scores of one row (16 of a
 // half tile's 32 keys, the other 16 in lane l ^ 32), and the bytes of its
 // weights are the second product's operand O^T += V^T P^T as they stand.
-//   SHARED: the waves hold 128 rows and walk the same tiles, which arrive in a
-//     ring of 4 LDS stages, three tiles ahead of their use.
+//   SHARED: the waves hold 128 rows and walk the same tiles, which arrive in
+//     rings of 4 K and 4 V tiles in LDS, three steps ahead of their use.
 //   otherwise: the waves hold the same 32 rows and take every fourth tile, each
 //     through an LDS slot of its own, K refilled while V is used and V refilled
 //     while the next K is, so no wave waits for another; their states are
 //     joined at the end.
+// Weights are 2^(s - m) for a reference m, the maximum of the first keys that the
+// row sees.  Scores above it need no rescaling, because the weights of 32 keys
+// carry an exponent of their own; only when one lies more than 2^60 above (2^14
+// among fp16 suffix keys) is the walk done again, with the row's true maximum.
 template <typename T, int D, bool SHARED>
-__global__ __launch_bounds__(256, D == 256 || (SHARED && D == 128) ? 1 : 2) void
+__global__ __launch_bounds__(256, D == 256 || SHARED ? 1 : 2) void
 block_attn_kernel(BlockAttnArgs a) {
   using S = Shape<D>;
   constexpr int NP = Pieces<T>::n, KS = S::KS, DT = S::DT;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   __shared__ float sm_m[4][32], sm_l[4][32];
+  __shared__ int sm_over[4];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -324,13 +283,6 @@ block_attn_kernel(BlockAttnArgs a) {
   const int bk = lid / a.nqblk / a.splits;
   const int kh = bk % a.HK, b = bk / a.HK;
   const int G = a.H / a.HK;
-
-  // this lane's row (rows past the end repeat the last one and are not stored)
-  const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
-  const int r = min(row0 + col, a.R - 1);
-  const int t = r % a.T, g = r / a.T % G, w = r / a.T / G;
-  const int64_t n = (int64_t)b * a.W + w;
-  const int h = kh * G + g;
 
   // ---- this wave's tiles of the prefix: first + stride * k, k < count.  (With one
   // range the first pages do not wait for the length.)
@@ -342,9 +294,10 @@ block_attn_kernel(BlockAttnArgs a) {
   const int count = __builtin_amdgcn_readfirstlane(
       SHARED ? end - begin : max((end - first + stride - 1) / stride, 0));
 
-  // Pages: lane i of a chunk of 32 tiles describes half tile i: its page
-  // (-1: none) and keys held | K's scale byte << 8 | V's << 16
-  int pg = -1, meta = 0;
+  // Pages: lane i of a chunk of 32 tiles describes half tile i: the offset of its
+  // codes, and keys held (0: no page) | K's scale byte << 8 | V's << 16
+  uint32_t code_lo = 0, code_hi = 0;
+  int meta = 0;
   auto half_at = [&](int chunk) {
     return (first + stride * (32 * chunk + (lane >> 1))) * kKeys + (lane & 1) * 32;
   };
@@ -353,27 +306,89 @@ block_attn_kernel(BlockAttnArgs a) {
   };
   auto describe = [&](int chunk, int id) {
     const int pos = half_at(chunk);
-    pg = -1;
     meta = 127 << 8 | 127 << 16;
     if (32 * chunk + (lane >> 1) < count && pos < len && id >= 0 && id < a.pages) {
       const int64_t ph = (int64_t)id * a.HK + kh;
-      pg = id;
+      const int64_t code = ((ph << a.lblock) + (pos & ((1 << a.lblock) - 1))) * D;
+      code_lo = (uint32_t)code;
+      code_hi = (uint32_t)(code >> 32);
       meta = min(len - pos, 32) | (int)a.ksc[ph] << 8 | (int)a.vsc[ph] << 16;
     }
   };
-  const int first_page = page_at(0);
+  int first_page = page_at(0);
 
-  // ---- Q: the row's elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7 as they
-  // are, and in e4m3 pieces against the row's power of two
+  // ---- this lane's row (rows past the end repeat the last one and are not stored)
+  const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
+  const int r = min(row0 + col, a.R - 1);
+  const int rt = r / a.T, t = r - rt * a.T, w = rt / G, g = rt - w * G;
+  const int64_t n = (int64_t)b * a.W + w;
+  const int h = kh * G + g;
   const T* const kind = nullptr;
-  u32x4 qr[4 * KS];
-  {
+
+  // ---- loads of a tile.  Instruction i of a K or V tile brings keys i * RPI +
+  // lane / CPR; at place lane % CPR of a key goes the chunk that the swizzle puts
+  // there.  Keys past those held arrive as zeros.
+  constexpr int IPH = S::LT / 2;                 // instructions per half tile
+  const int d_row = lane / S::CPR, d_pc = lane % S::CPR;
+  auto source = [&](const uint8_t* codes, uint32_t lo, uint32_t hi32, int held) {
+    const uint64_t p = (uint64_t)(uintptr_t)codes + ((uint64_t)hi32 << 32 | lo);
+    return u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)held * D, 0x00020000u};
+  };
+  // (the offset field adds (i % 4) KB to the source and the destination)
+  auto off_of = [&](int kv, int i) {
+    const int row = i * S::RPI + d_row;
+    return (uint32_t)((row & 31) * D - i % 4 * 1024 +
+                      (d_pc ^ (kv ? S::swv(row) : S::swk(row))) * 16);
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
+
+  // LDS offsets of the fragments
+  uint32_t k_off[KS][2];   // K: key col of a half, chunks 4 s + hi and 4 s + 2 + hi
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      k_off[s][c] = col * D + ((4 * s + 2 * c + hi) ^ S::swk(col)) * 16;
+  // V: key 8 (e / 4) + 4 hi + e % 4, e = (lane % 16) / 2; d = 32 dt + 16 (lane / 16 % 2) +
+  // 8 (lane % 2)
+  const int v_e = (lane & 15) >> 1;
+  const int v_row = 8 * (v_e >> 2) + 4 * hi + (v_e & 3);
+  uint32_t v_off[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    v_off[dt] = v_row * D + (lane & 1) * 8 + (((2 * dt + (lane >> 4 & 1)) ^ S::swv(v_row)) * 16);
+  auto read_k = [&](const uint8_t* ks, int hf, int s) {
+    const i32x4 x = *(const i32x4*)(ks + k_off[s][0] + hf * 32 * D);
+    const i32x4 y = *(const i32x4*)(ks + k_off[s][1] + hf * 32 * D);
+    return i32x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+  // 4 transpose reads of 8 keys (within 16 lanes, lane i receives byte i % 8 of
+  // the 8-byte pieces that lanes 2e + i / 8 address, e < 8)
+  auto read_v = [&](const uint8_t* vs, int dt) {
+    typedef __attribute__((address_space(3))) i32x2* piece_t;
+    const uint32_t at = (uint32_t)(uintptr_t)(lds_t*)vs + v_off[dt];
+    i32x8 f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((piece_t)(at + 16 * c * D));
+      f[2 * c] = x[0];
+      f[2 * c + 1] = x[1];
+    }
+    return f;
+  };
+
+  // ---- the row's state, over the walk
+  float m = -INFINITY, m_true, l;
+  bool over, spoilt = false;
+  f32x16 O[DT];
+  u32x4 qr[4 * KS];        // q: elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7
+  i32x8 qf[NP][KS];        // q in e4m3 pieces against the row's power of two
+  int qs[NP];
+  auto load_q = [&]() {
     const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h + 16 * hi;
 #pragma unroll
     for (int c = 0; c < 4 * KS; ++c) qr[c] = *(const u32x4*)(qrow + 32 * (c >> 1) + 8 * (c & 1));
-  }
-  i32x8 qf[NP][KS];
-  int qs[NP];
+  };
   auto split_q = [&]() {
     float amax = 0.f;
 #pragma unroll
@@ -396,25 +411,13 @@ block_attn_kernel(BlockAttnArgs a) {
       for (int p = 0; p < NP; ++p) {
         qf[p][c >> 2][2 * (c & 3)] = piece4(x, x);
         qf[p][c >> 2][2 * (c & 3) + 1] = piece4(x + 4, x + 4);
+        if (p + 1 < NP)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= 16.f;
       }
     }
 #pragma unroll
     for (int p = 0; p < NP; ++p) qs[p] = E - 4 * p + 127;
-  };
-
-  // ---- softmax state: weights are 2^(s - m) for a reference m that moves only
-  // when a score exceeds it by 2^kMaxUp
-  float m = -INFINITY, l = 0.f;
-  f32x16 O[DT];
-#pragma unroll
-  for (int i = 0; i < DT; ++i) O[i] = f32x16{};
-  auto raise = [&](float top, float slack) {   // m up to the row's `top` where that is far above
-    const float to = top > m + slack ? top : m;
-    const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
-    m = to;
-    l *= f;
-#pragma unroll
-    for (int i = 0; i < DT; ++i) scale_acc(O[i], f);
   };
 
   // ---- the beams' own suffixes.  The suffix keys of the wave's beams, in order,
@@ -424,7 +427,6 @@ block_attn_kernel(BlockAttnArgs a) {
   // finite would reach the rows that do not see it as 0 * inf, so a group that
   // holds one is multiplied without it, and the rows that do see it add it at the
   // end.
-  bool spoilt = false;
   const bool has_suffix = a.Tk > 0 && split == 0 && (SHARED || wave == 0);
   int vlo = 0, vhi = -1, keys = 0;                   // keys the row sees, keys of the wave
   const int w0 = row0 / a.T / G;
@@ -432,13 +434,12 @@ block_attn_kernel(BlockAttnArgs a) {
   constexpr int CPV = D / 8, RPV = 512 / D;          // chunks per V row, rows per load
   u32x4 kr[4 * KS];
   if (has_suffix) {
-    const int w1 = min(row0 + 31, a.R - 1) / a.T / G;
     vlo = (w - w0) * a.Tk;
     vhi = vlo + a.Tk - a.T + t;
     keys = vhi + 1;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o, 64));
-    keys = max(min(__builtin_amdgcn_readfirstlane(keys), (w1 - w0 + 1) * a.Tk), 1);
+    keys = __builtin_amdgcn_readfirstlane(keys);
   }
   auto of_lane = [](int64_t v, int from) {
     return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
@@ -454,7 +455,7 @@ block_attn_kernel(BlockAttnArgs a) {
       kr[c] = *(const u32x4*)(krow + 32 * (c >> 1) + 8 * (c & 1));
     const int64_t v_at = (n0 + beam) * a.ssv_n + (int64_t)token * a.ssv_t + kh * a.ssv_h;
     const int pieces = (keys - f0 > 16 ? 32 : 16) / RPV;   // 16 or 32 rows of V
-#pragma unroll 4
+#pragma unroll 2
     for (int i = 0; i < pieces; ++i) {
       const int row = i * RPV + lane / CPV;
       const int chunk = (lane % CPV) ^ (D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
@@ -464,6 +465,12 @@ block_attn_kernel(BlockAttnArgs a) {
   };
   // in_flight: loads issued after the first group's
   auto suffix = [&](uint8_t* area, int in_flight) {
+    const float mul = a.qmul * a.sl2;
+    constexpr float kUp = std::is_same<T, bf16_t>::value ? kMaxUp : 14.f;
+    const int gi = lane & 15, s_row = 4 * hi + (gi >> 2);
+    const int s_d = (lane >> 4 & 1) * 16 + (gi & 3) * 4;
+    const int s_sw = D == 64 ? (s_row >> 1 & 1) * 4 : (s_row & 3) * 4;
+#pragma unroll 1
     for (int f0 = 0; f0 < keys; f0 += 32) {
       const bool both = keys - f0 > 16;
       if (f0 > 0) {
@@ -473,7 +480,6 @@ block_attn_kernel(BlockAttnArgs a) {
       f32x16 st = f32x16{};
 #pragma unroll
       for (int c = 0; c < 4 * KS; ++c) st = mfma_wide(kind, kr[c], qr[c], st);
-      const float mul = a.qmul * a.sl2;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -482,8 +488,9 @@ block_attn_kernel(BlockAttnArgs a) {
         top = fmaxf(top, st[j]);
       }
       top = max_xor32(top);
+      m_true = fmaxf(m_true, top);
       if (m == -INFINITY) m = top;
-      if (__ballot(top > m) != 0) raise(top, 0.f);   // (so weights are at most 1)
+      over |= top > m + kUp;
       const float ref = m == -INFINITY ? 0.f : m;
       u32x4 pk[2];
       float sum = 0.f;
@@ -495,7 +502,7 @@ block_attn_kernel(BlockAttnArgs a) {
         pk[j >> 3][j >> 1 & 3] = pack2(kind, x, y);
       }
       l += add_xor32(sum);
-      if (f0 == 0 && in_flight) wait_vm(in_flight);
+      if (f0 == 0) wait_vm(in_flight);
       else wait_vm(0);
       // (each lane looks at what its own loads brought)
       uint32_t top_exp = 0;
@@ -516,381 +523,318 @@ block_attn_kernel(BlockAttnArgs a) {
         }
         __builtin_amdgcn_s_waitcnt(0xc07f);
       }
-      const int gi = lane & 15, v_row = 4 * hi + (gi >> 2);
-      const int v_d = (lane >> 4 & 1) * 16 + (gi & 3) * 4;
-      const int v_sw = D == 64 ? (v_row >> 1 & 1) * 4 : (v_row & 3) * 4;
+      spoilt |= bad;
+#pragma unroll 1
       for (int ks = 0; ks < (both ? 2 : 1); ++ks) {
         const uint32_t base =
-            (uint32_t)(uintptr_t)(area + (16 * ks + v_row) * D * 2 + (v_d & 7) * 2);
+            (uint32_t)(uintptr_t)(area + (16 * ks + s_row) * D * 2 + (s_d & 7) * 2);
+        const u32x4 p = ks ? pk[1] : pk[0];
 #pragma unroll
         for (int d2 = 0; d2 < DT / 2; ++d2) {
           u32x4 x, y;
-          read_wide2<D>(base + ((((64 * d2 + v_d) >> 3) ^ v_sw) * 16),
-                        base + ((((64 * d2 + 32 + v_d) >> 3) ^ v_sw) * 16), x, y);
-          O[2 * d2] = mfma_wide(kind, x, ks ? pk[1] : pk[0], O[2 * d2]);
-          O[2 * d2 + 1] = mfma_wide(kind, y, ks ? pk[1] : pk[0], O[2 * d2 + 1]);
+          read_wide2<D>(base + ((((64 * d2 + s_d) >> 3) ^ s_sw) * 16),
+                        base + ((((64 * d2 + 32 + s_d) >> 3) ^ s_sw) * 16), x, y);
+          O[2 * d2] = mfma_wide(kind, x, p, O[2 * d2]);
+          O[2 * d2 + 1] = mfma_wide(kind, y, p, O[2 * d2 + 1]);
         }
       }
-      spoilt |= bad;
     }
   };
 
-  // load instruction i of a K (kv 0) or V tile: key i * RPI + lane / CPR, at place
-  // lane % CPR the chunk that the swizzle puts there; page and meta describe
-  // the half tile it lies in, pos is the tile's first key
-  const int d_row = lane / S::CPR, d_pc = lane % S::CPR;
-  auto load1 = [&](int kv, int page, int meta_of, int pos, int i, uint32_t dst) {
-    const int row = i * S::RPI + d_row;
-    const int64_t key = (((int64_t)max(page, 0) * a.HK + kh) << a.lblock) +
-                        ((pos + i * S::RPI / 32 * 32) & ((1 << a.lblock) - 1));
-    const int off = (row & 31) * D + (d_pc ^ (kv ? S::swv(row) : S::swk(row))) * 16;
-    load_lds16((kv ? a.vc : a.kc) + key * D, (meta_of & 0xff) * D, off, dst + i * 1024);
-  };
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
-
-  // LDS offsets of the fragments
-  uint32_t k_off[KS][2];   // K: key col of a half, chunks 4 s + hi and 4 s + 2 + hi
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      k_off[s][c] = col * D + ((4 * s + 2 * c + hi) ^ S::swk(col)) * 16;
-  // V: key 8 (e / 4) + 4 hi + e % 4, e = (lane % 16) / 2; d = 32 dt + 16 (lane / 16 % 2) +
-  // 8 (lane % 2)
-  const int v_e = (lane & 15) >> 1;
-  const int v_row = 8 * (v_e >> 2) + 4 * hi + (v_e & 3);
-  uint32_t v_off[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-    v_off[dt] = v_row * D + (lane & 1) * 8 + (((2 * dt + (lane >> 4 & 1)) ^ S::swv(v_row)) * 16);
-
-  // ---- one tile in LDS: scores, weights, output
-  int m0 = 0, m1 = 0;   // meta of the tile's halves
-  auto scores = [&](const uint8_t* ks, f32x16* st) {
+  // ---- the scores st of a tile (of halves holding held[] keys) to weights
+  i32x8 pf[NP];
+  int ps;                  // the scale byte of this lane's block of weights
+  auto scores = [&](const uint8_t* ks, int meta0, int meta1, f32x16* st) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       st[hf] = f32x16{};
-      const int sk = (hf ? m1 : m0) >> 8 & 0xff;
+      const int sk = (hf ? meta1 : meta0) >> 8 & 0xff;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const i32x4 x = *(const i32x4*)(ks + k_off[s][0] + hf * 32 * D);
-        const i32x4 y = *(const i32x4*)(ks + k_off[s][1] + hf * 32 * D);
-        const i32x8 kf = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        const i32x8 kf = read_k(ks, hf, s);
 #pragma unroll
         for (int p = 0; p < NP; ++p) st[hf] = mfma_scaled(kf, qf[p][s], st[hf], sk, qs[p]);
       }
     }
   };
-  i32x8 pf[NP];
-  int ps[NP];
-  auto weights = [&](f32x16* st) {
-    const int held[2] = {m0 & 0xff, m1 & 0xff};
-    float top[2];
+  auto mask = [&](int meta0, int meta1, f32x16* st) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      if (held[hf] < 32) {
+      const int held = (hf ? meta1 : meta0) & 0xff;
+      if (held < 32) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          st[hf][j] = 8 * (j >> 2) + 4 * hi + (j & 3) < held[hf] ? st[hf][j] : -INFINITY;
-      }
-      float x = st[hf][0];
-#pragma unroll
-      for (int j = 1; j < 16; ++j) x = fmaxf(x, st[hf][j]);
-      top[hf] = max_xor32(x) * a.sl2;
-    }
-    const float both = fmaxf(top[0], top[1]);
-    if (m == -INFINITY) m = both;
-    if (__ballot(both > m + kMaxUp) != 0) raise(both, kMaxUp);
-    const float ref = m == -INFINITY ? 0.f : m;
-    int e[2];
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      e[hf] = (int)fmaxf(ceilf(top[hf] - ref), -100.f);
-      const float nm = (float)(8 - e[hf]) - ref;
-      float sum = 0.f;
-#pragma unroll
-      for (int j4 = 0; j4 < 4; ++j4) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[i] = __builtin_amdgcn_exp2f(fmaf(st[hf][4 * j4 + i], a.sl2, nm));
-          sum += y[i];
-        }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) pf[p][4 * hf + j4] = piece4(y, y);
-      }
-      l = fmaf(add_xor32(sum), pow2i(e[hf] - 8), l);
-    }
-    const int own = hi ? e[1] : e[0];
-#pragma unroll
-    for (int p = 0; p < NP; ++p) ps[p] = own - 8 - 4 * p + 127;
-  };
-  auto outputs = [&](const uint8_t* vs) {
-    const int sv = (hi ? m1 : m0) >> 16 & 0xff;
-    const uint32_t base = (uint32_t)(uintptr_t)vs;
-#pragma unroll
-    for (int d2 = 0; d2 < DT / 2; ++d2) {
-      i32x8 f0, f1;
-      read_v2<D>(base + v_off[2 * d2], base + v_off[2 * d2 + 1], f0, f1);
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        O[2 * d2] = mfma_scaled(f0, pf[p], O[2 * d2], sv, ps[p]);
-        O[2 * d2 + 1] = mfma_scaled(f1, pf[p], O[2 * d2 + 1], sv, ps[p]);
+          st[hf][j] = 8 * (j >> 2) + 4 * hi + (j & 3) < held ? st[hf][j] : -INFINITY;
       }
     }
   };
-  auto take_meta = [&](int k) {
-    m0 = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
-    m1 = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
-  };
-
-  if constexpr (SHARED) {
-    // Two rings of 4 tiles, K's and then V's.  Step k forms the scores of tile
-    // k + 1 and adds tile k - 1 to the output while the vector unit turns tile k's
-    // scores into weights: the three are independent, so the products run
-    // without a pause (a step's vector work takes about 3/4 of their time at D =
-    // 256).  K(k) and V(k - 2) have been used by then, and K(k + 4) and V(k + 2)
-    // are loaded into their places, three steps before their use; wave w loads
-    // the w-th quarter of each.  Tiles past the last are loaded as zeros, which
-    // keeps the counts of loads in flight the same.
-    constexpr int LW = S::LT / 4;
-    int ring_pg[6][2], ring_meta[6][2];     // halves of the tiles k - 1 .. k + 4 (-1: none)
-    auto read_ring = [&](int x, int k) {
+  // The work on a tile's scores in slices: 8 of maxima, 1 of references, 24 of
+  // weights.  A half's weights are 2^(s - ref - e + 8), e the least whole number
+  // that keeps them at most 2^8, and their pieces' scales 2^(e - 8): what two
+  // (three) pieces leave of a weight is at most 2^-8 (2^-12) of it, or 2^-18 of
+  // the half's largest.
+  float top[2], nm[2], sum[2], y4[4];
+  int e_of[2];
+  auto slice = [&](auto c_c, const f32x16* cur, i32x8* pc, int& pcs) {
+    constexpr int c = decltype(c_c)::value;
+    if constexpr (c < 8) {
+      constexpr int hf = c / 4, q4 = c % 4;
+      const float x = max3(cur[hf][4 * q4 + 1], cur[hf][4 * q4 + 2], cur[hf][4 * q4 + 3]);
+      top[hf] = max3(q4 == 0 ? x : top[hf], cur[hf][4 * q4], x);
+    } else if constexpr (c == 8) {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) top[hf] = max_xor32(top[hf]) * a.sl2;
+      const float both = fmaxf(top[0], top[1]);
+      m_true = fmaxf(m_true, both);
+      m = m == -INFINITY ? both : m;
+      over |= both > m + kMaxUp;
+      const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        ring_pg[x][hf] = __builtin_amdgcn_readlane(pg, 2 * (k & 31) + hf);
-        ring_meta[x][hf] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + hf);
+        const float e = fmaxf(ceilf(top[hf] - ref), -100.f);
+        e_of[hf] = (int)fminf(e, 100.f);
+        nm[hf] = 8.f - (float)e_of[hf] - ref;
+        sum[hf] = 0.f;
       }
-    };
-    auto issue = [&](int kv, int x, int k) {  // tile k, described in ring[x]
-      const uint32_t dst = lds0 + (4 * kv + (k & 3)) * S::tile;
+      pcs = (hi ? e_of[1] : e_of[0]) - 8 + 127;
+    } else {
+      constexpr int q = (c - 9) / 3, part = (c - 9) % 3, hf = q / 4, j4 = q % 4;
+      if constexpr (part < 2) {
+#pragma unroll
+        for (int i = 2 * part; i < 2 * part + 2; ++i) {
+          y4[i] = __builtin_amdgcn_exp2f(fmaf(cur[hf][4 * j4 + i], a.sl2, nm[hf]));
+          sum[hf] += y4[i];
+        }
+        asm volatile("" ::"v"(sum[hf]));   // (here, not where it is used)
+      } else {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          const int word = piece4(y4, y4);
+          asm volatile("" ::"v"(word));
+          pc[p][4 * hf + j4] = word;
+        }
+      }
+    }
+  };
+  auto add_sums = [&]() {
+    l += add_xor32(sum[0]) * pow2i(e_of[0] - 8) + add_xor32(sum[1]) * pow2i(e_of[1] - 8);
+  };
+  constexpr int SL = 33;
+
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    l = 0.f;
+    m_true = -INFINITY;
+    over = false;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) O[i] = f32x16{};
+    load_q();
+    if constexpr (SHARED) {
+      // Two rings of 4 tiles, K's and then V's.  Step k forms the scores of tile
+      // k + 1 and adds tile k - 1 to the output while the vector unit turns tile
+      // k's scores into weights: the three are independent, so products and
+      // vector work overlap.  K(k) and V(k - 2) have been used by then, and K(k +
+      // 4) and V(k + 2) are loaded into their places, three steps before their
+      // use; wave w loads the w-th quarter of each, which lies in half w / 2.
+      // Tiles past the last are loaded as zeros, which keeps the counts of loads
+      // in flight the same.
+      constexpr int LW = S::LT / 4;
+      uint32_t k_src[LW], v_src[LW];
 #pragma unroll
       for (int i = 0; i < LW; ++i) {
-        const int at = wave * LW + i, hf = at * S::RPI / 32;
-        load1(kv, hf ? ring_pg[x][1] : ring_pg[x][0], hf ? ring_meta[x][1] : ring_meta[x][0],
-              (first + k) * kKeys, at, dst);
+        k_src[i] = off_of(0, wave * LW + i) + (LW < 4 ? (wave * LW + i) % 4 * 1024 : 0);
+        v_src[i] = off_of(1, wave * LW + i) + (LW < 4 ? (wave * LW + i) % 4 * 1024 : 0);
       }
-    };
-    uint8_t* area = smem + (4 + wave) * S::tile;   // the suffix: where V's tiles go
-    if (has_suffix) suffix_load(area, 0);
-    describe(0, first_page);
-    ring_pg[0][0] = ring_pg[0][1] = -1;
-    ring_meta[0][0] = ring_meta[0][1] = 127 << 8 | 127 << 16;
+      auto issue = [&](int kv, int k, u32x4 rsrc) {
+        const uint32_t dst = lds0 + (4 * kv + (k & 3)) * S::tile + wave * LW * 1024;
+        static_for<LW>([&](auto i_c) {
+          constexpr int i = decltype(i_c)::value;
+          if constexpr (LW == 4) load_lds16<i * 1024>(rsrc, kv ? v_src[i] : k_src[i], dst);
+          else load_lds16<0>(rsrc, kv ? v_src[i] : k_src[i], dst + i * 1024);
+        });
+      };
+      int ring[6][2];                       // meta of the halves of tiles k - 1 .. k + 4
+      uint32_t own_lo[3], own_hi[3], own_held[3];   // this wave's half of tiles k + 2 .. k + 4
+      auto read_half = [&](int x, int k) {
+        const int at = 2 * (k & 31);
+        own_lo[x] = __builtin_amdgcn_readlane(code_lo, at + (wave >> 1));
+        own_hi[x] = __builtin_amdgcn_readlane(code_hi, at + (wave >> 1));
+        own_held[x] = __builtin_amdgcn_readlane(meta, at + (wave >> 1)) & 0xff;
+      };
+      auto read_ring = [&](int x, int k) {
+        ring[x][0] = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
+        ring[x][1] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
+      };
+      uint8_t* area = smem + (4 + wave) * S::tile;   // the suffix: where V's tiles go
+      if (has_suffix) suffix_load(area, 0);
+      describe(0, first_page);
+      ring[0][0] = ring[0][1] = 127 << 8 | 127 << 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      read_ring(k + 1, k);
-      issue(0, k + 1, k);
-    }
-    if (has_suffix) {
-      suffix(area, 4 * LW);
+      for (int k = 0; k < 4; ++k) {
+        read_ring(k + 1, k);
+        read_half(k < 2 ? 2 : k - 2, k);
+        issue(0, k, source(a.kc, own_lo[k < 2 ? 2 : k - 2], own_hi[k < 2 ? 2 : k - 2],
+                           own_held[k < 2 ? 2 : k - 2]));
+      }
+      if (has_suffix) {
+        suffix(area, 4 * LW);
+        tile_barrier();
+      }
+      issue(1, -1, source(a.vc, 0, 0, 0));
+      read_half(2, 0);
+      issue(1, 0, source(a.vc, own_lo[2], own_hi[2], own_held[2]));
+      read_half(2, 1);
+      issue(1, 1, source(a.vc, own_lo[2], own_hi[2], own_held[2]));
+      split_q();
+      f32x16 st[2];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) pf[p] = i32x8{};
+      ps = 127;
+      wait_vm(6 * LW);                        // K(0)
       tile_barrier();
-    }
-    issue(1, 0, -1);
-    issue(1, 1, 0);
-    issue(1, 2, 1);
-    ring_pg[5][0] = ring_pg[5][1] = ring_meta[5][0] = ring_meta[5][1] = 0;
-    split_q();
-    f32x16 st[2];
-#pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      pf[p] = i32x8{};
-      ps[p] = 127;
-    }
-    wait_vm(6 * LW);                        // K(0)
-    tile_barrier();
-    m0 = ring_meta[1][0];
-    m1 = ring_meta[1][1];
-    scores(smem, st);
+      scores(smem, ring[1][0], ring[1][1], st);
 
-    auto read_v = [&](const uint8_t* vs, int dt) {
-      typedef __attribute__((address_space(3))) i32x2* piece_t;
-      const uint32_t at = (uint32_t)(uintptr_t)(lds_t*)vs + v_off[dt];
-      i32x8 f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((piece_t)(at + 16 * c * D));
-        f[2 * c] = x[0];
-        f[2 * c + 1] = x[1];
-      }
-      return f;
-    };
 #pragma unroll 1
-    for (int k = 0; k < count; ++k) {
-      f32x16 cur[2] = {st[0], st[1]};
-      i32x8 pc[NP];
-      int pcs[NP];
-      if (k >= 2) wait_vm(4 * LW);          // K(k + 1) and V(k - 1)
-      else wait_vm(2 * LW);
-      tile_barrier();
+      for (int k = 0; k < count; ++k) {
+        if (k >= 2) wait_vm(4 * LW);          // K(k + 1) and V(k - 1)
+        else wait_vm(2 * LW);
+        tile_barrier();
+        const uint8_t* ks = smem + (k + 1 & 3) * S::tile;
+        const uint8_t* vs = smem + (4 + (k - 1 & 3)) * S::tile;
+        constexpr int NF = 4 * KS, MF = NF * NP;
+        i32x8 fr[3];
+        auto fetch = [&](auto f_c) {
+          constexpr int f = decltype(f_c)::value;
+          if constexpr (f < 2 * KS) fr[f % 3] = read_k(ks, f / KS, f % KS);
+          else if constexpr (f < NF) fr[f % 3] = read_v(vs, f - 2 * KS);
+        };
+        fetch(std::integral_constant<int, 0>{});
+        fetch(std::integral_constant<int, 1>{});
+        if ((k + 4 & 31) == 0) describe((k + 4) >> 5, page_at((k + 4) >> 5));
+        read_ring(5, k + 4);
+        read_half(2, k + 4);
+        f32x16 cur[2] = {st[0], st[1]};
+        mask(ring[1][0], ring[1][1], cur);
+        i32x8 pc[NP];
+        int pcs;
+        const int sk[2] = {ring[2][0] >> 8 & 0xff, ring[2][1] >> 8 & 0xff};
+        const int sv = (hi ? ring[0][1] : ring[0][0]) >> 16 & 0xff;
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<MF>([&](auto i_c) {
+          constexpr int i = decltype(i_c)::value, f = i / NP, p = i % NP;
+          if constexpr (p == 0) fetch(std::integral_constant<int, f + 2>{});
+          if constexpr (f < 2 * KS) {
+            constexpr int hf = f / KS, s = f % KS;
+            if constexpr (s == 0 && p == 0)
+              st[hf] = mfma_scaled(fr[f % 3], qf[p][s], f32x16{}, sk[hf], qs[p]);
+            else
+              st[hf] = mfma_scaled(fr[f % 3], qf[p][s], st[hf], sk[hf], qs[p]);
+          } else {
+            constexpr int dt = f - 2 * KS;
+            O[dt] = mfma_scaled(fr[f % 3], pf[p], O[dt], sv, ps);
+          }
+          // K(k + 4) is loaded half way, V(k + 2) three quarters on
+          if constexpr (i == MF / 2)
+            issue(0, k + 4, source(a.kc, own_lo[2], own_hi[2], own_held[2]));
+          if constexpr (i == 3 * MF / 4)
+            issue(1, k + 2, source(a.vc, own_lo[0], own_hi[0], own_held[0]));
+          constexpr int c0 = i * SL / MF, c1 = (i + 1) * SL / MF;
+          static_for<c1 - c0>([&](auto x_c) {
+            slice(std::integral_constant<int, c0 + decltype(x_c)::value>{}, cur, pc, pcs);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        // (the products above stay here, not where their results are used)
+        asm volatile("" ::"a"(st[0]), "a"(st[1]));
+        add_sums();
 #pragma unroll
-      for (int x = 0; x < 5; ++x)
+        for (int p = 0; p < NP; ++p) pf[p] = pc[p];
+        ps = pcs;
+#pragma unroll
+        for (int x = 0; x < 5; ++x) {
+          ring[x][0] = ring[x + 1][0];
+          ring[x][1] = ring[x + 1][1];
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          own_lo[x] = own_lo[x + 1];
+          own_hi[x] = own_hi[x + 1];
+          own_held[x] = own_held[x + 1];
+        }
+      }
+      // the last tile's output
+      const bool any = __ballot(over) != 0;
+      if (lane == 0) sm_over[wave] = any;
+      wait_vm(0);
+      __syncthreads();
+      if (count > 0) {
+        const uint8_t* vs = smem + (4 + (count - 1 & 3)) * S::tile;
+        const int sv = (hi ? ring[0][1] : ring[0][0]) >> 16 & 0xff;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const i32x8 f = read_v(vs, dt);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[p], O[dt], sv, ps);
+        }
+      }
+      if (pass == 1 || (sm_over[0] | sm_over[1] | sm_over[2] | sm_over[3]) == 0) break;
+      __syncthreads();
+    } else {
+      uint8_t* mine = smem + wave * S::slot;
+      const uint32_t mine_at = lds0 + wave * S::slot;
+      auto issue = [&](int kv, int k) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          if (k > 0) ring_pg[x][hf] = ring_pg[x + 1][hf];
-          if (k > 0) ring_meta[x][hf] = ring_meta[x + 1][hf];
-        }
-      if ((k + 4 & 31) == 0) describe((k + 4) >> 5, page_at((k + 4) >> 5));
-      read_ring(5, k + 4);
-      issue(0, 5, k + 4);
-      issue(1, 3, k + 2);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int held = ring_meta[1][hf] & 0xff;
-        if (held < 32) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            cur[hf][j] = 8 * (j >> 2) + 4 * hi + (j & 3) < held ? cur[hf][j] : -INFINITY;
-        }
-      }
-      const uint8_t* ks = smem + (k + 1 & 3) * S::tile;
-      const uint8_t* vs = smem + (4 + (k - 1 & 3)) * S::tile;
-      const int sk[2] = {ring_meta[2][0] >> 8 & 0xff, ring_meta[2][1] >> 8 & 0xff};
-      const int sv = (hi ? ring_meta[0][1] : ring_meta[0][0]) >> 16 & 0xff;
-      // the vector work in slices: 8 of maxima, 1 of references, 24 of weights
-      float top[2] = {-INFINITY, -INFINITY}, nm[2], sum[2] = {0.f, 0.f}, y[4], fac = 1.f;
-      int e[2];
-      bool moved = false;
-      auto slice = [&](auto c_c) {
-        constexpr int c = decltype(c_c)::value;
-        if constexpr (c < 8) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top[c / 4] = fmaxf(top[c / 4], cur[c / 4][4 * (c % 4) + j]);
-        } else if constexpr (c == 8) {
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) top[hf] = max_xor32(top[hf]) * a.sl2;
-          const float both = fmaxf(top[0], top[1]);
-          moved = both > m + kMaxUp && m != -INFINITY;
-          const float to = m == -INFINITY || moved ? both : m;
-          fac = moved ? __builtin_amdgcn_exp2f(m - to) : 1.f;
-          m = to;
-          const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            e[hf] = (int)fmaxf(ceilf(top[hf] - ref), -100.f);
-            nm[hf] = (float)(8 - e[hf]) - ref;
-          }
-          const int own = hi ? e[1] : e[0];
-#pragma unroll
-          for (int p = 0; p < NP; ++p) pcs[p] = own - 8 - 4 * p + 127;
-        } else {
-          constexpr int g = (c - 9) / 3, part = (c - 9) % 3, hf = g / 4, j4 = g % 4;
-          if constexpr (part < 2) {
-#pragma unroll
-            for (int i = 2 * part; i < 2 * part + 2; ++i) {
-              y[i] = __builtin_amdgcn_exp2f(fmaf(cur[hf][4 * j4 + i], a.sl2, nm[hf]));
-              sum[hf] += y[i];
-            }
-            asm volatile("" ::"v"(sum[hf]));   // (here, not where it is used)
-          } else {
-#pragma unroll
-            for (int p = 0; p < NP; ++p) {
-              const int word = piece4(y, y);
-              asm volatile("" ::"v"(word));
-              pc[p][4 * hf + j4] = word;
-            }
-          }
+          const int at = 2 * (k & 31) + hf;
+          const u32x4 rsrc = source(kv ? a.vc : a.kc, __builtin_amdgcn_readlane(code_lo, at),
+                                    __builtin_amdgcn_readlane(code_hi, at),
+                                    __builtin_amdgcn_readlane(meta, at) & 0xff);
+          const uint32_t dst = mine_at + kv * S::tile + hf * IPH * 1024;
+          static_for<IPH>([&](auto i_c) {
+            constexpr int i = decltype(i_c)::value;
+            load_lds16<i % 4 * 1024>(rsrc, off_of(kv, i), dst + i / 4 * 4096);
+          });
         }
       };
-      constexpr int NF = 4 * KS, MF = NF * NP, SL = 33;
-      i32x8 fr[3];
-      auto fetch = [&](auto f_c) {
-        constexpr int f = decltype(f_c)::value;
-        if constexpr (f < 2 * KS) {
-          constexpr int hf = f / KS, s = f % KS;
-          const i32x4 x = *(const i32x4*)(ks + k_off[s][0] + hf * 32 * D);
-          const i32x4 z = *(const i32x4*)(ks + k_off[s][1] + hf * 32 * D);
-          fr[f % 3] = i32x8{x[0], x[1], x[2], x[3], z[0], z[1], z[2], z[3]};
-        } else if constexpr (f < NF) {
-          fr[f % 3] = read_v(vs, f - 2 * KS);
-        }
-      };
-      __builtin_amdgcn_sched_barrier(0);
-      fetch(std::integral_constant<int, 0>{});
-      fetch(std::integral_constant<int, 1>{});
-      static_for<MF>([&](auto i_c) {
-        constexpr int i = decltype(i_c)::value, f = i / NP, p = i % NP;
-        if constexpr (p == 0) fetch(std::integral_constant<int, f + 2>{});
-        if constexpr (f < 2 * KS) {
-          constexpr int hf = f / KS, s = f % KS;
-          if constexpr (s == 0 && p == 0)
-            st[hf] = mfma_scaled(fr[f % 3], qf[p][s], f32x16{}, sk[hf], qs[p]);
-          else
-            st[hf] = mfma_scaled(fr[f % 3], qf[p][s], st[hf], sk[hf], qs[p]);
-        } else {
-          constexpr int dt = f - 2 * KS;
-          O[dt] = mfma_scaled(fr[f % 3], pf[p], O[dt], sv, ps[p]);
-        }
-        constexpr int c0 = i * SL / MF, c1 = (i + 1) * SL / MF;
-        static_for<c1 - c0>([&](auto x_c) {
-          slice(std::integral_constant<int, c0 + decltype(x_c)::value>{});
-        });
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      // (the products above stay here, not where their results are used)
-      asm volatile("" ::"a"(st[0]), "a"(st[1]));
-      l = l * fac + add_xor32(sum[0]) * pow2i(e[0] - 8) + add_xor32(sum[1]) * pow2i(e[1] - 8);
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        pf[p] = pc[p];
-        ps[p] = pcs[p];
-      }
-      if (__ballot(moved) != 0) {
-#pragma unroll
-        for (int i = 0; i < DT; ++i) scale_acc(O[i], fac);
-      }
-    }
-    // the last tile's output
-    wait_vm(0);
-    tile_barrier();
-    if (count > 0) {
-      const uint8_t* vs = smem + (4 + (count - 1 & 3)) * S::tile;
-      const int sv = (hi ? ring_meta[1][1] : ring_meta[1][0]) >> 16 & 0xff;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const i32x8 f = read_v(vs, dt);
-#pragma unroll
-        for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[p], O[dt], sv, ps[p]);
-      }
-    }
-  } else {
-    uint8_t* mine = smem + wave * S::slot;
-    const uint32_t mine_at = lds0 + wave * S::slot;
-    auto issue = [&](int kv, int k) {
-#pragma unroll
-      for (int i = 0; i < S::LT; ++i) {
-        const int at = 2 * (k & 31) + i * S::RPI / 32;       // the lane that describes the half
-        load1(kv, __builtin_amdgcn_readlane(pg, at), __builtin_amdgcn_readlane(meta, at),
-              (first + stride * k) * kKeys, i, mine_at + kv * S::tile);
-      }
-    };
-    if (has_suffix) suffix_load(mine + S::tile, 0);   // where V goes
-    describe(0, first_page);
-    if (count > 0) issue(0, 0);
-    if (has_suffix) {
-      if (count > 0) suffix(mine + S::tile, S::LT);
-      else suffix(mine + S::tile, 0);
-    }
-    if (count > 0) issue(1, 0);
-    split_q();
-    for (int k = 0; k < count; ++k) {
-      take_meta(k);
-      wait_vm(S::LT);              // K of tile k is there, V may be on its way
-      f32x16 st[2];
-      scores(mine, st);
-      // the next tile's K goes where this one's was, once its reads are done
-      // (the products above have taken them)
-      if (k + 1 < count) {
+      if (has_suffix) suffix_load(mine + S::tile, 0);   // where V goes
+      describe(0, first_page);
+      issue(0, 0);
+      if (has_suffix) suffix(mine + S::tile, S::LT);
+      issue(1, 0);
+      split_q();
+#pragma unroll 1
+      for (int k = 0; k < count; ++k) {
+        const int m0 = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
+        const int m1 = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
+        wait_vm(S::LT);              // K of tile k is there, V may be on its way
+        f32x16 st[2];
+        scores(mine, m0, m1, st);
+        // the next tile's K goes where this one's was, once its reads are done
+        // (the products above have taken them)
         if ((k + 1 & 31) == 0) describe((k + 1) >> 5, page_at((k + 1) >> 5));
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0)
         __builtin_amdgcn_sched_barrier(0);
         issue(0, k + 1);
+        mask(m0, m1, st);
+        static_for<SL>([&](auto c_c) { slice(c_c, st, pf, ps); });
+        add_sums();
+        wait_vm(S::LT);
+        const int sv = (hi ? m1 : m0) >> 16 & 0xff;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const i32x8 f = read_v(mine + S::tile, dt);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[p], O[dt], sv, ps);
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        __builtin_amdgcn_sched_barrier(0);
+        issue(1, k + 1);
       }
-      weights(st);
-      if (k + 1 < count) wait_vm(S::LT);
-      else wait_vm(0);
-      outputs(mine + S::tile);
-      if (k + 1 < count) issue(1, k + 1);     // outputs() waits for its own reads
+      wait_vm(0);
+      if (pass == 1 || __ballot(over) == 0) break;
     }
+    m = over ? m_true : m;
+    first_page = page_at(0);
   }
 
   // ---- the rows: O^T through LDS, joined over the waves that hold the same
