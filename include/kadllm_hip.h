@@ -613,8 +613,7 @@ int kad_write_prefix_blocks(const void* k, int64_t sk_b, int64_t sk_t, int64_t s
  * (n, t, h) see the first lengths[b] cached tokens of their request b = n / W
  * and the suffix keys j <= Tk - T + t of their beam (Tk = 0: no suffix).  bf16
  * or fp16 queries, suffixes, gate (may be null) and out; last dimensions
- * contiguous; query and suffix rows 16-byte, gate and out rows 8-byte aligned.
- * A row that sees no key gives zeros.  The workspace (its size from
+ * contiguous and every row 16-byte aligned.  A row that sees no key gives zeros.  The workspace (its size from
  * kad_block_prefix_attention_workspace_bytes, 0 where none is needed) holds
  * the partial results of a prefix that is split over workgroups. */
 int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, int H, int HK, int D,

@@ -27,6 +27,22 @@
 
 namespace {
 
+// n / d for 0 <= n < 2^31 as n m / 2^(31 + s), m = floor(2^(31 + s) / d) + 1 and s =
+// ceil(log2 d): 0 < m d - 2^(31 + s) <= d <= 2^s, so the quotient is over n / d by
+// less than 1 / d
+struct Divide {
+  uint32_t m;
+  int s, d;
+};
+inline Divide divide_by(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return Divide{(uint32_t)((1ull << (31 + s)) / (uint32_t)d + 1), 31 + s, d};
+}
+__device__ __forceinline__ int operator/(int n, Divide by) {
+  return (int)((uint64_t)(uint32_t)n * by.m >> by.s);
+}
+
 struct BlockAttnArgs {
   const void* q;
   int64_t sq_n, sq_t, sq_h;
@@ -43,8 +59,9 @@ struct BlockAttnArgs {
   int64_t so_n, so_t, so_h;
   float* part_o;    // splits > 1: [split][B*HK][R][D] unnormalised outputs
   float* part_ml;   // and [split][B*HK][R][2]: the exponent they are relative to, the sum
-  int pages, width, B, W, T, Tk, H, HK, lblock;
+  int pages, width, B, W, T, Tk, H, HK, G, lblock;
   int splits, nqblk;
+  Divide by_splits, by_nqblk, by_HK, by_G, by_T, by_Tk;
   int R;            // query rows of a request and KV head, W * T * (H / HK)
   float qmul, sl2;  // sign of the scale (0 for none), |scale| in log2 units
 };
@@ -75,7 +92,9 @@ __device__ __forceinline__ f32x16 mfma_scaled(i32x8 a, i32x8 b, f32x16 c, int sa
 
 // 4 floats to a dword of e4m3 codes, and what they leave
 __device__ __forceinline__ int piece4(const float* y, float* rest) {
-  int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  int c;
+  asm("" : "=v"(c));              // (both halves are written below)
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], c, false);
   c = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(c, false);
   const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
@@ -228,25 +247,29 @@ __device__ __forceinline__ void load_lds16(const void* src, uint32_t lds) {
       : "memory");
 }
 
-// 4 elements of an output row: times inv, gated, rounded once (the gate's
-// sigmoid by the hardware's reciprocal, 1 ulp)
+// y times the sigmoid of a gate element (by the hardware's reciprocal, 1 ulp)
+__device__ __forceinline__ float gate1(float g, float y) {
+  return y * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+}
+template <typename T>
+__device__ __forceinline__ void gate8(const T* kind, u32x4 gate, float* y) {
+  float g[8];
+  widen8(kind, gate, g);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = gate1(g[i], y[i]);
+}
+// 4 elements of an output row: times inv, gated, rounded once
 template <typename T>
 __device__ __forceinline__ void store_row4(T* out, const float* o, float inv, bool gated,
                                            u32x2 gate) {
-  float y[4];
-  typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-  const f16x4 gh = __builtin_bit_cast(f16x4, gate);
+  const T* const kind = nullptr;
+  float y[4], g[8];
+  widen8(kind, u32x4{gate[0], gate[1], 0u, 0u}, g);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     y[e] = o[e] * inv;
-    if (gated) {
-      const float g = std::is_same<T, bf16_t>::value
-                          ? __uint_as_float(e & 1 ? gate[e >> 1] & 0xffff0000u : gate[e >> 1] << 16)
-                          : (float)gh[e];
-      y[e] *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
-    }
+    if (gated) y[e] = gate1(g[e], y[e]);
   }
-  const T* const kind = nullptr;
   *(u32x2*)out = u32x2{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3])};
 }
 
@@ -279,17 +302,21 @@ block_attn_kernel(BlockAttnArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hi = lane >> 5, col = lane & 31;
   const int lid = xcd_logical_id(blockIdx.x, gridDim.x);
-  const int qb = lid % a.nqblk, split = lid / a.nqblk % a.splits;
-  const int bk = lid / a.nqblk / a.splits;
-  const int kh = bk % a.HK, b = bk / a.HK;
-  const int G = a.H / a.HK;
+  const int bks = lid / a.by_nqblk, bk = bks / a.by_splits, b = bk / a.by_HK;
+  const int qb = lid - bks * a.nqblk, split = bks - bk * a.splits, kh = bk - b * a.HK;
+  const int G = a.G;
 
   // ---- this wave's tiles of the prefix: first + stride * k, k < count.  (With one
   // range the first pages do not wait for the length.)
+  int first_page = 0;
+  const int* table = a.tables + (int64_t)b * a.width;
+  if (a.splits == 1)
+    first_page = table[min(((SHARED ? 0 : wave) + (SHARED ? 1 : 4) * (lane >> 1)) * 2 + (lane & 1)
+                           >> (a.lblock - 5), a.width - 1)];
   const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
   const int tiles = (len + kKeys - 1) / kKeys;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int begin = split == 0 ? 0 : min(split * per, tiles), end = min(begin + per, tiles);
+  const int per = (tiles + a.splits - 1) / a.by_splits;
+  const int begin = min(split * per, tiles), end = min(begin + per, tiles);
   const int first = begin + (SHARED ? 0 : wave), stride = SHARED ? 1 : 4;
   const int count = __builtin_amdgcn_readfirstlane(
       SHARED ? end - begin : max((end - first + stride - 1) / stride, 0));
@@ -302,7 +329,7 @@ block_attn_kernel(BlockAttnArgs a) {
     return (first + stride * (32 * chunk + (lane >> 1))) * kKeys + (lane & 1) * 32;
   };
   auto page_at = [&](int chunk) {
-    return a.tables[(int64_t)b * a.width + min(half_at(chunk) >> a.lblock, a.width - 1)];
+    return table[min(half_at(chunk) >> a.lblock, a.width - 1)];
   };
   auto describe = [&](int chunk, int id) {
     const int pos = half_at(chunk);
@@ -315,12 +342,12 @@ block_attn_kernel(BlockAttnArgs a) {
       meta = min(len - pos, 32) | (int)a.ksc[ph] << 8 | (int)a.vsc[ph] << 16;
     }
   };
-  int first_page = page_at(0);
+  if (a.splits > 1) first_page = page_at(0);
 
   // ---- this lane's row (rows past the end repeat the last one and are not stored)
   const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
   const int r = min(row0 + col, a.R - 1);
-  const int rt = r / a.T, t = r - rt * a.T, w = rt / G, g = rt - w * G;
+  const int rt = r / a.by_T, t = r - rt * a.T, w = rt / a.by_G, g = rt - w * G;
   const int64_t n = (int64_t)b * a.W + w;
   const int h = kh * G + g;
   const T* const kind = nullptr;
@@ -429,7 +456,7 @@ block_attn_kernel(BlockAttnArgs a) {
   // end.
   const bool has_suffix = a.Tk > 0 && split == 0 && (SHARED || wave == 0);
   int vlo = 0, vhi = -1, keys = 0;                   // keys the row sees, keys of the wave
-  const int w0 = row0 / a.T / G;
+  const int w0 = min(row0, a.R - 1) / a.by_T / a.by_G;
   const int64_t n0 = (int64_t)b * a.W + w0;
   constexpr int CPV = D / 8, RPV = 512 / D;          // chunks per V row, rows per load
   u32x4 kr[4 * KS];
@@ -447,7 +474,7 @@ block_attn_kernel(BlockAttnArgs a) {
   };
   auto suffix_load = [&](uint8_t* area, int f0) {
     const uint32_t area_at = (uint32_t)(uintptr_t)(lds_t*)area;
-    const int f = min(f0 + col, keys - 1), beam = f / a.Tk, token = f - beam * a.Tk;
+    const int f = min(f0 + col, keys - 1), beam = f / a.by_Tk, token = f - beam * a.Tk;
     const T* krow = (const T*)a.sk + (n0 + beam) * a.ssk_n + (int64_t)token * a.ssk_t +
                     kh * a.ssk_h + 16 * hi;
 #pragma unroll
@@ -837,17 +864,83 @@ block_attn_kernel(BlockAttnArgs a) {
     first_page = page_at(0);
   }
 
-  // ---- the rows: O^T through LDS, joined over the waves that hold the same
-  // rows, then stored whole (or as a partial result).  A wave takes 256 / D rows
-  // at a time, 4 elements a lane; the gates of 8 such steps are loaded while the
-  // 8 before them are stored.
-  constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
-  constexpr int STEPS = SHARED ? 32 / RPS : (32 / RPS + 3) / 4, BATCH = STEPS < 8 ? STEPS : 8;
-  const int sub = lane / LPR, d0 = lane % LPR * 4;
   const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
   const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
   const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
-  auto first_row = [&](int s) { return (SHARED ? s : 4 * s + wave) * RPS; };
+  const bool gated = a.gate != nullptr && a.splits == 1;
+  if constexpr (SHARED) {
+    // ---- each lane has its row's elements 8 q + 4 hi + 0..3; lanes l and l ^ 32
+    // exchange halves, so that each holds 8 in a row, 16 bytes of the output
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const bool mine = col < rows;
+    const int64_t part = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + col;
+    if (mine) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(O[dt][8 * j + i]),
+                                                            __float_as_uint(O[dt][8 * j + 4 + i]),
+                                                            false, false);
+            y[i] = __uint_as_float(x[0]);
+            y[4 + i] = __uint_as_float(x[1]);
+          }
+          const int d = 32 * dt + 16 * j + 8 * hi;
+          if (a.splits > 1) {
+            *(f32x4*)(a.part_o + part * D + d) = f32x4{y[0], y[1], y[2], y[3]};
+            *(f32x4*)(a.part_o + part * D + d + 4) = f32x4{y[4], y[5], y[6], y[7]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] *= inv;
+            if (gated) gate8(kind, *(const u32x4*)((const T*)a.gate + gate_at + d), y);
+            *(u32x4*)((T*)a.out + out_at + d) =
+                u32x4{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3]), pack2(kind, y[4], y[5]),
+                      pack2(kind, y[6], y[7])};
+          }
+        }
+      if (a.splits > 1 && hi == 0) {
+        a.part_ml[2 * part] = m;
+        a.part_ml[2 * part + 1] = l;
+      }
+    }
+    if (spoilt) {
+      // values that are not finite, to the rows that see them: their sum is the
+      // element, whatever the weights
+      wait_vm(0);
+      const int64_t v_at = n * a.ssv_n + kh * a.ssv_h;
+#pragma unroll 1
+      for (int i = 0; i < rows; ++i) {
+        const T* vr = (const T*)a.sv + of_lane(v_at, i);
+        const int last = a.Tk - a.T + __shfl(t, i, 64);
+        T* out = (T*)a.out + of_lane(out_at, i);
+        float* o = a.part_o + of_lane(part, i) * D;
+#pragma unroll 1
+        for (int d = lane; d < D; d += 64) {
+          float sum_bad = 0.f;
+          for (int j = 0; j <= last; ++j) {
+            const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + d]);
+            if (!(fabsf(x) < INFINITY)) sum_bad += x;
+          }
+          if (sum_bad != 0.f) {
+            if (a.splits > 1) o[d] = sum_bad;
+            else out[d] = Elem<T>::from_f(sum_bad);
+          }
+        }
+      }
+    }
+    return;
+  }
+
+  // ---- O^T through LDS, joined over the waves that hold the same rows, then stored
+  // (or left as a partial result).  A wave takes 256 / D rows at a time, 4 elements
+  // a lane.
+  constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
+  constexpr int STEPS = (32 / RPS + 3) / 4;
+  const int sub = lane / LPR, d0 = lane % LPR * 4;
+  auto first_row = [&](int s) { return (4 * s + wave) * RPS; };
   // the value of the row that this lane stores in step s
   auto of_row = [&](int64_t v, int s) {
     if constexpr (RPS == 1) {
@@ -858,16 +951,6 @@ block_attn_kernel(BlockAttnArgs a) {
       return of_lane(v, first_row(s) + sub);
     }
   };
-  const bool gated = a.gate != nullptr && a.splits == 1;
-  u32x2 gv[BATCH];
-  auto load_gates = [&](int s0) {
-#pragma unroll
-    for (int s = 0; s < BATCH; ++s) {
-      gv[s] = u32x2{};
-      if (gated) gv[s] = *(const u32x2*)((const T*)a.gate + of_row(gate_at, s0 + s) + d0);
-    }
-  };
-  load_gates(0);
   wait_vm(0);
   __syncthreads();
   float* ep = (float*)smem + wave * 32 * S::EpiLd;
@@ -892,54 +975,36 @@ block_attn_kernel(BlockAttnArgs a) {
   }
   if (hi == 0) {
     sm_m[wave][col] = m;
-    sm_l[wave][col] = SHARED && a.splits == 1 ? (l == 0.f ? 0.f : 1.f / l) : l;
+    sm_l[wave][col] = l;
   }
   __syncthreads();
 #pragma unroll 1
-  for (int s0 = 0; s0 < STEPS && first_row(s0) < rows; s0 += BATCH) {
-    u32x2 gate[BATCH];
+  for (int s = 0; s < STEPS && first_row(s) < rows; ++s) {
+    const int i = first_row(s) + sub;
+    const int64_t to = of_row(out_at, s), gate_to = of_row(gate_at, s);
+    u32x2 gate = u32x2{};
+    if (gated) gate = *(const u32x2*)((const T*)a.gate + gate_to + d0);
+    const float mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
+    float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < BATCH; ++s) gate[s] = gv[s];
-    if (s0 + BATCH < STEPS && first_row(s0 + BATCH) < rows) load_gates(s0 + BATCH);
+    for (int x = 0; x < 4; ++x) {
+      const float mx = sm_m[x][i];
+      const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mm);
+      ll = fmaf(f, sm_l[x][i], ll);
+      const f32x4 y = *(const f32x4*)((float*)smem + (x * 32 + i) * S::EpiLd + d0);
 #pragma unroll
-    for (int s = 0; s < BATCH; ++s) {
-      const int i = first_row(s0 + s) + sub;
-      const int64_t to = of_row(out_at, s0 + s);
-      if (first_row(s0 + s) >= rows) break;
-      float o[4], ll, mm;
-      if constexpr (SHARED) {
-        mm = sm_m[wave][i];
-        ll = sm_l[wave][i];
-        const f32x4 x = *(const f32x4*)(ep + i * S::EpiLd + d0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = x[e];
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
+    }
+    if (i < rows) {
+      if (a.splits > 1) {
+        const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + i;
+        *(f32x4*)(a.part_o + at * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
+        if (d0 == 0) {
+          a.part_ml[2 * at] = mm;
+          a.part_ml[2 * at + 1] = ll;
+        }
       } else {
-        mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
-        ll = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = 0.f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float mx = sm_m[x][i];
-          const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mm);
-          ll = fmaf(f, sm_l[x][i], ll);
-          const f32x4 y = *(const f32x4*)((float*)smem + (x * 32 + i) * S::EpiLd + d0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
-        }
-        if (a.splits == 1) ll = ll == 0.f ? 0.f : 1.f / ll;
-      }
-      if (i < rows) {
-        if (a.splits > 1) {
-          const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + i;
-          *(f32x4*)(a.part_o + at * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
-          if (d0 == 0) {
-            a.part_ml[2 * at] = mm;
-            a.part_ml[2 * at + 1] = ll;
-          }
-        } else {
-          store_row4<T>((T*)a.out + to + d0, o, ll, gated, gate[s]);
-        }
+        store_row4<T>((T*)a.out + to + d0, o, ll == 0.f ? 0.f : 1.f / ll, gated, gate);
       }
     }
   }
@@ -954,11 +1019,11 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
   const int d0 = threadIdx.x % LPR * 4;
   if (row >= rows) return;
-  const int G = a.H / a.HK;
-  const int rr = (int)(row % a.R), bk = (int)(row / a.R);
-  const int t = rr % a.T, g = rr / a.T % G, w = rr / a.T / G;
-  const int64_t n = (int64_t)(bk / a.HK) * a.W + w;
-  const int h = bk % a.HK * G + g;
+  const int bk = (int)(row / a.R), rr = (int)(row - (int64_t)bk * a.R);
+  const int b = bk / a.by_HK, kh = bk - b * a.HK;
+  const int rt = rr / a.by_T, t = rr - rt * a.T, w = rt / a.by_G, g = rt - w * a.G;
+  const int64_t n = (int64_t)b * a.W + w;
+  const int h = kh * a.G + g;
   u32x2 gate = u32x2{};
   if (a.gate)
     gate = *(const u32x2*)((const T*)a.gate + n * a.sg_n + t * a.sg_t + h * a.sg_h + d0);
@@ -1086,8 +1151,8 @@ extern "C" int kad_block_prefix_attention(
   KAD_REQUIRE(Tk == 0 || (aligned(suffix_k, ssk_n, ssk_t, ssk_h, 8) &&
                           aligned(suffix_v, ssv_n, ssv_t, ssv_h, 8)),
               "suffix rows must be 16-byte aligned");
-  KAD_REQUIRE(aligned(out, so_n, so_t, so_h, 4) && (!gate || aligned(gate, sg_n, sg_t, sg_h, 4)),
-              "gate and output rows must be 8-byte aligned");
+  KAD_REQUIRE(aligned(out, so_n, so_t, so_h, 8) && (!gate || aligned(gate, sg_n, sg_t, sg_h, 8)),
+              "gate and output rows must be 16-byte aligned");
   if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
     KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
   int64_t need = 0;
@@ -1113,7 +1178,10 @@ extern "C" int kad_block_prefix_attention(
   a.part_ml = a.part_o + (int64_t)p.splits * B * HK * R * D;
   a.pages = pages; a.width = width; a.B = B; a.W = W; a.T = T; a.Tk = Tk; a.H = H; a.HK = HK;
   a.lblock = block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : 8;
-  a.splits = p.splits; a.nqblk = p.nqblk; a.R = R;
+  a.splits = p.splits; a.nqblk = p.nqblk; a.R = R; a.G = H / HK;
+  a.by_splits = divide_by(a.splits); a.by_nqblk = divide_by(a.nqblk);
+  a.by_HK = divide_by(HK); a.by_G = divide_by(a.G); a.by_T = divide_by(T);
+  a.by_Tk = divide_by(Tk > 0 ? Tk : 1);
   const float log2e = 1.4426950408889634f;
   a.qmul = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale == 0.f ? 0.f : scale;
   a.sl2 = scale == 0.f ? log2e : fabsf(scale) * log2e;

@@ -246,7 +246,7 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
     _device_of(q, tables, lengths, suffix_k, suffix_v, gate, *blocks)
     gate_strides = None
     if gate is not None:
-        gate = _rows(gate, 4)
+        gate = _rows(gate, 8)
         gate_strides = (gate.stride(0), gate.stride(1), D)
     return _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
                             D ** -0.5 if scale is None else scale, gate, gate_strides)
