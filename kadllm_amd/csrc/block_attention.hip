@@ -306,6 +306,79 @@ block_attn_kernel(BlockAttnArgs a) {
   const int qb = lid - bks * a.nqblk, split = bks - bk * a.splits, kh = bk - b * a.HK;
   const int G = a.G;
 
+  // ---- this lane's row (rows past the end repeat the last one and are not stored)
+  const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
+  const int r = min(row0 + col, a.R - 1);
+  const int rt = r / a.by_T, t = r - rt * a.T, w = rt / a.by_G, g = rt - w * G;
+  const int64_t n = (int64_t)b * a.W + w;
+  const int h = kh * G + g;
+  const T* const kind = nullptr;
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
+  u32x4 qr[4 * KS];        // q: elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7
+  // 16-bit rows (of q, of the suffix) into LDS, `count` of them (16 or 32), lane i's
+  // `at` the offset of row i: whole rows at a time, chunk c of row r at place c ^
+  // sw(r)
+  constexpr int CPV = D / 8, RPV = 512 / D;          // 16-byte chunks per row, rows per load
+  auto of_lane = [](int64_t v, int from) {
+    return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
+                     (uint64_t)(uint32_t)__shfl((int)(v >> 32), from, 64) << 32);
+  };
+  auto load_rows = [&](auto count_c, auto values_c, const T* base, int64_t at, uint32_t dst) {
+    constexpr bool kValues = decltype(values_c)::value;   // (read by transposes)
+    constexpr int LOADS = decltype(count_c)::value / RPV;
+    const T* src[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = i * RPV + lane / CPV;
+      const int sw = !kValues ? row & 7 : D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4;
+      src[i] = base + of_lane(at, row) + ((lane % CPV) ^ sw) * 8;
+    }
+    __builtin_amdgcn_sched_barrier(0);   // (the exchanges first, all at once)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load_lds16(src[i], dst + i * 1024);
+  };
+  auto row_chunk = [&](const uint8_t* area, int row, int c) {
+    const int chunk = 8 * (c >> 2) + 4 * (c >> 1 & 1) + 2 * hi + (c & 1);
+    return *(const u32x4*)(area + row * 2 * D + (chunk ^ (row & 7)) * 16);
+  };
+  using n16 = std::integral_constant<int, 16>;
+  using n32 = std::integral_constant<int, 32>;
+  using yes = std::integral_constant<bool, true>;
+  using no = std::integral_constant<bool, false>;
+  auto load_q = [&](uint32_t dst) {
+    load_rows(n32{}, no{}, (const T*)a.q, n * a.sq_n + t * a.sq_t + h * a.sq_h, dst);
+  };
+  auto take_q = [&](const uint8_t* area) {
+#pragma unroll
+    for (int c = 0; c < 4 * KS; ++c) qr[c] = row_chunk(area, col, c);
+  };
+  const bool has_suffix = a.Tk > 0 && split == 0 && (SHARED || wave == 3);
+  int vlo = 0, vhi = -1, keys = 0;                   // keys the row sees, keys of the wave
+  const int w0 = min(row0, a.R - 1) / a.by_T / a.by_G;
+  const int64_t n0 = (int64_t)b * a.W + w0;
+  if (has_suffix) {
+    vlo = (w - w0) * a.Tk;
+    vhi = vlo + a.Tk - a.T + t;
+    keys = vhi + 1;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o, 64));
+    keys = __builtin_amdgcn_readfirstlane(keys);
+  }
+  auto suffix_load = [&](uint32_t dst, int f0) {
+    const int f = min(f0 + (lane & 15), keys - 1), beam = f / a.by_Tk, token = f - beam * a.Tk;
+    load_rows(n16{}, no{}, (const T*)a.sk,
+              (n0 + beam) * a.ssk_n + (int64_t)token * a.ssk_t + kh * a.ssk_h, dst);
+    load_rows(n16{}, yes{}, (const T*)a.sv,
+              (n0 + beam) * a.ssv_n + (int64_t)token * a.ssv_t + kh * a.ssv_h, dst + 32 * D);
+  };
+  // q and the suffix, where a V tile and a K tile will go
+  auto load_first = [&]() {
+    load_q(lds0 + (SHARED ? 4 + wave : 2 * wave + 1) * S::tile);
+    if (has_suffix) suffix_load(lds0 + (SHARED ? wave : 2 * wave) * S::tile, 0);
+  };
+  load_first();
+
   // ---- this wave's tiles of the prefix: first + stride * k, k < count.  (With one
   // range the first pages do not wait for the length.)
   int first_page = 0;
@@ -344,14 +417,6 @@ block_attn_kernel(BlockAttnArgs a) {
   };
   if (a.splits > 1) first_page = page_at(0);
 
-  // ---- this lane's row (rows past the end repeat the last one and are not stored)
-  const int row0 = qb * (SHARED ? 128 : 32) + (SHARED ? wave * 32 : 0);
-  const int r = min(row0 + col, a.R - 1);
-  const int rt = r / a.by_T, t = r - rt * a.T, w = rt / a.by_G, g = rt - w * G;
-  const int64_t n = (int64_t)b * a.W + w;
-  const int h = kh * G + g;
-  const T* const kind = nullptr;
-
   // ---- loads of a tile.  Instruction i of a K or V tile brings keys i * RPI +
   // lane / CPR; at place lane % CPR of a key goes the chunk that the swizzle puts
   // there.  Keys past those held arrive as zeros.
@@ -367,7 +432,6 @@ block_attn_kernel(BlockAttnArgs a) {
     return (uint32_t)((row & 31) * D - i % 4 * 1024 +
                       (d_pc ^ (kv ? S::swv(row) : S::swk(row))) * 16);
   };
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
 
   // LDS offsets of the fragments
   uint32_t k_off[KS][2];   // K: key col of a half, chunks 4 s + hi and 4 s + 2 + hi
@@ -408,14 +472,8 @@ block_attn_kernel(BlockAttnArgs a) {
   float m = -INFINITY, m_true, l;
   bool over, spoilt = false;
   f32x16 O[DT];
-  u32x4 qr[4 * KS];        // q: elements 64 s + 32 (c / 2) + 16 hi + 8 (c % 2) + 0..7
   i32x8 qf[NP][KS];        // q in e4m3 pieces against the row's power of two
   int qs[NP];
-  auto load_q = [&]() {
-    const T* qrow = (const T*)a.q + n * a.sq_n + t * a.sq_t + h * a.sq_h + 16 * hi;
-#pragma unroll
-    for (int c = 0; c < 4 * KS; ++c) qr[c] = *(const u32x4*)(qrow + 32 * (c >> 1) + 8 * (c & 1));
-  };
   auto split_q = [&]() {
     float amax = 0.f;
 #pragma unroll
@@ -448,68 +506,35 @@ block_attn_kernel(BlockAttnArgs a) {
   };
 
   // ---- the beams' own suffixes.  The suffix keys of the wave's beams, in order,
-  // are its key rows: of group after group of 32, S^T = K Q^T over all of them,
+  // are its key rows: of group after group of 16, S^T = K Q^T over all of them,
   // masked to each row's beam and to the tokens before its own, then O^T += V^T
-  // P^T from LDS (area: 64 * D bytes of the wave's own).  A value that is not
+  // P^T, both from LDS (area: 64 * D bytes of the wave's own).  A value that is not
   // finite would reach the rows that do not see it as 0 * inf, so a group that
   // holds one is multiplied without it, and the rows that do see it add it at the
-  // end.
-  const bool has_suffix = a.Tk > 0 && split == 0 && (SHARED || wave == 0);
-  int vlo = 0, vhi = -1, keys = 0;                   // keys the row sees, keys of the wave
-  const int w0 = min(row0, a.R - 1) / a.by_T / a.by_G;
-  const int64_t n0 = (int64_t)b * a.W + w0;
-  constexpr int CPV = D / 8, RPV = 512 / D;          // chunks per V row, rows per load
-  u32x4 kr[4 * KS];
-  if (has_suffix) {
-    vlo = (w - w0) * a.Tk;
-    vhi = vlo + a.Tk - a.T + t;
-    keys = vhi + 1;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) keys = max(keys, __shfl_xor(keys, o, 64));
-    keys = __builtin_amdgcn_readfirstlane(keys);
-  }
-  auto of_lane = [](int64_t v, int from) {
-    return (int64_t)((uint64_t)(uint32_t)__shfl((int)v, from, 64) |
-                     (uint64_t)(uint32_t)__shfl((int)(v >> 32), from, 64) << 32);
-  };
-  auto suffix_load = [&](uint8_t* area, int f0) {
-    const uint32_t area_at = (uint32_t)(uintptr_t)(lds_t*)area;
-    const int f = min(f0 + col, keys - 1), beam = f / a.by_Tk, token = f - beam * a.Tk;
-    const T* krow = (const T*)a.sk + (n0 + beam) * a.ssk_n + (int64_t)token * a.ssk_t +
-                    kh * a.ssk_h + 16 * hi;
-#pragma unroll
-    for (int c = 0; c < 4 * KS; ++c)
-      kr[c] = *(const u32x4*)(krow + 32 * (c >> 1) + 8 * (c & 1));
-    const int64_t v_at = (n0 + beam) * a.ssv_n + (int64_t)token * a.ssv_t + kh * a.ssv_h;
-    const int pieces = (keys - f0 > 16 ? 32 : 16) / RPV;   // 16 or 32 rows of V
-#pragma unroll 2
-    for (int i = 0; i < pieces; ++i) {
-      const int row = i * RPV + lane / CPV;
-      const int chunk = (lane % CPV) ^ (D == 64 ? (row >> 1 & 1) * 4 : (row & 3) * 4);
-      const T* src = (const T*)a.sv + of_lane(v_at, row) + chunk * 8;
-      load_lds16(src, area_at + i * 1024);
-    }
-  };
-  // in_flight: loads issued after the first group's
-  auto suffix = [&](uint8_t* area, int in_flight) {
+  // end.  (In the private form the last wave does it, which has the fewest tiles.)
+  // (the first group is there)
+  auto suffix = [&](uint8_t* area, uint32_t area_at) {
     const float mul = a.qmul * a.sl2;
     constexpr float kUp = std::is_same<T, bf16_t>::value ? kMaxUp : 14.f;
+    const uint8_t* values = area + 32 * D;
     const int gi = lane & 15, s_row = 4 * hi + (gi >> 2);
     const int s_d = (lane >> 4 & 1) * 16 + (gi & 3) * 4;
     const int s_sw = D == 64 ? (s_row >> 1 & 1) * 4 : (s_row & 3) * 4;
+    const uint32_t base = area_at + 32 * D + s_row * D * 2 + (s_d & 7) * 2;
 #pragma unroll 1
-    for (int f0 = 0; f0 < keys; f0 += 32) {
-      const bool both = keys - f0 > 16;
+    for (int f0 = 0; f0 < keys; f0 += 16) {
       if (f0 > 0) {
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-        suffix_load(area, f0);
+        suffix_load(area_at, f0);
+        wait_vm(0);
       }
       f32x16 st = f32x16{};
 #pragma unroll
-      for (int c = 0; c < 4 * KS; ++c) st = mfma_wide(kind, kr[c], qr[c], st);
+      for (int c = 0; c < 4 * KS; ++c)
+        st = mfma_wide(kind, row_chunk(area, col & 15, c), qr[c], st);
+      // (key rows 16 to 31 repeat the first ones)
       float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const int f = f0 + 8 * (j >> 2) + 4 * hi + (j & 3);
         st[j] = f >= vlo && f <= vhi ? st[j] * mul : -INFINITY;
         top = fmaxf(top, st[j]);
@@ -519,31 +544,30 @@ block_attn_kernel(BlockAttnArgs a) {
       if (m == -INFINITY) m = top;
       over |= top > m + kUp;
       const float ref = m == -INFINITY ? 0.f : m;
-      u32x4 pk[2];
+      u32x4 p;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
+      for (int j = 0; j < 8; j += 2) {
         const float x = __builtin_amdgcn_exp2f(st[j] - ref);
         const float y = __builtin_amdgcn_exp2f(st[j + 1] - ref);
         sum += x + y;
-        pk[j >> 3][j >> 1 & 3] = pack2(kind, x, y);
+        p[j >> 1] = pack2(kind, x, y);
       }
       l += add_xor32(sum);
-      if (f0 == 0) wait_vm(in_flight);
-      else wait_vm(0);
       // (each lane looks at what its own loads brought)
       uint32_t top_exp = 0;
-      const int pieces = (both ? 32 : 16) / RPV;
-      for (int i = 0; i < pieces; ++i) {
-        const u32x4 x = *(const u32x4*)(area + i * 1024 + lane * 16);
+#pragma unroll
+      for (int i = 0; i < 16 / RPV; ++i) {
+        const u32x4 x = *(const u32x4*)(values + i * 1024 + lane * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) top_exp = max_u16x2(top_exp, x[e] & kExponents<T>);
       }
       const uint32_t full = kExponents<T> & 0xffffu;
       const bool bad = __ballot((top_exp & 0xffffu) == full || top_exp >> 16 == full) != 0;
       if (bad) {
-        for (int i = 0; i < pieces; ++i) {
-          uint16_t* x = (uint16_t*)(area + i * 1024 + lane * 16);
+#pragma unroll 1
+        for (int i = 0; i < 16 / RPV; ++i) {
+          uint16_t* x = (uint16_t*)(values + i * 1024 + lane * 16);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if ((x[e] & full) == full) x[e] = 0;
@@ -551,19 +575,13 @@ block_attn_kernel(BlockAttnArgs a) {
         __builtin_amdgcn_s_waitcnt(0xc07f);
       }
       spoilt |= bad;
-#pragma unroll 1
-      for (int ks = 0; ks < (both ? 2 : 1); ++ks) {
-        const uint32_t base =
-            (uint32_t)(uintptr_t)(area + (16 * ks + s_row) * D * 2 + (s_d & 7) * 2);
-        const u32x4 p = ks ? pk[1] : pk[0];
 #pragma unroll
-        for (int d2 = 0; d2 < DT / 2; ++d2) {
-          u32x4 x, y;
-          read_wide2<D>(base + ((((64 * d2 + s_d) >> 3) ^ s_sw) * 16),
-                        base + ((((64 * d2 + 32 + s_d) >> 3) ^ s_sw) * 16), x, y);
-          O[2 * d2] = mfma_wide(kind, x, p, O[2 * d2]);
-          O[2 * d2 + 1] = mfma_wide(kind, y, p, O[2 * d2 + 1]);
-        }
+      for (int d2 = 0; d2 < DT / 2; ++d2) {
+        u32x4 x, y;
+        read_wide2<D>(base + ((((64 * d2 + s_d) >> 3) ^ s_sw) * 16),
+                      base + ((((64 * d2 + 32 + s_d) >> 3) ^ s_sw) * 16), x, y);
+        O[2 * d2] = mfma_wide(kind, x, p, O[2 * d2]);
+        O[2 * d2 + 1] = mfma_wide(kind, y, p, O[2 * d2 + 1]);
       }
     }
   };
@@ -648,6 +666,14 @@ block_attn_kernel(BlockAttnArgs a) {
   };
   constexpr int SL = 33;
 
+  const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
+  const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
+  const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
+  const bool gated = a.gate != nullptr && a.splits == 1;
+  constexpr int STEPS = 32 / RPV;                // SHARED: RPV rows a step, 8 elements a lane
+  const int sub = lane / CPV, d0 = lane % CPV * 8;
+  u32x4 gv[STEPS];
+
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
     l = 0.f;
@@ -655,7 +681,6 @@ block_attn_kernel(BlockAttnArgs a) {
     over = false;
 #pragma unroll
     for (int i = 0; i < DT; ++i) O[i] = f32x16{};
-    load_q();
     if constexpr (SHARED) {
       // Two rings of 4 tiles, K's and then V's.  Step k forms the scores of tile
       // k + 1 and adds tile k - 1 to the output while the vector unit turns tile
@@ -692,9 +717,13 @@ block_attn_kernel(BlockAttnArgs a) {
         ring[x][0] = __builtin_amdgcn_readlane(meta, 2 * (k & 31));
         ring[x][1] = __builtin_amdgcn_readlane(meta, 2 * (k & 31) + 1);
       };
-      uint8_t* area = smem + (4 + wave) * S::tile;   // the suffix: where V's tiles go
-      if (has_suffix) suffix_load(area, 0);
+      if (pass > 0) load_first();
       describe(0, first_page);
+      wait_vm(0);
+      take_q(smem + (4 + wave) * S::tile);
+      if (has_suffix) suffix(smem + wave * S::tile, lds0 + wave * S::tile);
+      __builtin_amdgcn_s_waitcnt(0xc07f);     // (q is read)
+      tile_barrier();
       ring[0][0] = ring[0][1] = 127 << 8 | 127 << 16;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -702,10 +731,6 @@ block_attn_kernel(BlockAttnArgs a) {
         read_half(k < 2 ? 2 : k - 2, k);
         issue(0, k, source(a.kc, own_lo[k < 2 ? 2 : k - 2], own_hi[k < 2 ? 2 : k - 2],
                            own_held[k < 2 ? 2 : k - 2]));
-      }
-      if (has_suffix) {
-        suffix(area, 4 * LW);
-        tile_barrier();
       }
       issue(1, -1, source(a.vc, 0, 0, 0));
       read_half(2, 0);
@@ -789,6 +814,17 @@ block_attn_kernel(BlockAttnArgs a) {
           own_held[x] = own_held[x + 1];
         }
       }
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) gv[s] = u32x4{};
+      if (gated) {                            // (on their way during the last tile)
+        const T* src[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+          src[s] = (const T*)a.gate + of_lane(gate_at, s * RPV + sub) + d0;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) gv[s] = *(const u32x4*)src[s];
+        __builtin_amdgcn_sched_barrier(0);
+      }
       // the last tile's output
       const bool any = __ballot(over) != 0;
       if (lane == 0) sm_over[wave] = any;
@@ -823,10 +859,18 @@ block_attn_kernel(BlockAttnArgs a) {
           });
         }
       };
-      if (has_suffix) suffix_load(mine + S::tile, 0);   // where V goes
+      if (pass > 0) load_first();
       describe(0, first_page);
-      issue(0, 0);
-      if (has_suffix) suffix(mine + S::tile, S::LT);
+      if (!has_suffix) issue(0, 0);
+      if (has_suffix) wait_vm(0);
+      else wait_vm(S::LT);
+      take_q(mine + S::tile);
+      if (has_suffix) {
+        suffix(mine, mine_at);
+        issue(0, 0);
+      }
+      __builtin_amdgcn_s_waitcnt(0xc07f);     // (q is read)
+      __builtin_amdgcn_sched_barrier(0);
       issue(1, 0);
       split_q();
 #pragma unroll 1
@@ -864,72 +908,76 @@ block_attn_kernel(BlockAttnArgs a) {
     first_page = page_at(0);
   }
 
-  const int64_t out_at = n * a.so_n + t * a.so_t + h * a.so_h;
-  const int64_t gate_at = n * a.sg_n + t * a.sg_t + h * a.sg_h;
-  const int rows = min(32, a.R - row0);          // (none or fewer for waves past the end)
-  const bool gated = a.gate != nullptr && a.splits == 1;
-  if constexpr (SHARED) {
-    // ---- each lane has its row's elements 8 q + 4 hi + 0..3; lanes l and l ^ 32
-    // exchange halves, so that each holds 8 in a row, 16 bytes of the output
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const bool mine = col < rows;
-    const int64_t part = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + col;
-    if (mine) {
+  float* ep = (float*)smem + wave * 32 * S::EpiLd;
+  auto rows_to_lds = [&]() {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(O[dt][8 * j + i]),
-                                                            __float_as_uint(O[dt][8 * j + 4 + i]),
-                                                            false, false);
-            y[i] = __uint_as_float(x[0]);
-            y[4 + i] = __uint_as_float(x[1]);
-          }
-          const int d = 32 * dt + 16 * j + 8 * hi;
-          if (a.splits > 1) {
-            *(f32x4*)(a.part_o + part * D + d) = f32x4{y[0], y[1], y[2], y[3]};
-            *(f32x4*)(a.part_o + part * D + d + 4) = f32x4{y[4], y[5], y[6], y[7]};
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] *= inv;
-            if (gated) gate8(kind, *(const u32x4*)((const T*)a.gate + gate_at + d), y);
-            *(u32x4*)((T*)a.out + out_at + d) =
-                u32x4{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3]), pack2(kind, y[4], y[5]),
-                      pack2(kind, y[6], y[7])};
-          }
-        }
-      if (a.splits > 1 && hi == 0) {
-        a.part_ml[2 * part] = m;
-        a.part_ml[2 * part + 1] = l;
-      }
-    }
-    if (spoilt) {
-      // values that are not finite, to the rows that see them: their sum is the
-      // element, whatever the weights
-      wait_vm(0);
+      for (int q4 = 0; q4 < 4; ++q4)
+        *(f32x4*)(ep + col * S::EpiLd + 32 * dt + 8 * q4 + 4 * hi) =
+            f32x4{O[dt][4 * q4], O[dt][4 * q4 + 1], O[dt][4 * q4 + 2], O[dt][4 * q4 + 3]};
+    if (spoilt) {   // values that are not finite to the rows that see them
       const int64_t v_at = n * a.ssv_n + kh * a.ssv_h;
 #pragma unroll 1
-      for (int i = 0; i < rows; ++i) {
+      for (int i = 0; i < 32; ++i) {
         const T* vr = (const T*)a.sv + of_lane(v_at, i);
         const int last = a.Tk - a.T + __shfl(t, i, 64);
-        T* out = (T*)a.out + of_lane(out_at, i);
-        float* o = a.part_o + of_lane(part, i) * D;
 #pragma unroll 1
-        for (int d = lane; d < D; d += 64) {
-          float sum_bad = 0.f;
-          for (int j = 0; j <= last; ++j) {
-            const float x = Elem<T>::to_f(vr[(int64_t)j * a.ssv_t + d]);
-            if (!(fabsf(x) < INFINITY)) sum_bad += x;
-          }
-          if (sum_bad != 0.f) {
-            if (a.splits > 1) o[d] = sum_bad;
-            else out[d] = Elem<T>::from_f(sum_bad);
-          }
+        for (int e = lane; e < (last + 1) * D; e += 64) {
+          const float x = Elem<T>::to_f(vr[(int64_t)(e / D) * a.ssv_t + e % D]);
+          if (!(fabsf(x) < INFINITY)) ep[i * S::EpiLd + e % D] += x;
         }
       }
+    }
+  };
+  if constexpr (SHARED) {
+    // ---- the wave's rows through LDS, RPV rows at a time, 8 elements a lane: whole
+    // rows of gates in and of results out
+    __syncthreads();                // the rings are free
+    rows_to_lds();
+    if (a.splits > 1) {
+      const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + row0;
+      if (hi == 0 && col < rows) {
+        a.part_ml[2 * (at + col)] = m;
+        a.part_ml[2 * (at + col) + 1] = l;
+      }
+#pragma unroll 4
+      for (int s = 0; s < STEPS; ++s) {
+        const int i = s * RPV + sub;
+        if (i < rows) {
+          float* o = a.part_o + (at + i) * D + d0;
+          *(f32x4*)o = *(const f32x4*)(ep + i * S::EpiLd + d0);
+          *(f32x4*)(o + 4) = *(const f32x4*)(ep + i * S::EpiLd + d0 + 4);
+        }
+      }
+      return;
+    }
+    T* to[STEPS];
+    float inv[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      to[s] = (T*)a.out + of_lane(out_at, s * RPV + sub) + d0;
+      inv[s] = __shfl(l, s * RPV + sub, 64);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 x[2][2];
+    auto fetch = [&](int s) {
+      const float* o = ep + (s * RPV + sub) * S::EpiLd + d0;
+      x[s & 1][0] = *(const f32x4*)o;
+      x[s & 1][1] = *(const f32x4*)(o + 4);
+    };
+    fetch(0);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s + 1 < STEPS) fetch(s + 1);
+      const float f = inv[s] == 0.f ? 0.f : __builtin_amdgcn_rcpf(inv[s]);
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[s & 1][i >> 2][i & 3] * f;
+      if (gated) gate8(kind, gv[s], y);
+      if (s * RPV + sub < rows)
+        *(u32x4*)to[s] = u32x4{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3]),
+                               pack2(kind, y[4], y[5]), pack2(kind, y[6], y[7])};
     }
     return;
   }
@@ -938,8 +986,8 @@ block_attn_kernel(BlockAttnArgs a) {
   // (or left as a partial result).  A wave takes 256 / D rows at a time, 4 elements
   // a lane.
   constexpr int LPR = D / 4, RPS = 64 / LPR;     // lanes per row, rows per step
-  constexpr int STEPS = (32 / RPS + 3) / 4;
-  const int sub = lane / LPR, d0 = lane % LPR * 4;
+  constexpr int TURNS = (32 / RPS + 3) / 4;
+  const int psub = lane / LPR, pd0 = lane % LPR * 4;
   auto first_row = [&](int s) { return (4 * s + wave) * RPS; };
   // the value of the row that this lane stores in step s
   auto of_row = [&](int64_t v, int s) {
@@ -948,42 +996,23 @@ block_attn_kernel(BlockAttnArgs a) {
       return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, i) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32);
     } else {
-      return of_lane(v, first_row(s) + sub);
+      return of_lane(v, first_row(s) + psub);
     }
   };
   wait_vm(0);
   __syncthreads();
-  float* ep = (float*)smem + wave * 32 * S::EpiLd;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-      *(f32x4*)(ep + col * S::EpiLd + 32 * dt + 8 * q4 + 4 * hi) =
-          f32x4{O[dt][4 * q4], O[dt][4 * q4 + 1], O[dt][4 * q4 + 2], O[dt][4 * q4 + 3]};
-  if (spoilt) {   // values that are not finite to the rows that see them
-    const int64_t v_at = n * a.ssv_n + kh * a.ssv_h;
-#pragma unroll 1
-    for (int i = 0; i < 32; ++i) {
-      const T* vr = (const T*)a.sv + of_lane(v_at, i);
-      const int last = a.Tk - a.T + __shfl(t, i, 64);
-#pragma unroll 1
-      for (int e = lane; e < (last + 1) * D; e += 64) {
-        const float x = Elem<T>::to_f(vr[(int64_t)(e / D) * a.ssv_t + e % D]);
-        if (!(fabsf(x) < INFINITY)) ep[i * S::EpiLd + e % D] += x;
-      }
-    }
-  }
+  rows_to_lds();
   if (hi == 0) {
     sm_m[wave][col] = m;
     sm_l[wave][col] = l;
   }
   __syncthreads();
 #pragma unroll 1
-  for (int s = 0; s < STEPS && first_row(s) < rows; ++s) {
-    const int i = first_row(s) + sub;
+  for (int s = 0; s < TURNS && first_row(s) < rows; ++s) {
+    const int i = first_row(s) + psub;
     const int64_t to = of_row(out_at, s), gate_to = of_row(gate_at, s);
     u32x2 gate = u32x2{};
-    if (gated) gate = *(const u32x2*)((const T*)a.gate + gate_to + d0);
+    if (gated) gate = *(const u32x2*)((const T*)a.gate + gate_to + pd0);
     const float mm = fmaxf(fmaxf(sm_m[0][i], sm_m[1][i]), fmaxf(sm_m[2][i], sm_m[3][i]));
     float ll = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -991,20 +1020,20 @@ block_attn_kernel(BlockAttnArgs a) {
       const float mx = sm_m[x][i];
       const float f = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mm);
       ll = fmaf(f, sm_l[x][i], ll);
-      const f32x4 y = *(const f32x4*)((float*)smem + (x * 32 + i) * S::EpiLd + d0);
+      const f32x4 y = *(const f32x4*)((float*)smem + (x * 32 + i) * S::EpiLd + pd0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
     }
     if (i < rows) {
       if (a.splits > 1) {
         const int64_t at = ((int64_t)split * a.B * a.HK + bk) * a.R + row0 + i;
-        *(f32x4*)(a.part_o + at * D + d0) = f32x4{o[0], o[1], o[2], o[3]};
-        if (d0 == 0) {
+        *(f32x4*)(a.part_o + at * D + pd0) = f32x4{o[0], o[1], o[2], o[3]};
+        if (pd0 == 0) {
           a.part_ml[2 * at] = mm;
           a.part_ml[2 * at + 1] = ll;
         }
       } else {
-        store_row4<T>((T*)a.out + to + d0, o, ll == 0.f ? 0.f : 1.f / ll, gated, gate);
+        store_row4<T>((T*)a.out + to + pd0, o, ll == 0.f ? 0.f : 1.f / ll, gated, gate);
       }
     }
   }
