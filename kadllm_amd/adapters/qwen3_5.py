@@ -24,6 +24,7 @@ import torch
 from ..config import Qwen35Config
 from ..grbeam import PrefillResult
 from ..ops import _gdn_launch
+from ..prefix_cache import HEAD_DIMS, PagedPrefix, paged_prefixes
 from ..qwen35 import LMHead, Qwen35Runner, Qwen35TextModel
 from ..qwen35_f32 import Qwen35RunnerF16, Qwen35RunnerF32
 
@@ -52,10 +53,18 @@ class Qwen35GRBeamAdapter:
     gdn_triton_config keeps its validation (tile_v, warps, stages[, beam_group])
     and its requirement of gdn_backend='triton'; the HIP kernel picks its own
     tiling.
+
+    prefix_cache="e4m3" (bf16 models with attention heads of 64, 128 or 256)
+    keeps the prefixes of the attention layers in 8-bit pages
+    (kadllm_amd.prefix_cache) instead of bf16: half the memory, each key and
+    value rounded to an e4m3 multiple of its page's scale.  The attention layers
+    of such a prefix are PagedPrefix tuples, and decode_incremental's logits
+    equal decode's to rounding instead of bit for bit.
     """
 
     def __init__(self, text_model, lm_head, *, gdn_backend="torch", conv_backend="torch",
-                 attention_backend="torch", gdn_triton_config=None, head_tokens=None):
+                 attention_backend="torch", gdn_triton_config=None, head_tokens=None,
+                 prefix_cache=None):
         native = isinstance(text_model, Qwen35TextModel)
         if not native and not _is_transformers_text_model(text_model):
             raise TypeError("pass the dense Qwen3_5TextModel explicitly")
@@ -90,6 +99,12 @@ class Qwen35GRBeamAdapter:
         else:
             raise TypeError("the HIP GRBeam path runs bf16, fp16 or fp32 models with one dtype; "
                             "convert with .to()")
+        if prefix_cache not in (None, "e4m3"):
+            raise ValueError("prefix_cache must be None or 'e4m3'")
+        if prefix_cache is not None and (runner is not Qwen35Runner
+                                         or cfg.head_dim not in HEAD_DIMS):
+            raise ValueError("an 8-bit prefix cache needs a bf16 model with attention heads of "
+                             "64, 128 or 256")
         if device.type != "cuda":
             raise RuntimeError("the HIP GRBeam path needs the model on a ROCm device")
         self.layer_types = tuple(cfg.layer_types)
@@ -97,6 +112,7 @@ class Qwen35GRBeamAdapter:
         self.gdn_backend, self.conv_backend = gdn_backend, conv_backend
         self.attention_backend = attention_backend
         self.gdn_triton_config = gdn_triton_config
+        self.prefix_cache = prefix_cache
         self.config = cfg if native else Qwen35Config.from_hf(cfg)
         self.device = device
         self._runner = runner(self.config, text_model.state_dict(),
@@ -140,6 +156,16 @@ class Qwen35GRBeamAdapter:
         if lo < 0 or hi >= self.config.vocab_size:
             raise IndexError("index out of range in self")
 
+    def _store(self, layers):
+        """The prefix layers as this adapter keeps them."""
+        attention = [i for i, kind in enumerate(self.layer_types) if kind == "full_attention"]
+        if self.prefix_cache is None or not attention:
+            return tuple(layers)
+        layers = list(layers)
+        for i, paged in zip(attention, paged_prefixes([layers[i] for i in attention])):
+            layers[i] = paged
+        return tuple(layers)
+
     @torch.no_grad()
     def prefill(self, input_ids):
         self._check(input_ids)
@@ -147,6 +173,7 @@ class Qwen35GRBeamAdapter:
             raise ValueError("input_ids must be nonempty unpadded [B,L]")
         probe = self._range_probe(input_ids)
         logits, layers = self._runner.prefill(input_ids)
+        layers = self._store(layers)
         self._raise_out_of_range(probe)
         state = Qwen35Prefix(input_ids.shape[1], input_ids.shape[0], self._owner, layers)
         return PrefillResult(logits, state)
@@ -186,7 +213,7 @@ class Qwen35GRBeamAdapter:
             else:
                 layers.append((a.to(self.device, act), b.to(self.device, act)))
         batch = layers[0][0].shape[0]
-        return Qwen35Prefix(int(length), batch, self._owner, tuple(layers))
+        return Qwen35Prefix(int(length), batch, self._owner, self._store(layers))
 
     def prefix_to_cache(self, state, hf_config=None):
         """A transformers DynamicCache holding this adapter's prefix."""
@@ -194,6 +221,8 @@ class Qwen35GRBeamAdapter:
 
         if not isinstance(state, Qwen35Prefix) or state.owner is not self._owner:
             raise ValueError("prefix belongs to a different adapter")
+        if any(isinstance(layer, PagedPrefix) for layer in state.layers):
+            raise ValueError("an 8-bit prefix has no transformers form")
         return cache_from_prefix_layers(state.layers, self.layer_types,
                                         hf_config if hf_config is not None else self.config.to_hf())
 

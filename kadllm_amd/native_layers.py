@@ -10,6 +10,7 @@ import operator
 import torch
 
 from . import _lib
+from .prefix_cache import PagedPrefix
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -163,6 +164,8 @@ class NativeLayers:
         """Whether kad_qwen_decode_step takes this level: two tokens at most,
         attention prefixes it can read in place."""
         if not self.step_shapes or T > 2:
+            return False
+        if any(isinstance(layer, PagedPrefix) for layer in prefix_layers):
             return False
         for (a, b), lin in zip(prefix_layers, self.linear):
             if a.dtype != torch.bfloat16:

@@ -238,30 +238,25 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
             raise ValueError("attention inputs must have the same dtype")
     if gate is not None and (gate.shape != (BW, T, H * D) or gate.dtype is not dtype):
         raise ValueError("gate must be [B*W, T, H*D] in the query dtype")
-    if torch.is_grad_enabled() and (
-            q.requires_grad or (suffix_k is not None and (suffix_k.requires_grad
-                                                          or suffix_v.requires_grad))
-            or (gate is not None and gate.requires_grad)):
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad
+                                       for x in (q, suffix_k, suffix_v, gate)):
         raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
     _device_of(q, tables, lengths, suffix_k, suffix_v, gate, *blocks)
-    gate_strides = None
-    if gate is not None:
-        gate = _rows(gate, 8)
-        gate_strides = (gate.stride(0), gate.stride(1), D)
     return _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width,
-                            D ** -0.5 if scale is None else scale, gate, gate_strides)
+                            D ** -0.5 if scale is None else scale,
+                            gate if gate is None else gate.view(BW, T, H, D))
 
 
-def _rows(t, elements):
-    """t, or a copy whose rows start at multiples of ``elements`` (a power of
-    two) 16-bit elements."""
-    *outer, inner = t.stride()
-    bits = 0
-    for s in outer:
-        bits |= s
-    if inner == 1 and not bits % elements and not t.data_ptr() % (2 * elements):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows(t):
+    """(t, its address, its first three strides); a copy where t's rows do not
+    start at 16-byte boundaries (of 16-bit elements)."""
+    a, b, c, d = t.stride()
+    p = t.data_ptr()
+    if d != 1 or (a | b | c) & 7 or p & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        a, b, c, _ = t.stride()
+        p = t.data_ptr()
+    return t, p, a, b, c
 
 
 @functools.lru_cache(maxsize=1024)
@@ -271,33 +266,61 @@ def _workspace_bytes(*sizes):
     return need.value
 
 
-_NONE = (None, 0, 0, 0)
+_NONE = (None, None, 0, 0, 0)
 
 
-def _strided(t):
-    return (t.data_ptr(), *t.stride()[:3])
-
-
-def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale, gate=None,
-                     gate_strides=None):
-    """block_prefix_attention on checked arguments; ``gate`` any tensor whose
-    data pointer is head 0's gate with element strides ``gate_strides`` =
-    (beam, token, head)."""
+def _block_attention(q, blocks, tables, lengths, suffix_k, suffix_v, beam_width, scale,
+                     gate=None):
+    """block_prefix_attention on checked arguments, with ``gate`` [B*W, T, H, D]
+    of any strides."""
     BW, T, H, D = q.shape
-    pages, HK, block, _ = blocks.k.shape
+    k, v, k_scale, v_scale = blocks
+    pages, HK, block, _ = k.shape
     B, width = BW // beam_width, tables.shape[1]
-    q = _rows(q, 8)
-    Tk, sk, sv, g = 0, _NONE, _NONE, _NONE
-    if suffix_k is not None:
-        suffix_k, suffix_v = _rows(suffix_k, 8), _rows(suffix_v, 8)
-        Tk, sk, sv = suffix_k.shape[1], _strided(suffix_k), _strided(suffix_v)
-    if gate is not None:
-        g = (gate.data_ptr(), *gate_strides)
-    out = torch.empty((BW, T, H, D), dtype=q.dtype, device=q.device)
+    q, *q_at = _rows(q)
+    Tk = 0 if suffix_k is None else suffix_k.shape[1]
+    sk, *sk_at = _NONE if suffix_k is None else _rows(suffix_k)
+    sv, *sv_at = _NONE if suffix_v is None else _rows(suffix_v)
+    g, *g_at = _NONE if gate is None else _rows(gate)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     need = _workspace_bytes(B, beam_width, T, H, HK, D, width, block)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch(q.get_device(), "kad_block_prefix_attention", *_strided(q),
-            *[x.data_ptr() for x in blocks], pages, tables.data_ptr(), width, lengths.data_ptr(),
-            *sk, *sv, *g, out.data_ptr(), T * H * D, H * D, D, _lib.ptr(ws), need, B, beam_width,
-            T, Tk, H, HK, D, block, _lib.DTYPE_CODES[q.dtype], float(scale))
+    _launch(q.get_device(), "kad_block_prefix_attention", *q_at, k.data_ptr(), v.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), pages, tables.data_ptr(), width,
+            lengths.data_ptr(), *sk_at, *sv_at, *g_at, out.data_ptr(), T * H * D, H * D, D,
+            _lib.ptr(ws), need, B, beam_width, T, Tk, H, HK, D, block, _lib.DTYPE_CODES[q.dtype],
+            float(scale))
     return out
+
+
+class PagedPrefix(NamedTuple):
+    """An attention layer's prefix in the 8-bit cache, in the place of the
+    layer's (K, V) pair."""
+
+    blocks: PrefixBlocks
+    tables: torch.Tensor
+    lengths: torch.Tensor
+
+
+def paged_prefixes(pairs, *, block_size=64):
+    """PagedPrefix for each (K, V) of ``pairs``, all [B, L, HK, D] of one shape: one
+    table for all layers, a pool each."""
+    K = pairs[0][0]
+    B, L, HK, D = K.shape
+    device = K.device
+    width = -(-L // block_size)
+    lengths = torch.full((B,), L, dtype=torch.int32, device=device)
+    tables, _ = prefix_block_tables(lengths, torch.arange(B * width, dtype=torch.int32,
+                                                          device=device),
+                                    block_size=block_size, max_length=L)
+    return [PagedPrefix(write_prefix_blocks(
+        PrefixBlocks.empty(B * width, HK, D, block_size=block_size, device=device), k, v, tables,
+        lengths), tables, lengths) for k, v in pairs]
+
+
+def paged_attention_decode(q, prefix, suffix_k, suffix_v, beam_width, scale, gate, gate_strides):
+    """attention.prefix_attention_decode over a PagedPrefix: ``gate`` any tensor
+    whose data pointer is head 0's gate with strides ``gate_strides`` = (beam,
+    token, head)."""
+    gate = gate.as_strided(q.shape, (*gate_strides, 1))
+    return _block_attention(q, *prefix, suffix_k, suffix_v, beam_width, scale, gate)

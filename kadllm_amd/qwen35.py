@@ -29,6 +29,17 @@ from . import _lib, layers
 from .native_layers import NativeLayers
 from .attention import attention_prefill, prefix_attention_decode
 from .ops import REPLAY_MAX_T
+from .prefix_cache import PagedPrefix, paged_attention_decode
+
+
+def _attend(q, prefix, k, v, W, scale, gate, gate_strides):
+    """Decode attention of an attention layer over its prefix, (K, V) in the
+    model's type or a PagedPrefix, and the suffixes k, v."""
+    if isinstance(prefix, PagedPrefix):
+        return paged_attention_decode(q, prefix, k, v, W, scale, gate, gate_strides)
+    return prefix_attention_decode(q, prefix[0], prefix[1], k, v, W, None, scale, gate=gate,
+                                   gate_strides=gate_strides)
+
 
 _BLOCK = 32  # gate/up interleave granularity of the SwiGLU epilogue
 
@@ -541,9 +552,8 @@ class Qwen35Runner:
                                     (0, nkv * hd, hd), R, R, hd, self.rot, self.inv_freq,
                                     prefix_length, T, cfg.rms_norm_eps)
                 v = proj[:, (2 * nh + nkv) * hd:].as_strided((BW, T, nkv, hd), (T * ld, ld, hd, 1))
-                att = prefix_attention_decode(q, cached[0], cached[1], k, v, W, None,
-                                              hd ** -0.5, gate=last_rows[:, hd:],
-                                              gate_strides=(T * ld, T * ld, 2 * hd))
+                att = _attend(q, cached, k, v, W, hd ** -0.5, last_rows[:, hd:],
+                              (T * ld, T * ld, 2 * hd))
                 layers.gemm(att.view(BW, nh * hd), lyr.w_o, out=x_last,
                             epilogue=layers.EPI_RESIDUAL, residual=x_last)
             else:
@@ -558,9 +568,8 @@ class Qwen35Runner:
                                     (0, nkv * hd, hd), R, R, hd, self.rot, self.inv_freq,
                                     prefix_length, T, cfg.rms_norm_eps)
                 v = proj[:, (2 * nh + nkv) * hd:].as_strided((BW, T, nkv, hd), (T * ld, ld, hd, 1))
-                att = prefix_attention_decode(q, cached[0], cached[1], k, v, W, None,
-                                              hd ** -0.5, gate=proj[:, hd:],
-                                              gate_strides=(T * ld, ld, 2 * hd))
+                att = _attend(q, cached, k, v, W, hd ** -0.5, proj[:, hd:],
+                              (T * ld, ld, 2 * hd))
                 layers.gemm(att.view(R, nh * hd), lyr.w_o, out=x,
                             epilogue=layers.EPI_RESIDUAL, residual=x)
             if terminal:
@@ -673,9 +682,8 @@ class Qwen35Runner:
                                     cfg.rms_norm_eps)
                 layers.scatter_heads(proj[:, (2 * nh + nkv) * hd:], ld, nkv, hd, v_all[:, T - 1],
                                      tok, BW, BW)
-                att = prefix_attention_decode(q, cached[0], cached[1], k_all, v_all, W, None,
-                                              hd ** -0.5, gate=proj[:, hd:],
-                                              gate_strides=(ld, ld, 2 * hd))
+                att = _attend(q, cached, k_all, v_all, W, hd ** -0.5, proj[:, hd:],
+                              (ld, ld, 2 * hd))
                 layers.gemm(att.view(BW, nh * hd), lyr.w_o, out=x, epilogue=layers.EPI_RESIDUAL,
                             residual=x)
                 if keep_cache:
