@@ -1056,18 +1056,36 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
   u32x2 gate = u32x2{};
   if (a.gate)
     gate = *(const u32x2*)((const T*)a.gate + n * a.sg_n + t * a.sg_t + h * a.sg_h + d0);
-  float mm = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part_ml[2 * (s * rows + row)]);
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = s * rows + row;
-    const float ms = a.part_ml[2 * at], ls = a.part_ml[2 * at + 1];
-    const f32x4 x = *(const f32x4*)(a.part_o + at * D + d0);
-    const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms - mm);
-    ll = fmaf(f, ls, ll);
+  // 8 ranges' loads at a time (those past the last repeat it, at no weight)
+  const float* ml = a.part_ml + 2 * row;
+  const float* po = a.part_o + row * D + d0;
+  float mm = -INFINITY, o[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    f32x4 x[8];
+    float ms[8], ls[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, x[e], o[e]);
+    for (int i = 0; i < 8; ++i) {
+      const int64_t s = min(s0 + i, a.splits - 1) * rows;
+      ms[i] = ml[2 * s];
+      ls[i] = ml[2 * s + 1];
+      x[i] = *(const f32x4*)(po + s * D);
+    }
+    float top = mm;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, ms[i]);
+    const float keep = mm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mm - top);
+    mm = top;
+    ll *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool none = ms[i] == -INFINITY || s0 + i >= a.splits;
+      const float f = none ? 0.f : __builtin_amdgcn_exp2f(ms[i] - mm);
+      ll = fmaf(f, ls[i], ll);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = none ? o[e] : fmaf(f, x[i][e], o[e]);
+    }
   }
   store_row4<T>((T*)a.out + n * a.so_n + t * a.so_t + h * a.so_h + d0, o,
                 ll == 0.f ? 0.f : 1.f / ll, a.gate != nullptr, gate);
