@@ -1109,11 +1109,11 @@ Plan plan_of(int B, int HK, int R, int D, int keys) {
   const int64_t blocks = (int64_t)B * HK * p.nqblk;
   const int64_t slots = D == 256 ? 256 : 512;      // workgroups that run at once
   const int step = p.shared ? 1 : 4;               // tiles a workgroup takes side by side
-  const int64_t tiles = kad_cdiv(keys, kKeys);
+  const int tiles = (int)kad_cdiv(keys, kKeys);
   p.splits = 1;
   int64_t best = INT64_MAX;
-  for (int s = 1; s <= 64 && (s == 1 || tiles >= (int64_t)s * step); ++s) {
-    const int64_t walk = kad_cdiv(kad_cdiv(tiles, s), step) + kStart;
+  for (int s = 1; s <= 64 && (s == 1 || tiles >= s * step); ++s) {
+    const int walk = ((tiles + s - 1) / s + step - 1) / step + kStart;
     const int64_t cost = kad_cdiv(blocks * s, slots) * walk + (s > 1 ? kJoin : 0);
     if (cost < best) {
       best = cost;
@@ -1121,6 +1121,10 @@ Plan plan_of(int B, int HK, int R, int D, int keys) {
     }
   }
   return p;
+}
+
+int64_t workspace_of(const Plan& p, int B, int HK, int R, int D) {
+  return p.splits > 1 ? (int64_t)p.splits * B * HK * R * (D + 2) * 4 : 0;
 }
 
 template <typename T, int D>
@@ -1168,8 +1172,7 @@ extern "C" int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, i
   KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
   const int64_t R = (int64_t)W * T * (H / HK);
   KAD_REQUIRE(R <= 0x7fffffff - 256, "%lld rows for a KV head", (long long)R);
-  const Plan p = plan_of(B, HK, (int)R, D, width * block);
-  *bytes = p.splits > 1 ? (int64_t)p.splits * B * HK * R * (D + 2) * 4 : 0;
+  *bytes = workspace_of(plan_of(B, HK, (int)R, D, width * block), B, HK, (int)R, D);
   return KAD_OK;
 }
 
@@ -1202,13 +1205,13 @@ extern "C" int kad_block_prefix_attention(
               "gate and output rows must be 16-byte aligned");
   if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
     KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
-  int64_t need = 0;
-  const int rc = kad_block_prefix_attention_workspace_bytes(B, W, T, H, HK, D, width, block, &need);
-  if (rc != KAD_OK) return rc;
-  KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
-              "a workspace of %lld bytes is needed", (long long)need);
+  KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
+  KAD_REQUIRE((int64_t)W * T * (H / HK) <= 0x7fffffff - 256, "too many rows for a KV head");
   const int R = W * T * (H / HK);
   const Plan p = plan_of(B, HK, R, D, width * block);
+  const int64_t need = workspace_of(p, B, HK, R, D);
+  KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+              "a workspace of %lld bytes is needed", (long long)need);
   KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff &&
                   kad_cdiv((int64_t)B * HK * R, 4) <= 0x7fffffff,
               "too many rows for a launch");

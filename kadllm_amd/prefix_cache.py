@@ -209,9 +209,8 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
     ``gate`` [B*W, T, H*D] multiplies the output by sigmoid(gate).  Returns
     [B*W, T, H, D] in q's type; a query that sees no key gets zeros.
     """
-    from .ops import _width
-
-    _width(beam_width)
+    if type(beam_width) is not int or beam_width <= 0:
+        raise ValueError("beam_width must be a positive integer")
     pages, HK, block, D = _check_blocks(blocks)
     shape = q.shape
     if len(shape) != 4 or shape[3] != D:
