@@ -273,6 +273,23 @@ __device__ __forceinline__ void store_row4(T* out, const float* o, float inv, bo
   *(u32x2*)out = u32x2{pack2(kind, y[0], y[1]), pack2(kind, y[2], y[3])};
 }
 
+// 4 accumulation registers cut to at most a bound each, which stays a rare branch
+// between products only if it leaves them where they are.  (The first nops cover
+// a product still writing them, the last one the next reader.)
+__device__ __forceinline__ void min_acc(float& x0, float& x1, float& x2, float& x3, f32x4 bound) {
+  float t0, t1, t2, t3;
+  asm volatile(
+      "s_nop 15\n\ts_nop 15\n\t"
+      "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\t"
+      "v_accvgpr_read_b32 %6, %2\n\tv_accvgpr_read_b32 %7, %3\n\ts_nop 1\n\t"
+      "v_min_f32 %4, %4, %8\n\tv_min_f32 %5, %5, %9\n\t"
+      "v_min_f32 %6, %6, %10\n\tv_min_f32 %7, %7, %11\n\ts_nop 1\n\t"
+      "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+      "v_accvgpr_write_b32 %2, %6\n\tv_accvgpr_write_b32 %3, %7\n\ts_nop 4"
+      : "+a"(x0), "+a"(x1), "+a"(x2), "+a"(x3), "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+      : "v"(bound[0]), "v"(bound[1]), "v"(bound[2]), "v"(bound[3]));
+}
+
 // A workgroup of 4 waves takes a request, a KV head, a range of the prefix
 // (one of `splits`) and query rows, ordered (beam, head in the group, token).
 // A wave holds 32 rows: Q's pieces, the output O^T and the softmax state stay
@@ -384,8 +401,8 @@ block_attn_kernel(BlockAttnArgs a) {
   int first_page = 0;
   const int* table = a.tables + (int64_t)b * a.width;
   if (a.splits == 1)
-    first_page = table[min(((SHARED ? 0 : wave) + (SHARED ? 1 : 4) * (lane >> 1)) * 2 + (lane & 1)
-                           >> (a.lblock - 5), a.width - 1)];
+    first_page = table[min((((SHARED ? 0 : wave) + (SHARED ? 1 : 4) * (lane >> 1)) * 2 + (lane & 1))
+                               >> (a.lblock - 5), a.width - 1)];
   const int len = max(min(a.lengths[b], a.width << a.lblock), 0);
   const int tiles = (len + kKeys - 1) / kKeys;
   const int per = (tiles + a.splits - 1) / a.by_splits;
@@ -424,7 +441,9 @@ block_attn_kernel(BlockAttnArgs a) {
   const int d_row = lane / S::CPR, d_pc = lane % S::CPR;
   auto source = [&](const uint8_t* codes, uint32_t lo, uint32_t hi32, int held) {
     const uint64_t p = (uint64_t)(uintptr_t)codes + ((uint64_t)hi32 << 32 | lo);
-    return u32x4{(uint32_t)p, (uint32_t)(p >> 32) & 0xffffu, (uint32_t)held * D, 0x00020000u};
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)p),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
+                 (uint32_t)__builtin_amdgcn_readfirstlane(held * D), 0x00020000u};
   };
   // (the offset field adds (i % 4) KB to the source and the destination)
   auto off_of = [&](int kv, int i) {
@@ -587,8 +606,6 @@ block_attn_kernel(BlockAttnArgs a) {
   };
 
   // ---- the scores st of a tile (of halves holding held[] keys) to weights
-  i32x8 pf[NP];
-  int ps;                  // the scale byte of this lane's block of weights
   auto scores = [&](const uint8_t* ks, int meta0, int meta1, f32x16* st) {
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -738,16 +755,19 @@ block_attn_kernel(BlockAttnArgs a) {
       read_half(2, 1);
       issue(1, 1, source(a.vc, own_lo[2], own_hi[2], own_held[2]));
       split_q();
-      f32x16 st[2];
+      // scores and weights of tile k in set k % 2
+      f32x16 st[2][2];
+      i32x8 pf[2][NP];
+      int ps[2];                              // the scale byte of this lane's block of weights
 #pragma unroll
-      for (int p = 0; p < NP; ++p) pf[p] = i32x8{};
-      ps = 127;
+      for (int p = 0; p < NP; ++p) pf[1][p] = i32x8{};
+      ps[1] = 127;
       wait_vm(6 * LW);                        // K(0)
       tile_barrier();
-      scores(smem, ring[1][0], ring[1][1], st);
+      scores(smem, ring[1][0], ring[1][1], st[0]);
 
-#pragma unroll 1
-      for (int k = 0; k < count; ++k) {
+      auto step = [&](auto x_c, int k) {
+        constexpr int x = decltype(x_c)::value, z = 1 - x;
         if (k >= 2) wait_vm(4 * LW);          // K(k + 1) and V(k - 1)
         else wait_vm(2 * LW);
         tile_barrier();
@@ -765,10 +785,26 @@ block_attn_kernel(BlockAttnArgs a) {
         if ((k + 4 & 31) == 0) describe((k + 4) >> 5, page_at((k + 4) >> 5));
         read_ring(5, k + 4);
         read_half(2, k + 4);
-        f32x16 cur[2] = {st[0], st[1]};
-        mask(ring[1][0], ring[1][1], cur);
-        i32x8 pc[NP];
-        int pcs;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int held = ring[1][hf] & 0xff;
+          if (held < 32) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              f32x4 bound;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                bound[i] = 2 * j + 4 * hi + i < held ? INFINITY : -INFINITY;
+              float x0 = st[x][hf][j], x1 = st[x][hf][j + 1], x2 = st[x][hf][j + 2],
+                    x3 = st[x][hf][j + 3];
+              min_acc(x0, x1, x2, x3, bound);
+              st[x][hf][j] = x0;
+              st[x][hf][j + 1] = x1;
+              st[x][hf][j + 2] = x2;
+              st[x][hf][j + 3] = x3;
+            }
+          }
+        }
         const int sk[2] = {ring[2][0] >> 8 & 0xff, ring[2][1] >> 8 & 0xff};
         const int sv = (hi ? ring[0][1] : ring[0][0]) >> 16 & 0xff;
         __builtin_amdgcn_sched_barrier(0);
@@ -778,12 +814,12 @@ block_attn_kernel(BlockAttnArgs a) {
           if constexpr (f < 2 * KS) {
             constexpr int hf = f / KS, s = f % KS;
             if constexpr (s == 0 && p == 0)
-              st[hf] = mfma_scaled(fr[f % 3], qf[p][s], f32x16{}, sk[hf], qs[p]);
+              st[z][hf] = mfma_scaled(fr[f % 3], qf[p][s], f32x16{}, sk[hf], qs[p]);
             else
-              st[hf] = mfma_scaled(fr[f % 3], qf[p][s], st[hf], sk[hf], qs[p]);
+              st[z][hf] = mfma_scaled(fr[f % 3], qf[p][s], st[z][hf], sk[hf], qs[p]);
           } else {
             constexpr int dt = f - 2 * KS;
-            O[dt] = mfma_scaled(fr[f % 3], pf[p], O[dt], sv, ps);
+            O[dt] = mfma_scaled(fr[f % 3], pf[z][p], O[dt], sv, ps[z]);
           }
           // K(k + 4) is loaded half way, V(k + 2) three quarters on
           if constexpr (i == MF / 2)
@@ -791,28 +827,38 @@ block_attn_kernel(BlockAttnArgs a) {
           if constexpr (i == 3 * MF / 4)
             issue(1, k + 2, source(a.vc, own_lo[0], own_hi[0], own_held[0]));
           constexpr int c0 = i * SL / MF, c1 = (i + 1) * SL / MF;
-          static_for<c1 - c0>([&](auto x_c) {
-            slice(std::integral_constant<int, c0 + decltype(x_c)::value>{}, cur, pc, pcs);
+          static_for<c1 - c0>([&](auto n_c) {
+            slice(std::integral_constant<int, c0 + decltype(n_c)::value>{}, st[x], pf[x], ps[x]);
           });
           __builtin_amdgcn_sched_barrier(0);
         });
         // (the products above stay here, not where their results are used)
-        asm volatile("" ::"a"(st[0]), "a"(st[1]));
+        asm volatile("" ::"a"(st[z][0]), "a"(st[z][1]));
         add_sums();
 #pragma unroll
-        for (int p = 0; p < NP; ++p) pf[p] = pc[p];
-        ps = pcs;
-#pragma unroll
-        for (int x = 0; x < 5; ++x) {
-          ring[x][0] = ring[x + 1][0];
-          ring[x][1] = ring[x + 1][1];
+        for (int i = 0; i < 5; ++i) {
+          ring[i][0] = ring[i + 1][0];
+          ring[i][1] = ring[i + 1][1];
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          own_lo[x] = own_lo[x + 1];
-          own_hi[x] = own_hi[x + 1];
-          own_held[x] = own_held[x + 1];
+        for (int i = 0; i < 2; ++i) {
+          own_lo[i] = own_lo[i + 1];
+          own_hi[i] = own_hi[i + 1];
+          own_held[i] = own_held[i + 1];
         }
+      };
+      using set0 = std::integral_constant<int, 0>;
+      using set1 = std::integral_constant<int, 1>;
+#pragma unroll 1
+      for (int k = 0; k < count; k += 2) {
+        step(set0{}, k);
+        if (k + 1 == count) {                 // (the last tile's weights to set 1)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) pf[1][p] = pf[0][p];
+          ps[1] = ps[0];
+          break;
+        }
+        step(set1{}, k + 1);
       }
 #pragma unroll
       for (int s = 0; s < STEPS; ++s) gv[s] = u32x4{};
@@ -837,7 +883,7 @@ block_attn_kernel(BlockAttnArgs a) {
         for (int dt = 0; dt < DT; ++dt) {
           const i32x8 f = read_v(vs, dt);
 #pragma unroll
-          for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[p], O[dt], sv, ps);
+          for (int p = 0; p < NP; ++p) O[dt] = mfma_scaled(f, pf[1][p], O[dt], sv, ps[1]);
         }
       }
       if (pass == 1 || (sm_over[0] | sm_over[1] | sm_over[2] | sm_over[3]) == 0) break;
@@ -865,6 +911,8 @@ block_attn_kernel(BlockAttnArgs a) {
       if (has_suffix) wait_vm(0);
       else wait_vm(S::LT);
       take_q(mine + S::tile);
+      i32x8 pf[NP];
+      int ps;
       if (has_suffix) {
         suffix(mine, mine_at);
         issue(0, 0);
