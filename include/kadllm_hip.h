@@ -585,7 +585,8 @@ int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step_args* a,
  * A pool of pages per layer: codes [pages, HK, block, D] e4m3 and scales
  * [pages, HK] e8m0 (2^(byte - 127)); a value is code * scale.  tables [B,
  * width] int32 name a request's pages in order; entries outside [0, pages)
- * name none.  Supported: D in {64, 128, 256}, block in {32, 64, 128, 256}.
+ * name none.  Supported: D in {64, 128, 256}, block in {32, 64, 128, 256}, up to
+ * 2^30 tokens a request (width * block).
  *
  * kad_prefix_block_tables: request b needs ceil(lengths[b] / block) -
  * ceil(starts[b] / block) pages more (starts may be null: none held), taken in

@@ -27,23 +27,22 @@ __global__ __launch_bounds__(256) void block_tables_kernel(
     const int* __restrict__ lengths, const int* __restrict__ starts, const int* __restrict__ old,
     int old_width, const int* __restrict__ free_blocks, int num_free, int* __restrict__ tables,
     int width, int* __restrict__ used, int B, int block, int max_length) {
-  __shared__ int part[256];
+  __shared__ int64_t part[4];
   const int tid = threadIdx.x, b = blockIdx.x;
-  // pages the requests before b need; the last workgroup adds its own
-  int before = 0;
+  // pages that the requests before b need (the sum can pass 32 bits, where the
+  // lengths do not fit the list anyway)
+  int64_t before = 0;
   for (int i = tid; i < b; i += 256) {
     const int held = starts ? pages_of(min(starts[i], max_length), block) : 0;
     before += max(pages_of(min(lengths[i], max_length), block) - held, 0);
   }
-  part[tid] = before;
-  __syncthreads();
-  for (int s = 128; s > 0; s >>= 1) {
-    if (tid < s) part[tid] += part[tid + s];
-    __syncthreads();
-  }
-  before = part[0];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+  if ((tid & 63) == 0) part[tid >> 6] = before;
   const int held = starts ? pages_of(min(starts[b], max_length), block) : 0;
   const int total = max(pages_of(min(lengths[b], max_length), block), held);
+  __syncthreads();
+  before = part[0] + part[1] + part[2] + part[3];
   for (int j = tid; j < width; j += 256) {
     int page = -1;
     if (j < held) {
@@ -53,7 +52,8 @@ __global__ __launch_bounds__(256) void block_tables_kernel(
     }
     tables[(int64_t)b * width + j] = page;
   }
-  if (b == B - 1 && tid == 0) *used = before + total - held;
+  if (b == B - 1 && tid == 0)
+    *used = (int)min(before + total - held, (int64_t)0x7fffffff);
 }
 
 extern "C" int kad_prefix_block_tables(const int32_t* lengths, const int32_t* starts,
@@ -67,6 +67,7 @@ extern "C" int kad_prefix_block_tables(const int32_t* lengths, const int32_t* st
               "tables of %d columns of %d tokens do not hold %d", width, block, max_length);
   KAD_REQUIRE(lengths && tables && used && (free_blocks || num_free == 0),
               "null pointer argument");
+  KAD_REQUIRE(max_length <= 1 << 30, "requests of %d tokens", max_length);
   KAD_REQUIRE(!old_tables || starts, "held tables need the tokens held");
   hipLaunchKernelGGL(block_tables_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream,
                      lengths, starts, old_tables, old_width, free_blocks, num_free, tables, width,
@@ -161,7 +162,8 @@ __global__ __launch_bounds__(1024) void write_blocks_kernel(WriteArgs a) {
   const int h = blockIdx.y, kv = blockIdx.z;
   const int start = a.starts ? max(a.starts[b], 0) : 0;
   const int64_t stop64 = min((int64_t)start + a.N, (int64_t)a.width * a.block);
-  const int stop = min(a.lengths[b], (int)stop64);   // one past the last new position
+  // one past the last new position; at least 0, so that no difference below wraps
+  const int stop = max(min(a.lengths[b], (int)stop64), 0);
   const int blk = start / a.block + u;
   if (blk >= a.width) return;
   const int lo = max(start - blk * a.block, 0), hi = min(stop - blk * a.block, a.block);
@@ -267,6 +269,7 @@ extern "C" int kad_write_prefix_blocks(
   a.touched = (int)(starts ? ((int64_t)N + block - 2) / block + 1 : kad_cdiv(N, block));
   if (a.touched > width) a.touched = width;
   KAD_REQUIRE((int64_t)a.touched * B <= 0x7fffffff && HK <= 65535, "too many pages for a launch");
+  KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
   KAD_REQUIRE(((uintptr_t)k_codes % 16) == 0 && ((uintptr_t)v_codes % 16) == 0,
               "codes must be 16-byte aligned");
   const int item = dtype == KAD_DTYPE_F32 ? 4 : 2;

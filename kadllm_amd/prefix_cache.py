@@ -122,7 +122,7 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
     ceil(starts / block_size) pages more, in request order from the front of
     ``free_blocks`` [F] int32.  Returns (tables [B, ceil(max_length /
     block_size)] int32 with -1 past a request's last page, used [1] int32: the
-    pages taken).  Where ``used`` exceeds F the list was too short: the entries
+    pages taken, at most 2**31 - 1).  Where ``used`` exceeds F the list was too short: the entries
     it could not fill are -1, and the other operators leave such tokens out.
     """
     if not isinstance(block_size, int) or block_size not in BLOCK_SIZES:
@@ -184,8 +184,8 @@ def write_prefix_blocks(blocks, k, v, tables, lengths, *, starts=None):
     lengths = _check_int32("lengths", lengths, 1, B)
     if starts is not None:
         starts = _check_int32("starts", starts, 1, B)
-    if tables.shape[1] < 1:
-        raise ValueError("tables must have columns")
+    if not 0 < tables.shape[1] * block <= MAX_LENGTH:
+        raise ValueError(f"tables must have columns, for at most {MAX_LENGTH} tokens")
     device = _device_of(k, v, tables, lengths, starts, *blocks)
     k = k if k.stride(3) == 1 else k.contiguous()
     v = v if v.stride(3) == 1 else v.contiguous()

@@ -75,6 +75,18 @@ def test_tables_take_views_and_an_empty_list(device):
     assert got.tolist() == [[4, 5]] and used.item() == 0
 
 
+def test_tables_count_past_32_bits(device):
+    """Lengths whose pages add up to more than 2^31: no entry but the list's, and
+    a count that stays at its largest."""
+    most, B = 2**30, 65
+    lengths = torch.full((B,), most, dtype=I32, device=device)
+    got, used = prefix_block_tables(lengths, _ints([7, 8, 9], device), block_size=32,
+                                    max_length=most)
+    assert used.item() == 2**31 - 1
+    assert got[0, :4].tolist() == [7, 8, 9, -1]
+    assert (got[0, 3:] == -1).all() and all(bool((got[b] == -1).all()) for b in range(1, B))
+
+
 # ----------------------------------------------------------------------------
 # writing
 
@@ -197,6 +209,20 @@ def test_single_tokens_and_chunks_extend_pages(device, HK, D, block):
                             _ints(lengths, device), starts=_ints(starts, device))
         _check_write(blocks, before, k, v, tables.tolist(), lengths, starts)
         starts = lengths
+
+
+def test_write_ignores_starts_and_lengths_out_of_range(device):
+    """Starts at and past the tables' end, lengths past it and negative ones."""
+    big = 2**31 - 1
+    starts, lengths = [64, 63, big, 0, -5, 10], [70, big, big, -big - 1, 3, 5]
+    blocks = _pool(device, 13, 1, 32, 64, 7)
+    before = _clone(blocks)
+    tables = torch.arange(12).view(6, 2)
+    k, v = (torch.randn(6, 40, 1, 64, generator=torch.Generator().manual_seed(7))
+            for _ in range(2))
+    write_prefix_blocks(blocks, k.to(device), v.to(device), tables.int().to(device),
+                        _ints(lengths, device), starts=_ints(starts, device))
+    _check_write(blocks, before, k, v, tables.tolist(), lengths, starts)
 
 
 # ----------------------------------------------------------------------------
@@ -427,6 +453,25 @@ def test_requests_share_pages(device):
     lengths = [96, 41]
     out = block_prefix_attention(q, blocks, tables, _ints(lengths, device), sk, sv, beam_width=2)
     _check_attention(out, q, blocks, tables.tolist(), lengths, sk, sv, 2)
+
+
+def test_lengths_out_of_range(device):
+    """Lengths past the tables' columns see what the columns hold, negative ones
+    nothing."""
+    q, blocks, tables, _, sk, sv, _ = _problem(device, [64, 64, 64], 2, 1, 1, 2, 1, 64, 32,
+                                               torch.bfloat16, seed=16)
+    lengths = [2**31 - 1, -3, -2**31]
+    out = block_prefix_attention(q, blocks, tables, _ints(lengths, device), sk, sv, beam_width=2)
+    _check_attention(out, q, blocks, tables.tolist(), [max(n, 0) for n in lengths], sk, sv, 2)
+
+
+@pytest.mark.parametrize("W, T, Tk, lengths", [(300, 1, 1, [70]), (1, 1, 0, [9000]),
+                                               (17, 2, 20, [40, 0])])
+def test_every_dim_in_both_forms(device, W, T, Tk, lengths):
+    """Many rows and few rows, split and whole, with suffixes over several groups."""
+    for D in (64, 128, 256):
+        for dtype in (torch.bfloat16, torch.float16):
+            _run_and_check(device, lengths, W, T, Tk, 2, 2, D, 32, dtype, seed=17)
 
 
 def test_scale_and_its_sign(device):

@@ -131,9 +131,10 @@ def test_entry_points_refuse_before_any_launch():
         k.get("most", 100), None)
     assert tables(lengths=None) == tables(width=1) == tables(old=p) == tables(most=0) == -1
     write = lambda **k: lib.kad_write_prefix_blocks(  # noqa: E731
-        k.get("k", p), 0, 0, 0, p, 0, 0, 0, k.get("dtype", 0), p, 1, p, None, p, p, p, p, 1,
-        k.get("B", 1), 1, 1, k.get("D", 64), k.get("block", 64), None)
+        k.get("k", p), 0, 0, 0, p, 0, 0, 0, k.get("dtype", 0), p, k.get("width", 1), p, None, p, p, p,
+        p, 1, k.get("B", 1), 1, 1, k.get("D", 64), k.get("block", 64), None)
     assert write(k=None) == write(B=0) == write(D=96) == write(block=48) == -1
+    assert write(width=2**30) == -1
     assert write(dtype=7) == -2
     attend = lambda **k: lib.kad_block_prefix_attention(  # noqa: E731
         k.get("q", p), 0, 0, k.get("sq", 0), p, p, p, p, 1, p, k.get("width", 1), p, k.get("sk", None), 0, 0, 0, None, 0, 0, 0,
