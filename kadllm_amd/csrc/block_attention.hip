@@ -21,6 +21,7 @@
 // power of two, which the second product's scale operand restores: 2^-8
 // relative per weight with two pieces (bf16), 2^-12 with three (fp16).
 
+#include <cmath>
 #include <type_traits>
 
 #include "kad_common.h"
@@ -633,7 +634,7 @@ block_attn_kernel(BlockAttnArgs a) {
   // The work on a tile's scores in slices: 8 of maxima, 1 of references, 24 of
   // weights.  A half's weights are 2^(s - ref - e + 8), e the least whole number
   // that keeps them at most 2^8, and their pieces' scales 2^(e - 8): what two
-  // (three) pieces leave of a weight is at most 2^-8 (2^-12) of it, or 2^-18 of
+  // (three) pieces leave of a weight is at most 2^-8 (2^-12) of it, or 2^-17 of
   // the half's largest.
   float top[2], nm[2], sum[2], y4[4];
   int e_of[2];
@@ -1140,35 +1141,57 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
 }
 
 // The launch of a call: whether the waves share tiles, and the ranges the
-// prefix is split into.  More ranges fill the GPU and shorten each workgroup's
-// walk, but every workgroup starts and ends at a cost of about kStart tiles, and
-// the second kernel costs about kJoin of them; the cheapest number of ranges
-// by that count is taken.
+// prefix is split into, whichever a count of nanoseconds finds cheapest.
+// 256 workgroups (one a CU) run as a round; a round costs 30 D to start and end,
+// and for each step of its walk
+//   private: 600 + 6 D (four tiles for 32 rows; each wave waits for its own),
+//   shared:  800 + 3 D (one tile for 128 rows), and 2000 a call, its rings' filling
+// and a split costs 2000 for the second kernel and 0.3 a KB of partial results.
+// Fitted to 3507 measured (form, ranges) of 376 calls, D 64 to 256, 1 to 100
+// requests, 256 to 20000 keys and 4 to 1024 rows: what it takes is 0.6% slower than
+// the best measured choice in the mean and 12% at worst.  (A limit in rows alone,
+// shared from 65 on, lost 7 to 25% in the mean and up to 2.6 times.)  Both sides, us,
+// bf16, 2 KV heads:
+//                                    private  shared
+//   D 256,  64 requests,  256 keys,   64 rows   18.4    23.4
+//                                     96 rows   33.4    23.8
+//                                   1024 rows  232.5    98.0
+//   D 256,   1 request,  8192 keys,  128 rows   23.0    28.5
+//                                   1024 rows   39.4    46.0
+//   D 128,   8 requests, 4096 keys, 1024 rows   58.0    63.8
+//   D 128, 100 requests,  640 keys,   96 rows   27.9    25.5
 struct Plan {
   bool shared;
   int nqblk, splits;
 };
-constexpr int kStart = 6, kJoin = 6;
 
 Plan plan_of(int B, int HK, int R, int D, int keys) {
-  Plan p;
-  p.shared = R > 64;
-  p.nqblk = (int)kad_cdiv(R, p.shared ? 128 : 32);
-  const int64_t blocks = (int64_t)B * HK * p.nqblk;
-  const int64_t slots = D == 256 ? 256 : 512;      // workgroups that run at once
-  const int step = p.shared ? 1 : 4;               // tiles a workgroup takes side by side
+  Plan p = {};
   const int tiles = (int)kad_cdiv(keys, kKeys);
-  p.splits = 1;
-  int64_t best = INT64_MAX;
-  for (int s = 1; s <= 64 && (s == 1 || tiles >= s * step); ++s) {
-    const int walk = ((tiles + s - 1) / s + step - 1) / step + kStart;
-    const int64_t cost = kad_cdiv(blocks * s, slots) * walk + (s > 1 ? kJoin : 0);
-    if (cost < best) {
-      best = cost;
-      p.splits = s;
+  double best = INFINITY;
+  for (int form = 0; form < 2; ++form) {
+    const bool shared = form == 1;
+    const int nqblk = (int)kad_cdiv(R, shared ? 128 : 32), step = shared ? 1 : 4;
+    const double per_step = shared ? 800 + 3 * D : 600 + 6 * D;
+    for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      if (s > 1 && tiles < s * step) break;
+      const int walk = ((tiles + s - 1) / s + step - 1) / step;
+      const double rounds = std::ceil((double)B * HK * nqblk * s / 256);
+      double cost = rounds * (30 * D + walk * per_step) + (shared ? 2000 : 0);
+      if (s > 1) cost += 2000 + 0.0003 * s * B * HK * R * D * 4;
+      if (cost < best) {
+        best = cost;
+        p = Plan{shared, nqblk, s};
+      }
     }
   }
   return p;
+}
+
+// a KV head's rows and a launch's workgroups in 32 bits (doubles hold any product)
+bool rows_fit(int B, int W, int T, int H, int HK) {
+  const double R = (double)W * T * (H / HK);
+  return R <= 0x7fffffff - 256 && B * (double)HK * R / 4 <= 0x7fffffff;
 }
 
 int64_t workspace_of(const Plan& p, int B, int HK, int R, int D) {
@@ -1218,8 +1241,8 @@ extern "C" int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, i
   KAD_REQUIRE(B > 0 && W > 0 && T > 0 && H > 0 && HK > 0 && H % HK == 0 && width > 0,
               "empty dimensions");
   KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
+  KAD_REQUIRE(rows_fit(B, W, T, H, HK), "too many rows for a launch");
   const int64_t R = (int64_t)W * T * (H / HK);
-  KAD_REQUIRE(R <= 0x7fffffff - 256, "%lld rows for a KV head", (long long)R);
   *bytes = workspace_of(plan_of(B, HK, (int)R, D, width * block), B, HK, (int)R, D);
   return KAD_OK;
 }
@@ -1254,15 +1277,13 @@ extern "C" int kad_block_prefix_attention(
   if (dtype != KAD_DTYPE_BF16 && dtype != KAD_DTYPE_F16)
     KAD_UNSUPPORTED("dtype code %d: queries are bf16 or fp16", dtype);
   KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
-  KAD_REQUIRE((int64_t)W * T * (H / HK) <= 0x7fffffff - 256, "too many rows for a KV head");
+  KAD_REQUIRE(rows_fit(B, W, T, H, HK), "too many rows for a launch");
   const int R = W * T * (H / HK);
   const Plan p = plan_of(B, HK, R, D, width * block);
   const int64_t need = workspace_of(p, B, HK, R, D);
   KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
               "a workspace of %lld bytes is needed", (long long)need);
-  KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff &&
-                  kad_cdiv((int64_t)B * HK * R, 4) <= 0x7fffffff,
-              "too many rows for a launch");
+  KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff, "too many rows for a launch");
   BlockAttnArgs a = {};
   a.q = q; a.sq_n = sq_n; a.sq_t = sq_t; a.sq_h = sq_h;
   a.kc = (const uint8_t*)k_codes; a.vc = (const uint8_t*)v_codes;

@@ -7,9 +7,10 @@ for bf16, 2^-11 for fp16; e4m3's is 2^-4):
   - the softmax weights' rounding before the second product: two e4m3 pieces
     for bf16 (2^-8), three for fp16 (2^-12), or the suffix's weights in the
     queries' own type (u): u sum_j p_j |v_j|;
-  - pieces below e4m3's range: a piece's subnormal step is 2^-9, half of it
-    2^-10, and the last piece carries at least another 2^-4 while 32 weights
-    share a scale that puts their largest, at most 1, above 2^7: 2^-21 |v_j|
+  - pieces below e4m3's range: a piece's subnormal step is 2^-9, so its rounding
+    is off by at most 2^-10 of its scale.  All pieces of 32 weights share one
+    scale, which puts their largest, at most 1, at 2^7 or above, so the scale is
+    at most 2^-7 and the last piece leaves 2^-10 * 2^-7 = 2^-17 |v_j| at most,
     for each cached key's weight before the division by l;
   - the scores: an fp32 sum of D products, (D + 4) 2^-24 sum_d |q_d k_d|, and
     a query element's piece, 2^-21 max|q| sum_d |k_d| for the row; twice the
@@ -247,7 +248,7 @@ def _attention_bound(q, pool_k, y, weight, slack, suffix_k, scale):
     p = max(_u(dtype), 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -12)
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     return (_u(dtype) * y.abs() + (p + 2 * score + 2.0 ** -19) * (1 + _u(dtype)) * weight
-            + 2.0 ** -21 * slack + tiny)
+            + 2.0 ** -17 * slack + tiny)
 
 
 def _check_attention(out, q, blocks, tables, lengths, sk, sv, W, gate=None, scale=None):
@@ -472,6 +473,82 @@ def test_every_dim_in_both_forms(device, W, T, Tk, lengths):
     for D in (64, 128, 256):
         for dtype in (torch.bfloat16, torch.float16):
             _run_and_check(device, lengths, W, T, Tk, 2, 2, D, 32, dtype, seed=17)
+
+
+# Batches large enough that the waves of a workgroup share their tiles: a few
+# requests many times over, the first ones against the oracle and the copies
+# bit for bit against them.
+
+def _copies(times, *xs):
+    return [None if x is None else x.repeat(times, *[1] * (x.dim() - 1)) for x in xs]
+
+
+def _run_copies(times, W, q, blocks, tables, lens, sk, sv, gate=None):
+    """The attention of ``times`` copies; (one copy, equal to the others)."""
+    many = _copies(times, q, tables, lens, sk, sv, gate)
+    out = block_prefix_attention(many[0], blocks, *many[1:5], beam_width=W, gate=many[5])
+    out = out.view(times, *q.shape)
+    assert torch.equal(out.view(torch.int16), out[:1].expand_as(out).view(torch.int16))
+    return out[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths, times, W, T, Tk, H, HK, block", [
+    ([64, 33, 0], 32, 13, 1, 1, 5, 1, 32),            # 65 rows, one tile
+    ([320, 257, 1], 32, 25, 1, 0, 4, 1, 64),          # 100 rows, no suffix
+    ([190, 65], 64, 11, 3, 4, 6, 2, 128),             # 99 rows
+    ([70, 600, 256], 42, 50, 1, 17, 4, 1, 256),       # 200 rows, two groups of suffix keys
+    ([2048, 1500], 48, 13, 1, 1, 5, 1, 64),           # split (D >= 128)
+    ([2000, 1921], 40, 97, 1, 2, 1, 1, 64),           # split
+])
+def test_attention_of_large_batches(device, dtype, D, lengths, times, W, T, Tk, H, HK, block):
+    q, blocks, tables, lens, sk, sv, gate = _problem(device, lengths, W, T, Tk, H, HK, D, block,
+                                                     dtype, gated=T == 3, seed=18)
+    out = _run_copies(times, W, q, blocks, tables, lens, sk, sv, gate)
+    _check_attention(out, q, blocks, tables.tolist(), lengths, sk, sv, W, gate)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_large_batches_scores_far_apart(device, D):
+    lengths, W = [320, 320], 25
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, lengths, W, 1, 1, 4, 1, D, 32,
+                                                  torch.bfloat16, seed=19)
+    scales = blocks.k_scale.view(torch.uint8)
+    for j in range(tables.shape[1]):
+        scales[tables[0, j].long()] = 122 + 2 * j
+        scales[tables[1, j].long()] = 140 - 2 * j
+    out = _run_copies(72, W, q, blocks, tables, lens, sk, sv)
+    assert out.isfinite().all()
+    y, _, _ = ref.attention(q, ref.decode(blocks.k, blocks.k_scale),
+                            ref.decode(blocks.v, blocks.v_scale), tables.tolist(), lengths,
+                            sk, sv, W, D ** -0.5)
+    near = (out.double().cpu() - y).abs().amax(3) <= 2.0 ** -7 * y.abs().amax(3) + 2.0 ** -8
+    assert near.float().mean() > 0.9
+
+
+def test_large_batches_ignore_what_lies_behind_the_lengths(device):
+    lengths, W, block = [70, 33, 0], 25, 32
+    q, blocks, tables, lens, sk, sv, _ = _problem(device, lengths, W, 2, 2, 4, 2, 128, block,
+                                                  torch.bfloat16, seed=20)
+    want = _run_copies(32, W, q, blocks, tables, lens, sk, sv)
+    _check_attention(want, q, blocks, tables.tolist(), lengths, sk, sv, W)
+    for b, n in enumerate(lengths):
+        for j, page in enumerate(tables[b].tolist()):
+            if page >= 0:
+                for x in (blocks.k, blocks.v):
+                    x.view(torch.uint8)[page, :, max(0, n - j * block):] = 0x7f
+    tables = torch.where(tables < 0, 10**9, tables)
+    assert torch.equal(_run_copies(32, W, q, blocks, tables, lens, sk, sv), want)
+    for bad in (torch.nan, torch.inf):        # the second token's suffix key of one beam
+        ks, vs = sk.clone(), sv.clone()
+        ks[6, 1], vs[6, 1] = bad, bad
+        many = _copies(32, q, tables, lens, ks, vs)
+        got = block_prefix_attention(many[0], blocks, *many[1:], beam_width=W)[:3 * W]
+        others = [n for n in range(3 * W) if n != 6]
+        assert torch.equal(got[others], want[others])
+        assert torch.equal(got[6, 0], want[6, 0])
+        assert not got[6, 1].isfinite().all()
 
 
 def test_scale_and_its_sign(device):
