@@ -18,6 +18,10 @@
 //   old[b][j]                              j <  ceil(starts / block)
 //   free[sum of need before b + j - held]  j <  ceil(lengths / block)
 //   -1                                     otherwise, or when `free` is used up.
+// One workgroup a request, which adds up what the requests before it need by
+// itself: B / 2 lengths on average out of L2, and no second launch or wait between
+// workgroups.  Bound by latency: 3.0 us for 32 requests of 1024 tokens, 5.3 us for
+// 1000 of 32768 that grow (3.1 MB).
 
 __device__ __forceinline__ int pages_of(int tokens, int block) {
   return (int)(((int64_t)max(tokens, 0) + block - 1) / block);
@@ -151,7 +155,10 @@ __device__ __forceinline__ void store16(uint8_t* p, const float* f, float scale)
 // A page and head is block * D / 16 pieces of 16 elements.  Each of up to 1024
 // threads keeps 4 of them in registers between the maximum and the rounding, so
 // the input is read once and the codes are written once, 16 bytes a lane.
-// VEC: rows of the input start at 16-byte boundaries.
+// Bound by HBM: 32 requests of 1024 tokens (bf16, 2 KV heads of 256; 101 MB) in 19.2 us,
+// 5.2 TB/s, and 8 of up to 20000 (fp16, 8 heads of 128; 492 MB) in 98 us, 5.0 TB/s, the
+// rate of a large copy (5.18).  One token for each of 256 requests: 5.6 us.
+// VEC: rows of the input start at 16-byte boundaries (else element by element).
 constexpr int kPieces = 4;
 
 template <typename T, bool VEC>
