@@ -612,11 +612,12 @@ int kad_write_prefix_blocks(const void* k, int64_t sk_b, int64_t sk_t, int64_t s
                             kad_stream_t stream);
 /* kad_prefix_attention_decode_ex's attention over such a prefix: query rows
  * (n, t, h) see the first lengths[b] cached tokens of their request b = n / W
- * and the suffix keys j <= Tk - T + t of their beam (Tk = 0: no suffix).  bf16
- * or fp16 queries, suffixes, gate (may be null) and out; last dimensions
- * contiguous and every row 16-byte aligned.  A row that sees no key gives zeros.  The workspace (its size from
- * kad_block_prefix_attention_workspace_bytes, 0 where none is needed) holds
- * the partial results of a prefix that is split over workgroups. */
+ * and the suffix keys j <= Tk - T + t of their beam (Tk = 0: no suffix; at most
+ * 2^22 keys).  bf16 or fp16 queries, suffixes, gate (may be null) and out; last
+ * dimensions contiguous and every row 16-byte aligned.  A row that sees no key
+ * gives zeros.  The workspace (16-byte aligned, its size from
+ * kad_block_prefix_attention_workspace_bytes, 0 where none is needed) holds the
+ * partial results of a prefix that is split over workgroups. */
 int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, int H, int HK, int D,
                                                int width, int block, int64_t* bytes);
 int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_t sq_h,

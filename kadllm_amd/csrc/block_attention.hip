@@ -1273,6 +1273,9 @@ extern "C" int kad_block_prefix_attention(
               "empty dimensions");
   KAD_REQUIRE(H % HK == 0, "%d heads over %d KV heads", H, HK);
   KAD_REQUIRE(Tk == 0 || Tk >= T, "a suffix of %d keys for %d queries", Tk, T);
+  // (a wave numbers the suffix keys of up to 32 beams, and the elements of one beam's
+  // values, in 32 bits)
+  KAD_REQUIRE(Tk <= 1 << 22, "a suffix of %d keys", Tk);
   KAD_REQUIRE(q && k_codes && v_codes && k_scale && v_scale && tables && lengths && out &&
                   (Tk == 0 || (suffix_k && suffix_v)),
               "null pointer argument");
@@ -1294,8 +1297,8 @@ extern "C" int kad_block_prefix_attention(
   const int R = W * T * (H / HK);
   const Plan p = plan_of(B, HK, R, D, width * block);
   const int64_t need = workspace_of(p, B, HK, R, D);
-  KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
-              "a workspace of %lld bytes is needed", (long long)need);
+  KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
+              "a workspace of %lld bytes at a 16-byte boundary is needed", (long long)need);
   KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff, "too many rows for a launch");
   BlockAttnArgs a = {};
   a.q = q; a.sq_n = sq_n; a.sq_t = sq_t; a.sq_h = sq_h;

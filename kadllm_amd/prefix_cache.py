@@ -28,6 +28,7 @@ from . import _lib
 BLOCK_SIZES = (32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 MAX_LENGTH = 2**30          # tokens of a request
+MAX_SUFFIX = 2**22          # suffix keys of a beam
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -122,8 +123,9 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
     ceil(starts / block_size) pages more, in request order from the front of
     ``free_blocks`` [F] int32.  Returns (tables [B, ceil(max_length /
     block_size)] int32 with -1 past a request's last page, used [1] int32: the
-    pages taken, at most 2**31 - 1).  Where ``used`` exceeds F the list was too short: the entries
-    it could not fill are -1, and the other operators leave such tokens out.
+    pages taken, at most 2**31 - 1).  Where ``used`` exceeds F the list was too
+    short: the entries it could not fill are -1, and the other operators leave
+    such tokens out.
     """
     if not isinstance(block_size, int) or block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
@@ -186,6 +188,8 @@ def write_prefix_blocks(blocks, k, v, tables, lengths, *, starts=None):
         starts = _check_int32("starts", starts, 1, B)
     if not 0 < tables.shape[1] * block <= MAX_LENGTH:
         raise ValueError(f"tables must have columns, for at most {MAX_LENGTH} tokens")
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
     device = _device_of(k, v, tables, lengths, starts, *blocks)
     k = k if k.stride(3) == 1 else k.contiguous()
     v = v if v.stride(3) == 1 else v.contiguous()
@@ -203,8 +207,8 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
     q [B*W, T, H, D] bf16 or fp16; tables [B, columns] and lengths [B] int32:
     a query sees the first lengths[b] cached tokens of its request, except any
     whose table entry names no page.  suffix_k, suffix_v [B*W, Tk, HK, D] in
-    q's type, Tk >= T: the beam's own tokens, of which the queries are the last
-    T (query t sees suffix keys up to Tk - T + t); None for none, as when the
+    q's type, T <= Tk <= 2**22: the beam's own tokens, of which the queries are the
+    last T (query t sees suffix keys up to Tk - T + t); None for none, as when the
     newest tokens are already in the cache.  ``scale`` defaults to D**-0.5;
     ``gate`` [B*W, T, H*D] multiplies the output by sigmoid(gate).  Returns
     [B*W, T, H, D] in q's type; a query that sees no key gets zeros.
@@ -233,6 +237,8 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
         if len(s) != 4 or s[0] != BW or s[1] < T or s[2] != HK or s[3] != D or \
                 suffix_v.shape != s:
             raise ValueError("suffix_k and suffix_v must be [B*W, Tk, HK, D] with Tk >= T")
+        if s[1] > MAX_SUFFIX:
+            raise ValueError(f"a suffix has at most {MAX_SUFFIX} keys")
         if suffix_k.dtype is not dtype or suffix_v.dtype is not dtype:
             raise ValueError("attention inputs must have the same dtype")
     if gate is not None and (gate.shape != (BW, T, H * D) or gate.dtype is not dtype):

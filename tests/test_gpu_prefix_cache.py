@@ -420,6 +420,25 @@ def test_attention_nan_in_a_visible_key(device):
     assert torch.equal(got[[3, 5]], want[[3, 5]])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_infinite_queries_and_gates(device, dtype):
+    """An infinite query element makes its row NaN (inf - inf) and no other; gates
+    of either infinity give the output itself and zeros."""
+    q, blocks, tables, lens, sk, sv, gate = _problem(device, [40, 99], 3, 1, 1, 2, 1, 64, 32,
+                                                     dtype, gated=True, seed=21)
+    want = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=3)
+    for bad in (torch.inf, -torch.inf):
+        qs = q.clone()
+        qs[4, 0, 1, 7] = bad
+        got = block_prefix_attention(qs, blocks, tables, lens, sk, sv, beam_width=3)
+        assert got[4, 0, 1].isnan().all()
+        got[4, 0, 1] = want[4, 0, 1]
+        assert torch.equal(got, want)
+    gate[:, :, :64], gate[:, :, 64:] = torch.inf, -torch.inf
+    got = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=3, gate=gate)
+    assert torch.equal(got[:, :, 0], want[:, :, 0]) and (got[:, :, 1] == 0).all()
+
+
 def test_attention_takes_strides(device):
     lengths, W, T, Tk, H, HK, D, block = [50, 90], 3, 2, 3, 4, 2, 64, 32
     q, blocks, tables, lens, sk, sv, gate = _problem(device, lengths, W, T, Tk, H, HK, D, block,

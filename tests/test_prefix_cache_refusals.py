@@ -77,6 +77,8 @@ def test_tables_refusals(change, error):
     (dict(tables=torch.zeros(2, 1, dtype=torch.int64)), TypeError),
     (dict(lengths=torch.zeros(1, dtype=I32)), ValueError),
     (dict(starts=torch.zeros(2, dtype=torch.int64)), TypeError),
+    (dict(k=torch.zeros(2, 5, 2, 64, dtype=torch.bfloat16).requires_grad_()), RuntimeError),
+    (dict(v=torch.zeros(2, 5, 2, 64, dtype=torch.bfloat16).requires_grad_()), RuntimeError),
     (dict(), RuntimeError),
 ])
 def test_write_refusals(change, error):
@@ -108,6 +110,8 @@ def _bf(*shape):
     (dict(suffix_k=_bf(4, 0, 2, 64), suffix_v=_bf(4, 0, 2, 64)), ValueError),
     (dict(suffix_k=_bf(4, 1, 4, 64), suffix_v=_bf(4, 1, 4, 64)), ValueError),
     (dict(suffix_k=_bf(4, 2, 2, 64), suffix_v=_bf(4, 1, 2, 64)), ValueError),
+    (dict(suffix_k=_bf(1, 1, 2, 64).expand(4, 2**22 + 1, 2, 64),
+          suffix_v=_bf(1, 1, 2, 64).expand(4, 2**22 + 1, 2, 64)), ValueError),
     (dict(suffix_k=_bf(4, 1, 2, 64).half(), suffix_v=_bf(4, 1, 2, 64)), ValueError),
     (dict(gate=_bf(4, 1, 64)), ValueError),
     (dict(gate=torch.zeros(4, 1, 256)), ValueError),
@@ -137,12 +141,16 @@ def test_entry_points_refuse_before_any_launch():
     assert write(width=2**30) == -1
     assert write(dtype=7) == -2
     attend = lambda **k: lib.kad_block_prefix_attention(  # noqa: E731
-        k.get("q", p), 0, 0, k.get("sq", 0), p, p, p, p, 1, p, k.get("width", 1), p, k.get("sk", None), 0, 0, 0, None, 0, 0, 0,
-        None, 0, 0, 0, p, 0, 0, 0, None, 0, k.get("B", 1), 1, 1, k.get("Tk", 0), k.get("H", 2), 2, k.get("D", 64),
-        k.get("block", 64), k.get("dtype", 0), 1.0, None)
+        k.get("q", p), 0, 0, k.get("sq", 0), p, p, p, p, 1, p, k.get("width", 1), p,
+        k.get("sk", None), 0, 0, 0, k.get("sk", None), 0, 0, 0, None, 0, 0, 0, p, 0, 0, 0,
+        k.get("ws", None), 2**40, k.get("B", 1), 1, 1, k.get("Tk", 0), k.get("H", 2), 2,
+        k.get("D", 64), k.get("block", 64), k.get("dtype", 0), 1.0, None)
     assert attend(q=None) == attend(Tk=1) == attend(H=3) == attend(D=32) == attend(block=16) == -1
     assert attend(sq=4) == attend(q=ctypes.c_void_p(264)) == attend(width=2**30) == -1
     assert attend(width=64) == -1 and b"workspace" in lib.kad_last_error()
+    assert attend(Tk=2**22 + 1, sk=p) == -1 and b"suffix" in lib.kad_last_error()
+    assert attend(width=64, ws=ctypes.c_void_p(264)) == -1
+    assert attend(B=2**30, H=2**20) == -1 and b"rows" in lib.kad_last_error()
     assert attend(dtype=2) == -2
     need = ctypes.c_int64(-1)
     size = lib.kad_block_prefix_attention_workspace_bytes
