@@ -156,7 +156,20 @@ __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
 }
 
 constexpr int kKeys = 64;       // keys per tile: two halves of 32, each within a page
-constexpr int kMaxUp = 60;      // a tile may exceed the row's reference by 2^60 before it moves
+// A row's scores may lie this far above its reference, in powers of two, before the
+// reference moves: by 60, or less where the values are so large that weights of
+// that size times them could pass 2^120.  Of up to 2^30 cached keys of V scale byte
+// sv the values are below 2^(sv - 118); a suffix has up to 2^22 keys, whose values may
+// reach 2^38 (kBigValue) under weights of up to 2^60.
+constexpr int kMaxUp = 60;
+constexpr uint32_t kBigValue = (127 + 38) << 7;   // as a bf16 (fp16 values end before it)
+__device__ __forceinline__ float climb_of(int sv) { return (float)min(kMaxUp, 208 - sv); }
+// A reference that has moved lies this far above the row's true maximum, so that
+// outputs stay below the largest value while they are summed (2^30 keys of weight
+// 2^-30).  Not in fp16, where suffix weights are fp16 and an output that passes fp32
+// on the way does not fit its type.
+template <typename T>
+constexpr float kRoom = std::is_same<T, bf16_t>::value ? 30.f : 0.f;
 
 template <int D>
 struct Shape {
@@ -306,7 +319,8 @@ __device__ __forceinline__ void min_acc(float& x0, float& x1, float& x2, float& 
 // Weights are 2^(s - m) for a reference m, the maximum of the first keys that the
 // row sees.  Scores above it need no rescaling, because the weights of 32 keys
 // carry an exponent of their own; only when one lies more than 2^60 above (2^14
-// among fp16 suffix keys) is the walk done again, with the row's true maximum.
+// among fp16 suffix keys, less among values past 2^30: climb_of) is the walk done
+// again, with the row's true maximum.
 // What bounds it, bf16, D 256, 2 KV heads for 8 heads:
 //   16 requests of 1 beam over 32768 keys: HBM, 94 to 99 us for 537 MB, 5.4 to 5.7 TB/s
 //     (private, 8 ranges each).
@@ -606,6 +620,18 @@ block_attn_kernel(BlockAttnArgs a) {
         __builtin_amdgcn_s_waitcnt(0xc07f);
       }
       spoilt |= bad;
+      if constexpr (std::is_same<T, bf16_t>::value) {   // a row that sees a big value
+        if (__ballot((top_exp & 0xffffu) >= kBigValue || top_exp >> 16 >= kBigValue) != 0) {
+          const int last = min(vhi - f0, 15);
+          uint32_t seen = 0;
+#pragma unroll 1
+          for (int i = max(vlo - f0, 0); i <= last; ++i)
+#pragma unroll 1
+            for (int e = 0; e < D / 2; ++e)
+              seen = max_u16x2(seen, ((const uint32_t*)(values + i * 2 * D))[e] & kExponents<T>);
+          over |= (seen & 0xffffu) >= kBigValue || seen >> 16 >= kBigValue;
+        }
+      }
 #pragma unroll
       for (int d2 = 0; d2 < DT / 2; ++d2) {
         u32x4 x, y;
@@ -647,7 +673,7 @@ block_attn_kernel(BlockAttnArgs a) {
   // that keeps them at most 2^8, and their pieces' scales 2^(e - 8): what two
   // (three) pieces leave of a weight is at most 2^-8 (2^-12) of it, or 2^-17 of
   // the half's largest.
-  float top[2], nm[2], sum[2], y4[4];
+  float top[2], nm[2], sum[2], y4[4], climb;   // climb: climb_of the tile's larger V scale
   int e_of[2];
   auto slice = [&](auto c_c, const f32x16* cur, i32x8* pc, int& pcs) {
     constexpr int c = decltype(c_c)::value;
@@ -661,7 +687,7 @@ block_attn_kernel(BlockAttnArgs a) {
       const float both = fmaxf(top[0], top[1]);
       m_true = fmaxf(m_true, both);
       m = m == -INFINITY ? both : m;
-      over |= both > m + kMaxUp;
+      over |= both > m + climb;
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
@@ -819,6 +845,7 @@ block_attn_kernel(BlockAttnArgs a) {
         }
         const int sk[2] = {ring[2][0] >> 8 & 0xff, ring[2][1] >> 8 & 0xff};
         const int sv = (hi ? ring[0][1] : ring[0][0]) >> 16 & 0xff;
+        climb = climb_of(max(ring[1][0], ring[1][1]) >> 16);
         __builtin_amdgcn_sched_barrier(0);
         static_for<MF>([&](auto i_c) {
           constexpr int i = decltype(i_c)::value, f = i / NP, p = i % NP;
@@ -947,6 +974,7 @@ block_attn_kernel(BlockAttnArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         issue(0, k + 1);
         mask(m0, m1, st);
+        climb = climb_of(max(m0, m1) >> 16);
         static_for<SL>([&](auto c_c) { slice(c_c, st, pf, ps); });
         add_sums();
         wait_vm(S::LT);
@@ -964,7 +992,7 @@ block_attn_kernel(BlockAttnArgs a) {
       wait_vm(0);
       if (pass == 1 || __ballot(over) == 0) break;
     }
-    m = over ? m_true : m;
+    m = over ? m_true + kRoom<T> : m;
     first_page = page_at(0);
   }
 

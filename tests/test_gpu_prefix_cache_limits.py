@@ -1,0 +1,79 @@
+"""The 8-bit prefix cache's operators at the ends of what they accept: scores
+that climb far above a row's first ones, values and queries of any magnitude.
+
+The bounds are those of test_gpu_prefix_cache (derived there).
+"""
+
+import pytest
+import torch
+
+import test_gpu_prefix_cache as base
+from kadllm_amd.ops import block_prefix_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def _climbing(device, lengths, W, T, Tk, H, HK, D, block, dtype, key_bytes, seed, suffix=None):
+    """A problem whose scores are near 11.5 * 2^(byte - 127) * f in log2 units: f is
+    the row's own, 0.4 to 1, and byte the scale byte of the key's page (key_bytes,
+    for every other request in reverse) or, for suffix key j, 127 + suffix(j)."""
+    q, blocks, tables, lens, sk, sv, gate = base._problem(device, lengths, W, T, Tk, H, HK, D,
+                                                          block, dtype, seed=seed)
+    gen = torch.Generator().manual_seed(seed + 1)
+    row = 0.4 + 0.6 * torch.rand(*q.shape[:3], 1, generator=gen)
+    # q . k D^-0.5 = 8 f with keys near 1
+    q = (row * 8 / D ** 0.5 * (1 + 0.05 * torch.randn(q.shape, generator=gen))).to(dtype)
+    near_one = lambda shape: 1 + 0.125 * torch.randint(-1, 2, shape, generator=gen)  # noqa: E731
+    blocks.k.copy_(near_one(blocks.k.shape).to(torch.float8_e4m3fn))
+    scales = blocks.k_scale.view(torch.uint8)
+    for b, pages in enumerate(tables.tolist()):
+        for j, page in enumerate(pages):
+            if page >= 0:
+                scales[page] = key_bytes[j if b % 2 == 0 else len(key_bytes) - 1 - j]
+    if suffix is not None:
+        rise = torch.tensor([2.0 ** suffix(j) for j in range(Tk)]).view(1, Tk, 1, 1)
+        sk = (near_one(sk.shape) * rise).to(dtype).to(device)
+    return q.to(device), blocks, tables, lens, sk, sv, gate
+
+
+def _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times=1):
+    """The attention of ``times`` copies against the oracle."""
+    if times == 1:
+        out = block_prefix_attention(q, blocks, tables, lens, sk, sv, beam_width=W, gate=gate)
+    else:
+        out = base._run_copies(times, W, q, blocks, tables, lens, sk, sv, gate)
+    base._check_attention(out, q, blocks, tables.tolist(), lens.tolist(), sk, sv, W, gate)
+
+
+# (lengths, copies, W, H, block): few rows, few rows in ranges, 128 rows that share
+# tiles, and those in ranges
+FORMS = [([160, 130], 1, 3, 2, 32), ([1500], 1, 1, 2, 64), ([160, 130], 72, 25, 5, 32),
+         ([2000, 1921], 40, 97, 1, 64)]
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths, times, W, H, block", FORMS)
+@pytest.mark.parametrize("what", ["climb", "sum", "both"])
+def test_values_near_the_largest(device, D, lengths, times, W, H, block, what):
+    """Values of 2^100 and more under scores that climb by up to 35 (weights relative
+    to the first score of up to 2^35), values whose plain sum passes fp32's
+    largest, and both: the outputs, averages of the values, are finite."""
+    pages = -(-max(lengths) // block)
+    byte = [127 + 2 * (what != "sum" and j % 5 == 3) for j in range(pages)]
+    q, blocks, tables, lens, sk, sv, gate = _climbing(device, lengths, W, 1, 1, H, 1, D, block,
+                                                      torch.bfloat16, byte, seed=31,
+                                                      suffix=lambda j: 0)
+    blocks.v.view(torch.uint8).bitwise_and_(0x7f)
+    blocks.v_scale.view(torch.uint8).fill_(220 if what == "climb" else 245)
+    _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times)
+
+
+@pytest.mark.parametrize("lengths, times, W, H, block", [FORMS[0], FORMS[2]])
+@pytest.mark.parametrize("T, Tk, climb", [(1, 40, True), (2, 33, False), (1, 4, True)])
+def test_suffix_values_near_the_largest(device, lengths, times, W, H, block, T, Tk, climb):
+    byte = [127] * -(-max(lengths) // block)
+    q, blocks, tables, lens, sk, sv, gate = _climbing(
+        device, lengths, W, T, Tk, H, 1, 64, block, torch.bfloat16, byte, seed=32,
+        suffix=lambda j: 2 * (climb and j % 4 == 3))
+    sv = sv.abs() * 2.0 ** 125
+    _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times)
