@@ -13,7 +13,8 @@
 // + y2 / 256), each y the e4m3 rounding of 16 times what the pieces before it
 // left.  A piece keeps 4 significant bits, so two hold a bf16 value exactly
 // (8 bits) and three an fp16 one (11 bits), as far down as 2^-10 of the row's
-// largest element; below that the error is at most 2^-22 of the largest.  Two
+// largest element; below that the error is at most 2^-21 of the largest (the last
+// piece of two is off by up to 2^-10 / 16 where the largest is 2^7 or more).  Two
 // pieces cost what one bf16 product would (e4m3 runs at twice the rate), and
 // the cache is neither widened in registers nor stored wide in LDS.
 //
@@ -529,7 +530,9 @@ block_attn_kernel(BlockAttnArgs a) {
       for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
     }
     amax = max_xor32(amax);
-    const int E = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, -100);
+    // (held where the last piece's scale is the smallest e8m0; what a piece cannot
+    // hold there, 2^-137, is below every bf16 and fp16 number)
+    const int E = max((int)(__float_as_uint(amax) >> 23) - 127 - 7, 4 * (NP - 1) - 127);
     const float inv = pow2i(-E) * a.qmul;
 #pragma unroll
     for (int c = 0; c < 4 * KS; ++c) {

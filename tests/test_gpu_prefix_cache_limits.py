@@ -77,3 +77,15 @@ def test_suffix_values_near_the_largest(device, lengths, times, W, H, block, T, 
         suffix=lambda j: 2 * (climb and j % 4 == 3))
     sv = sv.abs() * 2.0 ** 125
     _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths, times, W, H, block", FORMS)
+@pytest.mark.parametrize("exponent", [-95, -108, -119, -126])
+def test_queries_of_any_magnitude(device, D, lengths, times, W, H, block, exponent):
+    """Queries down to bf16's smallest numbers, under keys as much larger."""
+    q, blocks, tables, lens, sk, sv, gate = base._problem(device, lengths, W, 1, 0, H, 1, D, block,
+                                                          torch.bfloat16, seed=33)
+    q = (q.double() * 2.0 ** exponent).bfloat16()
+    blocks.k_scale.view(torch.uint8).sub_(exponent % 256)
+    _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times)
