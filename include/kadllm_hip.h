@@ -603,7 +603,8 @@ int kad_prefix_block_tables(const int32_t* lengths, const int32_t* starts,
  * lengths[b].  A page's scale is the smallest power of two s >= 2^-100 with
  * amax <= 448 s over the finite values written, or the page's own where that
  * is larger and the page holds earlier tokens (whose codes are rounded again
- * when the scale grows).  Tokens without a page are left out. */
+ * when the scale grows; where it is NaN, it stays, and new codes are NaN).
+ * Tokens without a page are left out. */
 int kad_write_prefix_blocks(const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h,
                             const void* v, int64_t sv_b, int64_t sv_t, int64_t sv_h, int dtype,
                             const int32_t* tables, int width, const int32_t* lengths,

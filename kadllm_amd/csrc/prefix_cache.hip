@@ -86,7 +86,9 @@ extern "C" int kad_prefix_block_tables(const int32_t* lengths, const int32_t* st
 //   e_need = the smallest e >= -100 with amax <= 448 * 2^e over the finite new values
 //   e      = e_need, or max(e_need, the page's) when it holds earlier tokens
 //   code   = e4m3(x * 2^-e), to nearest even; infinities and NaN become NaN
-// and the earlier tokens' codes are rounded again when the scale has grown.
+// and the earlier tokens' codes are rounded again when the scale has grown.  A page
+// of earlier tokens whose scale is not a number (byte 255) stays one: new codes are
+// NaN too.
 // Rows past lengths[b] are left as they were.
 constexpr int kMinExp = -100;
 
@@ -97,8 +99,8 @@ __device__ __forceinline__ int scale_exp(float amax) {
   const int e = x - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return max(e, kMinExp);  // zeros and subnormals of fp32 give x = -127
 }
-__device__ __forceinline__ float pow2f(int e) {  // 2^e, -126 <= e <= 127
-  return __uint_as_float((uint32_t)(e + 127) << 23);
+__device__ __forceinline__ float pow2f(int e) {  // 2^e, -127 <= e <= 127
+  return __uint_as_float(e > -127 ? (uint32_t)(e + 127) << 23 : 1u << 22);
 }
 
 struct WriteArgs {
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(1024) void write_blocks_kernel(WriteArgs a) {
   for (int i = 0; i < threads / 64; ++i) amax = fmaxf(amax, part[i]);
   int e = scale_exp(amax);
   if (lo > 0) {
-    const int before = min((int)*scale - 127, 127);
+    const int before = (int)*scale - 127;             // (128: not a number)
     if (e > before) {                                 // the earlier rows to the new scale
       const float m = pow2f(max(before - e, -126));
       for (int i = tid; i < lo * ppr; i += threads) {
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(1024) void write_blocks_kernel(WriteArgs a) {
     }
     e = max(e, before);
   }
-  const float inv = pow2f(-e);
+  const float inv = e <= 127 ? pow2f(-e) : NAN;
 #pragma unroll
   for (int p = 0; p < kPieces; ++p) {
     const int i = tid + p * threads, row = i / ppr;

@@ -165,11 +165,12 @@ def write_prefix_blocks(blocks, k, v, tables, lengths, *, starts=None):
     A page's scale is the smallest power of two s >= 2**-100 with amax <= 448 s
     over the finite values written to it.  A page that holds earlier tokens
     keeps the larger of its scale and the new tokens'; when that grows, the
-    earlier codes are rounded to the new scale.  Codes are x / s to the nearest
-    e4m3 value (ties to even); infinities and NaN become NaN.  Rows behind
-    lengths[b] and pages the call does not reach are left as they were; tokens
-    whose table entry names no page are left out.  Two requests of one call
-    must not write to the same page.  Returns ``blocks``.
+    earlier codes are rounded to the new scale (a scale that is not a number
+    stays, and the new codes are NaN).  Codes are x / s to the nearest e4m3 value
+    (ties to even); infinities and NaN become NaN.  Rows behind lengths[b] and
+    pages the call does not reach are left as they were; tokens whose table
+    entry names no page are left out.  Two requests of one call must not write
+    to the same page.  Returns ``blocks``.
     """
     pages, HK, block, D = _check_blocks(blocks)
     shape = k.shape

@@ -20,11 +20,13 @@ def e4m3_values():
 
 
 def decode(codes, scales):
-    """(code values, scales) as float64 of float8_e4m3fn and float8_e8m0fnu tensors."""
+    """(code values, scales) as float64 of float8_e4m3fn and float8_e8m0fnu tensors
+    (NaN for the scale byte 255)."""
     table = e4m3_values()
+    byte = scales.cpu().view(torch.uint8).long()
+    powers = torch.ldexp(torch.ones((), dtype=torch.float64), byte - 127)
     return (table[codes.cpu().view(torch.uint8).long()],
-            torch.ldexp(torch.ones((), dtype=torch.float64),
-                        scales.cpu().view(torch.uint8).long() - 127))
+            torch.where(byte == 255, torch.nan, powers))
 
 
 def round_e4m3(x):
@@ -74,7 +76,7 @@ def write(codes, scales, x, tables, lengths, starts, block):
                     e += 1
                 s = 2.0 ** e
                 before = scales[page, h].item()
-                if lo and before >= s:
+                if lo and (before >= s or math.isnan(before)):
                     s = before
                 elif lo:
                     codes[page, h, :lo] = round_e4m3(codes[page, h, :lo] * (before / s))

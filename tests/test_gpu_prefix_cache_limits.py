@@ -8,7 +8,8 @@ import pytest
 import torch
 
 import test_gpu_prefix_cache as base
-from kadllm_amd.ops import block_prefix_attention
+from kadllm_amd.ops import block_prefix_attention, write_prefix_blocks
+from oracle import prefix_cache_ref as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,30 @@ def test_queries_of_any_magnitude(device, D, lengths, times, W, H, block, expone
     q = (q.double() * 2.0 ** exponent).bfloat16()
     blocks.k_scale.view(torch.uint8).sub_(exponent % 256)
     _attend_and_check(q, blocks, tables, lens, sk, sv, gate, W, times)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("byte", [252, 253, 254, 255])
+def test_pages_of_the_largest_scales_are_extended(device, dtype, byte):
+    """Pages whose scale is 2^125 to 2^127, and pages that are not numbers (255): the
+    earlier tokens stay what they are, new ones are codes of that scale."""
+    blocks = base._pool(device, 3, 2, 32, 64, 36)
+    blocks.k_scale.view(torch.uint8)[:2] = byte
+    blocks.v_scale.view(torch.uint8)[1:] = byte
+    before = base._clone(blocks)
+    gen = torch.Generator().manual_seed(36)
+    k, v = (torch.randn(3, 9, 2, 64, generator=gen).mul(2.0 ** 125).to(dtype) for _ in range(2))
+    tables, starts, lengths = [[0], [1], [2]], [20, 1, 31], [29, 10, 32]
+    write_prefix_blocks(blocks, k.to(device), v.to(device), base._ints(tables, device),
+                        base._ints(lengths, device), starts=base._ints(starts, device))
+    for x, now, was in ((k, (blocks.k, blocks.k_scale), (before.k, before.k_scale)),
+                        (v, (blocks.v, blocks.v_scale), (before.v, before.v_scale))):
+        codes, scales = ref.decode(*was)
+        ref.write(codes, scales, x.double(), tables, lengths, starts, 32)
+        got_codes, got_scales = ref.decode(*now)
+        assert torch.equal(got_scales.isnan(), scales.isnan())
+        assert torch.equal(got_scales.nan_to_num(0), scales.nan_to_num(0))
+        # a token's value: of a page that is not a number, none
+        got, want = (c * s[..., None, None] for c, s in ((got_codes, got_scales), (codes, scales)))
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
