@@ -593,11 +593,19 @@ int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step_args* a,
  * request order from the front of free_blocks; tables gets the held entries of
  * old_tables [B, old_width], then the new pages, then -1, and *used the pages
  * needed in all (above num_free: the entries past the list are -1).  Lengths
- * above max_length <= width * block are cut there. */
+ * above max_length <= width * block are cut there.
+ * kad_prefix_block_tables_ex: the same behind the first *taken pages of the list
+ * (may be null: 0), which *used then counts too; `used` and `taken` must not be
+ * the same place. */
 int kad_prefix_block_tables(const int32_t* lengths, const int32_t* starts,
                             const int32_t* old_tables, int old_width, const int32_t* free_blocks,
                             int num_free, int32_t* tables, int width, int32_t* used, int B,
                             int block, int max_length, kad_stream_t stream);
+int kad_prefix_block_tables_ex(const int32_t* lengths, const int32_t* starts,
+                               const int32_t* old_tables, int old_width,
+                               const int32_t* free_blocks, int num_free, const int32_t* taken,
+                               int32_t* tables, int width, int32_t* used, int B, int block,
+                               int max_length, kad_stream_t stream);
 /* Token i of request b (k, v at [b*s_b + i*s_t + h*s_h + d], bf16, fp16 or
  * fp32) to position starts[b] + i (starts may be null: 0) while that is below
  * lengths[b].  A page's scale is the smallest power of two s >= 2^-100 with

@@ -72,6 +72,7 @@ SIGNATURES = {
     "kad_qwen_prefill": "pps",
     "kad_qwen_decode_step": "pps",
     "kad_prefix_block_tables": "pppipipipiiis",
+    "kad_prefix_block_tables_ex": "pppipippipiiis",
     "kad_write_prefix_blocks": "plll" "plll" "i" "pipp" "pppp" "iiiiii" "s",
     "kad_block_prefix_attention_workspace_bytes": "iiiiiiiip",
     "kad_block_prefix_attention": "plll" "ppppi" "pip" "plll" "plll" "plll" "plll" "pl"

@@ -113,7 +113,8 @@ def _check_blocks(blocks):
     return shape
 
 
-def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=None, tables=None):
+def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=None, tables=None,
+                        taken=None):
     """Pages for requests of ``lengths`` tokens.
 
     lengths [B] int32 are the requests' tokens after this step, at most
@@ -121,11 +122,13 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
     they hold already (default none), in the pages of the earlier ``tables``
     [B, columns].  A request gets ceil(lengths / block_size) -
     ceil(starts / block_size) pages more, in request order from the front of
-    ``free_blocks`` [F] int32.  Returns (tables [B, ceil(max_length /
-    block_size)] int32 with -1 past a request's last page, used [1] int32: the
-    pages taken, at most 2**31 - 1).  Where ``used`` exceeds F the list was too
-    short: the entries it could not fill are -1, and the other operators leave
-    such tokens out.
+    ``free_blocks`` [F] int32, behind the first ``taken`` [1] int32 (default
+    none).  Returns (tables [B, ceil(max_length / block_size)] int32 with -1 past
+    a request's last page, used [1] int32: the pages of the list that are taken
+    now, those before this call included, at most 2**31 - 1).  Where ``used``
+    exceeds F the list was too short: the entries it could not fill are -1, and
+    the other operators leave such tokens out.  A loop that hands ``used`` on as
+    the next call's ``taken`` gives out no page twice.
     """
     if not isinstance(block_size, int) or block_size not in BLOCK_SIZES:
         raise ValueError(f"block_size must be one of {BLOCK_SIZES}")
@@ -143,14 +146,16 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
         if starts is None:
             raise ValueError("earlier tables need the tokens held (starts)")
         tables = _check_int32("tables", tables, 2, B)
-    device = _device_of(lengths, free_blocks, starts, tables)
+    if taken is not None:
+        taken = _check_int32("taken", taken, 1, 1)
+    device = _device_of(lengths, free_blocks, starts, tables, taken)
     width = -(-max_length // block_size)
     out = torch.empty((B, width), dtype=torch.int32, device=lengths.device)
     used = torch.empty(1, dtype=torch.int32, device=lengths.device)
-    _launch(device, "kad_prefix_block_tables", lengths.data_ptr(), _lib.ptr(starts),
+    _launch(device, "kad_prefix_block_tables_ex", lengths.data_ptr(), _lib.ptr(starts),
             _lib.ptr(tables), 0 if tables is None else tables.shape[1], free_blocks.data_ptr(),
-            free_blocks.shape[0], out.data_ptr(), width, used.data_ptr(), B, block_size,
-            max_length)
+            free_blocks.shape[0], _lib.ptr(taken), out.data_ptr(), width, used.data_ptr(), B,
+            block_size, max_length)
     return out, used
 
 

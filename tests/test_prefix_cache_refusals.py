@@ -177,3 +177,13 @@ def test_oracle_scale_is_the_smallest_that_holds_the_values():
         ref.write(codes, scales, x, [[0]], [2], [0], 32)
         assert scales.item() == want and codes.abs().max() <= 448
         assert codes[0, 0, 1, 5].item() * want == pytest.approx(-amax, rel=2 ** -4)
+
+
+def test_tables_refuse_a_count_of_another_kind():
+    lengths, free = torch.ones(2, dtype=I32), torch.arange(4, dtype=I32)
+    for taken, error in ((torch.zeros(1, dtype=torch.int64), TypeError),
+                         (torch.zeros(2, dtype=I32), ValueError),
+                         (torch.zeros((), dtype=I32), ValueError),
+                         (torch.zeros(1, dtype=I32), RuntimeError)):   # not on a ROCm device
+        with pytest.raises(error):
+            prefix_block_tables(lengths, free, block_size=64, max_length=100, taken=taken)
