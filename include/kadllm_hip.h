@@ -586,7 +586,8 @@ int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step_args* a,
  * [pages, HK] e8m0 (2^(byte - 127)); a value is code * scale.  tables [B,
  * width] int32 name a request's pages in order; entries outside [0, pages)
  * name none.  Supported: D in {64, 128, 256}, block in {32, 64, 128, 256}, up to
- * 2^30 tokens a request (width * block).
+ * 2^30 tokens a request (width * block).  Calls of more workgroups than a grid holds
+ * (2^32 work-items) are refused, and block tables of more than 2^20 requests.
  *
  * kad_prefix_block_tables: request b needs ceil(lengths[b] / block) -
  * ceil(starts[b] / block) pages more (starts may be null: none held), taken in

@@ -1204,6 +1204,8 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
 //                                   1024 rows   39.4    46.0
 //   D 128,   8 requests, 4096 keys, 1024 rows   58.0    63.8
 //   D 128, 100 requests,  640 keys,   96 rows   27.9    25.5
+// Of the choices that a grid holds: fewer than 2^32 work-items, so fewer than 2^24
+// workgroups of 256 (splits 0: there is none).
 struct Plan {
   bool shared;
   int nqblk, splits;
@@ -1212,6 +1214,7 @@ struct Plan {
 Plan plan_of(int B, int HK, int R, int D, int keys) {
   Plan p = {};
   const int tiles = (int)kad_cdiv(keys, kKeys);
+  const double most = (1 << 24) - 1;
   double best = INFINITY;
   for (int form = 0; form < 2; ++form) {
     const bool shared = form == 1;
@@ -1220,7 +1223,9 @@ Plan plan_of(int B, int HK, int R, int D, int keys) {
     for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
       if (s > 1 && tiles < s * step) break;
       const int walk = ((tiles + s - 1) / s + step - 1) / step;
-      const double rounds = std::ceil((double)B * HK * nqblk * s / 256);
+      const double blocks = (double)B * HK * nqblk * s;
+      if (blocks > most || (s > 1 && (double)B * HK * R / (1024 / D) > most)) break;
+      const double rounds = std::ceil(blocks / 256);
       double cost = rounds * (30 * D + walk * per_step) + (shared ? 2000 : 0);
       if (s > 1) cost += 2000 + 0.0003 * s * B * HK * R * D * 4;
       if (cost < best) {
@@ -1232,7 +1237,7 @@ Plan plan_of(int B, int HK, int R, int D, int keys) {
   return p;
 }
 
-// a KV head's rows and a launch's workgroups in 32 bits (doubles hold any product)
+// a KV head's rows in 32 bits and all rows in 64 (doubles hold any product)
 bool rows_fit(int B, int W, int T, int H, int HK) {
   const double R = (double)W * T * (H / HK);
   return R <= 0x7fffffff - 256 && B * (double)HK * R / 4 <= 0x7fffffff;
@@ -1284,10 +1289,14 @@ extern "C" int kad_block_prefix_attention_workspace_bytes(int B, int W, int T, i
   KAD_REQUIRE(bytes, "null pointer argument");
   KAD_REQUIRE(B > 0 && W > 0 && T > 0 && H > 0 && HK > 0 && H % HK == 0 && width > 0,
               "empty dimensions");
-  KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
+  KAD_REQUIRE(D == 64 || D == 128 || D == 256, "head dim %d is not 64, 128 or 256", D);
+  KAD_REQUIRE(block > 0 && (int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens",
+              width, block);
   KAD_REQUIRE(rows_fit(B, W, T, H, HK), "too many rows for a launch");
-  const int64_t R = (int64_t)W * T * (H / HK);
-  *bytes = workspace_of(plan_of(B, HK, (int)R, D, width * block), B, HK, (int)R, D);
+  const int R = W * T * (H / HK);
+  const Plan p = plan_of(B, HK, R, D, width * block);
+  KAD_REQUIRE(p.splits > 0, "too many rows for a launch");
+  *bytes = workspace_of(p, B, HK, R, D);
   return KAD_OK;
 }
 
@@ -1327,10 +1336,10 @@ extern "C" int kad_block_prefix_attention(
   KAD_REQUIRE(rows_fit(B, W, T, H, HK), "too many rows for a launch");
   const int R = W * T * (H / HK);
   const Plan p = plan_of(B, HK, R, D, width * block);
+  KAD_REQUIRE(p.splits > 0, "too many rows for a launch");
   const int64_t need = workspace_of(p, B, HK, R, D);
   KAD_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
               "a workspace of %lld bytes at a 16-byte boundary is needed", (long long)need);
-  KAD_REQUIRE((int64_t)B * HK * p.splits * p.nqblk <= 0x7fffffff, "too many rows for a launch");
   BlockAttnArgs a = {};
   a.q = q; a.sq_n = sq_n; a.sq_t = sq_t; a.sq_h = sq_h;
   a.kc = (const uint8_t*)k_codes; a.vc = (const uint8_t*)v_codes;

@@ -75,6 +75,8 @@ extern "C" int kad_prefix_block_tables_ex(const int32_t* lengths, const int32_t*
   KAD_REQUIRE(lengths && tables && used && (free_blocks || num_free == 0),
               "null pointer argument");
   KAD_REQUIRE(max_length <= 1 << 30, "requests of %d tokens", max_length);
+  // (each workgroup adds up the requests before its own, so the work grows with B^2)
+  KAD_REQUIRE(B <= 1 << 20, "block tables of %d requests", B);
   KAD_REQUIRE(!old_tables || starts, "held tables need the tokens held");
   hipLaunchKernelGGL(block_tables_kernel, dim3((unsigned)B), dim3(256), 0, (hipStream_t)stream,
                      lengths, starts, old_tables, old_width, free_blocks, num_free, taken, tables,
@@ -261,11 +263,13 @@ __global__ __launch_bounds__(1024) void write_blocks_kernel(WriteArgs a) {
   if (tid == 0) *scale = (uint8_t)(e + 127);
 }
 
+// 4 pieces a thread, whole waves
+static int write_threads(int block, int D) { return max(64, block * D / (16 * kPieces)); }
+
 template <typename T>
 static void launch_write(const WriteArgs& a, bool vec, hipStream_t stream) {
   const dim3 grid((unsigned)(a.touched * a.B), (unsigned)a.HK, 2);
-  // 4 pieces a thread, whole waves
-  const int threads = max(64, a.block * a.D / (16 * kPieces));
+  const int threads = write_threads(a.block, a.D);
   if (vec)
     hipLaunchKernelGGL((write_blocks_kernel<T, true>), grid, dim3(threads), 0, stream, a);
   else
@@ -289,7 +293,9 @@ extern "C" int kad_write_prefix_blocks(
   // N tokens reach into at most this many pages of a request
   a.touched = (int)(starts ? ((int64_t)N + block - 2) / block + 1 : kad_cdiv(N, block));
   if (a.touched > width) a.touched = width;
-  KAD_REQUIRE((int64_t)a.touched * B <= 0x7fffffff && HK <= 65535, "too many pages for a launch");
+  // (a grid holds fewer than 2^32 work-items a dimension)
+  KAD_REQUIRE((int64_t)a.touched * B < (1ll << 32) / write_threads(block, D) && HK <= 65535,
+              "too many pages for a launch");
   KAD_REQUIRE((int64_t)width * block <= 1 << 30, "tables of %d columns of %d tokens", width, block);
   KAD_REQUIRE(((uintptr_t)k_codes % 16) == 0 && ((uintptr_t)v_codes % 16) == 0,
               "codes must be 16-byte aligned");

@@ -28,6 +28,7 @@ from . import _lib
 BLOCK_SIZES = (32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 MAX_LENGTH = 2**30          # tokens of a request
+MAX_REQUESTS = 2**20        # rows of a block table
 MAX_SUFFIX = 2**22          # suffix keys of a beam
 _CODES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -117,8 +118,8 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
                         taken=None):
     """Pages for requests of ``lengths`` tokens.
 
-    lengths [B] int32 are the requests' tokens after this step, at most
-    ``max_length`` (longer ones are cut there); starts [B] int32 the tokens
+    lengths [B] int32, B <= 2**20, are the requests' tokens after this step, at
+    most ``max_length`` (longer ones are cut there); starts [B] int32 the tokens
     they hold already (default none), in the pages of the earlier ``tables``
     [B, columns].  A request gets ceil(lengths / block_size) -
     ceil(starts / block_size) pages more, in request order from the front of
@@ -138,8 +139,8 @@ def prefix_block_tables(lengths, free_blocks, *, block_size, max_length, starts=
     lengths = _check_int32("lengths", lengths, 1)
     free_blocks = _check_int32("free_blocks", free_blocks, 1)
     B = lengths.shape[0]
-    if B < 1:
-        raise ValueError("lengths must not be empty")
+    if not 0 < B <= MAX_REQUESTS:
+        raise ValueError(f"lengths must be those of 1 to {MAX_REQUESTS} requests")
     if starts is not None:
         starts = _check_int32("starts", starts, 1, B)
     if tables is not None:

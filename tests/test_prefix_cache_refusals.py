@@ -187,3 +187,37 @@ def test_tables_refuse_a_count_of_another_kind():
                          (torch.zeros(1, dtype=I32), RuntimeError)):   # not on a ROCm device
         with pytest.raises(error):
             prefix_block_tables(lengths, free, block_size=64, max_length=100, taken=taken)
+
+
+def test_launches_past_a_grid_are_refused():
+    """A grid holds fewer than 2^32 work-items a dimension.  Addresses are never
+    read: every call is refused on the host, and one below the limit is not made."""
+    lib, p = _lib.load(), ctypes.c_void_p(256)
+    assert lib.kad_prefix_block_tables(p, None, None, 0, p, 1, p, 2, p, 2**20 + 1, 64, 100,
+                                       None) == -1
+    assert b"requests" in lib.kad_last_error()
+    with pytest.raises(ValueError, match="requests"):
+        prefix_block_tables(torch.ones(1, dtype=I32).expand(2**20 + 1), torch.arange(4, dtype=I32),
+                            block_size=64, max_length=100)
+    # 1024, 64 and 128 threads a page
+    for B, N, D, block, starts in ((2**22, 1, 256, 256, None), (2**26, 1, 64, 32, None),
+                                   (2**16, 2**16, 64, 128, None), (2**25, 2, 64, 64, p)):
+        assert lib.kad_write_prefix_blocks(p, 0, 0, 0, p, 0, 0, 0, 0, p, 2**16, p, starts, p, p, p, p,
+                                           1, B, N, 1, D, block, None) == -1
+        assert b"pages" in lib.kad_last_error()
+    need = ctypes.c_int64()
+    for B, W, H, HK, D, width in ((2**24, 1, 1, 1, 64, 1), (2**23, 1, 2, 2, 256, 1),
+                                  (2, 2**30, 1, 1, 128, 1), (2, 2**30, 1, 1, 64, 64)):
+        assert lib.kad_block_prefix_attention_workspace_bytes(
+            B, W, 1, H, HK, D, width, 64, ctypes.byref(need)) == -1
+        assert b"rows" in lib.kad_last_error()
+        assert lib.kad_block_prefix_attention(
+            p, 0, 0, 0, p, p, p, p, 1, p, width, p, None, 0, 0, 0, None, 0, 0, 0, None, 0, 0, 0, p, 0,
+            0, 0, p, 2**62, B, W, 1, 0, H, HK, D, 64, 0, 1.0, None) == -1
+        assert b"rows" in lib.kad_last_error()
+    size = lib.kad_block_prefix_attention_workspace_bytes
+    assert size(1, 1, 1, 2, 2, 96, 1, 64, ctypes.byref(need)) == -1
+    assert size(1, 1, 1, 2, 2, 64, 1, -64, ctypes.byref(need)) == -1
+    # one form's workgroups fit where the other's do not
+    assert size(1, 2**30, 1, 1, 1, 64, 1, 64, ctypes.byref(need)) == 0 and need.value == 0
+    assert size(2**24 - 1, 1, 1, 1, 1, 64, 1, 64, ctypes.byref(need)) == 0 and need.value == 0
