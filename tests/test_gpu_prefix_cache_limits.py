@@ -117,3 +117,28 @@ def test_pages_of_the_largest_scales_are_extended(device, dtype, byte):
         got, want = (c * s[..., None, None] for c, s in ((got_codes, got_scales), (codes, scales)))
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths, times, W, H, block", FORMS)
+def test_scores_that_climb_past_the_first_walk(device, dtype, D, lengths, times, W, H, block):
+    """Scores up to 174 above the first ones: past 2^60 in some rows and not in others, so
+    that some take their weights from a second walk.  Every output is held to its bound."""
+    pages = -(-max(lengths) // block)
+    _attend_and_check(*_climbing(device, lengths, W, 1, 1, H, 1, D, block, dtype,
+                                 [127 + j % 5 for j in range(pages)], seed=34), W, times)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("lengths, times, W, H, block", [FORMS[0], FORMS[2]])
+@pytest.mark.parametrize("T, Tk", [(1, 33), (3, 50)])
+def test_suffix_scores_that_climb_past_the_first_walk(device, dtype, D, lengths, times, W, H, block,
+                                                      T, Tk):
+    """Suffix scores that lie up to 12 above the first ones from key 16 on and up to 81
+    from key 32 on (a first walk holds fp16 suffix weights up to 2^14, bf16 ones up to
+    2^60)."""
+    byte = [127] * -(-max(lengths) // block)
+    _attend_and_check(*_climbing(device, lengths, W, T, Tk, H, 1, D, block, dtype, byte, seed=35,
+                                 suffix=lambda j: j // 16 + (j >= 32)), W, times)

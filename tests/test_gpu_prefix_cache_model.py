@@ -145,3 +145,23 @@ def test_refusals(device, tiny):
         plain.decode(ids[:, None], state)
     with pytest.raises(ValueError, match="transformers"):
         paged.prefix_to_cache(state)
+
+
+def test_prefixes_from_a_transformers_cache(device, tiny):
+    """The pages that prefix_from_cache fills are those that the prefill fills."""
+    cfg, _, plain, paged = tiny
+    ids = torch.randint(0, cfg.vocab_size, (2, 77),
+                        generator=torch.Generator().manual_seed(4)).to(device)
+    want = paged.prefill(ids).state
+    got = paged.prefix_from_cache(plain.prefix_to_cache(plain.prefill(ids).state), 77)
+    assert (got.length, got.batch) == (77, 2)
+    for kind, a, b in zip(cfg.layer_types, got.layers, want.layers):
+        assert isinstance(a, PagedPrefix) == (kind == "full_attention")
+        if isinstance(a, PagedPrefix):
+            for x, y in zip((*a.blocks, a.tables, a.lengths), (*b.blocks, b.tables, b.lengths)):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+        else:
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    history = torch.randint(0, cfg.vocab_size, (2, 5, 2),
+                            generator=torch.Generator().manual_seed(5)).to(device)
+    assert torch.equal(paged.decode(history, got), paged.decode(history, want))
