@@ -322,17 +322,24 @@ __device__ __forceinline__ void min_acc(float& x0, float& x1, float& x2, float& 
 // carry an exponent of their own; only when one lies more than 2^60 above (2^14
 // among fp16 suffix keys, less among values past 2^30: climb_of) is the walk done
 // again, with the row's true maximum.
-// What bounds it, bf16, D 256, 2 KV heads for 8 heads:
-//   16 requests of 1 beam over 32768 keys: HBM, 94 to 99 us for 537 MB, 5.4 to 5.7 TB/s
-//     (private, 8 ranges each).
-//   32 requests of 256 beams over 1024 keys, gated: 102 us for 69 GFLOP and 168 MB,
-//     two rounds of workgroups that load q, walk and store together.  A step of the
-//     walk takes about 2900 cycles where its 32 MFMAs take 2048: the softmax and the
-//     pieces of the weights fill the issue slots between them.  Half the first round
-//     started late, to set the phases apart, measured the same.
-//   1 request of 256 beams over 8192 keys: 35 to 37 us, the walk at the same rate.
-//   1 request of 1 beam over 100 keys: 10.5 us, latency: q, page numbers, keys, values,
-//     the join of four waves and the store one after another.
+// What bounds it, bf16, D 256, 2 KV heads for 8 heads (traced kernel times, which are
+// some us longer than those of calls that follow each other):
+//   16 requests of 1 beam over 32768 keys: HBM, 95 to 100 us for 537 MB (private, 8
+//     ranges each), and 5 us of join.
+//   32 requests of 256 beams over 1024 keys, gated: 106 to 112 us (102 in a row of
+//     calls) for 69 GFLOP and 168 MB, two rounds of workgroups that load q, walk and
+//     store together.  Fitted over calls without a gate, a step of the walk takes 1.8 us
+//     (its 32 MFMAs 2048 cycles, about half of that; the softmax and the pieces of the
+//     weights are the rest) and a round 19 us besides: q and its pieces, the first
+//     tiles, the results through LDS and out, with no other workgroup on the CU (512
+//     registers and 133 KB of LDS).  Half the first round started late, to set the
+//     phases apart, measured the same.  fp16, with three pieces: 145 to 150 us; 2.6 us a
+//     step and 24 us a round.
+//   1 request of 256 beams over 8192 keys: 35 to 37 us (private, 4 ranges; 2.5 us a step
+//     of four tiles, 13 us besides), and 4 us of join.
+//   1 request of 1 beam over 100 keys: 10.5 us, most of it that fixed part.
+// Vector registers that do not fit and go to scratch: 6 in the shared form of bf16 at
+// D 256, 54 in that of fp16, 12 in the private form of fp16 at D 128.
 template <typename T, int D, bool SHARED>
 __global__ __launch_bounds__(256, D == 256 || SHARED ? 1 : 2) void
 block_attn_kernel(BlockAttnArgs a) {
@@ -1191,9 +1198,11 @@ __global__ __launch_bounds__(256) void block_attn_join_kernel(BlockAttnArgs a) {
 //   private: 600 + 6 D (four tiles for 32 rows; each wave waits for its own),
 //   shared:  800 + 3 D (one tile for 128 rows), and 2000 a call, its rings' filling
 // and a split costs 2000 for the second kernel and 0.3 a KB of partial results.
-// Fitted to 3507 measured (form, ranges) of 376 calls, D 64 to 256, 1 to 100
-// requests, 256 to 20000 keys and 4 to 1024 rows: what it takes is 0.6% slower than
-// the best measured choice in the mean and 12% at worst.  (A limit in rows alone,
+// Fitted to 3507 measured (form, ranges) of 306 calls, bf16 and fp16, D 64 to 256, 1 to
+// 100 requests, 256 to 20000 keys, 4 to 1024 rows and one suffix key: what it takes is
+// 0.6% slower than the best measured choice in the mean and 12% at worst.  It counts
+// the tokens that the tables can hold, as the lengths are on the GPU, and neither the
+// suffix nor the pieces.  (A limit in rows alone,
 // shared from 65 on, lost 7 to 25% in the mean and up to 2.6 times.)  Both sides, us,
 // bf16, 2 KV heads:
 //                                    private  shared

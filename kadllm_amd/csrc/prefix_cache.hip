@@ -171,9 +171,10 @@ __device__ __forceinline__ void store16(uint8_t* p, const float* f, float scale)
 // A page and head is block * D / 16 pieces of 16 elements.  Each of up to 1024
 // threads keeps 4 of them in registers between the maximum and the rounding, so
 // the input is read once and the codes are written once, 16 bytes a lane.
-// Bound by HBM: 32 requests of 1024 tokens (bf16, 2 KV heads of 256; 101 MB) in 19.2 us,
-// 5.2 TB/s, and 8 of up to 20000 (fp16, 8 heads of 128; 492 MB) in 98 us, 5.0 TB/s, the
-// rate of a large copy (5.18).  One token for each of 256 requests: 5.6 us.
+// Bound by HBM: 32 requests of 1024 tokens (bf16, 2 KV heads of 256; 101 MB) in 19.4 us,
+// 5.2 TB/s, and 8 of up to 20000 (fp16, 8 heads of 128; 492 MB) in 98 to 100 us, 4.9 to
+// 5.0 TB/s, the rate of a large copy (5.18).  The 32 in fp32 (168 MB, part of it from the
+// memory-side cache in repeated calls): 25 us.  One token for each of 256 requests: 5.7 us.
 // VEC: rows of the input start at 16-byte boundaries (else element by element).
 constexpr int kPieces = 4;
 

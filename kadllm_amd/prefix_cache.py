@@ -173,10 +173,12 @@ def write_prefix_blocks(blocks, k, v, tables, lengths, *, starts=None):
     keeps the larger of its scale and the new tokens'; when that grows, the
     earlier codes are rounded to the new scale (a scale that is not a number
     stays, and the new codes are NaN).  Codes are x / s to the nearest e4m3 value
-    (ties to even); infinities and NaN become NaN.  Rows behind lengths[b] and
-    pages the call does not reach are left as they were; tokens whose table
-    entry names no page are left out.  Two requests of one call must not write
-    to the same page.  Returns ``blocks``.
+    (ties to even): off by up to 2**-4 of x, or by 2**-10 s where that is more;
+    infinities and NaN become NaN.  Rows behind lengths[b] and pages the call
+    does not reach are left as they were; tokens whose table entry names no page
+    are left out.  Tokens are written in order: codes behind the last one written
+    to a page stay, but not the scale they were made for.  One call must not
+    write to a page twice.  Returns ``blocks``.
     """
     pages, HK, block, D = _check_blocks(blocks)
     shape = k.shape
@@ -219,6 +221,14 @@ def block_prefix_attention(q, blocks, tables, lengths, suffix_k=None, suffix_v=N
     newest tokens are already in the cache.  ``scale`` defaults to D**-0.5;
     ``gate`` [B*W, T, H*D] multiplies the output by sigmoid(gate).  Returns
     [B*W, T, H, D] in q's type; a query that sees no key gets zeros.
+
+    Scores, sums and the output are held in fp32.  The softmax weights of cached
+    keys are off by up to 2**-8 of themselves for bf16 and 2**-12 for fp16, or 2**-17
+    of the largest where that is more; those of suffix keys are rounded to q's
+    type; elements of q below 2**-10 of their row's largest are off by up to 2**-21
+    of it.  A suffix is walked 16 keys at a time by a part of the workgroups, which
+    suits the few tokens of a search; the bulk of a long one is better written to
+    the cache first.
     """
     if type(beam_width) is not int or beam_width <= 0:
         raise ValueError("beam_width must be a positive integer")
