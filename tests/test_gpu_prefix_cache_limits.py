@@ -142,3 +142,24 @@ def test_suffix_scores_that_climb_past_the_first_walk(device, dtype, D, lengths,
     byte = [127] * -(-max(lengths) // block)
     _attend_and_check(*_climbing(device, lengths, W, T, Tk, H, 1, D, block, dtype, byte, seed=35,
                                  suffix=lambda j: j // 16 + (j >= 32)), W, times)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths, times, W, T, Tk, H, D", [
+    ([100], 1, 1, 1, 1, 2, 256), ([1, 0, 33, 700], 1, 5, 2, 2, 4, 64),
+    ([100, 0], 40, 97, 1, 2, 1, 128), ([65, 1], 40, 97, 1, 0, 1, 256)])
+def test_tables_much_wider_than_the_lengths(device, dtype, lengths, times, W, T, Tk, H, D):
+    """Tables of 4096 tokens over short requests: most of the ranges that the prefix is
+    split into hold no keys, some requests none at all."""
+    q, blocks, tables, lens, sk, sv, gate = base._problem(device, lengths, W, T, Tk, H, 1, D, 64,
+                                                          dtype, gated=True, seed=37)
+    wide = torch.full((len(lengths), 64), 10**6, dtype=torch.int32, device=device)
+    wide[:, ::3] = -1
+    wide[:, :tables.shape[1]] = tables
+    _attend_and_check(q, blocks, wide, lens, sk, sv, gate, W, times)
+    if times == 1:      # what lies in the columns behind the lengths does not matter
+        other = wide.clone()
+        other[:, tables.shape[1]:] = 0
+        a, b = (block_prefix_attention(q, blocks, t, lens, sk, sv, beam_width=W, gate=gate)
+                for t in (wide, other))
+        assert torch.equal(a, b)
