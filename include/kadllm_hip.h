@@ -642,6 +642,48 @@ int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_
                                float scale, kad_stream_t stream);
 
 /* --------------------------------------------------------------------------
+ * Weights in 4 bits, and products with them (no reference counterpart: its weights
+ * stay in the model's type, src/kadllm/adapters/qwen3_5.py:144-235).
+ *
+ * A weight [N, K] in groups of 32 neighbours of a row: e2m1 codes (0, 1/2, 1, 3/2, 2,
+ * 3, 4, 6 and their negatives) and an e8m0 scale 2^(byte - 127) for each; a value is
+ * code * scale.  Rows padded to 16 and columns to 128 with zero codes; codes
+ * [N/16][K/128][64][16 bytes]: entry l of a block holds row l % 16, columns 32 (l / 16)
+ * .. +31, the even column in a byte's low half; scales [N/16][K/512][64][4]: byte j of
+ * entry l is that group's in the j-th of four blocks.  Scales are from 2^-100 to 2^125, or NaN
+ * (255).  Both arrays 16-byte aligned.  K up to 2^20, N up to 2^26.
+ *
+ * kad_quantize_weight: w [N, K] (bf16, fp16 or fp32, rows at stride ldw); a group's
+ * scale is the smallest with amax <= 7 * scale, the codes w / scale to the nearest,
+ * ties to the even code, at most 6; a group with an infinity or NaN gets the NaN scale.
+ * kad_dequantize_weight: the values, rounded to the type of out. */
+int kad_quantize_weight(const void* w, int64_t ldw, int dtype, void* codes, void* scales, int N,
+                        int K, kad_stream_t stream);
+int kad_dequantize_weight(const void* codes, const void* scales, void* out, int64_t ldo, int dtype,
+                          int N, int K, kad_stream_t stream);
+/* y[M, N] = x[M, K] W^T + residual[M, N] (may be null, may be y), all of one dtype
+ * (bf16, fp16, fp32) with rows at strides ldx, ldy, ldr; fp32 sums, rounded once.  The
+ * workspace (16-byte aligned) has the size that kad_quantized_linear_workspace_bytes
+ * gives for the same x, ldx and sizes (0: none); calls that overlap need one each. */
+int kad_quantized_linear_workspace_bytes(const void* x, int64_t ldx, int dtype, int M, int N,
+                                         int K, int64_t* bytes);
+int kad_quantized_linear(const void* x, int64_t ldx, int dtype, const void* codes,
+                         const void* scales, const void* residual, int64_t ldr, void* y,
+                         int64_t ldy, void* workspace, int64_t workspace_bytes, int M, int N,
+                         int K, kad_stream_t stream);
+/* y[M, H] = (silu(x G^T) * (x U^T)) D^T + residual, x [M, H], G and U [F, H], D [H, F];
+ * strides, types and workspace as above.  The product in the middle is held in
+ * bf16 for bf16 rows (2^-8 of itself), to 2^-15 for fp16 and 2^-22 for fp32. */
+int kad_quantized_gated_ffn_workspace_bytes(const void* x, int64_t ldx, int dtype, int M, int H,
+                                            int F, int64_t* bytes);
+int kad_quantized_gated_ffn(const void* x, int64_t ldx, int dtype, const void* gate_codes,
+                            const void* gate_scales, const void* up_codes, const void* up_scales,
+                            const void* down_codes, const void* down_scales,
+                            const void* residual, int64_t ldr, void* y, int64_t ldy,
+                            void* workspace, int64_t workspace_bytes, int M, int H, int F,
+                            kad_stream_t stream);
+
+/* --------------------------------------------------------------------------
  * MFMA lane-layout self-test (no reference counterpart): C[16x16] = A[16x32]
  * B[32x16] (bf16 in, fp32 out, all row-major) computed by one wave with the
  * operand layout the kernels above assume for v_mfma_f32_16x16x32_bf16, and

@@ -10,9 +10,10 @@ not provided.
 """
 
 from kadllm_amd import (Constraint, GRBeamAdapter, GRBeamResult, PrefillResult, PrefixBlocks,
-                        block_prefix_attention, causal_conv1d, conditional_search, gated_delta,
-                        grbeam_search, merge_attention, prefix_attention, prefix_block_tables,
-                        write_prefix_blocks)
+                        QuantizedWeight, block_prefix_attention, causal_conv1d,
+                        conditional_search, dequantize_weight, gated_delta, grbeam_search,
+                        merge_attention, prefix_attention, prefix_block_tables, quantize_weight,
+                        quantized_gated_ffn, quantized_linear, write_prefix_blocks)
 
 from . import adapters, grbeam, ops  # noqa: E402  (the reference's submodules)
 
@@ -31,4 +32,9 @@ __all__ = [
     "prefix_block_tables",
     "write_prefix_blocks",
     "block_prefix_attention",
+    "QuantizedWeight",
+    "quantize_weight",
+    "dequantize_weight",
+    "quantized_linear",
+    "quantized_gated_ffn",
 ]

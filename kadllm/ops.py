@@ -2,7 +2,8 @@
 the validation helpers the reference's benchmark imports (``_gdn_launch``,
 benchmarks/grbeam.py:99)."""
 
-from kadllm_amd.ops import (PrefixBlocks, _backend, _gdn_launch, _same_device,  # noqa: F401
-                            _width, block_prefix_attention, causal_conv1d, gated_delta,
-                            merge_attention, prefix_attention, prefix_block_tables,
-                            write_prefix_blocks)
+from kadllm_amd.ops import (PrefixBlocks, QuantizedWeight, _backend, _gdn_launch,  # noqa: F401
+                            _same_device, _width, block_prefix_attention, causal_conv1d,
+                            dequantize_weight, gated_delta, merge_attention, prefix_attention,
+                            prefix_block_tables, quantize_weight, quantized_gated_ffn,
+                            quantized_linear, write_prefix_blocks)

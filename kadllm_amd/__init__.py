@@ -4,8 +4,9 @@ Public names follow the reference package (src/kadllm/__init__.py:3-18):
 ``grbeam_search``, ``GRBeamAdapter``, ``PrefillResult``, ``GRBeamResult``,
 the operators ``gated_delta``, ``causal_conv1d``, ``prefix_attention`` and the
 adapter ``adapters.Qwen35GRBeamAdapter``; beyond them ``conditional_search``
-(coarse levels, then per-coarse-beam quotas) and the 8-bit prefix cache
-(``PrefixBlocks`` and its three operators).  All numerics run in the HIP
+(coarse levels, then per-coarse-beam quotas), the 8-bit prefix cache
+(``PrefixBlocks`` and its three operators) and 4-bit weights
+(``QuantizedWeight`` and its four operators).  All numerics run in the HIP
 kernels of ``libkadllm_hip.so`` (built by ``python -m kadllm_amd.csrc.build``).
 """
 
@@ -14,6 +15,8 @@ from .grbeam import (Constraint, GRBeamAdapter, GRBeamResult, PrefillResult, con
 from .ops import causal_conv1d, gated_delta, merge_attention, prefix_attention
 from .prefix_cache import (PrefixBlocks, block_prefix_attention, prefix_block_tables,
                            write_prefix_blocks)
+from .quantized import (QuantizedWeight, dequantize_weight, quantize_weight,
+                        quantized_gated_ffn, quantized_linear)
 
 __all__ = [
     "GRBeamResult",
@@ -30,4 +33,9 @@ __all__ = [
     "prefix_block_tables",
     "write_prefix_blocks",
     "block_prefix_attention",
+    "QuantizedWeight",
+    "quantize_weight",
+    "dequantize_weight",
+    "quantized_linear",
+    "quantized_gated_ffn",
 ]

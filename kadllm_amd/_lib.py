@@ -77,6 +77,12 @@ SIGNATURES = {
     "kad_block_prefix_attention_workspace_bytes": "iiiiiiiip",
     "kad_block_prefix_attention": "plll" "ppppi" "pip" "plll" "plll" "plll" "plll" "pl"
                                   "iiiiiiiii" "f" "s",
+    "kad_quantize_weight": "plippiis",
+    "kad_dequantize_weight": "pppliiis",
+    "kad_quantized_linear_workspace_bytes": "pliiiip",
+    "kad_quantized_linear": "pli" "pp" "plpl" "pl" "iii" "s",
+    "kad_quantized_gated_ffn_workspace_bytes": "pliiiip",
+    "kad_quantized_gated_ffn": "pli" "pppppp" "plpl" "pl" "iii" "s",
     "kad_selftest_mfma_f32": "ppps",
     "kad_selftest_mfma16": "ppps",
     "kad_selftest_mfma32": "ppps",

@@ -20,6 +20,8 @@ import torch
 from . import _lib
 from .prefix_cache import (PrefixBlocks, block_prefix_attention,  # noqa: F401
                            prefix_block_tables, write_prefix_blocks)
+from .quantized import (QuantizedWeight, dequantize_weight, quantize_weight,  # noqa: F401
+                        quantized_gated_ffn, quantized_linear)
 
 
 def _backend(name, tensors):

@@ -1,0 +1,257 @@
+"""Weights in 4 bits, and products with them.
+
+A ``QuantizedWeight`` holds a weight [N, K] in groups of 32 neighbours of a row:
+e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives) and one e8m0 scale (a
+power of two) for each group, 4.25 bits an element.  A value is code * scale, which is
+exact in bf16.
+
+    q = quantize_weight(w)                       # or QuantizedWeight.pack(codes, scales)
+    y = quantized_linear(x, q, residual=r)       # x W^T + r
+    y = quantized_gated_ffn(x, gate, up, down)   # (silu(x G^T) * (x U^T)) D^T
+
+Everything runs on the GPU without a host synchronisation (but for ``pack``, which
+looks at the scales once); no counterpart in the reference, whose weights stay in the
+model's type (src/kadllm/adapters/qwen3_5.py:144-235).
+"""
+
+import ctypes
+import functools
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .prefix_cache import _device_of, _launch
+
+GROUP = 32                  # columns of a row that share a scale
+MAX_COLS = 2**20            # columns of a weight
+MAX_WEIGHT_ROWS = 2**26     # rows of a weight
+MAX_ROWS = 16 * 65535       # rows of x
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_SCALES = torch.float8_e8m0fnu
+
+
+def _padded(rows, cols):
+    """The shapes of a weight's codes and scales."""
+    nb, kb = -(-rows // 16), -(-cols // 128)
+    return (nb, kb, 64, 16), (nb, -(-kb // 4), 64, 4)
+
+
+class QuantizedWeight(NamedTuple):
+    """A weight [rows, cols] in 4 bits, as quantized_linear reads it: codes uint8
+    [rows/16, cols/128, 64, 16] and scales torch.float8_e8m0fnu [rows/16, cols/512,
+    64, 4] (sizes rounded up), of which entry l of a block is row l % 16, columns
+    32 (l // 16) to + 31."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    cols: int
+
+    @classmethod
+    def pack(cls, codes, scales, *, cols=None):
+        """From row-major parts: codes [N, ceil(K / 2)] (uint8, or
+        torch.float4_e2m1fn_x2, the even column in a byte's low half) and scales
+        [N, ceil(K / 32)] (torch.float8_e8m0fnu or its bytes as uint8), from 2**-100
+        to 2**125 or NaN.  ``cols`` is K (default: two for each byte)."""
+        if codes.dtype is torch.float4_e2m1fn_x2:
+            codes = codes.view(torch.uint8)
+        if scales.dtype is _SCALES:
+            scales = scales.view(torch.uint8)
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
+            raise TypeError("codes are uint8 or float4_e2m1fn_x2, scales float8_e8m0fnu or uint8")
+        if codes.ndim != 2 or scales.ndim != 2 or 0 in codes.shape:
+            raise ValueError("codes must be [N, K / 2] and scales [N, K / 32]")
+        N, half = codes.shape
+        K = 2 * half if cols is None else cols
+        _check_size(N, K)
+        if half != -(-K // 2) or scales.shape != (N, -(-K // GROUP)):
+            raise ValueError("codes must be [N, K / 2] and scales [N, K / 32]")
+        if codes.device != scales.device:
+            raise ValueError("all tensors must be on the same device")
+        if bool(((scales < 27) | ((scales > 252) & (scales < 255))).any()):
+            raise ValueError("scales must be from 2**-100 to 2**125, or NaN")
+        if K % 2:
+            codes = torch.cat((codes[:, :-1], codes[:, -1:] & 15), 1)
+        (nb, kb, _, _), (_, k4, _, _) = _padded(N, K)
+        pad = torch.nn.functional.pad
+        codes = pad(codes, (0, kb * 64 - half, 0, nb * 16 - N))
+        codes = codes.view(nb, 16, kb, 4, 16).permute(0, 2, 3, 1, 4)
+        scales = pad(scales, (0, k4 * 16 - scales.shape[1], 0, nb * 16 - N), value=27)
+        scales = scales.view(nb, 16, k4, 4, 4).permute(0, 2, 4, 1, 3)
+        return cls(codes.reshape(nb, kb, 64, 16), scales.reshape(nb, k4, 64, 4).view(_SCALES), N, K)
+
+    def unpack(self):
+        """(codes [N, ceil(K / 2)] uint8, scales [N, ceil(K / 32)] float8_e8m0fnu):
+        the row-major parts that ``pack`` takes."""
+        _check_weight(self)
+        nb, kb, k4 = self.codes.shape[0], self.codes.shape[1], self.scales.shape[1]
+        codes = self.codes.view(nb, kb, 4, 16, 16).permute(0, 3, 1, 2, 4).reshape(nb * 16, -1)
+        scales = self.scales.view(torch.uint8).view(nb, k4, 4, 16, 4).permute(0, 3, 1, 4, 2)
+        scales = scales.reshape(nb * 16, -1)[:self.rows, :-(-self.cols // GROUP)]
+        return (codes[:self.rows, :-(-self.cols // 2)].contiguous(),
+                scales.contiguous().view(_SCALES))
+
+
+def _check_size(rows, cols):
+    if type(rows) is not int or type(cols) is not int or not 0 < rows <= MAX_WEIGHT_ROWS or \
+            not 0 < cols <= MAX_COLS:
+        raise ValueError(f"a weight has 1 to {MAX_WEIGHT_ROWS} rows of 1 to {MAX_COLS} columns")
+
+
+def _check_weight(w, name="weight"):
+    if not isinstance(w, QuantizedWeight):
+        raise TypeError(f"{name} must be a QuantizedWeight")
+    if w.codes.dtype is not torch.uint8 or w.scales.dtype is not _SCALES:
+        raise TypeError("the codes of a weight are uint8 and its scales float8_e8m0fnu")
+    _check_size(w.rows, w.cols)
+    if (w.codes.shape, w.scales.shape) != _padded(w.rows, w.cols):
+        raise ValueError("codes and scales do not fit the weight's size")
+    if not (w.codes.is_contiguous() and w.scales.is_contiguous()):
+        raise ValueError("the tensors of a 4-bit weight must be contiguous")
+
+
+def _no_gradients(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
+
+
+def _rows(t):
+    """t [M, C] with a contiguous last dimension and rows that do not overlap, and
+    the stride of its rows."""
+    M, C = t.shape
+    if t.stride(1) != 1 and C > 1 or t.stride(0) < C and M > 1:
+        t = t.contiguous()
+    return t, max(t.stride(0), C)
+
+
+def quantize_weight(weight):
+    """``weight`` [N, K] (bf16, fp16 or fp32, any strides) in 4 bits.
+
+    A group's scale is the smallest power of two s, from 2**-100 to 2**125, with amax <=
+    7 s; its codes are w / s to the nearest e2m1 value, ties to the even code, at
+    most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s and s above.
+    A group that holds an infinity or NaN reads as NaN.  Columns past K and rows past N
+    of the padded arrays are zeros.  Returns a QuantizedWeight."""
+    if weight.ndim != 2 or 0 in weight.shape:
+        raise ValueError("a weight must be [N, K]")
+    if weight.dtype not in _TYPES:
+        raise TypeError("weights must be bf16, fp16 or fp32")
+    N, K = weight.shape
+    _check_size(N, K)
+    _no_gradients(weight)
+    device = _device_of(weight)
+    weight, ld = _rows(weight)
+    shapes = _padded(N, K)
+    codes = torch.empty(shapes[0], dtype=torch.uint8, device=weight.device)
+    scales = torch.empty(shapes[1], dtype=torch.uint8, device=weight.device).view(_SCALES)
+    _launch(device, "kad_quantize_weight", weight.data_ptr(), ld, _lib.dtype_code(weight.dtype),
+            codes.data_ptr(), scales.data_ptr(), N, K)
+    return QuantizedWeight(codes, scales, N, K)
+
+
+def dequantize_weight(weight, dtype=torch.bfloat16):
+    """The values [N, K] of a QuantizedWeight in ``dtype`` (bf16 and fp32: exactly)."""
+    _check_weight(weight)
+    if dtype not in _TYPES:
+        raise TypeError("weights must be bf16, fp16 or fp32")
+    device = _device_of(weight.codes, weight.scales)
+    out = torch.empty(weight.rows, weight.cols, dtype=dtype, device=weight.codes.device)
+    _launch(device, "kad_dequantize_weight", weight.codes.data_ptr(), weight.scales.data_ptr(),
+            out.data_ptr(), weight.cols, _lib.dtype_code(dtype), weight.rows, weight.cols)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, offset, *sizes):
+    """Of a call whose x is ``offset`` bytes past a 16-byte boundary."""
+    need = ctypes.c_int64(0)
+    _lib.call(name, offset, *sizes, ctypes.byref(need))
+    return need.value
+
+
+def _workspace(name, x, *sizes):
+    """(buffer or None, its bytes) for a call on x."""
+    need = _workspace_bytes(name + "_workspace_bytes", x.data_ptr() & 15, *sizes)
+    return (torch.empty(need, dtype=torch.uint8, device=x.device) if need else None), need
+
+
+def _check_rows(x, cols, out_cols, residual):
+    """x [..., cols] and residual [..., out_cols] (or None) as 2-D rows."""
+    if x.ndim < 1 or x.shape[-1] != cols or 0 in x.shape:
+        raise ValueError(f"x must be [..., {cols}], the weight's columns, and not empty")
+    if x.dtype not in _TYPES:
+        raise TypeError("x must be bf16, fp16 or fp32")
+    if residual is not None:
+        if residual.shape != (*x.shape[:-1], out_cols):
+            raise ValueError(f"residual must be x's rows of {out_cols}")
+        if residual.dtype is not x.dtype:
+            raise ValueError("x and residual must have the same dtype")
+        residual = residual.reshape(-1, out_cols)
+    x = x.reshape(-1, cols)
+    if x.shape[0] > MAX_ROWS:
+        raise ValueError(f"x has at most {MAX_ROWS} rows")
+    return x, residual
+
+
+def quantized_linear(x, weight, *, residual=None):
+    """x W^T (+ residual) for a QuantizedWeight W [N, K].
+
+    x [..., K] bf16, fp16 or fp32 (any strides); residual [..., N] of x's type.
+    Returns [..., N] in x's type.  Products are exact, sums are fp32 and are rounded
+    once, with the residual added."""
+    _check_weight(weight)
+    rows, r = _check_rows(x, weight.cols, weight.rows, residual)
+    _no_gradients(x, residual)
+    _device_of(x, residual, weight.codes, weight.scales)
+    out = torch.empty(rows.shape[0], weight.rows, dtype=x.dtype, device=x.device)
+    return _linear(rows, weight, out, r).view(*x.shape[:-1], weight.rows)
+
+
+def _linear(x, weight, out, residual=None):
+    """quantized_linear on checked 2-D rows, into ``out`` (rows of any stride; it
+    may be ``residual``)."""
+    x, ldx = _rows(x)
+    M, N, K = x.shape[0], weight.rows, weight.cols
+    r, ldr = (None, 0) if residual is None else _rows(residual)
+    code = _lib.DTYPE_CODES[x.dtype]
+    ws, need = _workspace("kad_quantized_linear", x, ldx, code, M, N, K)
+    _launch(x.get_device(), "kad_quantized_linear", x.data_ptr(), ldx, code,
+            weight.codes.data_ptr(), weight.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(),
+            max(out.stride(0), N), _lib.ptr(ws), need, M, N, K)
+    return out
+
+
+def quantized_gated_ffn(x, gate, up, down, *, residual=None):
+    """(silu(x G^T) * (x U^T)) D^T (+ residual) for QuantizedWeights gate and up
+    [F, H] and down [H, F].
+
+    x [..., H] bf16, fp16 or fp32 (any strides); residual [..., H] of x's type.
+    Returns [..., H] in x's type.  Sums are fp32.  The product of the two
+    projections, whose SiLU is computed in fp32, is held in bf16 for bf16 rows (off
+    by up to 2**-8 of itself), to 2**-15 for fp16 and 2**-22 for fp32."""
+    for name, w in (("gate", gate), ("up", up), ("down", down)):
+        _check_weight(w, name)
+    F, H = gate.rows, gate.cols
+    if (up.rows, up.cols) != (F, H) or (down.rows, down.cols) != (H, F):
+        raise ValueError("gate and up must be [F, H] and down [H, F]")
+    rows, r = _check_rows(x, H, H, residual)
+    _no_gradients(x, residual)
+    _device_of(x, residual, *(t for w in (gate, up, down) for t in (w.codes, w.scales)))
+    out = torch.empty(rows.shape[0], H, dtype=x.dtype, device=x.device)
+    return _gated_ffn(rows, gate, up, down, out, r).view(x.shape)
+
+
+def _gated_ffn(x, gate, up, down, out, residual=None):
+    """quantized_gated_ffn on checked 2-D rows, into ``out`` (rows of any stride; it
+    may be ``residual``)."""
+    x, ldx = _rows(x)
+    M, F, H = x.shape[0], gate.rows, gate.cols
+    r, ldr = (None, 0) if residual is None else _rows(residual)
+    code = _lib.DTYPE_CODES[x.dtype]
+    ws, need = _workspace("kad_quantized_gated_ffn", x, ldx, code, M, H, F)
+    _launch(x.get_device(), "kad_quantized_gated_ffn", x.data_ptr(), ldx, code,
+            gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
+            up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), _lib.ptr(r), ldr,
+            out.data_ptr(), max(out.stride(0), H), _lib.ptr(ws), need, M, H, F)
+    return out
