@@ -648,10 +648,10 @@ int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_
  * A weight [N, K] in groups of 32 neighbours of a row: e2m1 codes (0, 1/2, 1, 3/2, 2,
  * 3, 4, 6 and their negatives) and an e8m0 scale 2^(byte - 127) for each; a value is
  * code * scale.  Rows padded to 16 and columns to 128 with zero codes; codes
- * [N/16][K/128][64][16 bytes]: entry l of a block holds row l % 16, columns 32 (l / 16)
- * .. +31, the even column in a byte's low half; scales [N/16][K/512][64][4]: byte j of
- * entry l is that group's in the j-th of four blocks.  Scales are from 2^-100 to 2^125, or NaN
- * (255).  Both arrays 16-byte aligned.  K up to 2^20, N up to 2^26.
+ * [N/16][K/128][64][4 words]: word j of entry l of a block holds row l % 16, columns 32 j +
+ * 8 (l / 16) .. +7, the first in the lowest bits; scales [N/16][K/128][16 rows][4 groups].
+ * Scales are from 2^-100 to 2^125, or NaN (255).  Both arrays 16-byte aligned.  K up to 2^20,
+ * N up to 2^26.
  *
  * kad_quantize_weight: w [N, K] (bf16, fp16 or fp32, rows at stride ldw); a group's
  * scale is the smallest with amax <= 7 * scale, the codes w / scale to the nearest,

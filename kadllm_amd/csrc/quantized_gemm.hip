@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ x
 }
 
 struct Args {
-  const bf16_t* x;           // pieces of the rows: (p, m, k) at x[p * xp + m * ldx + k]
+  const void* x;             // rows of T, or their pieces: (p, m, k) at x[p * xp + m * ldx + k]
   int64_t ldx, xp;
   const uint8_t* codes[2];   // the weight, or gate and up
   const uint8_t* scales[2];
@@ -81,7 +81,7 @@ struct Args {
   int64_t ldr;
   void* y;                   // linear: rows of T; gated: pieces, (p, m, n) as for x
   int64_t ldy, yp;
-  int M, N, KB;
+  int M, N, K, KB;           // KB blocks of 128 columns
   int cols;                  // columns that are written: N, or (gated) N padded to 128
   int vec;                   // 4 neighbours of y (and r) may go as one access
 };
@@ -139,47 +139,354 @@ __device__ __forceinline__ void finish(const Args& a, int m, int n, const f32x4*
   }
 }
 
-// One workgroup: 16 rows of x and 16 of the weight(s), K split over its 4 waves, whose
-// sums meet in LDS.
-template <typename T, bool GATED>
-__global__ __launch_bounds__(256) void q4_kernel(Args a) {
-  constexpr int P = kPieces<T>, W = GATED ? 2 : 1, KS = 4;
-  __shared__ f32x4 part[KS][W][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-  const int nt = blockIdx.x, m0 = blockIdx.y * 16;
-  const int NB = (a.N + 15) / 16, nb = min(nt, NB - 1), K4 = (a.KB + 3) / 4;
-  f32x4 acc[W];
+// A wave's blocks of 128 columns: codes and scales of NW row blocks of the weight(s).
+template <int NW>
+struct Codes {
+  u32x4 c[NW];
+  uint32_t s[NW];  // a row's scales of the block's four groups
+};
+__device__ __forceinline__ bf16x8 operand(u32x4 c, uint32_t s, int j) {
+  return operand(c[j], __uint_as_float((s >> (8 * j) & 255u) << 23));
+}
+
+// The row blocks' codes and scales, by their first block of 128 columns.
+template <int NW>
+struct Source {
+  const uint8_t* c[NW];
+  const uint8_t* s[NW];
+  __device__ __forceinline__ void load(Codes<NW>& f, int kb, int lane) const {
 #pragma unroll
-  for (int w = 0; w < W; ++w) acc[w] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const bf16_t* x = a.x + (int64_t)min(m0 + fr, a.M - 1) * a.ldx + fq * 32;
-  for (int kb = wave; kb < a.KB; kb += KS) {
-    u32x4 c[W];
-    float scale[W];
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      c[w] = *(const u32x4*)(a.codes[w] + (((int64_t)nb * a.KB + kb) * 64 + lane) * 16);
-      const uint32_t s =
-          a.scales[w][(((int64_t)nb * K4 + (kb >> 2)) * 64 + lane) * 4 + (kb & 3)];
-      scale[w] = __uint_as_float(s << 23);
+    for (int n = 0; n < NW; ++n) {
+      f.c[n] = *(const u32x4*)(c[n] + (int64_t)kb * 1024 + lane * 16);
+      f.s[n] = *(const uint32_t*)(s[n] + (int64_t)kb * 64 + (lane & 15) * 4);
     }
+  }
+};
+// blocks first .. first + NW / W - 1 of each of W weights (past the last: the last)
+template <int NW, int W>
+__device__ __forceinline__ Source<NW> source(const Args& a, int first) {
+  Source<NW> f;
+  const int NB = (a.N + 15) / 16;
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+  for (int n = 0; n < NW; ++n) {
+    const int w = n / (NW / W), nb = min(first + n % (NW / W), NB - 1);
+    f.c[n] = a.codes[w] + (int64_t)nb * a.KB * 1024;
+    f.s[n] = a.scales[w] + (int64_t)nb * a.KB * 64;
+  }
+  return f;
+}
+
+// 8 neighbours of a row as they are in memory, and as MFMA operands.
+template <typename T, bool RAW>
+struct Chunk {
+  // pieces: one operand each
+  u32x4 v[kPieces<T>];
+  __device__ __forceinline__ void load(const Args& a, int64_t at) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bf16x8 xf = as_bf16x8(*(const u32x4*)(x + p * a.xp + kb * 128 + j * 8));
+    for (int p = 0; p < kPieces<T>; ++p)
+      v[p] = *(const u32x4*)((const bf16_t*)a.x + p * a.xp + at);
+  }
+  __device__ __forceinline__ void pieces(bf16x8 (&p)[kPieces<T>]) const {
 #pragma unroll
-        for (int w = 0; w < W; ++w) acc[w] = mfma16x16x32(operand(c[w][j], scale[w]), xf, acc[w]);
+    for (int i = 0; i < kPieces<T>; ++i) p[i] = as_bf16x8(v[i]);
+  }
+};
+template <typename T>
+struct Chunk<T, true> {
+  static constexpr int P = kPieces<T>, V = sizeof(T) / 2;
+  u32x4 v[V];
+  __device__ __forceinline__ void load(const Args& a, int64_t at) {
+    // (rows may begin anywhere: the loads need no alignment)
+    __builtin_memcpy(v, (const T*)a.x + at, sizeof(v));
+  }
+  // the first `left` elements, zeros behind them
+  __device__ __forceinline__ void load_part(const Args& a, int64_t at, int left) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = i < left ? ((const T*)a.x)[at + i] : T(0);
+    __builtin_memcpy(v, t, sizeof(v));
+  }
+  // split() of all 8: the leading halves by byte permutes, the rest by packed conversions.
+  // (What is left of an infinity or NaN, a NaN, becomes any finite number: it is added to
+  // the infinity or NaN in the first piece.)
+  __device__ __forceinline__ void pieces(bf16x8 (&p)[P]) const {
+    if constexpr (P == 1) {
+      p[0] = as_bf16x8(v[0]);
+    } else {
+      float f[8];
+      T t[8];
+      __builtin_memcpy(t, v, sizeof(v));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        f[i] = P == 2 ? (float)t[i] : __builtin_canonicalizef((float)t[i]);
+      u32x4 w[P];
+#pragma unroll
+      for (int q = 0; q < P - 1; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t lo = __float_as_uint(f[2 * i]), hi = __float_as_uint(f[2 * i + 1]);
+          w[q][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+          f[2 * i] = rest(f[2 * i], lo);
+          f[2 * i + 1] = rest(f[2 * i + 1], hi);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[P - 1][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+#pragma unroll
+      for (int q = 0; q < P; ++q) p[q] = as_bf16x8(w[q]);
+    }
+  }
+  static __device__ __forceinline__ float rest(float f, uint32_t bits) {
+    return fmaxf(f - __uint_as_float(bits & 0xffff0000u), -0x1p126f);
+  }
+};
+
+// Few rows: a workgroup has 16 MT rows of x and 16 NT columns of y, K split over its KS
+// waves, whose sums meet in LDS.  Operands go from memory to registers, D blocks of 128
+// columns ahead.  RAW: x is the rows themselves, whatever their type, alignment and length; else
+// their pieces, padded to whole blocks.
+template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D>
+__global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
+  constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NW = W * NT;
+  __shared__ f32x4 part[KS][NW * MT][64];
+  const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nt = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+  f32x4 acc[NW][MT];
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const Source<NW> src = source<NW, W>(a, nt);
+  int64_t row[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    row[i] = (int64_t)min(m0 + i * 16 + fr, a.M - 1) * a.ldx + fq * 8;
+  struct Block {
+    Codes<NW> w;
+    Chunk<T, RAW> x[MT][4];
+  };
+  auto load = [&](Block& b, int kb) {
+    src.load(b.w, kb, lane);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b.x[i][j].load(a, row[i] + kb * 128 + j * 32);
+  };
+  auto mul = [&](const Block& b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 xf[MT][P];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) b.x[i][j].pieces(xf[i]);
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        const bf16x8 wf = operand(b.w.c[n], b.w.s[n], j);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[n][i] = mfma16x16x32(wf, xf[i][p], acc[n][i]);
       }
-  }
+    }
+  };
+  // this wave's whole blocks: wave, wave + KS, ..  (No load below hangs on a condition: the
+  // compiler's waits would then allow for its absence, and nothing stay in flight.)
+  const int whole = RAW ? a.K / 128 : a.KB;
+  const int n = wave < whole ? (whole - wave + KS - 1) / KS : 0;
+  if (n > 0) {
+    Block b[D];
+    auto fill = [&](Block& f, int i) { load(f, wave + KS * min(i, n - 1)); };
 #pragma unroll
-  for (int w = 0; w < W; ++w) part[wave][w][lane] = acc[w];
-  __syncthreads();
-  if (wave == 0) {
+    for (int d = 0; d < D; ++d) fill(b[d], d);
+    int i = 0;
+    for (; i + D < n; i += D)
 #pragma unroll
-    for (int w = 0; w < W; ++w)
-      for (int i = 1; i < KS; ++i) acc[w] += part[i][w][lane];
-    finish<T, GATED>(a, m0 + fr, nt * 16 + fq * 4, acc);
+      for (int d = 0; d < D; ++d) {
+        mul(b[d]);
+        fill(b[d], i + D + d);
+      }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (i + d < n) mul(b[d]);
   }
+  if constexpr (RAW) {
+    if (whole < a.KB && whole % KS == wave) {  // the last columns, which are no whole block
+      Block f;
+      src.load(f.w, whole, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = whole * 128 + j * 32;
+          f.x[i][j].load_part(a, row[i] + k, a.K - k - fq * 8);
+        }
+      mul(f);
+    }
+  }
+  if constexpr (KS > 1) {
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) part[wave][n * MT + i][lane] = acc[n][i];
+    __syncthreads();
+    // tile (t, i) of y by wave (t * MT + i) % KS
+#pragma unroll
+    for (int t = 0; t < NT * MT; ++t) {
+      if (t % KS != wave) continue;
+      f32x4 s[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        s[w] = part[0][w * NT * MT + t][lane];
+#pragma unroll
+        for (int k = 1; k < KS; ++k) s[w] += part[k][w * NT * MT + t][lane];
+      }
+      finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < NT * MT; ++t) {
+      f32x4 s[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) s[w] = acc[w * NT + t / MT][t % MT];
+      finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
+    }
+  }
+}
+
+typedef __attribute__((address_space(3))) void lds_void_t;
+
+// Many rows: a workgroup has 16 MT rows of x, which 4 waves share through LDS in slices of
+// BK columns, and each of the waves NW row blocks of the weight (gated: half of them the
+// gate's), whose codes it reads by itself, D - 1 blocks of 128 ahead.  A ring of SLOTS slices
+// is filled by direct loads.
+template <typename T, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+__global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int ntiles) {
+  constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NT = NW / W;
+  constexpr int BM = 16 * MT, GROUP = 8;
+  constexpr int CPR = BK / 8, RPI = 64 / CPR;  // chunks of 8 in a slice row, rows a load
+  constexpr int LPW = BM / RPI / 4;            // loads per wave and slice
+  constexpr int HALVES = 128 / BK, STEPS = BK / 32;
+  // PIPE: a slice goes to registers while the one before multiplies
+  constexpr bool PIPE = MT <= 4;
+  constexpr int AHEAD = PIPE ? SLOTS : SLOTS - 1;  // slices loaded ahead
+  // loads that a wave issues after a slice's own before it waits for that slice: those of
+  // SLOTS - 2 later ones, and the codes' and scales' of the blocks that begin meanwhile
+  constexpr int LATER = LPW * (SLOTS - 2) + 2 * NW * ((SLOTS - 2) / (HALVES * P));
+  static_assert(D * HALVES * P % 2 == 0, "slices alternate between two sets of registers");
+  static_assert(LPW * RPI * 4 == BM && LATER < 64, "loads");
+  __shared__ __attribute__((aligned(1024))) bf16_t ring[SLOTS][BM * BK];
+  const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lid = xcd_logical_id(blockIdx.x, gridDim.x);
+  // runs of 8 row tiles a column tile, so that an XCD's L2 holds what its run shares
+  const int g0 = lid / (GROUP * ntiles) * GROUP, in_group = lid - g0 * ntiles;
+  const int gm = min(GROUP, mtiles - g0);
+  const int m0 = (g0 + in_group % gm) * BM, nt = (in_group / gm * 4 + wave) * NT;
+
+  // Chunk c (of 8 columns) of slice row r is at chunk c ^ swizzle(r), so that the 16 rows
+  // of a fragment read hit 16 distinct bank groups.
+  auto swizzle = [](int r) { return BK == 64 ? (r >> 1) & 7 : r & 15; };
+  const bf16_t* src[LPW];
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int r = (wave + 4 * i) * RPI + lane / CPR;
+    src[i] = (const bf16_t*)a.x + (int64_t)min(m0 + r, a.M - 1) * a.ldx +
+             ((lane % CPR) ^ swizzle(r)) * 8;
+  }
+  const int slices = a.KB * HALVES * P;
+  int64_t next_at = 0;  // of the next slice to load: columns + piece
+  int next = 0, next_p = 0;
+  auto issue = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < LPW; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (__attribute__((address_space(1))) void*)(src[i] + next_at),
+          (lds_void_t*)(ring[slot] + (wave + 4 * i) * RPI * BK), 16, 0, 0);
+    // past the last slice, that one again (never read)
+    if (next + 1 < slices) {
+      ++next;
+      if (++next_p == P) next_p = 0, next_at += BK - (P - 1) * a.xp;
+      else next_at += a.xp;
+    }
+  };
+  const Source<NW> w = source<NW, W>(a, nt);
+  f32x4 acc[NW][MT];
+#pragma unroll
+  for (int n = 0; n < NW; ++n)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Codes<NW> codes[D];
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) w.load(codes[d], min(d, a.KB - 1), lane);
+#pragma unroll
+  for (int t = 0; t < AHEAD; ++t) issue(t);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  bf16x8 frags[PIPE ? 2 : 1][STEPS][MT];
+  auto read = [&](bf16x8 (&f)[STEPS][MT], int at) {
+    const bf16_t* x = ring[at] + fr * BK;
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)  // (rows differ by multiples of 16)
+        f[j][i] = as_bf16x8(*(const u32x4*)(x + i * 16 * BK + ((j * 4 + fq) ^ swizzle(fr)) * 8));
+  };
+  int slot = 0;
+  if constexpr (PIPE) {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(frags[0], 0);
+  }
+  for (int kb0 = 0; kb0 < a.KB; kb0 += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int kb = kb0 + d;
+      if (kb >= a.KB) break;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          constexpr int two = PIPE ? 2 : 1;
+          const int set = ((d * HALVES + h) * P + p) % two;
+          // PIPE: the next slice has landed (later ones may be in flight), and every wave
+          // has this one in registers, so its slot takes the slice SLOTS ahead.  Else: this
+          // slice has landed, and every wave has read the one before.
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(LATER) : "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (h == 0 && p == 0)
+            w.load(codes[(d + D - 1) % D], min(kb + D - 1, a.KB - 1), lane);
+          const int after = slot == SLOTS - 1 ? 0 : slot + 1;
+          if constexpr (PIPE) {
+            read(frags[set ^ 1], after);
+            issue(slot);
+          } else {
+            issue(slot == 0 ? SLOTS - 1 : slot - 1);
+            read(frags[0], slot);
+          }
+          slot = after;
+#pragma unroll
+          for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+            for (int n = 0; n < NW; ++n) {
+              const bf16x8 wf = operand(codes[d].c[n], codes[d].s[n], h * STEPS + j);
+#pragma unroll
+              for (int i = 0; i < MT; ++i)
+                acc[n][i] = mfma16x16x32(wf, frags[set][j][i], acc[n][i]);
+            }
+          if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+  // no load may land in LDS that is another workgroup's by then
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      f32x4 s[W];
+#pragma unroll
+      for (int v = 0; v < W; ++v) s[v] = acc[v * NT + t][i];
+      finish<T, GATED>(a, m0 + i * 16 + fr, (nt + t) * 16 + fq * 4, s);
+    }
 }
 
 int64_t pad128(int64_t k) { return kad_cdiv(k, 128) * 128; }
@@ -189,62 +496,146 @@ bool in_place(const void* x, int64_t ldx, int K) {
   return kPieces<T> == 1 && K % 128 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0;
 }
 
-// bytes of the rows' pieces; 0 where the rows can be read as they are
+// Which kernel and tile.  n: rows of the weights in all (gated: the gate's and the up's).
+// Up to one workgroup a CU (256) a call takes what one workgroup's walk over K takes, so the
+// smallest tile that needs no more wins, and beyond two a CU the largest.  Cold weights, us,
+// of tiles of rows x weight rows (those up to 32 x 64 the kernel of few rows):
+//   M x N x K            16x16 16x32 16x64 32x64 32x128 64x128 64x256 128x256
+//   64 x 1024 x 3584       5.9   6.1   6.7   9.7  13.5   19.9
+//   128 x 1024 x 3584      9.6   6.2   6.8  10.3  13.5   19.9
+//   256 x 1024 x 3584     17.3  10.2   6.9  10.4  13.5   19.9
+//   64 x 8192 x 8192      62.9  36.8  24.2  21.4  31.5   45     71     114
+//   128 x 8192 x 8192            68   42    38    32     45     70     116
+//   512 x 8192 x 8192                             76     64     73     118
+//   1024 x 8192 x 8192                           141    122    107     122
+//   4096 x 32768 x 1024                          375    354    277     247
+// The kernel of few rows reads fp16 and fp32 rows as they are, where the other needs a
+// pass that splits them: it keeps tiles of up to two workgroups a CU (256 x 4096 x 4096
+// fp16 25.5 us against 28.7, fp32 38.7 against 40.8).
 template <typename T>
-int64_t piece_bytes(const void* x, int64_t ldx, int M, int K) {
-  return in_place<T>(x, ldx, K) ? 0 : kPieces<T> * (int64_t)M * pad128(K) * 2;
+bool few(int64_t M, int64_t n) {
+  return M <= 16 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= (kPieces<T> == 1 ? 256 : 512);
 }
 
-// a.x, a.ldx, a.xp for the rows, split into `ws` where they cannot be read in place
+// bytes of the rows' pieces; 0 where the rows are read as they are
 template <typename T>
-void rows_of(Args& a, const void* x, int64_t ldx, void* ws, int M, int K, hipStream_t s) {
-  if (in_place<T>(x, ldx, K)) {
-    a.x = (const bf16_t*)x, a.ldx = ldx, a.xp = 0;
-    return;
+int64_t piece_bytes(const void* x, int64_t ldx, int64_t M, int64_t n, int K) {
+  return few<T>(M, n) || in_place<T>(x, ldx, K) ? 0 : kPieces<T> * M * pad128(K) * 2;
+}
+
+template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D>
+void launch_stream(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)kad_cdiv(a.cols, 16 * NT), (unsigned)kad_cdiv(a.M, 16 * MT));
+  hipLaunchKernelGGL((q4_stream_kernel<T, RAW, GATED, MT, NT, KS, D>), grid, dim3(64 * KS), 0, s,
+                     a);
+}
+
+template <typename T, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+void launch_tile(const Args& a, hipStream_t s) {
+  const int64_t mtiles = kad_cdiv(a.M, 16 * MT);
+  const int64_t ntiles = kad_cdiv(a.cols, 64 * NW / (GATED ? 2 : 1));
+  hipLaunchKernelGGL((q4_tile_kernel<T, GATED, MT, NW, BK, SLOTS, D>),
+                     dim3((unsigned)(mtiles * ntiles)), dim3(256), 0, s, a, (int)mtiles,
+                     (int)ntiles);
+}
+
+template <typename T, bool RAW, bool GATED>
+void stream(const Args& a, hipStream_t s) {
+  constexpr int W = GATED ? 2 : 1, P = kPieces<T>;
+  const int64_t rows = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
+  // 8 waves share K where each has 3 blocks or more of it (1 x 2048 x 16384: 9.9 us, 4 waves
+  // 11.7; fp16 1 x 1024 x 3584 5.2 and 6.0); else 4 (1 x 1024 x 1024 2.2 us, 8 waves 3.0)
+  const bool wide = a.KB >= 24;
+  constexpr int D = sizeof(T) == 2 ? 4 : 2;
+  if constexpr (!GATED)
+    if (rows * kad_cdiv(n, 16) <= 256) {
+      if (wide) return launch_stream<T, RAW, GATED, 1, 1, 8, D>(a, s);
+      return launch_stream<T, RAW, GATED, 1, 1, 4, 2>(a, s);
+    }
+  if (rows * kad_cdiv(n, 32) <= 256) {
+    if (wide) return launch_stream<T, RAW, GATED, 1, 2 / W, 8, D>(a, s);
+    return launch_stream<T, RAW, GATED, 1, 2 / W, 4, 2>(a, s);
   }
-  const int KP = (int)pad128(K);
-  a.x = (const bf16_t*)ws, a.ldx = KP, a.xp = (int64_t)M * KP;
-  hipLaunchKernelGGL((split_rows_kernel<T>), dim3((unsigned)kad_cdiv((int64_t)M * (KP / 8), 256)),
-                     dim3(256), 0, s, (const T*)x, ldx, (bf16_t*)ws, M, K, KP);
+  if (a.M <= 16 || rows * kad_cdiv(n, 64) <= (P == 3 ? 512 : 256)) {
+    if (wide) return launch_stream<T, RAW, GATED, 1, 4 / W, 8, 2>(a, s);
+    return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2>(a, s);
+  }
+  return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 3 ? 1 : 2>(a, s);
 }
 
 template <typename T, bool GATED>
-void launch(const Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)kad_cdiv(a.cols, 16), (unsigned)kad_cdiv(a.M, 16));
-  hipLaunchKernelGGL((q4_kernel<T, GATED>), grid, dim3(256), 0, s, a);
+void tiles(const Args& a, hipStream_t s) {
+  constexpr int P = kPieces<T>;
+  const int64_t n = (int64_t)a.cols * (GATED ? 2 : 1);
+  auto count = [&](int rows, int cols) { return kad_cdiv(a.M, rows) * kad_cdiv(n, cols); };
+  if (count(32, 128) <= 512) return launch_tile<T, GATED, 2, 2, 128, 4, 4>(a, s);
+  if (count(64, 128) <= 512) return launch_tile<T, GATED, 4, 2, 128, 4, P == 1 ? 4 : 2>(a, s);
+  // Two of the largest tiles run on a CU at a time, and take twice as long as four of half
+  // the size, or somewhat less: the larger ones where that halves the rounds (192 x
+  // 100000 x 1024, 2 rounds against 3: 61.9 us, smaller 54.0; 256 rows, 2 against 4: 63.5 and 65.9).
+  // fp16 and fp32 rows have no registers for them.
+  if constexpr (kPieces<T> == 1)
+    if (2 * kad_cdiv(count(128, 256), 512) <= kad_cdiv(count(64, 256), 512))
+      return launch_tile<T, GATED, 8, 4, 64, 4, 2>(a, s);
+  return launch_tile<T, GATED, 4, 4, 64, 4, 2>(a, s);
+}
+
+// a product of the rows x as they are, or of their pieces in `ws`
+template <typename T, bool GATED>
+void multiply(Args a, const void* x, int64_t ldx, void* ws, hipStream_t s) {
+  a.x = x, a.ldx = ldx, a.xp = 0;
+  if (few<T>(a.M, (int64_t)a.cols * (GATED ? 2 : 1))) return stream<T, true, GATED>(a, s);
+  if (!in_place<T>(x, ldx, a.K)) {
+    const int KP = (int)pad128(a.K);
+    a.x = ws, a.ldx = KP, a.xp = (int64_t)a.M * KP;
+    hipLaunchKernelGGL((split_rows_kernel<T>),
+                       dim3((unsigned)kad_cdiv((int64_t)a.M * (KP / 8), 256)), dim3(256), 0, s,
+                       (const T*)x, ldx, (bf16_t*)ws, a.M, a.K, KP);
+  }
+  tiles<T, GATED>(a, s);
+}
+
+// the same of rows that are pieces already, padded to whole blocks
+template <typename T>
+void multiply_pieces(Args a, const bf16_t* x, hipStream_t s) {
+  a.x = x, a.ldx = pad128(a.K), a.xp = a.M * a.ldx, a.K = (int)a.ldx;
+  if (few<T>(a.M, a.cols)) return stream<T, kPieces<T> == 1, false>(a, s);
+  tiles<T, false>(a, s);
 }
 
 struct Weight {
   const void *codes, *scales;
 };
 
+// everything of a product but its rows
 template <typename T>
-void linear(Args a, Weight w, const void* r, int64_t ldr, void* y, int64_t ldy, int M, int N,
-            int K, hipStream_t s) {
+Args linear(Weight w, const void* r, int64_t ldr, void* y, int64_t ldy, int M, int N, int K) {
+  Args a{};
   a.codes[0] = a.codes[1] = (const uint8_t*)w.codes;
   a.scales[0] = a.scales[1] = (const uint8_t*)w.scales;
   a.r = r, a.ldr = ldr, a.y = y, a.ldy = ldy, a.yp = 0;
-  a.M = M, a.N = N, a.KB = (int)kad_cdiv(K, 128), a.cols = N;
+  a.M = M, a.N = N, a.K = K, a.KB = (int)kad_cdiv(K, 128), a.cols = N;
   const int bytes = 4 * (int)sizeof(T);
   a.vec = N % 4 == 0 && (uintptr_t)y % bytes == 0 && ldy % 4 == 0 &&
           (!r || ((uintptr_t)r % bytes == 0 && ldr % 4 == 0));
-  launch<T, false>(a, s);
+  return a;
 }
 
-template <typename T>
-void gated(Args a, Weight g, Weight u, bf16_t* h, int M, int F, int K, hipStream_t s) {
+Args gated(Weight g, Weight u, bf16_t* h, int M, int F, int K) {
+  Args a{};
   a.codes[0] = (const uint8_t*)g.codes, a.codes[1] = (const uint8_t*)u.codes;
   a.scales[0] = (const uint8_t*)g.scales, a.scales[1] = (const uint8_t*)u.scales;
   a.r = nullptr, a.ldr = 0, a.y = h, a.ldy = pad128(F), a.yp = M * pad128(F);
-  a.M = M, a.N = F, a.KB = (int)kad_cdiv(K, 128), a.cols = (int)pad128(F), a.vec = 1;
-  launch<T, true>(a, s);
+  a.M = M, a.N = F, a.K = K, a.KB = (int)kad_cdiv(K, 128), a.cols = (int)pad128(F), a.vec = 1;
+  return a;
 }
 
-int check_sizes(int M, int N, int K) {
+int check_sizes(int64_t M, int64_t N, int K) {
   KAD_REQUIRE(M > 0 && N > 0 && K > 0, "empty dimensions");
-  KAD_REQUIRE(K <= kMaxK, "rows of %d columns", K);
-  // (a grid holds fewer than 2^32 work-items a dimension)
-  KAD_REQUIRE(kad_cdiv(M, 16) <= 65535 && N <= kMaxN, "a product of %d x %d outputs", M, N);
+  KAD_REQUIRE(K <= kMaxK && N <= kMaxN, "a weight of %lld rows of %d columns", (long long)N, K);
+  // (a grid holds fewer than 2^32 work-items a dimension, and 65535 rows of tiles)
+  KAD_REQUIRE(M <= 16 * 65535 && kad_cdiv(M, 32) * kad_cdiv(2 * N, 128) < (1ll << 32) / 256,
+              "a product of %lld x %lld outputs", (long long)M, (long long)N);
   return KAD_OK;
 }
 
@@ -276,7 +667,7 @@ extern "C" int kad_quantized_linear_workspace_bytes(const void* x, int64_t ldx, 
   KAD_REQUIRE(bytes, "null pointer argument");
   KAD_TRY(check_sizes(M, N, K));
   return for_dtype(dtype, [&](auto t) {
-    *bytes = piece_bytes<decltype(t)>(x, ldx, M, K);
+    *bytes = piece_bytes<decltype(t)>(x, ldx, M, N, K);
     return KAD_OK;
   });
 }
@@ -295,10 +686,9 @@ extern "C" int kad_quantized_linear(const void* x, int64_t ldx, int dtype, const
               (long long)workspace_bytes, (long long)need);
   return for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    Args a{};
-    rows_of<T>(a, x, ldx, workspace, M, K, (hipStream_t)stream);
-    linear<T>(a, {codes, scales}, residual, ldr, y, ldy, M, N, K, (hipStream_t)stream);
-    return kad_launch_status("q4_kernel");
+    multiply<T, false>(linear<T>({codes, scales}, residual, ldr, y, ldy, M, N, K), x, ldx,
+                       workspace, (hipStream_t)stream);
+    return kad_launch_status("quantized product");
   });
 }
 
@@ -309,7 +699,7 @@ extern "C" int kad_quantized_gated_ffn_workspace_bytes(const void* x, int64_t ld
   KAD_TRY(check_sizes(M, H, F));
   return for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    *bytes = piece_bytes<T>(x, ldx, M, H) + kPieces<T> * (int64_t)M * pad128(F) * 2;
+    *bytes = piece_bytes<T>(x, ldx, M, 2 * pad128(F), H) + kPieces<T> * (int64_t)M * pad128(F) * 2;
     return KAD_OK;
   });
 }
@@ -335,12 +725,9 @@ extern "C" int kad_quantized_gated_ffn(const void* x, int64_t ldx, int dtype,
   return for_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     const hipStream_t s = (hipStream_t)stream;
-    Args a{};
-    rows_of<T>(a, x, ldx, workspace, M, H, s);
-    bf16_t* h = (bf16_t*)((char*)workspace + piece_bytes<T>(x, ldx, M, H));
-    gated<T>(a, g, u, h, M, F, H, s);
-    a.x = h, a.ldx = pad128(F), a.xp = M * pad128(F);
-    linear<T>(a, d, residual, ldr, y, ldy, M, H, F, s);
-    return kad_launch_status("q4_kernel");
+    bf16_t* h = (bf16_t*)((char*)workspace + piece_bytes<T>(x, ldx, M, 2 * pad128(F), H));
+    multiply<T, true>(gated(g, u, h, M, F, H), x, ldx, workspace, s);
+    multiply_pieces<T>(linear<T>(d, residual, ldr, y, ldy, M, H, F), h, s);
+    return kad_launch_status("quantized product");
   });
 }

@@ -6,10 +6,10 @@
 // bf16, and what the products of quantized_gemm.hip multiply by is the value itself.
 //
 // Rows are padded to 16 and columns to 128 with zero codes, and laid out as the
-// MFMA's operand takes them: codes [N/16][K/128][64 lanes][16 bytes], lane l the
-// 32 codes of row l % 16, columns 32 (l / 16) .. +31 (the even column in the low half
-// of a byte), so a wave loads 1 KB in one piece; scales [N/16][K/512][64 lanes][4],
-// byte j that lane's group in the j-th of four blocks of 128.
+// MFMA's operand takes them: codes [N/16][K/128][64 lanes][4 words], word j of lane l
+// the 8 codes of row l % 16, columns 32 j + 8 (l / 16) .. +7 (the first column in the lowest
+// bits), so a wave loads 1 KB in one piece and word j is the lane's part of the j-th
+// product of 32 columns; scales [N/16][K/128][16 rows][4 groups], a word a lane.
 
 #include "quantized_common.h"
 
@@ -80,8 +80,7 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
       for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
     }
   }
-  const int at = (c >> 2) * 16 + r;  // the lane that the product reads this group by
-  uint32_t bytes = 0;
+  const int at = ((c & 3) * 16 + r) * 16 + (c >> 2) * 4;  // of the codes' word in its block
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int kb = k4 * 4 + j;
@@ -91,7 +90,6 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
     amax = max_nan(amax, __shfl_xor(amax, 1, 64));
     amax = max_nan(amax, __shfl_xor(amax, 2, 64));
     const uint32_t s = scale_byte(amax);
-    bytes |= s << (8 * j);
     if (kb < KB) {
       uint32_t code = 0;
       const float scale = __uint_as_float(s << 23);
@@ -101,10 +99,10 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restric
         code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][4], f[j][5], scale, 2);
         code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][6], f[j][7], scale, 3);
       }
-      *(uint32_t*)(codes + ((nb * KB + kb) * 64 + at) * 16 + (c & 3) * 4) = code;
+      *(uint32_t*)(codes + (nb * KB + kb) * 1024 + at) = code;
+      if ((c & 3) == 0) scales[(nb * KB + kb) * 64 + r * 4 + (c >> 2)] = (uint8_t)s;
     }
   }
-  if ((c & 3) == 0) *(uint32_t*)(scales + ((nb * K4 + k4) * 64 + at) * 4) = bytes;
 }
 
 // The same split the other way.
@@ -118,21 +116,19 @@ __global__ __launch_bounds__(256) void dequantize_weight_kernel(
   const int k4 = (int)(blockIdx.x - nb * K4);
   const int64_t row = nb * 16 + r;
   if (row >= N) return;
-  const int at = (c >> 2) * 16 + r;
-  const uint32_t bytes = *(const uint32_t*)(scales + ((nb * K4 + k4) * 64 + at) * 4);
-  uint32_t code[4];
+  const int at = ((c & 3) * 16 + r) * 16 + (c >> 2) * 4;
+  uint32_t code[4], byte[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int kb = k4 * 4 + j;
-    code[j] = kb < KB ? *(const uint32_t*)(codes + ((nb * KB + kb) * 64 + at) * 16 + (c & 3) * 4)
-                      : 0u;
+    const int kb = min(k4 * 4 + j, KB - 1);
+    code[j] = *(const uint32_t*)(codes + (nb * KB + kb) * 1024 + at);
+    byte[j] = scales[(nb * KB + kb) * 64 + r * 4 + (c >> 2)];
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int k = (k4 * 4 + j) * 128 + c * 8;
     if (k >= K) continue;
-    const uint32_t s = (bytes >> (8 * j)) & 255u;
-    const float scale = scale_value(s);
+    const float scale = scale_value(byte[j]);
     float f[8];
     codes_to_float(code[j], f);
     T* dst = out + row * ldo + k;

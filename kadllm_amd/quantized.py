@@ -16,7 +16,6 @@ model's type (src/kadllm/adapters/qwen3_5.py:144-235).
 
 import ctypes
 import functools
-from typing import NamedTuple
 
 import torch
 
@@ -34,19 +33,43 @@ _SCALES = torch.float8_e8m0fnu
 def _padded(rows, cols):
     """The shapes of a weight's codes and scales."""
     nb, kb = -(-rows // 16), -(-cols // 128)
-    return (nb, kb, 64, 16), (nb, -(-kb // 4), 64, 4)
+    return (nb, kb, 64, 16), (nb, kb, 16, 4)
 
 
-class QuantizedWeight(NamedTuple):
+class QuantizedWeight:
     """A weight [rows, cols] in 4 bits, as quantized_linear reads it: codes uint8
-    [rows/16, cols/128, 64, 16] and scales torch.float8_e8m0fnu [rows/16, cols/512,
-    64, 4] (sizes rounded up), of which entry l of a block is row l % 16, columns
-    32 (l // 16) to + 31."""
+    [rows/16, cols/128, 64, 16] (sizes rounded up), of which bytes 4 j to 4 j + 3 of
+    entry l of a block are row l % 16, columns 32 j + 8 (l // 16) to + 7, and scales
+    torch.float8_e8m0fnu [rows/16, cols/128, 16 rows, 4 groups].  Checked when it is made,
+    and not changed afterwards."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    cols: int
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes, scales, rows, cols):
+        if codes.dtype is not torch.uint8 or scales.dtype is not _SCALES:
+            raise TypeError("the codes of a weight are uint8 and its scales float8_e8m0fnu")
+        _check_size(rows, cols)
+        if (codes.shape, scales.shape) != _padded(rows, cols):
+            raise ValueError("codes and scales do not fit the weight's size")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("the tensors of a 4-bit weight must be contiguous")
+        if codes.device != scales.device:
+            raise ValueError("all tensors must be on the same device")
+        for name, value in zip(self.__slots__, (codes, scales, rows, cols)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("a QuantizedWeight is not changed; make another")
+
+    def __reduce__(self):
+        return type(self), (self.codes, self.scales, self.rows, self.cols)
+
+    def __repr__(self):
+        return f"QuantizedWeight({self.rows} x {self.cols}, {self.codes.device})"
+
+    def to(self, device):
+        """This weight on another device."""
+        return QuantizedWeight(self.codes.to(device), self.scales.to(device), self.rows, self.cols)
 
     @classmethod
     def pack(cls, codes, scales, *, cols=None):
@@ -73,22 +96,21 @@ class QuantizedWeight(NamedTuple):
             raise ValueError("scales must be from 2**-100 to 2**125, or NaN")
         if K % 2:
             codes = torch.cat((codes[:, :-1], codes[:, -1:] & 15), 1)
-        (nb, kb, _, _), (_, k4, _, _) = _padded(N, K)
+        nb, kb = _padded(N, K)[0][:2]
         pad = torch.nn.functional.pad
         codes = pad(codes, (0, kb * 64 - half, 0, nb * 16 - N))
-        codes = codes.view(nb, 16, kb, 4, 16).permute(0, 2, 3, 1, 4)
-        scales = pad(scales, (0, k4 * 16 - scales.shape[1], 0, nb * 16 - N), value=27)
-        scales = scales.view(nb, 16, k4, 4, 4).permute(0, 2, 4, 1, 3)
-        return cls(codes.reshape(nb, kb, 64, 16), scales.reshape(nb, k4, 64, 4).view(_SCALES), N, K)
+        codes = codes.view(nb, 16, kb, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
+        scales = pad(scales, (0, kb * 4 - scales.shape[1], 0, nb * 16 - N), value=27)
+        scales = scales.view(nb, 16, kb, 4).transpose(1, 2)
+        return cls(codes.reshape(nb, kb, 64, 16), scales.contiguous().view(_SCALES), N, K)
 
     def unpack(self):
         """(codes [N, ceil(K / 2)] uint8, scales [N, ceil(K / 32)] float8_e8m0fnu):
         the row-major parts that ``pack`` takes."""
-        _check_weight(self)
-        nb, kb, k4 = self.codes.shape[0], self.codes.shape[1], self.scales.shape[1]
-        codes = self.codes.view(nb, kb, 4, 16, 16).permute(0, 3, 1, 2, 4).reshape(nb * 16, -1)
-        scales = self.scales.view(torch.uint8).view(nb, k4, 4, 16, 4).permute(0, 3, 1, 4, 2)
-        scales = scales.reshape(nb * 16, -1)[:self.rows, :-(-self.cols // GROUP)]
+        nb, kb = self.codes.shape[:2]
+        codes = self.codes.view(nb, kb, 4, 16, 4, 4).permute(0, 3, 1, 4, 2, 5).reshape(nb * 16, -1)
+        scales = self.scales.view(torch.uint8).transpose(1, 2).reshape(nb * 16, -1)
+        scales = scales[:self.rows, :-(-self.cols // GROUP)]
         return (codes[:self.rows, :-(-self.cols // 2)].contiguous(),
                 scales.contiguous().view(_SCALES))
 
@@ -100,29 +122,19 @@ def _check_size(rows, cols):
 
 
 def _check_weight(w, name="weight"):
-    if not isinstance(w, QuantizedWeight):
+    if type(w) is not QuantizedWeight:
         raise TypeError(f"{name} must be a QuantizedWeight")
-    if w.codes.dtype is not torch.uint8 or w.scales.dtype is not _SCALES:
-        raise TypeError("the codes of a weight are uint8 and its scales float8_e8m0fnu")
-    _check_size(w.rows, w.cols)
-    if (w.codes.shape, w.scales.shape) != _padded(w.rows, w.cols):
-        raise ValueError("codes and scales do not fit the weight's size")
-    if not (w.codes.is_contiguous() and w.scales.is_contiguous()):
-        raise ValueError("the tensors of a 4-bit weight must be contiguous")
-
-
-def _no_gradients(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
 
 
 def _rows(t):
     """t [M, C] with a contiguous last dimension and rows that do not overlap, and
     the stride of its rows."""
     M, C = t.shape
-    if t.stride(1) != 1 and C > 1 or t.stride(0) < C and M > 1:
+    ld, one = t.stride()
+    if one != 1 and C > 1 or ld < C and M > 1:
         t = t.contiguous()
-    return t, max(t.stride(0), C)
+        ld = C
+    return t, ld if ld > C else C
 
 
 def quantize_weight(weight):
@@ -139,7 +151,8 @@ def quantize_weight(weight):
         raise TypeError("weights must be bf16, fp16 or fp32")
     N, K = weight.shape
     _check_size(N, K)
-    _no_gradients(weight)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
     device = _device_of(weight)
     weight, ld = _rows(weight)
     shapes = _padded(N, K)
@@ -170,27 +183,29 @@ def _workspace_bytes(name, offset, *sizes):
     return need.value
 
 
-def _workspace(name, x, *sizes):
-    """(buffer or None, its bytes) for a call on x."""
-    need = _workspace_bytes(name + "_workspace_bytes", x.data_ptr() & 15, *sizes)
-    return (torch.empty(need, dtype=torch.uint8, device=x.device) if need else None), need
-
-
-def _check_rows(x, cols, out_cols, residual):
-    """x [..., cols] and residual [..., out_cols] (or None) as 2-D rows."""
-    if x.ndim < 1 or x.shape[-1] != cols or 0 in x.shape:
+def _check_rows(x, cols, out_cols, residual, weights):
+    """x [..., cols] and residual [..., out_cols] (or None) as 2-D rows, fit to be
+    multiplied by ``weights``."""
+    shape = x.shape
+    if not shape or shape[-1] != cols or 0 in shape:
         raise ValueError(f"x must be [..., {cols}], the weight's columns, and not empty")
-    if x.dtype not in _TYPES:
+    if x.numel() > MAX_ROWS * cols:
+        raise ValueError(f"x has at most {MAX_ROWS} rows")
+    dtype = x.dtype
+    if dtype not in _TYPES:
         raise TypeError("x must be bf16, fp16 or fp32")
     if residual is not None:
-        if residual.shape != (*x.shape[:-1], out_cols):
+        if residual.shape != (*shape[:-1], out_cols):
             raise ValueError(f"residual must be x's rows of {out_cols}")
-        if residual.dtype is not x.dtype:
+        if residual.dtype is not dtype:
             raise ValueError("x and residual must have the same dtype")
-        residual = residual.reshape(-1, out_cols)
-    x = x.reshape(-1, cols)
-    if x.shape[0] > MAX_ROWS:
-        raise ValueError(f"x has at most {MAX_ROWS} rows")
+    if torch.is_grad_enabled() and (x.requires_grad or
+                                    residual is not None and residual.requires_grad):
+        raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
+    _device_of(x, residual, *[w.codes for w in weights])
+    if len(shape) != 2:
+        x = x.reshape(-1, cols)
+        residual = residual if residual is None else residual.reshape(-1, out_cols)
     return x, residual
 
 
@@ -201,11 +216,9 @@ def quantized_linear(x, weight, *, residual=None):
     Returns [..., N] in x's type.  Products are exact, sums are fp32 and are rounded
     once, with the residual added."""
     _check_weight(weight)
-    rows, r = _check_rows(x, weight.cols, weight.rows, residual)
-    _no_gradients(x, residual)
-    _device_of(x, residual, weight.codes, weight.scales)
-    out = torch.empty(rows.shape[0], weight.rows, dtype=x.dtype, device=x.device)
-    return _linear(rows, weight, out, r).view(*x.shape[:-1], weight.rows)
+    rows, r = _check_rows(x, weight.cols, weight.rows, residual, (weight,))
+    out = _linear(rows, weight, rows.new_empty((rows.shape[0], weight.rows)), r)
+    return out if rows is x else out.view(*x.shape[:-1], weight.rows)
 
 
 def _linear(x, weight, out, residual=None):
@@ -214,11 +227,12 @@ def _linear(x, weight, out, residual=None):
     x, ldx = _rows(x)
     M, N, K = x.shape[0], weight.rows, weight.cols
     r, ldr = (None, 0) if residual is None else _rows(residual)
-    code = _lib.DTYPE_CODES[x.dtype]
-    ws, need = _workspace("kad_quantized_linear", x, ldx, code, M, N, K)
-    _launch(x.get_device(), "kad_quantized_linear", x.data_ptr(), ldx, code,
-            weight.codes.data_ptr(), weight.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(),
-            max(out.stride(0), N), _lib.ptr(ws), need, M, N, K)
+    code, at = _lib.DTYPE_CODES[x.dtype], x.data_ptr()
+    need = _workspace_bytes("kad_quantized_linear_workspace_bytes", at & 15, ldx, code, M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _launch(x.get_device(), "kad_quantized_linear", at, ldx, code, weight.codes.data_ptr(),
+            weight.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(), max(out.stride(0), N),
+            _lib.ptr(ws), need, M, N, K)
     return out
 
 
@@ -233,13 +247,11 @@ def quantized_gated_ffn(x, gate, up, down, *, residual=None):
     for name, w in (("gate", gate), ("up", up), ("down", down)):
         _check_weight(w, name)
     F, H = gate.rows, gate.cols
-    if (up.rows, up.cols) != (F, H) or (down.rows, down.cols) != (H, F):
+    if up.rows != F or up.cols != H or down.rows != H or down.cols != F:
         raise ValueError("gate and up must be [F, H] and down [H, F]")
-    rows, r = _check_rows(x, H, H, residual)
-    _no_gradients(x, residual)
-    _device_of(x, residual, *(t for w in (gate, up, down) for t in (w.codes, w.scales)))
-    out = torch.empty(rows.shape[0], H, dtype=x.dtype, device=x.device)
-    return _gated_ffn(rows, gate, up, down, out, r).view(x.shape)
+    rows, r = _check_rows(x, H, H, residual, (gate, up, down))
+    out = _gated_ffn(rows, gate, up, down, rows.new_empty(rows.shape), r)
+    return out if rows is x else out.view(x.shape)
 
 
 def _gated_ffn(x, gate, up, down, out, residual=None):
@@ -248,10 +260,11 @@ def _gated_ffn(x, gate, up, down, out, residual=None):
     x, ldx = _rows(x)
     M, F, H = x.shape[0], gate.rows, gate.cols
     r, ldr = (None, 0) if residual is None else _rows(residual)
-    code = _lib.DTYPE_CODES[x.dtype]
-    ws, need = _workspace("kad_quantized_gated_ffn", x, ldx, code, M, H, F)
-    _launch(x.get_device(), "kad_quantized_gated_ffn", x.data_ptr(), ldx, code,
-            gate.codes.data_ptr(), gate.scales.data_ptr(), up.codes.data_ptr(),
-            up.scales.data_ptr(), down.codes.data_ptr(), down.scales.data_ptr(), _lib.ptr(r), ldr,
-            out.data_ptr(), max(out.stride(0), H), _lib.ptr(ws), need, M, H, F)
+    code, at = _lib.DTYPE_CODES[x.dtype], x.data_ptr()
+    need = _workspace_bytes("kad_quantized_gated_ffn_workspace_bytes", at & 15, ldx, code, M, H, F)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _launch(x.get_device(), "kad_quantized_gated_ffn", at, ldx, code, gate.codes.data_ptr(),
+            gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
+            down.codes.data_ptr(), down.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(),
+            max(out.stride(0), H), ws.data_ptr(), need, M, H, F)
     return out

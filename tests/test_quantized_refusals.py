@@ -49,17 +49,16 @@ def test_pack_and_unpack(N, K):
     w = QuantizedWeight.pack(codes, scales.view(torch.float8_e8m0fnu), cols=K)
     assert (w.rows, w.cols) == (N, K)
     assert w.codes.shape == (-(-N // 16), -(-K // 128), 64, 16)
-    assert w.scales.shape == (-(-N // 16), -(-K // 512), 64, 4)
+    assert w.scales.shape == (-(-N // 16), -(-K // 128), 16, 4)
     back = w.unpack()
     assert torch.equal(back[0], codes)
     assert torch.equal(back[1].view(U8), scales)
-    # entry l of a block: row l % 16, columns 32 (l // 16) to + 31
+    # word j of entry l of a block: row l % 16, columns 32 j + 8 (l // 16) to + 7
     for n, k in {(0, 0), (N - 1, K - 1), (N // 2, K // 2), (N // 3, K - 1)}:
-        lane = n % 16 + 16 * (k % 128 // 32)
-        byte = int(w.codes[n // 16, k // 128, lane, k % 32 // 2])
+        lane, j = n % 16 + 16 * (k % 32 // 8), k % 128 // 32
+        byte = int(w.codes[n // 16, k // 128, lane, 4 * j + k % 8 // 2])
         assert byte >> 4 * (k % 2) & 15 == int(codes[n, k // 2]) >> 4 * (k % 2) & 15
-        assert int(w.scales.view(U8)[n // 16, k // 512, lane, k % 512 // 128]) == \
-            int(scales[n, k // 32])
+        assert int(w.scales.view(U8)[n // 16, k // 128, n % 16, j]) == int(scales[n, k // 32])
     # nothing but zeros past the weight's rows and columns
     assert int((w.codes != 0).sum()) <= int((codes != 0).sum())
 
@@ -109,32 +108,48 @@ def test_quantize_refusals(w, error):
         quantize_weight(w)
 
 
-BAD_WEIGHTS = [
-    (lambda w: tuple(w), TypeError),
-    (lambda w: w._replace(codes=w.codes.float()), TypeError),
-    (lambda w: w._replace(scales=w.scales.view(U8)), TypeError),
-    (lambda w: w._replace(rows=17), ValueError),
-    (lambda w: w._replace(rows=0), ValueError),
-    (lambda w: w._replace(cols=129), ValueError),
-    (lambda w: w._replace(cols=True), ValueError),
-    (lambda w: w._replace(codes=w.codes[:, :0]), ValueError),
-    (lambda w: w._replace(codes=torch.zeros(1, 1, 16, 64, dtype=U8).transpose(2, 3)), ValueError),
-    (lambda w: w, RuntimeError),  # well-formed, but not on a ROCm device
-]
-
-
-@pytest.mark.parametrize("bad, error", BAD_WEIGHTS)
-def test_weight_refusals(bad, error):
-    w = bad(_weight())
-    x = torch.zeros(3, 40, dtype=BF)
+@pytest.mark.parametrize("change, error", [
+    (dict(codes=torch.zeros(1, 1, 64, 16)), TypeError),
+    (dict(scales=torch.zeros(1, 1, 16, 4, dtype=U8)), TypeError),
+    (dict(rows=17), ValueError),
+    (dict(rows=0), ValueError),
+    (dict(cols=129), ValueError),
+    (dict(cols=True), ValueError),
+    (dict(codes=torch.zeros(1, 0, 64, 16, dtype=U8)), ValueError),
+    (dict(codes=torch.zeros(1, 1, 16, 64, dtype=U8).transpose(2, 3)), ValueError),
+])
+def test_weight_refusals(change, error):
+    w = _weight()
+    parts = dict(codes=w.codes, scales=w.scales, rows=w.rows, cols=w.cols)
+    QuantizedWeight(**parts)
     with pytest.raises(error):
+        QuantizedWeight(**{**parts, **change})
+
+
+def test_a_weight_is_not_changed():
+    w = _weight()
+    for name in ("codes", "rows", "other"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, 3)
+    assert "5 x 40" in repr(w)
+    import copy
+    other = copy.deepcopy(w)
+    assert torch.equal(other.codes, w.codes) and other.codes.data_ptr() != w.codes.data_ptr()
+    assert w.to("cpu").cols == 40
+
+
+def test_operators_take_only_weights():
+    w, x = _weight(), torch.zeros(3, 40, dtype=BF)
+    for bad in ((w.codes, w.scales, 5, 40), w.codes, None):
+        with pytest.raises(TypeError):
+            dequantize_weight(bad)
+        with pytest.raises(TypeError):
+            quantized_linear(x, bad)
+        for args in ((bad, w, w), (w, bad, w), (w, w, bad)):
+            with pytest.raises(TypeError):
+                quantized_gated_ffn(x, *args)
+    with pytest.raises(RuntimeError):  # well-formed, but not on a ROCm device
         dequantize_weight(w)
-    with pytest.raises(error):
-        quantized_linear(x, w)
-    gate, down = _weight(), _weight(40, 5)
-    for args in ((w, gate, down), (gate, w, down)):
-        with pytest.raises(error):
-            quantized_gated_ffn(x, *args)
 
 
 def test_dequantize_refuses_types():
@@ -202,7 +217,7 @@ def test_c_product_refusals():
                 bytes=1 << 30, M=3, N=32, K=64)
     for change in (dict(x=None), dict(codes=None), dict(scales=None), dict(y=None), dict(ldx=63),
                    dict(ldy=31), dict(r=P, ldr=31), dict(ws=None), dict(ws=P + 8), dict(bytes=10),
-                   dict(M=0), dict(N=0), dict(K=0), dict(N=2**26 + 1, ldy=2**27), dict(dtype=7),
+                   dict(M=0), dict(M=16 * 65535 + 1), dict(N=0), dict(K=0), dict(N=2**26 + 1, ldy=2**27), dict(dtype=7),
                    dict(codes=P + 4), dict(K=2**20 + 1, ldx=2**21)):
         a = {**good, **change}
         assert _rc("kad_quantized_linear", a["x"], a["ldx"], a["dtype"], a["codes"], a["scales"],
