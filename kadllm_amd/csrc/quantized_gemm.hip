@@ -11,6 +11,8 @@
 // bf16 piece for bf16 x (2^-8, as the model's own activation), else to as many
 // pieces as x has: 2^-15 for fp16, whose range h may leave, and 2^-22 for fp32.
 
+#include <type_traits>
+
 #include "quantized_common.h"
 
 namespace {
@@ -176,108 +178,124 @@ __device__ __forceinline__ Source<NW> source(const Args& a, int first) {
   return f;
 }
 
-// 8 neighbours of a row as they are in memory, and as MFMA operands.
-template <typename T, bool RAW>
-struct Chunk {
-  // pieces: one operand each
-  u32x4 v[kPieces<T>];
-  __device__ __forceinline__ void load(const Args& a, int64_t at) {
-#pragma unroll
-    for (int p = 0; p < kPieces<T>; ++p)
-      v[p] = *(const u32x4*)((const bf16_t*)a.x + p * a.xp + at);
-  }
-  __device__ __forceinline__ void pieces(bf16x8 (&p)[kPieces<T>]) const {
-#pragma unroll
-    for (int i = 0; i < kPieces<T>; ++i) p[i] = as_bf16x8(v[i]);
-  }
-};
+// 8 neighbours of a row of fp16 or fp32 (2 V words) as MFMA operands: split() of all, the
+// leading halves by byte permutes, the rest by packed conversions.  (What is left of an
+// infinity or NaN, a NaN, becomes any finite number: it is added to the infinity or NaN in
+// the first piece.)
+__device__ __forceinline__ float rest(float f, uint32_t bits) {
+  return fmaxf(f - __uint_as_float(bits & 0xffff0000u), -0x1p126f);
+}
 template <typename T>
-struct Chunk<T, true> {
-  static constexpr int P = kPieces<T>, V = sizeof(T) / 2;
-  u32x4 v[V];
-  __device__ __forceinline__ void load(const Args& a, int64_t at) {
-    // (rows may begin anywhere: the loads need no alignment)
-    __builtin_memcpy(v, (const T*)a.x + at, sizeof(v));
-  }
-  // the first `left` elements, zeros behind them
-  __device__ __forceinline__ void load_part(const Args& a, int64_t at, int left) {
+__device__ __forceinline__ void pieces_of(const u32x4 (&v)[sizeof(T) / 2],
+                                          bf16x8 (&p)[kPieces<T>]) {
+  constexpr int P = kPieces<T>;
+  if constexpr (P == 1) {
+    p[0] = as_bf16x8(v[0]);
+  } else {
+    float f[8];
     T t[8];
+    __builtin_memcpy(t, v, sizeof(v));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = i < left ? ((const T*)a.x)[at + i] : T(0);
-    __builtin_memcpy(v, t, sizeof(v));
+    for (int i = 0; i < 8; ++i) f[i] = P == 2 ? (float)t[i] : __builtin_canonicalizef((float)t[i]);
+    u32x4 w[P];
+#pragma unroll
+    for (int q = 0; q < P - 1; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = __float_as_uint(f[2 * i]), hi = __float_as_uint(f[2 * i + 1]);
+        w[q][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+        f[2 * i] = rest(f[2 * i], lo);
+        f[2 * i + 1] = rest(f[2 * i + 1], hi);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[P - 1][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+#pragma unroll
+    for (int q = 0; q < P; ++q) p[q] = as_bf16x8(w[q]);
   }
-  // split() of all 8: the leading halves by byte permutes, the rest by packed conversions.
-  // (What is left of an infinity or NaN, a NaN, becomes any finite number: it is added to
-  // the infinity or NaN in the first piece.)
-  __device__ __forceinline__ void pieces(bf16x8 (&p)[P]) const {
-    if constexpr (P == 1) {
-      p[0] = as_bf16x8(v[0]);
-    } else {
-      float f[8];
-      T t[8];
-      __builtin_memcpy(t, v, sizeof(v));
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        f[i] = P == 2 ? (float)t[i] : __builtin_canonicalizef((float)t[i]);
-      u32x4 w[P];
-#pragma unroll
-      for (int q = 0; q < P - 1; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t lo = __float_as_uint(f[2 * i]), hi = __float_as_uint(f[2 * i + 1]);
-          w[q][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
-          f[2 * i] = rest(f[2 * i], lo);
-          f[2 * i + 1] = rest(f[2 * i + 1], hi);
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[P - 1][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-#pragma unroll
-      for (int q = 0; q < P; ++q) p[q] = as_bf16x8(w[q]);
-    }
-  }
-  static __device__ __forceinline__ float rest(float f, uint32_t bits) {
-    return fmaxf(f - __uint_as_float(bits & 0xffff0000u), -0x1p126f);
-  }
-};
+}
 
 // Few rows: a workgroup has 16 MT rows of x and 16 NT columns of y, K split over its KS
-// waves, whose sums meet in LDS.  Operands go from memory to registers, D blocks of 128
-// columns ahead.  RAW: x is the rows themselves, whatever their type, alignment and length; else
-// their pieces, padded to whole blocks.
-template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D>
+// waves, whose sums meet in LDS.  Codes and rows are loaded D blocks of 128 columns ahead,
+// into registers.  A lane of the product holds 16 bytes of a row of its own, which the cache
+// would serve one by one; so rows are loaded in runs of 256 bytes and more, and take their
+// places through LDS, of which each wave has a part that no other touches.  RAW: x is the
+// rows themselves, whatever their type, alignment and length; else their pieces, padded to
+// whole blocks.  R: rows of a tile that are loaded, 16, or 4 where x has no more (the
+// product's other columns repeat them).
+template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R>
 __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NW = W * NT;
-  __shared__ f32x4 part[KS][NW * MT][64];
+  // a block's rows: planes (the pieces) of 16 MT rows of RB bytes, loaded L x 1 KB a tile
+  constexpr int PLANES = RAW ? 1 : P, RB = RAW ? 128 * (int)sizeof(T) : 256;
+  constexpr int CPR = RB / 16, RPI = 64 / CPR, L = R / RPI;
+  static_assert(R == 16 || (R == 4 && MT == 1), "whole tiles, or one of 4 rows");
+  constexpr int kRows = PLANES * MT * R * RB, kSums = NW * MT * 1024;
+  constexpr int kWave = kRows > kSums ? kRows : kSums;
+  __shared__ __attribute__((aligned(1024))) char lds[KS * kWave];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nt = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+  char* own = lds + wave * kWave;
   f32x4 acc[NW][MT];
 #pragma unroll
   for (int n = 0; n < NW; ++n)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const Source<NW> src = source<NW, W>(a, nt);
-  int64_t row[MT];
+  constexpr int kItem = RAW ? sizeof(T) : 2;
+  const int chunk = lane % CPR;
+  const char* row[MT][L];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
-    row[i] = (int64_t)min(m0 + i * 16 + fr, a.M - 1) * a.ldx + fq * 8;
+#pragma unroll
+    for (int t = 0; t < L; ++t)
+      row[i][t] = (const char*)a.x + chunk * 16 +
+                  (int64_t)min(m0 + i * 16 + t * RPI + lane / CPR, a.M - 1) * a.ldx * kItem;
   struct Block {
     Codes<NW> w;
-    Chunk<T, RAW> x[MT][4];
+    u32x4 x[PLANES][MT][L];
   };
   auto load = [&](Block& b, int kb) {
     src.load(b.w, kb, lane);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int p = 0; p < PLANES; ++p)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b.x[i][j].load(a, row[i] + kb * 128 + j * 32);
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < L; ++t)  // (rows may begin anywhere: no alignment is needed)
+          __builtin_memcpy(&b.x[p][i][t], row[i][t] + (p * a.xp + kb * 128) * kItem, 16);
   };
+  // 16 bytes, c-th of row r, are at c ^ r: neither side has bank conflicts
+  const int rr = fr % R;
   auto mul = [&](const Block& b) {
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          const int r = t * RPI + lane / CPR;
+          *(u32x4*)(own + ((p * MT + i) * R + r) * RB + (chunk ^ r) * 16) = b.x[p][i][t];
+        }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       bf16x8 xf[MT][P];
 #pragma unroll
-      for (int i = 0; i < MT; ++i) b.x[i][j].pieces(xf[i]);
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (RAW) {
+          constexpr int V = sizeof(T) / 2;
+          u32x4 v[V];
+#pragma unroll
+          for (int h = 0; h < V; ++h)
+            v[h] = *(const u32x4*)(own + (i * R + rr) * RB + (((j * 4 + fq) * V + h) ^ rr) * 16);
+          pieces_of<T>(v, xf[i]);
+        } else {
+#pragma unroll
+          for (int p = 0; p < P; ++p)
+            xf[i][p] = as_bf16x8(
+                *(const u32x4*)(own + ((p * MT + i) * R + rr) * RB + ((j * 4 + fq) ^ rr) * 16));
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NW; ++n) {
         const bf16x8 wf = operand(b.w.c[n], b.w.s[n], j);
@@ -312,32 +330,38 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
     if (whole < a.KB && whole % KS == wave) {  // the last columns, which are no whole block
       Block f;
       src.load(f.w, whole, lane);
+      constexpr int E = 16 / sizeof(T);
+      const int left = a.K - whole * 128 - chunk * E;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int k = whole * 128 + j * 32;
-          f.x[i][j].load_part(a, row[i] + k, a.K - k - fq * 8);
+        for (int t = 0; t < L; ++t) {
+          const T* from = (const T*)(row[i][t]) + whole * 128;
+          T part[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) part[e] = e < left ? from[e] : T(0);
+          __builtin_memcpy(&f.x[0][i][t], part, 16);
         }
       mul(f);
     }
   }
+  auto sums = [&](int k) { return (f32x4*)(lds + k * kWave) + lane; };
   if constexpr (KS > 1) {
 #pragma unroll
     for (int n = 0; n < NW; ++n)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) part[wave][n * MT + i][lane] = acc[n][i];
+      for (int i = 0; i < MT; ++i) sums(wave)[(n * MT + i) * 64] = acc[n][i];
     __syncthreads();
-    // tile (t, i) of y by wave (t * MT + i) % KS
+    // tile t of y by wave t % KS
 #pragma unroll
     for (int t = 0; t < NT * MT; ++t) {
       if (t % KS != wave) continue;
       f32x4 s[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        s[w] = part[0][w * NT * MT + t][lane];
+        s[w] = sums(0)[(w * NT * MT + t) * 64];
 #pragma unroll
-        for (int k = 1; k < KS; ++k) s[w] += part[k][w * NT * MT + t][lane];
+        for (int k = 1; k < KS; ++k) s[w] += sums(k)[(w * NT * MT + t) * 64];
       }
       finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
     }
@@ -497,24 +521,27 @@ bool in_place(const void* x, int64_t ldx, int K) {
 }
 
 // Which kernel and tile.  n: rows of the weights in all (gated: the gate's and the up's).
-// Up to one workgroup a CU (256) a call takes what one workgroup's walk over K takes, so the
-// smallest tile that needs no more wins, and beyond two a CU the largest.  Cold weights, us,
-// of tiles of rows x weight rows (those up to 32 x 64 the kernel of few rows):
-//   M x N x K            16x16 16x32 16x64 32x64 32x128 64x128 64x256 128x256
-//   64 x 1024 x 3584       5.9   6.1   6.7   9.7  13.5   19.9
-//   128 x 1024 x 3584      9.6   6.2   6.8  10.3  13.5   19.9
-//   256 x 1024 x 3584     17.3  10.2   6.9  10.4  13.5   19.9
-//   64 x 8192 x 8192      62.9  36.8  24.2  21.4  31.5   45     71     114
-//   128 x 8192 x 8192            68   42    38    32     45     70     116
-//   512 x 8192 x 8192                             76     64     73     118
-//   1024 x 8192 x 8192                           141    122    107     122
-//   4096 x 32768 x 1024                          375    354    277     247
-// The kernel of few rows reads fp16 and fp32 rows as they are, where the other needs a
-// pass that splits them: it keeps tiles of up to two workgroups a CU (256 x 4096 x 4096
-// fp16 25.5 us against 28.7, fp32 38.7 against 40.8).
+// While there is a CU for each workgroup (256) a call takes what one workgroup's walk over K
+// takes, so the smallest tile that needs no more wins; with many workgroups a CU, the
+// largest.  The kernel of few rows has tiles of up to 32 x 64 (rows x rows of the weights),
+// its largest up to two workgroups a CU, and takes up to 32 rows whatever the weight.  us,
+// weights from beyond the caches:
+//   M x N x K            16x16  16x32  16x64  32x64 | 32x128 64x128 64x256 128x256
+//   16 x 1024 x 3584       4.2    4.5    5.8
+//   64 x 1024 x 3584       4.4    4.6    5.8    8.9 |  13.5
+//   128 x 1024 x 3584      5.8    4.8    5.8    9.0 |  13.5
+//   256 x 1024 x 3584             6.6    6.0    9.2 |  13.5   19.3
+//   32 x 8192 x 8192             15.6   13.3   17   |  31     44
+//   64 x 8192 x 8192             21     19.8   17.1 |  31     44     70
+//   128 x 8192 x 8192                   31.2   28.1 |  31.6   45     70
+//   256 x 8192 x 8192                          47.4 |  43.1   45.2   70    116
+//   512 x 8192 x 8192                          93.5 |  76.9   66.3   73    118
+//   1024 x 8192 x 8192                        175   | 140    122    107    120
+//   32 x 100000 x 1024                  21.4   20.2 |  19.6   25     19.4   30
+//   1024 x 32768 x 1024                       110   |  99     87     70     66
 template <typename T>
 bool few(int64_t M, int64_t n) {
-  return M <= 16 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= (kPieces<T> == 1 ? 256 : 512);
+  return M <= 32 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 512;
 }
 
 // bytes of the rows' pieces; 0 where the rows are read as they are
@@ -523,11 +550,11 @@ int64_t piece_bytes(const void* x, int64_t ldx, int64_t M, int64_t n, int K) {
   return few<T>(M, n) || in_place<T>(x, ldx, K) ? 0 : kPieces<T> * M * pad128(K) * 2;
 }
 
-template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D>
+template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R = 16>
 void launch_stream(const Args& a, hipStream_t s) {
   const dim3 grid((unsigned)kad_cdiv(a.cols, 16 * NT), (unsigned)kad_cdiv(a.M, 16 * MT));
-  hipLaunchKernelGGL((q4_stream_kernel<T, RAW, GATED, MT, NT, KS, D>), grid, dim3(64 * KS), 0, s,
-                     a);
+  hipLaunchKernelGGL((q4_stream_kernel<T, RAW, GATED, MT, NT, KS, D, R>), grid, dim3(64 * KS), 0,
+                     s, a);
 }
 
 template <typename T, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
@@ -542,24 +569,29 @@ void launch_tile(const Args& a, hipStream_t s) {
 template <typename T, bool RAW, bool GATED>
 void stream(const Args& a, hipStream_t s) {
   constexpr int W = GATED ? 2 : 1, P = kPieces<T>;
-  const int64_t rows = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
-  // 8 waves share K where each has 3 blocks or more of it (1 x 2048 x 16384: 9.9 us, 4 waves
-  // 11.7; fp16 1 x 1024 x 3584 5.2 and 6.0); else 4 (1 x 1024 x 1024 2.2 us, 8 waves 3.0)
+  const int64_t tiles = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
+  // 8 waves share K where each has 3 blocks or more of it (16 x 2048 x 16384: 12.9 us, 4 waves
+  // 14.3; fp16 16 x 1024 x 3584 5.8 and 6.6); else 4 (1 x 1024 x 1024 2.2 us, 8 waves 2.9)
   const bool wide = a.KB >= 24;
   constexpr int D = sizeof(T) == 2 ? 4 : 2;
-  if constexpr (!GATED)
-    if (rows * kad_cdiv(n, 16) <= 256) {
-      if (wide) return launch_stream<T, RAW, GATED, 1, 1, 8, D>(a, s);
-      return launch_stream<T, RAW, GATED, 1, 1, 4, 2>(a, s);
+  // 4 rows or fewer load no more (1 x 1024 x 3584: 3.2 us, all 16 of the tile 3.9)
+  auto rows = [&](auto r) {
+    constexpr int R = decltype(r)::value;
+    if constexpr (!GATED)
+      if (tiles * kad_cdiv(n, 16) <= 256) {
+        if (wide) return launch_stream<T, RAW, GATED, 1, 1, 8, D, R>(a, s);
+        return launch_stream<T, RAW, GATED, 1, 1, 4, 2, R>(a, s);
+      }
+    if (tiles * kad_cdiv(n, 32) <= 256) {
+      if (wide) return launch_stream<T, RAW, GATED, 1, 2 / W, 8, 2, R>(a, s);
+      return launch_stream<T, RAW, GATED, 1, 2 / W, 4, 2, R>(a, s);
     }
-  if (rows * kad_cdiv(n, 32) <= 256) {
-    if (wide) return launch_stream<T, RAW, GATED, 1, 2 / W, 8, D>(a, s);
-    return launch_stream<T, RAW, GATED, 1, 2 / W, 4, 2>(a, s);
-  }
-  if (a.M <= 16 || rows * kad_cdiv(n, 64) <= (P == 3 ? 512 : 256)) {
-    if (wide) return launch_stream<T, RAW, GATED, 1, 4 / W, 8, 2>(a, s);
-    return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2>(a, s);
-  }
+    if (wide) return launch_stream<T, RAW, GATED, 1, 4 / W, 8, 2, R>(a, s);
+    return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2, R>(a, s);
+  };
+  if (a.M <= 4) return rows(std::integral_constant<int, 4>{});
+  if (a.M <= 16 || tiles * kad_cdiv(n, 64) <= (P > 1 ? 512 : 256))
+    return rows(std::integral_constant<int, 16>{});
   return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 3 ? 1 : 2>(a, s);
 }
 
