@@ -514,6 +514,9 @@ int kad_cache_prefetch(const void* p0, int64_t bytes0, const void* p1, int64_t b
  *   blocks, w_down [hidden, ffn], w_in [conv_dim + vd, hidden] (q | k | v | z),
  *   w_ab [ab_rows, hidden] (a | b), w_qkv [(2 q_heads + 2 kv_heads) head_dim,
  *   hidden]; conv_dim = 2 kd + vd; rows of gdn_cols hold [q|k|v | z | a|b | pad].
+ *   A layer with scales s_* has its weights but w_ab in 4 bits (kad_quantize_weight's
+ *   codes, w_gu the gate's and w_up the up's): hidden, ffn, vd and q_heads head_dim
+ *   multiples of 128 and fuse_conv 0.
  * kad_qwen_prefill  layers 0 .. layers - 1 over x [B*L, hidden] (updated in
  *   place).  state0/1[i]: a linear layer's conv state [B, conv_dim, 4] and fp32
  *   state [B, v_heads, k_dim, v_dim], an attention layer's K and V
@@ -539,6 +542,7 @@ typedef struct {
   const void *input_norm, *post_norm, *w_gu, *w_down;
   const void *w_in, *w_ab, *conv_w, *A_log, *dt_bias, *norm_w, *w_out;
   const void *w_qkv, *q_norm, *k_norm, *w_o;
+  const void *w_up, *s_gate, *s_up, *s_down, *s_in, *s_out, *s_qkv, *s_o;
 } kad_qwen_layer;
 
 typedef struct {

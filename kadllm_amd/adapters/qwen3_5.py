@@ -60,11 +60,16 @@ class Qwen35GRBeamAdapter:
     value rounded to an e4m3 multiple of its page's scale.  The attention layers
     of such a prefix are PagedPrefix tuples, and decode_incremental's logits
     equal decode's to rounding instead of bit for bit.
+
+    weights="e2m1" (bf16 models) holds the projections, the FFN and the LM head
+    in 4 bits (kadllm_amd.quantized), quantised once, here; the embedding stays in
+    bf16.  Sums are in an order that depends on the rows of a call:
+    decode_incremental's logits equal decode's to rounding here too.
     """
 
     def __init__(self, text_model, lm_head, *, gdn_backend="torch", conv_backend="torch",
                  attention_backend="torch", gdn_triton_config=None, head_tokens=None,
-                 prefix_cache=None):
+                 prefix_cache=None, weights=None):
         native = isinstance(text_model, Qwen35TextModel)
         if not native and not _is_transformers_text_model(text_model):
             raise TypeError("pass the dense Qwen3_5TextModel explicitly")
@@ -105,6 +110,12 @@ class Qwen35GRBeamAdapter:
                                          or cfg.head_dim not in HEAD_DIMS):
             raise ValueError("an 8-bit prefix cache needs a bf16 model with attention heads of "
                              "64, 128 or 256")
+        if weights not in (None, "e2m1"):
+            raise ValueError("weights must be None or 'e2m1'")
+        if weights is not None and runner is not Qwen35Runner:
+            raise ValueError("4-bit weights need a bf16 model")
+        if weights is not None and cfg.num_attention_heads * cfg.head_dim % 8:
+            raise ValueError("4-bit weights need query rows in multiples of 16")
         if device.type != "cuda":
             raise RuntimeError("the HIP GRBeam path needs the model on a ROCm device")
         self.layer_types = tuple(cfg.layer_types)
@@ -112,12 +123,13 @@ class Qwen35GRBeamAdapter:
         self.gdn_backend, self.conv_backend = gdn_backend, conv_backend
         self.attention_backend = attention_backend
         self.gdn_triton_config = gdn_triton_config
-        self.prefix_cache = prefix_cache
+        self.prefix_cache, self.weights = prefix_cache, weights
         self.config = cfg if native else Qwen35Config.from_hf(cfg)
         self.device = device
+        more = {} if weights is None else {"weights": weights}
         self._runner = runner(self.config, text_model.state_dict(),
                               lm_head_weight=lm_head.weight, device=device,
-                              head_tokens=head_tokens)
+                              head_tokens=head_tokens, **more)
         if runner in (Qwen35RunnerF32, Qwen35RunnerF16):
             # fp32 and fp16 models replay the whole suffix at every level, as
             # the reference does

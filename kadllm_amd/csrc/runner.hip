@@ -35,6 +35,11 @@ int check_model(const kad_qwen_model* m) {
 int mlp(const kad_qwen_model& m, const kad_qwen_layer& l, void* x, void* n, void* h, int rows,
         bool prefetch, kad_stream_t s) {
   const int H = m.hidden, F = m.ffn;
+  if (l.s_down) {
+    KAD_TRY(kad_rmsnorm(x, H, l.post_norm, 1.f, n, H, rows, H, m.eps, s));
+    return kad_quantized_gated_ffn(n, H, kBf, l.w_gu, l.s_gate, l.w_up, l.s_up, l.w_down, l.s_down,
+                                   x, H, x, H, h, (int64_t)rows * F * 2, rows, H, F, s);
+  }
   if (prefetch)
     KAD_TRY(kad_cache_prefetch(l.w_gu, (int64_t)4 * F * H, l.w_down, (int64_t)2 * F * H, s));
   KAD_TRY(kad_rmsnorm(x, H, l.post_norm, 1.f, n, H, rows, H, m.eps, s));
@@ -42,9 +47,20 @@ int mlp(const kad_qwen_model& m, const kad_qwen_layer& l, void* x, void* n, void
   return kad_gemm_bf16(h, F, l.w_down, F, x, H, x, H, rows, H, F, KAD_EPI_RESIDUAL, s);
 }
 
-int store(const void* a, int64_t lda, const void* w, void* c, int64_t ldc, int M, int N, int K,
-          kad_stream_t s) {
+// a product with a bf16 weight, or (scales) a 4-bit one
+int store(const void* a, int64_t lda, const void* w, const void* scales, void* c, int64_t ldc,
+          int M, int N, int K, kad_stream_t s) {
+  if (scales)
+    return kad_quantized_linear(a, lda, kBf, w, scales, nullptr, 0, c, ldc, nullptr, 0, M, N, K, s);
   return kad_gemm_bf16(a, lda, w, K, c, ldc, nullptr, 0, M, N, K, KAD_EPI_STORE, s);
+}
+
+// the same added into x
+int add(const void* a, int64_t lda, const void* w, const void* scales, void* x, int M, int N,
+        int K, kad_stream_t s) {
+  if (scales)
+    return kad_quantized_linear(a, lda, kBf, w, scales, x, N, x, N, nullptr, 0, M, N, K, s);
+  return kad_gemm_bf16(a, lda, w, K, x, N, x, N, M, N, K, KAD_EPI_RESIDUAL, s);
 }
 
 }  // namespace
@@ -65,14 +81,14 @@ extern "C" int kad_qwen_prefill(const kad_qwen_model* m, const kad_qwen_prefill_
     KAD_TRY(kad_rmsnorm(a->x, H, l.input_norm, 1.f, a->n, H, rows, H, m->eps, s));
     if (l.linear) {
       // the gate projection first, while n is in the caches
-      KAD_TRY(store(a->n, H, l.w_ab, at(a->proj, c), cols, rows, m->ab_rows, H, s));
+      KAD_TRY(store(a->n, H, l.w_ab, nullptr, at(a->proj, c), cols, rows, m->ab_rows, H, s));
       const void* conv = a->proj;
       int64_t ldc = cols;
       if (a->fuse_conv) {
         KAD_TRY(kad_gemm_bf16_conv(a->n, H, l.w_in, H, a->proj, cols, rows, c, H, C, l.conv_w, L,
                                    a->state0[i], a->conv, a->conv_bytes, s));
       } else {
-        KAD_TRY(store(a->n, H, l.w_in, a->proj, cols, rows, c, H, s));
+        KAD_TRY(store(a->n, H, l.w_in, l.s_in, a->proj, cols, rows, c, H, s));
         KAD_TRY(kad_causal_conv_prefill(a->proj, cols, l.conv_w, a->conv, C, a->state0[i], B, L, C,
                                         1, s));
         conv = a->conv;
@@ -85,11 +101,10 @@ extern "C" int kad_qwen_prefill(const kad_qwen_model* m, const kad_qwen_prefill_
                                   (float*)a->state1[i], a->chunk_ws, a->chunk_bytes, B, L,
                                   m->k_heads, HV, m->k_dim, m->v_dim, m->gdn_scale,
                                   at(a->proj, C), cols, l.norm_w, m->eps, s));
-      KAD_TRY(kad_gemm_bf16(a->mixed, m->vd, l.w_out, m->vd, a->x, H, a->x, H, rows, H, m->vd,
-                            KAD_EPI_RESIDUAL, s));
+      KAD_TRY(add(a->mixed, m->vd, l.w_out, l.s_out, a->x, rows, H, m->vd, s));
     } else {
       const int ld = (2 * nh + 2 * nkv) * hd;
-      KAD_TRY(store(a->n, H, l.w_qkv, a->proj, ld, rows, ld, H, s));
+      KAD_TRY(store(a->n, H, l.w_qkv, l.s_qkv, a->proj, ld, rows, ld, H, s));
       KAD_TRY(kad_qk_norm_rope(a->proj, ld, 2 * hd, nh, l.q_norm, a->q, rows, 0, nh * hd, hd, rows,
                                hd, m->rot, m->inv_freq, 0, L, m->eps, 1, s));
       const int64_t sb = (int64_t)nkv * L * hd, sh = (int64_t)L * hd;
@@ -101,8 +116,7 @@ extern "C" int kad_qwen_prefill(const kad_qwen_model* m, const kad_qwen_prefill_
       KAD_TRY(kad_attention_prefill(a->q, qb, nh * hd, hd, a->state0[i], a->state1[i], sb, hd, sh,
                                     at(a->proj, hd), (int64_t)L * ld, ld, 2 * hd, a->mixed, qb,
                                     nh * hd, hd, B, L, nh, nkv, hd, m->attn_scale, s));
-      KAD_TRY(kad_gemm_bf16(a->mixed, nh * hd, l.w_o, nh * hd, a->x, H, a->x, H, rows, H, nh * hd,
-                            KAD_EPI_RESIDUAL, s));
+      KAD_TRY(add(a->mixed, nh * hd, l.w_o, l.s_o, a->x, rows, H, nh * hd, s));
     }
     KAD_TRY(mlp(*m, l, a->x, a->n, a->h, rows, false, s));
   }
@@ -130,7 +144,7 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
   for (int i = 0; i < m->n_layers; ++i) {
     const kad_qwen_layer& l = m->layers[i];
     const kad_qwen_prefix& p = a->prefix[i];
-    if (a->prefetch && !l.linear)
+    if (a->prefetch && !l.linear && !l.s_qkv)
       KAD_TRY(kad_cache_prefetch(l.w_qkv, (int64_t)(2 * nh + 2 * nkv) * hd * H * 2, nullptr, 0, s));
     KAD_TRY(kad_rmsnorm(a->x, H, l.input_norm, 1.f, a->n, H, BW, H, m->eps, s));
     if (l.linear) {
@@ -138,8 +152,9 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
         // the earlier token's rows in place in the parents' cache: only its
         // gate inputs are gathered, in whole 16-byte pieces
         KAD_TRY(follow(at(a->prev0[i], c), (int64_t)cols * 2, a->ab, nab * 2, nab * 2));
-        KAD_TRY(store(a->n, H, l.w_ab, at(a->ab, (T - 1) * nab), T * nab, BW, nab, H, s));
-        KAD_TRY(store(a->n, H, l.w_in, a->rows_ws, cols, BW, c, H, s));
+        KAD_TRY(store(a->n, H, l.w_ab, nullptr, at(a->ab, (T - 1) * nab), T * nab, BW, nab, H,
+                      s));
+        KAD_TRY(store(a->n, H, l.w_in, l.s_in, a->rows_ws, cols, BW, c, H, s));
         KAD_TRY(kad_gdn_gates(a->ab, nab, at(a->ab, HV), nab, l.A_log, l.dt_bias, a->g, a->beta,
                               (int64_t)BW * T, HV, s));
         KAD_TRY(kad_gdn_suffix_replay_conv_gated_parents(
@@ -153,8 +168,9 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
           KAD_TRY(follow(a->prev0[i], (int64_t)cols * 2, rows, (int64_t)cols * 2,
                          (int64_t)cols * 2));
         void* last = at(rows, (int64_t)(T - 1) * cols);
-        KAD_TRY(store(a->n, H, l.w_ab, at(last, c), (int64_t)T * cols, BW, nab, H, s));
-        KAD_TRY(store(a->n, H, l.w_in, last, (int64_t)T * cols, BW, c, H, s));
+        KAD_TRY(store(a->n, H, l.w_ab, nullptr, at(last, c), (int64_t)T * cols, BW, nab, H,
+                      s));
+        KAD_TRY(store(a->n, H, l.w_in, l.s_in, last, (int64_t)T * cols, BW, c, H, s));
         KAD_TRY(kad_gdn_gates(at(rows, c), cols, at(rows, c + HV), cols, l.A_log, l.dt_bias, a->g,
                               a->beta, (int64_t)BW * T, HV, s));
         KAD_TRY(kad_gdn_suffix_replay_conv_gated(
@@ -162,12 +178,11 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
             p.p1, p.dtype, at(rows, C), cols, l.norm_w, m->eps, 1, a->mixed, m->vd, B, W, T,
             m->k_heads, HV, m->k_dim, m->v_dim, m->gdn_scale, s));
       }
-      KAD_TRY(kad_gemm_bf16(a->mixed, m->vd, l.w_out, m->vd, a->x, H, a->x, H, BW, H, m->vd,
-                            KAD_EPI_RESIDUAL, s));
+      KAD_TRY(add(a->mixed, m->vd, l.w_out, l.s_out, a->x, BW, H, m->vd, s));
     } else {
       const int ld = (2 * nh + 2 * nkv) * hd;
       const int64_t row = (int64_t)nkv * hd;
-      KAD_TRY(store(a->n, H, l.w_qkv, a->qkv, ld, BW, ld, H, s));
+      KAD_TRY(store(a->n, H, l.w_qkv, l.s_qkv, a->qkv, ld, BW, ld, H, s));
       void* k = a->keep ? a->next0[i] : a->k_ws;
       void* v = a->keep ? a->next1[i] : a->v_ws;
       KAD_REQUIRE(k && v, "null pointer argument");
@@ -186,8 +201,7 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
           a->q, nh * hd, nh * hd, hd, p.p0, p.p1, p.s0, p.s1, p.s2, k, T * row, row, hd, v,
           T * row, row, hd, nullptr, at(a->qkv, hd), ld, ld, 2 * hd, a->mixed, nh * hd, nh * hd, hd,
           B, W, 1, T, nh, nkv, p.history, hd, m->attn_scale, s));
-      KAD_TRY(kad_gemm_bf16(a->mixed, nh * hd, l.w_o, nh * hd, a->x, H, a->x, H, BW, H, nh * hd,
-                            KAD_EPI_RESIDUAL, s));
+      KAD_TRY(add(a->mixed, nh * hd, l.w_o, l.s_o, a->x, BW, H, nh * hd, s));
     }
     KAD_TRY(mlp(*m, l, a->x, a->n, a->h, BW, a->prefetch != 0, s));
   }

@@ -8,17 +8,23 @@ checked by the C ABI, which raises KadLibraryError on a violation.
 import torch
 
 from . import _lib
+from .quantized import QuantizedWeight, _linear
 
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 
 def gemm(a, w, out=None, *, epilogue=EPI_STORE, residual=None):
     """out[M, N'] = epilogue(a[M, K] @ w[N, K]^T) (bf16, fp32 accumulate).
 
-    a, w, out may be row-strided 2-D views (last dim contiguous).  For the
+    w may be a QuantizedWeight (without the SwiGLU epilogue; rounded once, with the
+    residual added).  a, w, out may be row-strided 2-D views (last dim contiguous).  For the
     SwiGLU epilogue N' = N/2; for the residual epilogue ``residual`` [M, N]
     is added (it may be ``out`` itself).
     """
     M, K = a.shape
+    if type(w) is QuantizedWeight:
+        if out is None:
+            out = torch.empty(M, w.rows, dtype=torch.bfloat16, device=a.device)
+        return _linear(a, w, out, residual)
     N = w.shape[0]
     n_out = N // 2 if epilogue == EPI_SWIGLU else N
     if out is None:

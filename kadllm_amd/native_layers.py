@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 from .prefix_cache import PagedPrefix
+from .quantized import QuantizedWeight
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
@@ -18,7 +19,8 @@ _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 class _Layer(ctypes.Structure):
     _fields_ = [("linear", _I)] + [(n, _P) for n in (
         "input_norm", "post_norm", "w_gu", "w_down", "w_in", "w_ab", "conv_w", "A_log", "dt_bias",
-        "norm_w", "w_out", "w_qkv", "q_norm", "k_norm", "w_o")]
+        "norm_w", "w_out", "w_qkv", "q_norm", "k_norm", "w_o", "w_up", "s_gate", "s_up", "s_down",
+        "s_in", "s_out", "s_qkv", "s_o")]
 
 
 class _Model(ctypes.Structure):
@@ -56,11 +58,28 @@ _ATTENTION = _COMMON + ("w_qkv", "q_norm", "k_norm", "w_o")
 _get_linear, _get_attention = operator.attrgetter(*_LINEAR), operator.attrgetter(*_ATTENTION)
 
 
+def _fields(lyr):
+    """(field of _Layer, tensor) for each of a layer's weights."""
+    for name in _LINEAR if hasattr(lyr, "w_in") else _ATTENTION:
+        w = getattr(lyr, name)
+        if name == "w_gu" and type(w) is tuple:
+            gate, up = w
+            yield from (("w_gu", gate.codes), ("s_gate", gate.scales), ("w_up", up.codes),
+                        ("s_up", up.scales))
+        elif type(w) is QuantizedWeight:
+            yield from ((name, w.codes), ("s" + name[1:], w.scales))
+        else:
+            yield name, w
+
+
 def _weights(runner):
     """Every tensor whose address kad_qwen_model holds."""
     out = [runner.inv_freq]
     for lyr in runner.layers:
-        out += _get_linear(lyr) if hasattr(lyr, "w_in") else _get_attention(lyr)
+        if runner.weights is not None:
+            out += [t for _, t in _fields(lyr)]
+        else:
+            out += _get_linear(lyr) if hasattr(lyr, "w_in") else _get_attention(lyr)
     return out
 
 
@@ -74,18 +93,27 @@ class NativeLayers:
         for dst, src in zip(layers, runner.layers):
             dst.linear = int(hasattr(src, "w_in"))
             self.linear.append(bool(dst.linear))
-            for name in _LINEAR if dst.linear else _ATTENTION:
-                setattr(dst, name, getattr(src, name).data_ptr())
+            for name, tensor in _fields(src):
+                setattr(dst, name, tensor.data_ptr())
         # the tensors are held, so that no address outlives its memory
         self._layers, self._tensors = layers, _weights(runner)
         self._addresses = list(map(torch.Tensor.data_ptr, self._tensors))
         # the passes name no strides and no types
-        self.plain = all(t.is_contiguous() and t.dtype == (
-            torch.float32 if t is runner.inv_freq else torch.bfloat16) for t in self._tensors)
+        held = (torch.bfloat16,) if runner.weights is None else (
+            torch.bfloat16, torch.uint8, torch.float8_e8m0fnu)
+        self.plain = all(t.is_contiguous() and (
+            t.dtype == torch.float32 if t is runner.inv_freq else t.dtype in held)
+            for t in self._tensors)
         self.ab_rows = 2 * cfg.linear_num_value_heads
-        self.ffn = runner.layers[0].w_down.shape[1]
+        widths = [w.cols if type(w) is QuantizedWeight else w.shape[1]
+                  for w in (lyr.w_down for lyr in runner.layers)]
+        self.ffn = widths[0]
         # one width throughout (the padded packing of every layer's MLP)
-        self.uniform = all(lyr.w_down.shape[1] == self.ffn for lyr in runner.layers)
+        self.uniform = all(w == self.ffn for w in widths)
+        if runner.weights is not None:
+            # products of whole blocks of columns need no workspace
+            self.plain = self.plain and not any(n % 128 for n in (
+                cfg.hidden_size, self.ffn, runner.vd, cfg.num_attention_heads * cfg.head_dim))
         self.model = _Model(
             layers, runner.inv_freq.data_ptr(), len(runner.layers), cfg.hidden_size, self.ffn,
             runner.conv_dim, runner.kd, runner.vd, runner.gdn_cols, self.ab_rows,

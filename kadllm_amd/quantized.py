@@ -55,8 +55,12 @@ class QuantizedWeight:
             raise ValueError("the tensors of a 4-bit weight must be contiguous")
         if codes.device != scales.device:
             raise ValueError("all tensors must be on the same device")
-        for name, value in zip(self.__slots__, (codes, scales, rows, cols)):
+        self._set(codes, scales, rows, cols)
+
+    def _set(self, *values):
+        for name, value in zip(self.__slots__, values):
             object.__setattr__(self, name, value)
+        return self
 
     def __setattr__(self, name, value):
         raise AttributeError("a QuantizedWeight is not changed; make another")
@@ -66,6 +70,13 @@ class QuantizedWeight:
 
     def __repr__(self):
         return f"QuantizedWeight({self.rows} x {self.cols}, {self.codes.device})"
+
+    def row_range(self, first, last):
+        """The rows first to last - 1 (multiples of 16, or the end), sharing memory."""
+        if first % 16 or last % 16 and last != self.rows or not 0 <= first < last <= self.rows:
+            raise ValueError("a range of rows begins and ends at multiples of 16")
+        blocks = slice(first // 16, -(-last // 16))
+        return QuantizedWeight(self.codes[blocks], self.scales[blocks], last - first, self.cols)
 
     def to(self, device):
         """This weight on another device."""
@@ -131,10 +142,11 @@ def _rows(t):
     the stride of its rows."""
     M, C = t.shape
     ld, one = t.stride()
-    if one != 1 and C > 1 or ld < C and M > 1:
+    if one == 1 and ld >= C:
+        return t, ld
+    if one != 1 and C > 1 or M > 1:
         t = t.contiguous()
-        ld = C
-    return t, ld if ld > C else C
+    return t, C
 
 
 def quantize_weight(weight):
@@ -157,10 +169,10 @@ def quantize_weight(weight):
     weight, ld = _rows(weight)
     shapes = _padded(N, K)
     codes = torch.empty(shapes[0], dtype=torch.uint8, device=weight.device)
-    scales = torch.empty(shapes[1], dtype=torch.uint8, device=weight.device).view(_SCALES)
+    scales = torch.empty(shapes[1], dtype=_SCALES, device=weight.device)
     _launch(device, "kad_quantize_weight", weight.data_ptr(), ld, _lib.dtype_code(weight.dtype),
             codes.data_ptr(), scales.data_ptr(), N, K)
-    return QuantizedWeight(codes, scales, N, K)
+    return QuantizedWeight.__new__(QuantizedWeight)._set(codes, scales, N, K)
 
 
 def dequantize_weight(weight, dtype=torch.bfloat16):
@@ -183,9 +195,8 @@ def _workspace_bytes(name, offset, *sizes):
     return need.value
 
 
-def _check_rows(x, cols, out_cols, residual, weights):
-    """x [..., cols] and residual [..., out_cols] (or None) as 2-D rows, fit to be
-    multiplied by ``weights``."""
+def _check_rows(x, cols, out_cols, residual):
+    """x [..., cols] and residual [..., out_cols] (or None) as 2-D rows."""
     shape = x.shape
     if not shape or shape[-1] != cols or 0 in shape:
         raise ValueError(f"x must be [..., {cols}], the weight's columns, and not empty")
@@ -202,7 +213,6 @@ def _check_rows(x, cols, out_cols, residual, weights):
     if torch.is_grad_enabled() and (x.requires_grad or
                                     residual is not None and residual.requires_grad):
         raise RuntimeError("kadllm_amd operators are inference-only; disable gradients")
-    _device_of(x, residual, *[w.codes for w in weights])
     if len(shape) != 2:
         x = x.reshape(-1, cols)
         residual = residual if residual is None else residual.reshape(-1, out_cols)
@@ -216,7 +226,8 @@ def quantized_linear(x, weight, *, residual=None):
     Returns [..., N] in x's type.  Products are exact, sums are fp32 and are rounded
     once, with the residual added."""
     _check_weight(weight)
-    rows, r = _check_rows(x, weight.cols, weight.rows, residual, (weight,))
+    rows, r = _check_rows(x, weight.cols, weight.rows, residual)
+    _device_of(x, weight.codes, residual)
     out = _linear(rows, weight, rows.new_empty((rows.shape[0], weight.rows)), r)
     return out if rows is x else out.view(*x.shape[:-1], weight.rows)
 
@@ -249,7 +260,8 @@ def quantized_gated_ffn(x, gate, up, down, *, residual=None):
     F, H = gate.rows, gate.cols
     if up.rows != F or up.cols != H or down.rows != H or down.cols != F:
         raise ValueError("gate and up must be [F, H] and down [H, F]")
-    rows, r = _check_rows(x, H, H, residual, (gate, up, down))
+    rows, r = _check_rows(x, H, H, residual)
+    _device_of(x, gate.codes, up.codes, down.codes, residual)
     out = _gated_ffn(rows, gate, up, down, rows.new_empty(rows.shape), r)
     return out if rows is x else out.view(x.shape)
 

@@ -30,6 +30,7 @@ from .native_layers import NativeLayers
 from .attention import attention_prefill, prefix_attention_decode
 from .ops import REPLAY_MAX_T
 from .prefix_cache import PagedPrefix, paged_attention_decode
+from .quantized import QuantizedWeight, _gated_ffn, quantize_weight
 
 
 def _attend(q, prefix, k, v, W, scale, gate, gate_strides):
@@ -63,6 +64,13 @@ def reject_biases(cfg, state_dict):
         raise ValueError(f"the HIP runner has no projection biases; checkpoint holds {biased[:3]}")
 
 
+def _split_rows(w, rows):
+    """(the first ``rows`` rows of a weight, the others)"""
+    if type(w) is QuantizedWeight:
+        return w.row_range(0, rows), w.row_range(rows, w.rows)
+    return w[:rows], w[rows:]
+
+
 @dataclass
 class _GdnLayer:
     input_norm: torch.Tensor
@@ -74,7 +82,7 @@ class _GdnLayer:
     dt_bias: torch.Tensor
     norm_w: torch.Tensor      # [dv]
     w_out: torch.Tensor       # [H, Vd]
-    w_gu: torch.Tensor        # [2F, H] interleaved
+    w_gu: torch.Tensor        # [2F, H] interleaved; in 4 bits (gate, up)
     w_down: torch.Tensor      # [H, F]
 
 
@@ -122,12 +130,19 @@ class Qwen35Runner:
     head projects only to those tokens (README.md:164, the production head that
     projects to the semantic-ID tokens), logits column c is token
     head_tokens[c], and the softmax of a search runs over that sub-vocabulary.
+
+    ``weights`` "e2m1" holds the projections, the FFN and the LM head in 4 bits
+    (QuantizedWeight); the embedding and the 2 HV rows of a GDN layer's gate projection
+    stay in bf16.
     """
 
     dtype = torch.bfloat16
 
-    def __init__(self, cfg, state_dict, lm_head_weight=None, device=None, head_tokens=None):
+    def __init__(self, cfg, state_dict, lm_head_weight=None, device=None, head_tokens=None,
+                 weights=None):
         self.cfg = cfg
+        self.weights = weights
+        pack = (lambda w: w) if weights is None else quantize_weight
         self.device = torch.device(device) if device is not None else \
             state_dict["embed_tokens.weight"].device
         if self.device.type != "cuda":
@@ -153,6 +168,7 @@ class Qwen35Runner:
                 raise ValueError("head_tokens must be a nonempty 1-D list of vocabulary ids")
             self.head_ids = ids.contiguous()
             self.lm_head = self.lm_head.index_select(0, self.head_ids).contiguous()
+        self.lm_head = pack(self.lm_head)
         self.norm_w = get("norm.weight")
         self.kd = cfg.linear_num_key_heads * cfg.linear_key_head_dim
         self.vd = cfg.linear_num_value_heads * cfg.linear_value_head_dim
@@ -163,8 +179,11 @@ class Qwen35Runner:
         self.layers = []
         for i, kind in enumerate(cfg.layer_types):
             p = f"layers.{i}."
-            w_gu, w_down = pack_mlp(get(p + "mlp.gate_proj.weight"), get(p + "mlp.up_proj.weight"),
-                                    get(p + "mlp.down_proj.weight"))
+            gate, up, down = (get(p + f"mlp.{n}_proj.weight") for n in ("gate", "up", "down"))
+            if weights is None:
+                w_gu, w_down = pack_mlp(gate, up, down)
+            else:
+                w_gu, w_down = (pack(gate), pack(up)), pack(down)
             common = dict(input_norm=get(p + "input_layernorm.weight"),
                           post_norm=get(p + "post_attention_layernorm.weight"),
                           w_gu=w_gu, w_down=w_down)
@@ -181,16 +200,16 @@ class Qwen35Runner:
                 if cfg.linear_conv_kernel_dim != 4:
                     raise ValueError("the conv kernels are specialised for width 4")
                 self.layers.append(_GdnLayer(
-                    w_in=w_in, w_ab=w_ab, conv_w=get(a + "conv1d.weight").reshape(self.conv_dim, 4).contiguous(),
+                    w_in=pack(w_in), w_ab=w_ab, conv_w=get(a + "conv1d.weight").reshape(self.conv_dim, 4).contiguous(),
                     A_log=get(a + "A_log"), dt_bias=get(a + "dt_bias"), norm_w=get(a + "norm.weight"),
-                    w_out=get(a + "out_proj.weight"), **common))
+                    w_out=pack(get(a + "out_proj.weight")), **common))
             else:
                 a = p + "self_attn."
                 w_qkv = torch.cat((get(a + "q_proj.weight"), get(a + "k_proj.weight"),
                                    get(a + "v_proj.weight")), 0).contiguous()
-                self.layers.append(_AttnLayer(w_qkv=w_qkv, q_norm=get(a + "q_norm.weight"),
+                self.layers.append(_AttnLayer(w_qkv=pack(w_qkv), q_norm=get(a + "q_norm.weight"),
                                               k_norm=get(a + "k_norm.weight"),
-                                              w_o=get(a + "o_proj.weight"), **common))
+                                              w_o=pack(get(a + "o_proj.weight")), **common))
         self._native = None
         # optional observer: trace(phase, layer, x) after each layer with a copy
         # of the residual stream rows (the last position only past a pruned
@@ -221,6 +240,9 @@ class Qwen35Runner:
         if prefetch:
             layers.cache_prefetch(lyr.w_gu, lyr.w_down)
         n2 = layers.rmsnorm(x, lyr.post_norm, cfg.rms_norm_eps)
+        if self.weights is not None:
+            _gated_ffn(n2, *lyr.w_gu, lyr.w_down, x, x)
+            return
         h = layers.gemm(n2, lyr.w_gu, epilogue=layers.EPI_SWIGLU)
         layers.gemm(h, lyr.w_down, out=x, epilogue=layers.EPI_RESIDUAL, residual=x)
 
@@ -238,7 +260,7 @@ class Qwen35Runner:
     def conv_fuses(self, rows, L, lyr):
         """Whether kad_gemm_bf16_conv takes a prefill's projection."""
         C = self.conv_dim
-        return (L % 128 == 0 and rows % 256 == 0 and (C + self.vd) % 256 == 0 and C % 256 == 0
+        return (self.weights is None and L % 128 == 0 and rows % 256 == 0 and (C + self.vd) % 256 == 0 and C % 256 == 0
                 and self.cfg.hidden_size % 64 == 0 and lyr.conv_w.is_contiguous()
                 and lyr.conv_w.data_ptr() % 16 == 0)
 
@@ -255,8 +277,8 @@ class Qwen35Runner:
         c = C + self.vd
         dev = n.device
         stream = _lib.stream_of(n)
-        w_in = lyr.w_in
         if self.conv_fuses(rows, L, lyr):
+            w_in = lyr.w_in
             proj = torch.empty(rows, self.gdn_cols, dtype=torch.bfloat16, device=dev)
             layers.gemm(n, lyr.w_ab, out=proj[:, c:c + lyr.w_ab.shape[0]])
             nb = ctypes.c_int64(0)
@@ -404,7 +426,8 @@ class Qwen35Runner:
         rows = n.shape[0]
         dev = n.device
         qcols = 2 * nh * hd
-        kv = layers.gemm(n, lyr.w_qkv[qcols:])                  # [rows, k | v]
+        w_q, w_kv = _split_rows(lyr.w_qkv, qcols)
+        kv = layers.gemm(n, w_kv)                               # [rows, k | v]
         ld = kv.stride(0)
         kc = torch.empty(B, nkv, L, hd, dtype=torch.bfloat16, device=dev)
         vc = torch.empty(B, nkv, L, hd, dtype=torch.bfloat16, device=dev)
@@ -412,7 +435,7 @@ class Qwen35Runner:
         layers.qk_norm_rope(kv, ld, hd, nkv, lyr.k_norm, kc, kv_strides, L, rows, hd, self.rot,
                             self.inv_freq, 0, L, cfg.rms_norm_eps)
         layers.scatter_heads(kv[:, nkv * hd:], ld, nkv, hd, vc, kv_strides, L, rows)
-        qg = layers.gemm(n.view(B, L, -1)[:, -1], lyr.w_qkv[:qcols])   # [B, q | gate per head]
+        qg = layers.gemm(n.view(B, L, -1)[:, -1], w_q)   # [B, q | gate per head]
         q = torch.empty(B, 1, nh, hd, dtype=torch.bfloat16, device=dev)
         layers.qk_norm_rope(qg, qg.stride(0), 2 * hd, nh, lyr.q_norm, q, (nh * hd, nh * hd, hd),
                             1, B, hd, self.rot, self.inv_freq, L - 1, 1, cfg.rms_norm_eps)
@@ -635,7 +658,8 @@ class Qwen35Runner:
         # times.  The prefill's 32,768-row GEMMs lose only 2-3 us cold, less
         # than the prefetch costs, and a GEMM of few rows reads its weight
         # once at HBM rate whether or not it was prefetched.
-        prefetch = 2048 <= BW <= 16384
+        # (4-bit weights are a quarter of that)
+        prefetch = 2048 <= BW <= 16384 and self.weights is None
         new_layers = []
         native = self._native_layers()
         batched = native is not None and native.step_fits(T, prefix_layers)
