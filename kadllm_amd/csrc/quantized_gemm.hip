@@ -395,7 +395,8 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
   // loads that a wave issues after a slice's own before it waits for that slice: those of
   // SLOTS - 2 later ones, and the codes' and scales' of the blocks that begin meanwhile
   constexpr int LATER = LPW * (SLOTS - 2) + 2 * NW * ((SLOTS - 2) / (HALVES * P));
-  static_assert(D * HALVES * P % 2 == 0, "slices alternate between two sets of registers");
+  static_assert(D * HALVES * P % SLOTS == 0 && SLOTS % 2 == 0,
+                "a slice's slot and registers are known when the D blocks are unrolled");
   static_assert(LPW * RPI * 4 == BM && LATER < 64, "loads");
   __shared__ __attribute__((aligned(1024))) bf16_t ring[SLOTS][BM * BK];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
@@ -416,21 +417,16 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
     src[i] = (const bf16_t*)a.x + (int64_t)min(m0 + r, a.M - 1) * a.ldx +
              ((lane % CPR) ^ swizzle(r)) * 8;
   }
-  const int slices = a.KB * HALVES * P;
-  int64_t next_at = 0;  // of the next slice to load: columns + piece
-  int next = 0, next_p = 0;
-  auto issue = [&](int slot) {
+  // slice t (counted from a block kb's first) to its slot; past the last block, that one's
+  // again (never multiplied)
+  auto issue = [&](int kb, int t) {
+    const int p = t % P, h = t / P % HALVES;
+    const int64_t from = (int64_t)min(kb + t / (P * HALVES), a.KB - 1) * 128 + h * BK + p * a.xp;
 #pragma unroll
     for (int i = 0; i < LPW; ++i)
       __builtin_amdgcn_global_load_lds(
-          (__attribute__((address_space(1))) void*)(src[i] + next_at),
-          (lds_void_t*)(ring[slot] + (wave + 4 * i) * RPI * BK), 16, 0, 0);
-    // past the last slice, that one again (never read)
-    if (next + 1 < slices) {
-      ++next;
-      if (++next_p == P) next_p = 0, next_at += BK - (P - 1) * a.xp;
-      else next_at += a.xp;
-    }
+          (__attribute__((address_space(1))) void*)(src[i] + from),
+          (lds_void_t*)(ring[t % SLOTS] + (wave + 4 * i) * RPI * BK), 16, 0, 0);
   };
   const Source<NW> w = source<NW, W>(a, nt);
   f32x4 acc[NW][MT];
@@ -442,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
 #pragma unroll
   for (int d = 0; d < D - 1; ++d) w.load(codes[d], min(d, a.KB - 1), lane);
 #pragma unroll
-  for (int t = 0; t < AHEAD; ++t) issue(t);
+  for (int t = 0; t < AHEAD; ++t) issue(0, t);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   bf16x8 frags[PIPE ? 2 : 1][STEPS][MT];
   auto read = [&](bf16x8 (&f)[STEPS][MT], int at) {
@@ -453,7 +449,6 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
       for (int i = 0; i < MT; ++i)  // (rows differ by multiples of 16)
         f[j][i] = as_bf16x8(*(const u32x4*)(x + i * 16 * BK + ((j * 4 + fq) ^ swizzle(fr)) * 8));
   };
-  int slot = 0;
   if constexpr (PIPE) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -468,8 +463,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
       for (int h = 0; h < HALVES; ++h)
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          constexpr int two = PIPE ? 2 : 1;
-          const int set = ((d * HALVES + h) * P + p) % two;
+          const int t = (d * HALVES + h) * P + p, set = PIPE ? t % 2 : 0;
           // PIPE: the next slice has landed (later ones may be in flight), and every wave
           // has this one in registers, so its slot takes the slice SLOTS ahead.  Else: this
           // slice has landed, and every wave has read the one before.
@@ -478,24 +472,22 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
           asm volatile("" ::: "memory");
           if (h == 0 && p == 0)
             w.load(codes[(d + D - 1) % D], min(kb + D - 1, a.KB - 1), lane);
-          const int after = slot == SLOTS - 1 ? 0 : slot + 1;
-          if constexpr (PIPE) {
-            read(frags[set ^ 1], after);
-            issue(slot);
-          } else {
-            issue(slot == 0 ? SLOTS - 1 : slot - 1);
-            read(frags[0], slot);
+          if constexpr (PIPE) read(frags[set ^ 1], (t + 1) % SLOTS);
+          issue(kb0, t + AHEAD);
+          if constexpr (!PIPE) read(frags[0], t % SLOTS);
+          // the next row block's operand is made among the products of the present one: a
+          // conversion right before the product that reads it holds up the matrix unit
+          bf16x8 wf = operand(codes[d].c[0], codes[d].s[0], h * STEPS);
+#pragma unroll
+          for (int jn = 0; jn < STEPS * NW; ++jn) {
+            const int j = jn / NW, n = jn % NW, jl = (jn + 1) / NW, nl = (jn + 1) % NW;
+            bf16x8 ahead = wf;
+            if (jn + 1 < STEPS * NW)
+              ahead = operand(codes[d].c[nl], codes[d].s[nl], h * STEPS + jl);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[n][i] = mfma16x16x32(wf, frags[set][j][i], acc[n][i]);
+            wf = ahead;
           }
-          slot = after;
-#pragma unroll
-          for (int j = 0; j < STEPS; ++j)
-#pragma unroll
-            for (int n = 0; n < NW; ++n) {
-              const bf16x8 wf = operand(codes[d].c[n], codes[d].s[n], h * STEPS + j);
-#pragma unroll
-              for (int i = 0; i < MT; ++i)
-                acc[n][i] = mfma16x16x32(wf, frags[set][j][i], acc[n][i]);
-            }
           if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -601,7 +593,7 @@ void tiles(const Args& a, hipStream_t s) {
   const int64_t n = (int64_t)a.cols * (GATED ? 2 : 1);
   auto count = [&](int rows, int cols) { return kad_cdiv(a.M, rows) * kad_cdiv(n, cols); };
   if (count(32, 128) <= 512) return launch_tile<T, GATED, 2, 2, 128, 4, 4>(a, s);
-  if (count(64, 128) <= 512) return launch_tile<T, GATED, 4, 2, 128, 4, P == 1 ? 4 : 2>(a, s);
+  if (count(64, 128) <= 512) return launch_tile<T, GATED, 4, 2, 128, 4, P == 2 ? 2 : 4>(a, s);
   // Two of the largest tiles run on a CU at a time, and take twice as long as four of half
   // the size, or somewhat less: the larger ones where that halves the rounds (192 x
   // 100000 x 1024, 2 rounds against 3: 61.9 us, smaller 54.0; 256 rows, 2 against 4: 63.5 and 65.9).
