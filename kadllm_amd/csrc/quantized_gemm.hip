@@ -345,34 +345,25 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
       mul(f);
     }
   }
+  // a wave's sums take the place of its rows
   auto sums = [&](int k) { return (f32x4*)(lds + k * kWave) + lane; };
-  if constexpr (KS > 1) {
 #pragma unroll
-    for (int n = 0; n < NW; ++n)
+  for (int n = 0; n < NW; ++n)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) sums(wave)[(n * MT + i) * 64] = acc[n][i];
-    __syncthreads();
-    // tile t of y by wave t % KS
+    for (int i = 0; i < MT; ++i) sums(wave)[(n * MT + i) * 64] = acc[n][i];
+  __syncthreads();
+  // tile t of y by wave t % KS
 #pragma unroll
-    for (int t = 0; t < NT * MT; ++t) {
-      if (t % KS != wave) continue;
-      f32x4 s[W];
+  for (int t = 0; t < NT * MT; ++t) {
+    if (t % KS != wave) continue;
+    f32x4 s[W];
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        s[w] = sums(0)[(w * NT * MT + t) * 64];
+    for (int w = 0; w < W; ++w) {
+      s[w] = sums(0)[(w * NT * MT + t) * 64];
 #pragma unroll
-        for (int k = 1; k < KS; ++k) s[w] += sums(k)[(w * NT * MT + t) * 64];
-      }
-      finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
+      for (int k = 1; k < KS; ++k) s[w] += sums(k)[(w * NT * MT + t) * 64];
     }
-  } else {
-#pragma unroll
-    for (int t = 0; t < NT * MT; ++t) {
-      f32x4 s[W];
-#pragma unroll
-      for (int w = 0; w < W; ++w) s[w] = acc[w * NT + t / MT][t % MT];
-      finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
-    }
+    finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
   }
 }
 
@@ -516,15 +507,17 @@ bool in_place(const void* x, int64_t ldx, int K) {
 // While there is a CU for each workgroup (256) a call takes what one workgroup's walk over K
 // takes, so the smallest tile that needs no more wins; with many workgroups a CU, the
 // largest.  The kernel of few rows has tiles of up to 32 x 64 (rows x rows of the weights),
-// its largest up to two workgroups a CU, and takes up to 32 rows whatever the weight.  us,
-// weights from beyond the caches:
+// its largest up to 640 workgroups (300 x 4096 x 2048, 640 of them: bf16 12.2 us against the
+// other kernel's 12.3, fp16 17.4 and 21.4, fp32 27.2 and 28.2; 400 rows, 832: 15.3 and 12.7,
+// 23.1 and 22.4, 35 and 30), and takes up to 32 rows whatever the weight.  us, weights from
+// beyond the caches:
 //   M x N x K            16x16  16x32  16x64  32x64 | 32x128 64x128 64x256 128x256
 //   16 x 1024 x 3584       4.2    4.5    5.8
 //   64 x 1024 x 3584       4.4    4.6    5.8    8.9 |  13.5
 //   128 x 1024 x 3584      5.8    4.8    5.8    9.0 |  13.5
-//   256 x 1024 x 3584             6.6    6.0    9.2 |  13.5   19.3
-//   32 x 8192 x 8192             15.6   13.3   17   |  31     44
-//   64 x 8192 x 8192             21     19.8   17.1 |  31     44     70
+//   256 x 1024 x 3584             6.9    5.8    8.9 |  13.5   19.3
+//   32 x 8192 x 8192             15.6   13.1   17   |  31     44
+//   64 x 8192 x 8192             21     20.2   17.3 |  31     44     70
 //   128 x 8192 x 8192                   31.2   28.1 |  31.6   45     70
 //   256 x 8192 x 8192                          47.4 |  43.1   45.2   70    116
 //   512 x 8192 x 8192                          93.5 |  76.9   66.3   73    118
@@ -533,7 +526,7 @@ bool in_place(const void* x, int64_t ldx, int K) {
 //   1024 x 32768 x 1024                       110   |  99     87     70     66
 template <typename T>
 bool few(int64_t M, int64_t n) {
-  return M <= 32 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 512;
+  return M <= 32 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 640;
 }
 
 // bytes of the rows' pieces; 0 where the rows are read as they are
@@ -562,27 +555,36 @@ template <typename T, bool RAW, bool GATED>
 void stream(const Args& a, hipStream_t s) {
   constexpr int W = GATED ? 2 : 1, P = kPieces<T>;
   const int64_t tiles = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
-  // 8 waves share K where each has 3 blocks or more of it (16 x 2048 x 16384: 12.9 us, 4 waves
-  // 14.3; fp16 16 x 1024 x 3584 5.8 and 6.6); else 4 (1 x 1024 x 1024 2.2 us, 8 waves 2.9)
-  const bool wide = a.KB >= 24;
-  constexpr int D = sizeof(T) == 2 ? 4 : 2;
+  // 8 waves share K from 12 blocks of it on (16 x 1024 x 1536 fp32: 4.9 us, 4 waves 5.5;
+  // 16 x 2048 x 16384: 12.9 and 14.3; 1 x 1024 x 1024, 8 blocks: 2.9 and 2.2)
+  const bool wide = a.KB >= 12;
   // 4 rows or fewer load no more (1 x 1024 x 3584: 3.2 us, all 16 of the tile 3.9)
   auto rows = [&](auto r) {
     constexpr int R = decltype(r)::value;
     if constexpr (!GATED)
       if (tiles * kad_cdiv(n, 16) <= 256) {
-        if (wide) return launch_stream<T, RAW, GATED, 1, 1, 8, D, R>(a, s);
+        // 4 blocks ahead where a wave has as many (1 x 2048 x 16384: 7.7 us, 2 ahead 9.4)
+        if constexpr (P < 3)
+          if (a.KB >= 24) return launch_stream<T, RAW, GATED, 1, 1, 8, 4, R>(a, s);
+        if (wide) return launch_stream<T, RAW, GATED, 1, 1, 8, 2, R>(a, s);
         return launch_stream<T, RAW, GATED, 1, 1, 4, 2, R>(a, s);
       }
     if (tiles * kad_cdiv(n, 32) <= 256) {
       if (wide) return launch_stream<T, RAW, GATED, 1, 2 / W, 8, 2, R>(a, s);
       return launch_stream<T, RAW, GATED, 1, 2 / W, 4, 2, R>(a, s);
     }
-    if (wide) return launch_stream<T, RAW, GATED, 1, 4 / W, 8, 2, R>(a, s);
+    // one block ahead leaves registers for more waves (fp16 128 x 4096 x 4096: 13.9 us, 2
+    // ahead 16.7; fp32 has too few blocks in flight then: 128 x 2048 x 16384 45 and 39, and
+    // with 2 ahead no registers for a second workgroup: 300 x 1024 x 2048, 304 of them, 14.6
+    // us, of 4 waves 12)
+    if (wide && (P < 3 || tiles * kad_cdiv(n, 64) <= 256))
+      return launch_stream<T, RAW, GATED, 1, 4 / W, 8, P == 3 ? 2 : 1, R>(a, s);
     return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2, R>(a, s);
   };
   if (a.M <= 4) return rows(std::integral_constant<int, 4>{});
-  if (a.M <= 16 || tiles * kad_cdiv(n, 64) <= (P > 1 ? 512 : 256))
+  // (128 x 4096 x 4096, 512 workgroups of 16 x 64: fp16 13.9 us, of 32 x 64 16.0; bf16 10.8
+  // and 10.1)
+  if (a.M <= 16 || tiles * kad_cdiv(n, 64) <= (P > 1 ? 512 : 320))
     return rows(std::integral_constant<int, 16>{});
   return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 3 ? 1 : 2>(a, s);
 }
@@ -660,6 +662,7 @@ int check_sizes(int64_t M, int64_t N, int K) {
   // (a grid holds fewer than 2^32 work-items a dimension, and 65535 rows of tiles)
   KAD_REQUIRE(M <= 16 * 65535 && kad_cdiv(M, 32) * kad_cdiv(2 * N, 128) < (1ll << 32) / 256,
               "a product of %lld x %lld outputs", (long long)M, (long long)N);
+  KAD_REQUIRE(M * pad128(K) < (1ll << 35), "%lld rows of %d columns", (long long)M, K);
   return KAD_OK;
 }
 

@@ -140,6 +140,57 @@ def test_linear(device, M, N, K, dtype):
     _assert_linear(quantized_linear(x, q, residual=r), x, dense, r)
 
 
+# one shape for each tile of the kernel of many rows, and for rows that it splits first
+LARGE = [(700, 1900, 256), (1100, 3000, 300), (1100, 5000, 128), (4000, 8192, 130),
+         (2000, 1030, 640)]
+
+
+def _assert_large(out, x, dense, residual=None):
+    """_assert_linear in float64 on the GPU."""
+    xd, w = x.double(), dense.cuda()
+    y, size = xd @ w.T, xd.abs() @ w.abs().T
+    if residual is not None:
+        y, size = y + residual.double(), size + residual.double().abs()
+    bound = _bound(y, size, PIECES[x.dtype] * x.shape[-1] + 2, x.dtype)
+    err = (out.double() - y).abs()
+    assert (err <= bound).all(), (err - bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, N, K", LARGE)
+def test_linear_of_many_rows(device, M, N, K, dtype):
+    q, dense = _weight(N, K, M + N)
+    x = _values((M, K), K, dtype)
+    r = _values((M, N), 7, dtype)
+    _assert_large(quantized_linear(x, q, residual=r), x, dense, r)
+    # rows inside a wider buffer, at odd places of it
+    wide = _values((M, K + 19), K + 1, dtype)
+    for x in (wide[:, 8:8 + K], wide[:, 3:3 + K]):
+        _assert_large(quantized_linear(x, q), x, dense)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, N, K", LARGE)
+def test_many_rows_exactly(device, M, N, K, dtype):
+    # whole numbers, every sum of which is one: nothing is lost or added
+    g = torch.Generator().manual_seed(M)
+    w = ref.values()[torch.randint(0, 16, (N, K), generator=g)].float()
+    w[:, ::32] = 6.0
+    q = quantize_weight(w.cuda())
+    x = torch.randint(-4, 5, (M, K), generator=g).cuda()
+    want = x.double() @ w.double().cuda().T
+    got = quantized_linear(x.to(dtype), q)
+    assert torch.equal(got, want.to(dtype))
+    # a row that is not finite leaves the others alone
+    y = x.to(dtype)
+    y[M // 2, K - 1] = float("inf")
+    y[M - 1, 0] = float("nan")
+    out = quantized_linear(y, q)
+    assert not out[M // 2].isfinite().any() and out[M - 1].isnan().all()
+    rest = [m for m in range(M) if m not in (M // 2, M - 1)]
+    assert torch.equal(out[rest], got[rest])
+
+
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("M", [1, 3, 16, 40, 100, 260, 600])
 def test_linear_whole_numbers_are_exact(device, M, dtype):
@@ -277,6 +328,17 @@ def test_ffn(device, M, H, F, dtype):
     _assert_ffn(quantized_gated_ffn(x, gate, up, down, residual=r), x, g, u, d, r)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, H, F", [(1000, 1100, 700), (1500, 256, 2000), (4000, 128, 4096)])
+def test_ffn_of_many_rows(device, M, H, F, dtype):
+    (gate, g), (up, u), (down, d) = _weight(F, H, 1), _weight(F, H, 2), _weight(H, F, 3)
+    x = _values((M, H), 4, dtype)
+    out = quantized_gated_ffn(x, gate, up, down, residual=x)
+    # every tile of rows, the last ones among them
+    rows = torch.cat((torch.arange(0, M, 37), torch.arange(M - 20, M)))
+    _assert_ffn(out[rows.cuda()], x[rows.cuda()], g, u, d, x[rows.cuda()])
+
+
 def test_ffn_strided_and_batched(device):
     H, F = 128, 96
     (gate, g), (up, u), (down, d) = _weight(F, H, 1), _weight(F, H, 2), _weight(H, F, 3)
@@ -393,7 +455,7 @@ def test_streams(device):
 
 
 def test_repeated_calls_give_the_same_bits(device):
-    for M in (1, 40, 300):
+    for M in (1, 40, 300, 2500):
         q, _ = _weight(1000, 3584, 1)
         x = _values((M, 3584), 2, BF)
         first = quantized_linear(x, q)

@@ -224,6 +224,8 @@ def test_c_product_refusals():
                    a["r"], a["ldr"], a["y"], a["ldy"], a["ws"], a["bytes"], a["M"], a["N"], a["K"],
                    None) < 0, change
     assert _rc("kad_quantized_linear_workspace_bytes", P, 64, 0, 3, 32, 64, None) < 0
+    assert _rc("kad_quantized_linear_workspace_bytes", P, 2**20, 2, 2**16, 1, 2**20,
+               ctypes.byref(n)) < 0
     assert _rc("kad_quantized_gated_ffn_workspace_bytes", P, 64, 0, 3, 32, 64, None) < 0
     assert _rc("kad_quantized_gated_ffn_workspace_bytes", P, 64, 0, 3, 64, 100,
                ctypes.byref(n)) == 0 and n.value > 0
