@@ -658,7 +658,7 @@ int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_
  * N up to 2^26.
  *
  * kad_quantize_weight: w [N, K] (bf16, fp16 or fp32, rows at stride ldw); a group's
- * scale is the smallest with amax <= 7 * scale, the codes w / scale to the nearest,
+ * scale is the smallest with amax <= 7 * scale (1 for zeros), the codes w / scale to the nearest,
  * ties to the even code, at most 6; a group with an infinity or NaN gets the NaN scale.
  * kad_dequantize_weight: the values, rounded to the type of out. */
 int kad_quantize_weight(const void* w, int64_t ldw, int dtype, void* codes, void* scales, int N,

@@ -5,8 +5,10 @@
 //
 // The weight's values are exact in bf16 and go to v_mfma_f32_16x16x32_bf16 as they
 // are; what x has more bits than bf16 goes as further products: x is the sum of
-// bf16 pieces, one for bf16, two for fp16 (11 bits) and three for fp32 (24 bits),
-// each the leading bits of what is left, so the sum is x itself.  Sums are fp32 and
+// bf16 pieces, two for fp16 (11 bits) and three for fp32 (24 bits), each the leading
+// bits of what is left, so the sum is x itself.  With scales from 2^-15 to 1 the weight's
+// values are exact in fp16 too, and rows of fp16 go to v_mfma_f32_16x16x32_f16 as they are,
+// in pieces only where a block of 128 columns has another scale.  Sums are fp32 and
 // are rounded once, with the residual added.  The gated product h is rounded to one
 // bf16 piece for bf16 x (2^-8, as the model's own activation), else to as many
 // pieces as x has: 2^-15 for fp16, whose range h may leave, and 2^-22 for fp32.
@@ -21,6 +23,9 @@ using namespace kad_q4;
 
 template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 2;
 template <> constexpr int kPieces<bf16_t> = 1;
+
+// what the kernel of many rows reads of x: rows of 16 bits as they are, fp32 in pieces
+template <typename T> constexpr int kPlanes = sizeof(T) == 2 ? 1 : kPieces<T>;
 
 // f as the sum of P bf16 pieces, the leading 8 bits each time (truncated, so that no
 // piece is infinite where f is finite) and the last one rounded.  Infinities and NaN
@@ -46,12 +51,12 @@ __device__ __forceinline__ void split(float f, bf16_t (&p)[P]) {
   }
 }
 
-// Rows of x as bf16 pieces [P][M][KP], zeros past column K.  8 elements a thread.
-template <typename T>
+// Rows of x as P bf16 pieces [P][M][KP], or (P = 1) rows of 16 bits as they are; zeros past
+// column K.  8 elements a thread.
+template <typename T, int P>
 __global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ x, int64_t ldx,
-                                                         bf16_t* __restrict__ out, int M, int K,
+                                                         uint16_t* __restrict__ out, int M, int K,
                                                          int KP) {
-  constexpr int P = kPieces<T>;
   const int per_row = KP / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t m = i / per_row;
@@ -60,9 +65,10 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ x
   uint32_t w[P][4];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float f = k + e < K ? Elem<T>::to_f(x[m * ldx + k + e]) : 0.f;
-    bf16_t p[P];
-    split<P>(f, p);
+    const T v = k + e < K ? x[m * ldx + k + e] : T(0);
+    uint16_t p[P];
+    if constexpr (P == 1) p[0] = __builtin_bit_cast(uint16_t, v);
+    else split<P>(Elem<T>::to_f(v), p);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       if (e & 1) w[j][e / 2] |= (uint32_t)p[j] << 16;
@@ -96,6 +102,20 @@ __device__ __forceinline__ bf16x8 operand(uint32_t codes, float scale) {
   const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
   const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// the same in fp16, for scales from 2^-15 to 1
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f16x8 operand_f16(uint32_t codes, float scale) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3);
+  return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 template <typename T>
@@ -147,8 +167,21 @@ struct Codes {
   u32x4 c[NW];
   uint32_t s[NW];  // a row's scales of the block's four groups
 };
+__device__ __forceinline__ float scale_of(uint32_t s, int j) {
+  return __uint_as_float((s >> (8 * j) & 255u) << 23);
+}
 __device__ __forceinline__ bf16x8 operand(u32x4 c, uint32_t s, int j) {
-  return operand(c[j], __uint_as_float((s >> (8 * j) & 255u) << 23));
+  return operand(c[j], scale_of(s, j));
+}
+// nonzero where a word of scales has one that is not from 2^-15 to 1
+__device__ __forceinline__ uint32_t not_f16(uint32_t s) { return (s & 0xf0f0f0f0u) ^ 0x70707070u; }
+// whether fp16 holds a block's values: the same for all lanes
+template <int NW>
+__device__ __forceinline__ bool fits_f16(const Codes<NW>& f) {
+  uint32_t other = 0;
+#pragma unroll
+  for (int n = 0; n < NW; ++n) other |= not_f16(f.s[n]);
+  return !__any(other != 0);
 }
 
 // The row blocks' codes and scales, by their first block of 128 columns.
@@ -156,6 +189,17 @@ template <int NW>
 struct Source {
   const uint8_t* c[NW];
   const uint8_t* s[NW];
+  // whether fp16 holds the values of all KB blocks of columns
+  __device__ __forceinline__ bool fits_f16(int KB, int lane) const {
+    uint32_t other = 0;
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+      for (int i = lane; i < KB * 4; i += 64) {
+        const u32x4 v = ((const u32x4*)s[n])[i];
+        other |= not_f16(v[0]) | not_f16(v[1]) | not_f16(v[2]) | not_f16(v[3]);
+      }
+    return !__any(other != 0);
+  }
   __device__ __forceinline__ void load(Codes<NW>& f, int kb, int lane) const {
 #pragma unroll
     for (int n = 0; n < NW; ++n) {
@@ -225,6 +269,7 @@ __device__ __forceinline__ void pieces_of(const u32x4 (&v)[sizeof(T) / 2],
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R>
 __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NW = W * NT;
+  constexpr bool HALF = RAW && std::is_same_v<T, _Float16>;
   // a block's rows: planes (the pieces) of 16 MT rows of RB bytes, loaded L x 1 KB a tile
   constexpr int PLANES = RAW ? 1 : P, RB = RAW ? 128 * (int)sizeof(T) : 256;
   constexpr int CPR = RB / 16, RPI = 64 / CPR, L = R / RPI;
@@ -277,6 +322,24 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
           const int r = t * RPI + lane / CPR;
           *(u32x4*)(own + ((p * MT + i) * R + r) * RB + (chunk ^ r) * 16) = b.x[p][i][t];
         }
+    if constexpr (HALF) {
+      if (__builtin_expect(fits_f16(b.w), true)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f16x8 xf[MT];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            xf[i] = *(const f16x8*)(own + (i * R + rr) * RB + ((j * 4 + fq) ^ rr) * 16);
+#pragma unroll
+          for (int n = 0; n < NW; ++n) {
+            const f16x8 wf = operand_f16(b.w.c[n][j], scale_of(b.w.s[n], j));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[n][i] = mfma_f16(wf, xf[i], acc[n][i]);
+          }
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       bf16x8 xf[MT][P];
@@ -373,9 +436,10 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 // BK columns, and each of the waves NW row blocks of the weight (gated: half of them the
 // gate's), whose codes it reads by itself, D - 1 blocks of 128 ahead.  A ring of SLOTS slices
 // is filled by direct loads.
-template <typename T, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+// HALF: x is rows of fp16, else pieces.
+template <typename T, bool HALF, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int ntiles) {
-  constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NT = NW / W;
+  constexpr int P = HALF ? 1 : kPieces<T>, W = GATED ? 2 : 1, NT = NW / W;
   constexpr int BM = 16 * MT, GROUP = 8;
   constexpr int CPR = BK / 8, RPI = 64 / CPR;  // chunks of 8 in a slice row, rows a load
   constexpr int LPW = BM / RPI / 4;            // loads per wave and slice
@@ -430,6 +494,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
   for (int d = 0; d < D - 1; ++d) w.load(codes[d], min(d, a.KB - 1), lane);
 #pragma unroll
   for (int t = 0; t < AHEAD; ++t) issue(0, t);
+  const bool fits = HALF && w.fits_f16(a.KB, lane);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   bf16x8 frags[PIPE ? 2 : 1][STEPS][MT];
   auto read = [&](bf16x8 (&f)[STEPS][MT], int at) {
@@ -445,44 +510,77 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
     asm volatile("" ::: "memory");
     read(frags[0], 0);
   }
-  for (int kb0 = 0; kb0 < a.KB; kb0 += D) {
+  // F16: the row blocks' values are all fp16's, and the rows multiply as they are
+  auto walk = [&](auto f16) {
+    constexpr bool F16 = decltype(f16)::value;
+    auto made = [&](const Codes<NW>& f, int j, int n) {
+      if constexpr (F16) return operand_f16(f.c[n][j], scale_of(f.s[n], j));
+      else return operand(f.c[n], f.s[n], j);
+    };
+    for (int kb0 = 0; kb0 < a.KB; kb0 += D) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int kb = kb0 + d;
-      if (kb >= a.KB) break;
+      for (int d = 0; d < D; ++d) {
+        const int kb = kb0 + d;
+        if (kb >= a.KB) break;
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h)
+        for (int h = 0; h < HALVES; ++h)
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const int t = (d * HALVES + h) * P + p, set = PIPE ? t % 2 : 0;
-          // PIPE: the next slice has landed (later ones may be in flight), and every wave
-          // has this one in registers, so its slot takes the slice SLOTS ahead.  Else: this
-          // slice has landed, and every wave has read the one before.
-          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(LATER) : "memory");
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
-          if (h == 0 && p == 0)
-            w.load(codes[(d + D - 1) % D], min(kb + D - 1, a.KB - 1), lane);
-          if constexpr (PIPE) read(frags[set ^ 1], (t + 1) % SLOTS);
-          issue(kb0, t + AHEAD);
-          if constexpr (!PIPE) read(frags[0], t % SLOTS);
-          // the next row block's operand is made among the products of the present one: a
-          // conversion right before the product that reads it holds up the matrix unit
-          bf16x8 wf = operand(codes[d].c[0], codes[d].s[0], h * STEPS);
+          for (int p = 0; p < P; ++p) {
+            const int t = (d * HALVES + h) * P + p, set = PIPE ? t % 2 : 0;
+            // PIPE: the next slice has landed (later ones may be in flight), and every wave
+            // has this one in registers, so its slot takes the slice SLOTS ahead.  Else: this
+            // slice has landed, and every wave has read the one before.
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(LATER) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (h == 0 && p == 0)
+              w.load(codes[(d + D - 1) % D], min(kb + D - 1, a.KB - 1), lane);
+            if constexpr (PIPE) read(frags[set ^ 1], (t + 1) % SLOTS);
+            issue(kb0, t + AHEAD);
+            if constexpr (!PIPE) read(frags[0], t % SLOTS);
+            if constexpr (HALF && !F16) {
 #pragma unroll
-          for (int jn = 0; jn < STEPS * NW; ++jn) {
-            const int j = jn / NW, n = jn % NW, jl = (jn + 1) / NW, nl = (jn + 1) % NW;
-            bf16x8 ahead = wf;
-            if (jn + 1 < STEPS * NW)
-              ahead = operand(codes[d].c[nl], codes[d].s[nl], h * STEPS + jl);
+              for (int j = 0; j < STEPS; ++j)
 #pragma unroll
-            for (int i = 0; i < MT; ++i) acc[n][i] = mfma16x16x32(wf, frags[set][j][i], acc[n][i]);
-            wf = ahead;
+                for (int i = 0; i < MT; ++i) {
+                  bf16x8 xf[kPieces<T>];
+                  pieces_of<T>({__builtin_bit_cast(u32x4, frags[set][j][i])}, xf);
+#pragma unroll
+                  for (int n = 0; n < NW; ++n)
+#pragma unroll
+                    for (int q = 0; q < kPieces<T>; ++q)
+                      acc[n][i] = mfma16x16x32(made(codes[d], h * STEPS + j, n), xf[q], acc[n][i]);
+                  __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
+                }
+            } else {
+              // the next row block's operand is made among the products of the present one:
+              // a conversion right before the product that reads it holds up the matrix unit
+              auto wf = made(codes[d], h * STEPS, 0);
+#pragma unroll
+              for (int jn = 0; jn < STEPS * NW; ++jn) {
+                const int j = jn / NW, n = jn % NW;
+                auto ahead = wf;
+                if (jn + 1 < STEPS * NW)
+                  ahead = made(codes[d], h * STEPS + (jn + 1) / NW, (jn + 1) % NW);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                  if constexpr (F16)
+                    acc[n][i] =
+                        mfma_f16(wf, __builtin_bit_cast(f16x8, frags[set][j][i]), acc[n][i]);
+                  else
+                    acc[n][i] = mfma16x16x32(wf, frags[set][j][i], acc[n][i]);
+                }
+                wf = ahead;
+              }
+            }
+            if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
           }
-          if constexpr (PIPE) __builtin_amdgcn_sched_barrier(0);
-        }
+      }
     }
-  }
+  };
+  // (every wave waits at the same barriers, whichever walk it takes)
+  if (HALF && fits) walk(std::integral_constant<bool, HALF>{});
+  else walk(std::integral_constant<bool, false>{});
   // no load may land in LDS that is another workgroup's by then
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -500,7 +598,7 @@ int64_t pad128(int64_t k) { return kad_cdiv(k, 128) * 128; }
 
 template <typename T>
 bool in_place(const void* x, int64_t ldx, int K) {
-  return kPieces<T> == 1 && K % 128 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0;
+  return sizeof(T) == 2 && K % 128 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0;
 }
 
 // Which kernel and tile.  n: rows of the weights in all (gated: the gate's and the up's).
@@ -524,7 +622,6 @@ bool in_place(const void* x, int64_t ldx, int K) {
 //   1024 x 8192 x 8192                        175   | 140    122    107    120
 //   32 x 100000 x 1024                  21.4   20.2 |  19.6   25     19.4   30
 //   1024 x 32768 x 1024                       110   |  99     87     70     66
-template <typename T>
 bool few(int64_t M, int64_t n) {
   return M <= 32 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 640;
 }
@@ -532,7 +629,7 @@ bool few(int64_t M, int64_t n) {
 // bytes of the rows' pieces; 0 where the rows are read as they are
 template <typename T>
 int64_t piece_bytes(const void* x, int64_t ldx, int64_t M, int64_t n, int K) {
-  return few<T>(M, n) || in_place<T>(x, ldx, K) ? 0 : kPieces<T> * M * pad128(K) * 2;
+  return few(M, n) || in_place<T>(x, ldx, K) ? 0 : kPlanes<T> * M * pad128(K) * 2;
 }
 
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R = 16>
@@ -542,18 +639,18 @@ void launch_stream(const Args& a, hipStream_t s) {
                      s, a);
 }
 
-template <typename T, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+template <typename T, bool HALF, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 void launch_tile(const Args& a, hipStream_t s) {
   const int64_t mtiles = kad_cdiv(a.M, 16 * MT);
   const int64_t ntiles = kad_cdiv(a.cols, 64 * NW / (GATED ? 2 : 1));
-  hipLaunchKernelGGL((q4_tile_kernel<T, GATED, MT, NW, BK, SLOTS, D>),
+  hipLaunchKernelGGL((q4_tile_kernel<T, HALF, GATED, MT, NW, BK, SLOTS, D>),
                      dim3((unsigned)(mtiles * ntiles)), dim3(256), 0, s, a, (int)mtiles,
                      (int)ntiles);
 }
 
 template <typename T, bool RAW, bool GATED>
 void stream(const Args& a, hipStream_t s) {
-  constexpr int W = GATED ? 2 : 1, P = kPieces<T>;
+  constexpr int W = GATED ? 2 : 1, P = RAW && sizeof(T) == 2 ? 1 : kPieces<T>;
   const int64_t tiles = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
   // 8 waves share K from 12 blocks of it on (16 x 1024 x 1536 fp32: 4.9 us, 4 waves 5.5;
   // 16 x 2048 x 16384: 12.9 and 14.3; 1 x 1024 x 1024, 8 blocks: 2.9 and 2.2)
@@ -589,44 +686,44 @@ void stream(const Args& a, hipStream_t s) {
   return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 3 ? 1 : 2>(a, s);
 }
 
-template <typename T, bool GATED>
+template <typename T, bool HALF, bool GATED>
 void tiles(const Args& a, hipStream_t s) {
-  constexpr int P = kPieces<T>;
+  constexpr int P = HALF ? 1 : kPieces<T>;
   const int64_t n = (int64_t)a.cols * (GATED ? 2 : 1);
   auto count = [&](int rows, int cols) { return kad_cdiv(a.M, rows) * kad_cdiv(n, cols); };
-  if (count(32, 128) <= 512) return launch_tile<T, GATED, 2, 2, 128, 4, 4>(a, s);
-  if (count(64, 128) <= 512) return launch_tile<T, GATED, 4, 2, 128, 4, P == 2 ? 2 : 4>(a, s);
+  if (count(32, 128) <= 512) return launch_tile<T, HALF, GATED, 2, 2, 128, 4, 4>(a, s);
+  if (count(64, 128) <= 512) return launch_tile<T, HALF, GATED, 4, 2, HALF ? 64 : 128, 4, HALF || P == 2 ? 2 : 4>(a, s);
   // Two of the largest tiles run on a CU at a time, and take twice as long as four of half
   // the size, or somewhat less: the larger ones where that halves the rounds (192 x
   // 100000 x 1024, 2 rounds against 3: 61.9 us, smaller 54.0; 256 rows, 2 against 4: 63.5 and 65.9).
   // fp16 and fp32 rows have no registers for them.
   if constexpr (kPieces<T> == 1)
     if (2 * kad_cdiv(count(128, 256), 512) <= kad_cdiv(count(64, 256), 512))
-      return launch_tile<T, GATED, 8, 4, 64, 4, 2>(a, s);
-  return launch_tile<T, GATED, 4, 4, 64, 4, 2>(a, s);
+      return launch_tile<T, HALF, GATED, 8, 4, 64, 4, 2>(a, s);
+  return launch_tile<T, HALF, GATED, 4, 4, 64, 4, 2>(a, s);
 }
 
 // a product of the rows x as they are, or of their pieces in `ws`
 template <typename T, bool GATED>
 void multiply(Args a, const void* x, int64_t ldx, void* ws, hipStream_t s) {
   a.x = x, a.ldx = ldx, a.xp = 0;
-  if (few<T>(a.M, (int64_t)a.cols * (GATED ? 2 : 1))) return stream<T, true, GATED>(a, s);
+  if (few(a.M, (int64_t)a.cols * (GATED ? 2 : 1))) return stream<T, true, GATED>(a, s);
   if (!in_place<T>(x, ldx, a.K)) {
     const int KP = (int)pad128(a.K);
     a.x = ws, a.ldx = KP, a.xp = (int64_t)a.M * KP;
-    hipLaunchKernelGGL((split_rows_kernel<T>),
+    hipLaunchKernelGGL((split_rows_kernel<T, kPlanes<T>>),
                        dim3((unsigned)kad_cdiv((int64_t)a.M * (KP / 8), 256)), dim3(256), 0, s,
-                       (const T*)x, ldx, (bf16_t*)ws, a.M, a.K, KP);
+                       (const T*)x, ldx, (uint16_t*)ws, a.M, a.K, KP);
   }
-  tiles<T, GATED>(a, s);
+  tiles<T, std::is_same_v<T, _Float16>, GATED>(a, s);
 }
 
 // the same of rows that are pieces already, padded to whole blocks
 template <typename T>
 void multiply_pieces(Args a, const bf16_t* x, hipStream_t s) {
   a.x = x, a.ldx = pad128(a.K), a.xp = a.M * a.ldx, a.K = (int)a.ldx;
-  if (few<T>(a.M, a.cols)) return stream<T, kPieces<T> == 1, false>(a, s);
-  tiles<T, false>(a, s);
+  if (few(a.M, a.cols)) return stream<T, kPieces<T> == 1, false>(a, s);
+  tiles<T, false, false>(a, s);
 }
 
 struct Weight {

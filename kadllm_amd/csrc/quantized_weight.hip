@@ -43,10 +43,12 @@ __device__ __forceinline__ void load8(const T* p, int left, float* f) {
 // The scale's byte of a group whose largest magnitude is amax: the smallest e in
 // [-100, 125] with amax <= 7 * 2^e.  Up to 7 the rounding of the largest element is
 // off by at most 2^e, half the step between 4 and 6; 125 keeps 6 * 2^e finite.
-// amax = 1.m * 2^x and 7 = 1.75 * 2^2.  255 (NaN) where amax is not finite.
+// amax = 1.m * 2^x and 7 = 1.75 * 2^2.  255 (NaN) where amax is not finite, and 2^0 for a
+// group of zeros (which the products take for a value like others').
 __device__ __forceinline__ uint32_t scale_byte(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   if (bits >= 0x7f800000u) return 255u;
+  if (bits == 0u) return 127u;
   const int e = (int)(bits >> 23) - 127 - 2 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return (uint32_t)(min(max(e, -100), 125) + 127);
 }

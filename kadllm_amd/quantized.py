@@ -111,7 +111,7 @@ class QuantizedWeight:
         pad = torch.nn.functional.pad
         codes = pad(codes, (0, kb * 64 - half, 0, nb * 16 - N))
         codes = codes.view(nb, 16, kb, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
-        scales = pad(scales, (0, kb * 4 - scales.shape[1], 0, nb * 16 - N), value=27)
+        scales = pad(scales, (0, kb * 4 - scales.shape[1], 0, nb * 16 - N), value=127)
         scales = scales.view(nb, 16, kb, 4).transpose(1, 2)
         return cls(codes.reshape(nb, kb, 64, 16), scales.contiguous().view(_SCALES), N, K)
 
@@ -153,7 +153,7 @@ def quantize_weight(weight):
     """``weight`` [N, K] (bf16, fp16 or fp32, any strides) in 4 bits.
 
     A group's scale is the smallest power of two s, from 2**-100 to 2**125, with amax <=
-    7 s; its codes are w / s to the nearest e2m1 value, ties to the even code, at
+    7 s (1 for a group of zeros); its codes are w / s to the nearest e2m1 value, ties to the even code, at
     most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s and s above.
     A group that holds an infinity or NaN reads as NaN.  Columns past K and rows past N
     of the padded arrays are zeros.  Returns a QuantizedWeight."""
@@ -224,7 +224,8 @@ def quantized_linear(x, weight, *, residual=None):
 
     x [..., K] bf16, fp16 or fp32 (any strides); residual [..., N] of x's type.
     Returns [..., N] in x's type.  Products are exact, sums are fp32 and are rounded
-    once, with the residual added."""
+    once, with the residual added.  fp16 rows take half as long where all scales are from
+    2**-15 to 1."""
     _check_weight(weight)
     rows, r = _check_rows(x, weight.cols, weight.rows, residual)
     _device_of(x, weight.codes, residual)

@@ -18,9 +18,9 @@ def values():
 
 
 def scale_exponent(amax):
-    """The smallest e in [-100, 125] with amax <= 7 * 2^e."""
+    """The smallest e in [-100, 125] with amax <= 7 * 2^e; 0 for zeros."""
     if amax == 0:
-        return -100
+        return 0
     frac, exp = math.frexp(amax)                    # frac in [1/2, 1)
     return min(max(exp - 3 + (frac > 7 / 8), -100), 125)
 

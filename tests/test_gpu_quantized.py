@@ -278,16 +278,42 @@ def test_linear_special_values(device, M, dtype):
     assert torch.equal(out[rest], clean[rest].double().cpu())
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("M", [1, 40, 300])
-def test_a_group_that_is_not_a_number(device, M):
+def test_a_group_that_is_not_a_number(device, M, dtype):
     w = _values((40, 200), 31)
     w[7, 50] = float("nan")
     w[20, 199] = float("inf")
     q = quantize_weight(w)
-    out = quantized_linear(_values((M, 200), 32, BF), q)
+    out = quantized_linear(_values((M, 200), 32, dtype), q)
     assert out[:, 7].isnan().all() and out[:, 20].isnan().all()
     rest = [n for n in range(40) if n not in (7, 20)]
     assert out[:, rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, N", [(1, 50), (4, 50), (5, 300), (40, 300), (700, 1900), (1100, 3000),
+                                  (1100, 5000), (4000, 8192)])
+def test_scales_of_every_size(device, M, N, dtype):
+    # most weights' scales are exact in fp16; here some groups' are far from it, in some row
+    # blocks and columns of all
+    K = 520
+    w = _values((N, K), 41) * 0.04
+    w[N // 3:N // 2, 130:250] *= 2.0 ** -25
+    w[-7:, :32] *= 2.0 ** -60
+    w[-1, 500:] *= 2.0 ** -100
+    x = _values((M, K), 42, dtype)
+    q = quantize_weight(w)
+    dense = dequantize_weight(q, F32).cpu().double()
+    _assert_large(quantized_linear(x, q), x, dense)
+    # tiny weights alone: only their own products may be off, and only by a sum's rounding
+    tiny = quantize_weight(w * 2.0 ** -25)
+    big = (_values((M, K), 43) * 2.0 ** 7).clamp(-60000, 60000).to(dtype)
+    _assert_large(quantized_linear(big, tiny), big, dequantize_weight(tiny, F32).cpu().double())
+    # and huge ones
+    huge = quantize_weight(w * 2.0 ** 20)
+    small = (x.float() * 2.0 ** -19).to(dtype)
+    _assert_large(quantized_linear(small, huge), small, dequantize_weight(huge, F32).cpu().double())
 
 
 # ----------------------------------------------------------------------------

@@ -34,7 +34,8 @@ def test_oracle_rounds_to_even_and_saturates():
     assert exps.tolist() == [[0]]
     assert ref.dense(codes, exps).tolist() == [[6, 4, 2, 2, 1, 1, 0, -4, 0.5, -6]]
     assert ref.quantize(torch.tensor([[7.001]]))[1].tolist() == [[1]]
-    assert ref.quantize(torch.zeros(1, 3))[1].tolist() == [[-100]]
+    assert ref.quantize(torch.zeros(1, 3))[1].tolist() == [[0]]
+    assert ref.quantize(torch.full((1, 3), 1e-40))[1].tolist() == [[-100]]
     assert ref.quantize(torch.tensor([[3e38]]))[1].tolist() == [[125]]
     assert ref.dense(*ref.quantize(torch.tensor([[1.0, float("inf")]]))).isnan().all()
 
