@@ -62,13 +62,19 @@ __global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ x
   const int64_t m = i / per_row;
   if (m >= M) return;
   const int k = (int)(i - m * per_row) * 8;
+  // one access, wherever the row begins; at its end the last 8, and the thread's own below
+  T v[8];
+  if (K >= 8) __builtin_memcpy(v, x + m * ldx + min(k, K - 8), sizeof(v));
+  if (k + 8 > K) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < K ? x[m * ldx + k + e] : T(0);
+  }
   uint32_t w[P][4];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const T v = k + e < K ? x[m * ldx + k + e] : T(0);
     uint16_t p[P];
-    if constexpr (P == 1) p[0] = __builtin_bit_cast(uint16_t, v);
-    else split<P>(Elem<T>::to_f(v), p);
+    if constexpr (P == 1) p[0] = __builtin_bit_cast(uint16_t, v[e]);
+    else split<P>(Elem<T>::to_f(v[e]), p);
 #pragma unroll
     for (int j = 0; j < P; ++j) {
       if (e & 1) w[j][e / 2] |= (uint32_t)p[j] << 16;
@@ -91,7 +97,6 @@ struct Args {
   int64_t ldy, yp;
   int M, N, K, KB;           // KB blocks of 128 columns
   int cols;                  // columns that are written: N, or (gated) N padded to 128
-  int vec;                   // 4 neighbours of y (and r) may go as one access
 };
 
 // a word of 8 codes times its group's scale, as an MFMA operand
@@ -124,9 +129,21 @@ __device__ __forceinline__ float silu_of(float g) {
   else return silu_f(g);
 }
 
+// The residual of outputs (m, n .. n + 3): loaded early, on no condition of the lane's, so
+// that the loads of a tile are in flight together.  (Lanes that have no whole four, at the
+// row's end or past it, read others' here and their own in finish.)
+template <typename T>
+struct Residual {
+  T v[4];
+  __device__ __forceinline__ void load(const Args& a, int m, int n) {
+    __builtin_memcpy(v, (const T*)a.r + min(m, a.M - 1) * a.ldr + min(n, a.N - 4), sizeof(v));
+  }
+};
+
 // Outputs (m, n .. n + 3) from their sums: s[0], or the gate's and the up's.
 template <typename T, bool GATED>
-__device__ __forceinline__ void finish(const Args& a, int m, int n, const f32x4* s) {
+__device__ __forceinline__ void finish(const Args& a, int m, int n, const f32x4* s,
+                                       const Residual<T>& res) {
   if (m >= a.M || n >= a.cols) return;
   if constexpr (GATED) {
     constexpr int P = kPieces<T>;
@@ -140,26 +157,36 @@ __device__ __forceinline__ void finish(const Args& a, int m, int n, const f32x4*
           u32x2{p[0][j] | (uint32_t)p[1][j] << 16, p[2][j] | (uint32_t)p[3][j] << 16};
   } else {
     T* y = (T*)a.y + m * a.ldy + n;
-    const T* r = (const T*)a.r + (a.r ? m * a.ldr + n : 0);
-    if (a.vec) {
-      typedef T vec4 __attribute__((ext_vector_type(4)));
-      f32x4 f = s[0];
-      if (a.r) {
-        const vec4 v = *(const vec4*)r;
+    if (n + 4 <= a.N) {  // one access, wherever it begins
+      T v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] += Elem<T>::to_f(v[i]);
-      }
-      vec4 o;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = Elem<T>::from_f(f[i]);
-      *(vec4*)y = o;
+      for (int i = 0; i < 4; ++i)
+        v[i] = Elem<T>::from_f(a.r ? s[0][i] + Elem<T>::to_f(res.v[i]) : s[0][i]);
+      __builtin_memcpy(y, v, sizeof(v));
     } else {
+      const T* r = (const T*)a.r + (a.r ? m * a.ldr + n : 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (n + i < a.N) y[i] = Elem<T>::from_f(a.r ? s[0][i] + Elem<T>::to_f(r[i]) : s[0][i]);
     }
   }
 }
+
+// A lane of the product has 4 neighbours of a row of its own, so what a wave stores at once
+// would lie in 16 rows.  NT tiles of sums (16 rows x 16 columns, side by side) change places
+// through LDS first: taken lane by lane they are 16 / NT whole rows of 16 NT columns a time.
+// Neither side has bank conflicts.
+template <int NT>
+struct Sums {
+  static __device__ __forceinline__ int slot(int tile, int row, int quad) {
+    return tile * 64 + quad * 16 + (row ^ (quad * 4 + tile * (4 / NT)));
+  }
+  // the q-th of 64 NT quads of columns, rows first
+  int tile, row, quad;
+  __device__ __forceinline__ explicit Sums(int q)
+      : tile(q % (4 * NT) / 4), row(q / (4 * NT)), quad(q % 4) {}
+  __device__ __forceinline__ int slot() const { return slot(tile, row, quad); }
+};
 
 // A wave's blocks of 128 columns: codes and scales of NW row blocks of the weight(s).
 template <int NW>
@@ -286,6 +313,17 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   for (int n = 0; n < NW; ++n)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[n][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the wave's share of y: quads of columns t * 64 + lane of the row tiles, t = wave, wave + KS, ..
+  constexpr int kShare = (NT * MT + KS - 1) / KS;
+  Residual<T> res[kShare];
+  if (!GATED && a.r && a.N >= 4) {
+#pragma unroll
+    for (int u = 0; u < kShare; ++u) {
+      const int t = u * KS + wave;
+      const Sums<NT> at(t % NT * 64 + lane);
+      res[u].load(a, m0 + t / NT * 16 + at.row, (nt + at.tile) * 16 + at.quad * 4);
+    }
+  }
   const Source<NW> src = source<NW, W>(a, nt);
   constexpr int kItem = RAW ? sizeof(T) : 2;
   const int chunk = lane % CPR;
@@ -409,24 +447,28 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
     }
   }
   // a wave's sums take the place of its rows
-  auto sums = [&](int k) { return (f32x4*)(lds + k * kWave) + lane; };
+  auto sums = [&](int k, int w, int i) {
+    return (f32x4*)(lds + k * kWave) + (i * NW + w * NT) * 64;
+  };
 #pragma unroll
   for (int n = 0; n < NW; ++n)
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sums(wave)[(n * MT + i) * 64] = acc[n][i];
+    for (int i = 0; i < MT; ++i)
+      sums(wave, n / NT, i)[Sums<NT>::slot(n % NT, fr, fq)] = acc[n][i];
   __syncthreads();
-  // tile t of y by wave t % KS
 #pragma unroll
-  for (int t = 0; t < NT * MT; ++t) {
-    if (t % KS != wave) continue;
+  for (int u = 0; u < kShare; ++u) {
+    const int t = u * KS + wave;
+    if (t >= NT * MT) break;
+    const Sums<NT> at(t % NT * 64 + lane);
     f32x4 s[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      s[w] = sums(0)[(w * NT * MT + t) * 64];
+      s[w] = sums(0, w, t / NT)[at.slot()];
 #pragma unroll
-      for (int k = 1; k < KS; ++k) s[w] += sums(k)[(w * NT * MT + t) * 64];
+      for (int k = 1; k < KS; ++k) s[w] += sums(k, w, t / NT)[at.slot()];
     }
-    finish<T, GATED>(a, m0 + t % MT * 16 + fr, (nt + t / MT) * 16 + fq * 4, s);
+    finish<T, GATED>(a, m0 + t / NT * 16 + at.row, (nt + at.tile) * 16 + at.quad * 4, s, res[u]);
   }
 }
 
@@ -581,17 +623,36 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
   // (every wave waits at the same barriers, whichever walk it takes)
   if (HALF && fits) walk(std::integral_constant<bool, HALF>{});
   else walk(std::integral_constant<bool, false>{});
-  // no load may land in LDS that is another workgroup's by then
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  Residual<T> res[MT][NT];
+  if (!GATED && a.r && a.N >= 4) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const Sums<NT> at(t * 64 + lane);
+        res[i][t].load(a, m0 + i * 16 + at.row, (nt + at.tile) * 16 + at.quad * 4);
+      }
+  }
+  // the ring is free once every wave's loads have landed and been read
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  static_assert(sizeof(ring) >= 4 * 2 * NW * 1024, "two row tiles' sums a wave");
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    f32x4* sums = (f32x4*)ring + (wave * 2 + i % 2) * NW * 64;
+#pragma unroll
+    for (int n = 0; n < NW; ++n)
+      sums[n / NT * NT * 64 + Sums<NT>::slot(n % NT, fr, fq)] = acc[n][i];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      const Sums<NT> at(t * 64 + lane);
       f32x4 s[W];
 #pragma unroll
-      for (int v = 0; v < W; ++v) s[v] = acc[v * NT + t][i];
-      finish<T, GATED>(a, m0 + i * 16 + fr, (nt + t) * 16 + fq * 4, s);
+      for (int v = 0; v < W; ++v) s[v] = sums[v * NT * 64 + at.slot()];
+      finish<T, GATED>(a, m0 + i * 16 + at.row, (nt + at.tile) * 16 + at.quad * 4, s, res[i][t]);
     }
+  }
 }
 
 int64_t pad128(int64_t k) { return kad_cdiv(k, 128) * 128; }
@@ -683,7 +744,9 @@ void stream(const Args& a, hipStream_t s) {
   // and 10.1)
   if (a.M <= 16 || tiles * kad_cdiv(n, 64) <= (P > 1 ? 512 : 320))
     return rows(std::integral_constant<int, 16>{});
-  return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 3 ? 1 : 2>(a, s);
+  // (pieces two blocks ahead leave registers for one workgroup a CU: fp16 block of 600 x 1024 x
+  // 1024, one ahead 18.3 us, two 22.2)
+  return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 1 ? 2 : 1>(a, s);
 }
 
 template <typename T, bool HALF, bool GATED>
@@ -738,9 +801,6 @@ Args linear(Weight w, const void* r, int64_t ldr, void* y, int64_t ldy, int M, i
   a.scales[0] = a.scales[1] = (const uint8_t*)w.scales;
   a.r = r, a.ldr = ldr, a.y = y, a.ldy = ldy, a.yp = 0;
   a.M = M, a.N = N, a.K = K, a.KB = (int)kad_cdiv(K, 128), a.cols = N;
-  const int bytes = 4 * (int)sizeof(T);
-  a.vec = N % 4 == 0 && (uintptr_t)y % bytes == 0 && ldy % 4 == 0 &&
-          (!r || ((uintptr_t)r % bytes == 0 && ldr % 4 == 0));
   return a;
 }
 
@@ -749,7 +809,7 @@ Args gated(Weight g, Weight u, bf16_t* h, int M, int F, int K) {
   a.codes[0] = (const uint8_t*)g.codes, a.codes[1] = (const uint8_t*)u.codes;
   a.scales[0] = (const uint8_t*)g.scales, a.scales[1] = (const uint8_t*)u.scales;
   a.r = nullptr, a.ldr = 0, a.y = h, a.ldy = pad128(F), a.yp = M * pad128(F);
-  a.M = M, a.N = F, a.K = K, a.KB = (int)kad_cdiv(K, 128), a.cols = (int)pad128(F), a.vec = 1;
+  a.M = M, a.N = F, a.K = K, a.KB = (int)kad_cdiv(K, 128), a.cols = (int)pad128(F);
   return a;
 }
 

@@ -17,29 +17,6 @@ namespace {
 
 using namespace kad_q4;
 
-// 8 neighbours of a row as floats; zeros past the row's end
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int left, float* f) {
-  if (VEC && left >= 8) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const f32x4 x = *(const f32x4*)(p + 4 * v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[4 * v + i] = x[i];
-      }
-    } else {
-      typedef T vec8 __attribute__((ext_vector_type(8)));
-      const vec8 x = *(const vec8*)p;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f(x[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? Elem<T>::to_f(p[i]) : 0.f;
-  }
-}
-
 // The scale's byte of a group whose largest magnitude is amax: the smallest e in
 // [-100, 125] with amax <= 7 * 2^e.  Up to 7 the rounding of the largest element is
 // off by at most 2^e, half the step between 4 and 6; 125 keeps 6 * 2^e finite.
@@ -58,101 +35,108 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return (__float_as_uint(a) > __float_as_uint(b)) ? a : b;  // (non-negative or NaN)
 }
 
-// One workgroup takes 16 rows and 512 columns: a wave 4 rows, 16 lanes a row and
-// block of 128, so that a load instruction reads 4 whole runs of 16 x 8 elements.  A
-// group is 4 lanes.  Everything is loaded before the first use.
-template <typename T, bool VEC>
+// One workgroup takes 4 blocks of 16 rows and 128 columns, in a row of blocks' order: a wave
+// 4 rows, 16 lanes a row, so that a load instruction reads 4 whole runs of 16 x 8 elements.
+// A group is 4 lanes.  Everything is loaded before the first use.
+template <typename T>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ w, int64_t ldw,
                                                               uint8_t* __restrict__ codes,
                                                               uint8_t* __restrict__ scales, int N,
                                                               int K, int KB) {
   const int lane = threadIdx.x & 63, r = (threadIdx.x >> 6) * 4 + (lane >> 4), c = lane & 15;
-  const int K4 = (KB + 3) / 4;
-  const int64_t nb = blockIdx.x / K4;
-  const int k4 = (int)(blockIdx.x - nb * K4);
-  const int64_t row = nb * 16 + r;
-  float f[4][8];
+  const int NB = (N + 15) / 16;
+  int nb[4], kb[4], left[4];
+  const T* row[4];
+  T v[4][8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int k = (k4 * 4 + j) * 128 + c * 8;
-    if (row < N && k < K) {
-      load8<T, VEC>(w + row * ldw + k, K - k, f[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[j][i] = 0.f;
-    }
+    const uint32_t b = blockIdx.x * 4 + j;
+    nb[j] = (int)(b / (uint32_t)KB), kb[j] = (int)(b - (uint32_t)nb[j] * (uint32_t)KB);
+    const int n = nb[j] * 16 + r;
+    row[j] = w + min(n, N - 1) * ldw;
+    left[j] = n < N ? K - (kb[j] * 128 + c * 8) : 0;
   }
+  // one access, wherever it begins, and on no condition of the lane's, so that the four go
+  // out together; lanes at the row's end read its last 8, and their own below
+  if (K >= 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      __builtin_memcpy(v[j], row[j] + min(kb[j] * 128 + c * 8, K - 8), sizeof(v[j]));
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (left[j] < 8) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = i < left[j] ? row[j][K - left[j] + i] : T(0);
+    }
   const int at = ((c & 3) * 16 + r) * 16 + (c >> 2) * 4;  // of the codes' word in its block
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int kb = k4 * 4 + j;
-    float amax = 0.f;
+    float f[8], amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(f[j][i]));
+    for (int i = 0; i < 8; ++i) {
+      f[i] = Elem<T>::to_f(v[j][i]);
+      amax = max_nan(amax, fabsf(f[i]));
+    }
     amax = max_nan(amax, __shfl_xor(amax, 1, 64));
     amax = max_nan(amax, __shfl_xor(amax, 2, 64));
     const uint32_t s = scale_byte(amax);
-    if (kb < KB) {
+    if (nb[j] < NB) {
+      const int64_t block = (int64_t)nb[j] * KB + kb[j];
       uint32_t code = 0;
       const float scale = __uint_as_float(s << 23);
       if (s != 255u) {
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][0], f[j][1], scale, 0);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][2], f[j][3], scale, 1);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][4], f[j][5], scale, 2);
-        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[j][6], f[j][7], scale, 3);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[0], f[1], scale, 0);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[2], f[3], scale, 1);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[4], f[5], scale, 2);
+        code = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(code, f[6], f[7], scale, 3);
       }
-      *(uint32_t*)(codes + (nb * KB + kb) * 1024 + at) = code;
-      if ((c & 3) == 0) scales[(nb * KB + kb) * 64 + r * 4 + (c >> 2)] = (uint8_t)s;
+      *(uint32_t*)(codes + block * 1024 + at) = code;
+      if ((c & 3) == 0) scales[block * 64 + r * 4 + (c >> 2)] = (uint8_t)s;
     }
   }
 }
 
 // The same split the other way.
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void dequantize_weight_kernel(
     const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
     int64_t ldo, int N, int K, int KB) {
   const int lane = threadIdx.x & 63, r = (threadIdx.x >> 6) * 4 + (lane >> 4), c = lane & 15;
-  const int K4 = (KB + 3) / 4;
-  const int64_t nb = blockIdx.x / K4;
-  const int k4 = (int)(blockIdx.x - nb * K4);
-  const int64_t row = nb * 16 + r;
-  if (row >= N) return;
+  const int NB = (N + 15) / 16;
   const int at = ((c & 3) * 16 + r) * 16 + (c >> 2) * 4;
+  int nb[4], kb[4];
   uint32_t code[4], byte[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int kb = min(k4 * 4 + j, KB - 1);
-    code[j] = *(const uint32_t*)(codes + (nb * KB + kb) * 1024 + at);
-    byte[j] = scales[(nb * KB + kb) * 64 + r * 4 + (c >> 2)];
+    const uint32_t b = blockIdx.x * 4 + j;
+    nb[j] = (int)(b / (uint32_t)KB), kb[j] = (int)(b - (uint32_t)nb[j] * (uint32_t)KB);
+    const int64_t block = (int64_t)min(nb[j], NB - 1) * KB + kb[j];
+    code[j] = *(const uint32_t*)(codes + block * 1024 + at);
+    byte[j] = scales[block * 64 + r * 4 + (c >> 2)];
   }
+  T y[4][8], *dst[4];
+  int left[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int k = (k4 * 4 + j) * 128 + c * 8;
-    if (k >= K) continue;
+    const int n = nb[j] * 16 + r, k = kb[j] * 128 + c * 8;
+    dst[j] = out + n * ldo + k;
+    left[j] = n < N ? K - k : 0;
     const float scale = scale_value(byte[j]);
     float f[8];
     codes_to_float(code[j], f);
-    T* dst = out + row * ldo + k;
-    T y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = Elem<T>::from_f(f[i] * scale);
-    if (VEC && K - k >= 8) {
-      u32x4 v[sizeof(T) / 2];
-      __builtin_memcpy(v, y, sizeof(y));
+    for (int i = 0; i < 8; ++i) y[j][i] = Elem<T>::from_f(f[i] * scale);
+    if (left[j] >= 8) __builtin_memcpy(dst[j], y[j], sizeof(y[j]));  // (wherever it begins)
+  }
+  // the rows' ends (beside the whole 8 the compiler would split those for what both store)
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((u32x4*)dst)[i] = v[i];
-    } else {
+  for (int j = 0; j < 4; ++j)
+    if (left[j] < 8) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < K - k) dst[i] = y[i];
+        if (i < left[j]) dst[j][i] = y[j][i];
     }
-  }
-}
-
-template <typename T>
-bool rows16(const T* p, int64_t ld) {
-  return (uintptr_t)p % 16 == 0 && ld * (int64_t)sizeof(T) % 16 == 0;
 }
 
 int check(const void* w, const void* codes, const void* scales, int N, int K, int64_t ld) {
@@ -163,34 +147,26 @@ int check(const void* w, const void* codes, const void* scales, int N, int K, in
   KAD_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0,
               "codes and scales must be 16-byte aligned");
   // (a grid holds fewer than 2^32 work-items a dimension)
-  KAD_REQUIRE(kad_cdiv(N, 16) * kad_cdiv(K, 512) < (1ll << 32) / 256, "too large a weight");
+  KAD_REQUIRE(kad_cdiv(N, 16) * kad_cdiv(K, 128) < (1ll << 26), "too large a weight");
   return KAD_OK;
 }
 
 template <typename T>
 void launch_quantize(const void* w, int64_t ldw, void* codes, void* scales, int N, int K,
                      hipStream_t s) {
-  const dim3 grid((unsigned)(kad_cdiv(N, 16) * kad_cdiv(K, 512)));
   const int KB = (int)kad_cdiv(K, 128);
-  if (rows16((const T*)w, ldw))
-    hipLaunchKernelGGL((quantize_weight_kernel<T, true>), grid, dim3(256), 0, s, (const T*)w, ldw,
-                       (uint8_t*)codes, (uint8_t*)scales, N, K, KB);
-  else
-    hipLaunchKernelGGL((quantize_weight_kernel<T, false>), grid, dim3(256), 0, s, (const T*)w, ldw,
-                       (uint8_t*)codes, (uint8_t*)scales, N, K, KB);
+  const dim3 grid((unsigned)kad_cdiv(kad_cdiv(N, 16) * KB, 4));
+  hipLaunchKernelGGL(quantize_weight_kernel<T>, grid, dim3(256), 0, s, (const T*)w, ldw,
+                     (uint8_t*)codes, (uint8_t*)scales, N, K, KB);
 }
 
 template <typename T>
 void launch_dequantize(const void* codes, const void* scales, void* out, int64_t ldo, int N, int K,
                        hipStream_t s) {
-  const dim3 grid((unsigned)(kad_cdiv(N, 16) * kad_cdiv(K, 512)));
   const int KB = (int)kad_cdiv(K, 128);
-  if (rows16((const T*)out, ldo))
-    hipLaunchKernelGGL((dequantize_weight_kernel<T, true>), grid, dim3(256), 0, s,
-                       (const uint8_t*)codes, (const uint8_t*)scales, (T*)out, ldo, N, K, KB);
-  else
-    hipLaunchKernelGGL((dequantize_weight_kernel<T, false>), grid, dim3(256), 0, s,
-                       (const uint8_t*)codes, (const uint8_t*)scales, (T*)out, ldo, N, K, KB);
+  const dim3 grid((unsigned)kad_cdiv(kad_cdiv(N, 16) * KB, 4));
+  hipLaunchKernelGGL(dequantize_weight_kernel<T>, grid, dim3(256), 0, s, (const uint8_t*)codes,
+                     (const uint8_t*)scales, (T*)out, ldo, N, K, KB);
 }
 
 }  // namespace

@@ -56,6 +56,17 @@ def test_quantize_and_read_back(device, N, K, dtype):
         assert torch.equal(dequantize_weight(q, out).cpu(), exact.to(out)), out
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("N, K", [(5, 2), (20, 7), (33, 8), (18, 9), (300, 131), (70, 260)])
+def test_quantize_rows_that_begin_anywhere(device, N, K, dtype):
+    # rows shorter and longer than what is loaded at once, each at another alignment
+    w = _values((N, K + 5), N + K, dtype)[:, 3:3 + K]
+    q = quantize_weight(w)
+    codes, exps = _check_parts(q, w)
+    exact = ref.dense(codes, exps)
+    assert torch.equal(dequantize_weight(q, dtype).cpu(), exact.to(dtype))
+
+
 def test_quantize_every_midpoint(device):
     # every code, every midpoint and its neighbours, for scales over the whole range
     a = torch.tensor([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7],
@@ -189,6 +200,18 @@ def test_many_rows_exactly(device, M, N, K, dtype):
     assert not out[M // 2].isfinite().any() and out[M - 1].isnan().all()
     rest = [m for m in range(M) if m not in (M // 2, M - 1)]
     assert torch.equal(out[rest], got[rest])
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, K", [(3, 40), (70, 200), (21000, 40)])
+@pytest.mark.parametrize("N", [1, 2, 3, 4, 5])
+def test_linear_of_few_columns(device, M, N, K, dtype):
+    # fewer columns than are stored at once; a residual inside a wider buffer, at an odd place
+    q, dense = _weight(N, K, M + N)
+    x = _values((M, K), K, dtype)
+    r = _values((M, N + 6), 7, dtype)[:, 3:3 + N]
+    _assert_large(quantized_linear(x, q, residual=r), x, dense, r)
+    _assert_large(quantized_linear(x, q), x, dense)
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
