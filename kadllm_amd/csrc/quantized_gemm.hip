@@ -666,25 +666,27 @@ bool in_place(const void* x, int64_t ldx, int K) {
 // While there is a CU for each workgroup (256) a call takes what one workgroup's walk over K
 // takes, so the smallest tile that needs no more wins; with many workgroups a CU, the
 // largest.  The kernel of few rows has tiles of up to 32 x 64 (rows x rows of the weights),
-// its largest up to 640 workgroups (300 x 4096 x 2048, 640 of them: bf16 12.2 us against the
-// other kernel's 12.3, fp16 17.4 and 21.4, fp32 27.2 and 28.2; 400 rows, 832: 15.3 and 12.7,
-// 23.1 and 22.4, 35 and 30), and takes up to 32 rows whatever the weight.  us, weights from
+// its largest up to 640 workgroups (32 x 30000 x 8192, 469 of them: bf16 39 us, the other
+// kernel 42, fp16 38 and 45, fp32 72 and 68; 300 x 4096 x 2048, 640: 12.5 and 12.7, 12.4 and
+// 13.3, 29 and 27; 32 x 50000 x 1024, 782: 12.8 and 11.1, 12.6 and 11.5, 24 and 18), and up
+// to 16 rows its tile of 16 x 64 whatever the weight (16 x 248320 x 1024: 33.4 us, of the
+// other kernel's 32.1 at best; fp16 33.6 and 36.4, fp32 46 and 54).  bf16, us, weights from
 // beyond the caches:
 //   M x N x K            16x16  16x32  16x64  32x64 | 32x128 64x128 64x256 128x256
-//   16 x 1024 x 3584       4.2    4.5    5.8
-//   64 x 1024 x 3584       4.4    4.6    5.8    8.9 |  13.5
-//   128 x 1024 x 3584      5.8    4.8    5.8    9.0 |  13.5
-//   256 x 1024 x 3584             6.9    5.8    8.9 |  13.5   19.3
-//   32 x 8192 x 8192             15.6   13.1   17   |  31     44
-//   64 x 8192 x 8192             21     20.2   17.3 |  31     44     70
-//   128 x 8192 x 8192                   31.2   28.1 |  31.6   45     70
-//   256 x 8192 x 8192                          47.4 |  43.1   45.2   70    116
-//   512 x 8192 x 8192                          93.5 |  76.9   66.3   73    118
-//   1024 x 8192 x 8192                        175   | 140    122    107    120
-//   32 x 100000 x 1024                  21.4   20.2 |  19.6   25     19.4   30
-//   1024 x 32768 x 1024                       110   |  99     87     70     66
+//   16 x 1024 x 3584       5.0    5.6    6.9    8.4 |  17     21     30      45
+//   128 x 1024 x 3584      7.5    5.4    6.4    8.9 |  17     22     31      47
+//   256 x 1024 x 3584     11.9    7.3    6.4    8.8 |  17     22     31      47
+//   32 x 8192 x 8192      26     16     13.2   17.9 |  36     44     65     106
+//   64 x 8192 x 8192      45     25     20.4   17.5 |  36     46     67     106
+//   128 x 8192 x 8192     85     43     33     29   |  37     46     66     108
+//   256 x 8192 x 8192    161     79     59     50   |  46     47     66     108
+//   512 x 8192 x 8192    307    158    112     89   |  81     64     70     108
+//   1024 x 8192 x 8192                        171   | 143    124    107     117
+//   32 x 100000 x 1024    98     38     25     20.8 |  19.8   23.5   19.4    28.6
+//   64 x 100000 x 1024   185     66     42     32   |  28.8   26.5   21.0    29.7
+//   1024 x 32768 x 1024                       115   | 100     89     69      62
 bool few(int64_t M, int64_t n) {
-  return M <= 32 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 640;
+  return M <= 16 || kad_cdiv(M, 32) * kad_cdiv(n, 64) <= 640;
 }
 
 // bytes of the rows' pieces; 0 where the rows are read as they are
@@ -711,6 +713,8 @@ void launch_tile(const Args& a, hipStream_t s) {
 
 template <typename T, bool RAW, bool GATED>
 void stream(const Args& a, hipStream_t s) {
+  // (P: the products a row block and step take; rows of fp16 are pieces in the second half of
+  // a feed-forward block alone)
   constexpr int W = GATED ? 2 : 1, P = RAW && sizeof(T) == 2 ? 1 : kPieces<T>;
   const int64_t tiles = kad_cdiv(a.M, 16), n = (int64_t)a.cols * W;
   // 8 waves share K from 12 blocks of it on (16 x 1024 x 1536 fp32: 4.9 us, 4 waves 5.5;
@@ -731,17 +735,16 @@ void stream(const Args& a, hipStream_t s) {
       if (wide) return launch_stream<T, RAW, GATED, 1, 2 / W, 8, 2, R>(a, s);
       return launch_stream<T, RAW, GATED, 1, 2 / W, 4, 2, R>(a, s);
     }
-    // one block ahead leaves registers for more waves (fp16 128 x 4096 x 4096: 13.9 us, 2
-    // ahead 16.7; fp32 has too few blocks in flight then: 128 x 2048 x 16384 45 and 39, and
-    // with 2 ahead no registers for a second workgroup: 300 x 1024 x 2048, 304 of them, 14.6
-    // us, of 4 waves 12)
+    // (fp32 rows, one block ahead, have too few in flight: 128 x 2048 x 16384 45 us, two ahead
+    // 39; and with two ahead no registers for a second workgroup: 300 x 1024 x 2048, 304 of
+    // them, 14.6 us, of 4 waves 12)
     if (wide && (P < 3 || tiles * kad_cdiv(n, 64) <= 256))
       return launch_stream<T, RAW, GATED, 1, 4 / W, 8, P == 3 ? 2 : 1, R>(a, s);
     return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2, R>(a, s);
   };
   if (a.M <= 4) return rows(std::integral_constant<int, 4>{});
-  // (128 x 4096 x 4096, 512 workgroups of 16 x 64: fp16 13.9 us, of 32 x 64 16.0; bf16 10.8
-  // and 10.1)
+  // (128 x 4096 x 4096, 512 workgroups of 16 x 64: fp32 21.3 us, of 32 x 64 25; bf16 10.3 and
+  // 9.7)
   if (a.M <= 16 || tiles * kad_cdiv(n, 64) <= (P > 1 ? 512 : 320))
     return rows(std::integral_constant<int, 16>{});
   // (pieces two blocks ahead leave registers for one workgroup a CU: fp16 block of 600 x 1024 x
@@ -754,12 +757,21 @@ void tiles(const Args& a, hipStream_t s) {
   constexpr int P = HALF ? 1 : kPieces<T>;
   const int64_t n = (int64_t)a.cols * (GATED ? 2 : 1);
   auto count = [&](int rows, int cols) { return kad_cdiv(a.M, rows) * kad_cdiv(n, cols); };
-  if (count(32, 128) <= 512) return launch_tile<T, HALF, GATED, 2, 2, 128, 4, 4>(a, s);
-  if (count(64, 128) <= 512) return launch_tile<T, HALF, GATED, 4, 2, HALF ? 64 : 128, 4, HALF || P == 2 ? 2 : 4>(a, s);
+  // up to two workgroups a CU, and up to 32 rows (32 x 248320 x 1024: bf16 35.3 us, 64 x 128
+  // 45.9, 64 x 256 36.9; fp32 61, 83 and 72)
+  if (count(32, 128) <= 512 || a.M <= 32)
+    return launch_tile<T, HALF, GATED, 2, 2, 128, 4, 4>(a, s);
+  // slices of 64 columns and fewer codes ahead where the pieces of fp16 rows leave no
+  // registers for more
+  if (count(64, 128) <= 512) {
+    constexpr int BK = HALF ? 64 : 128, D = HALF || P == 2 ? 2 : 4;
+    return launch_tile<T, HALF, GATED, 4, 2, BK, 4, D>(a, s);
+  }
   // Two of the largest tiles run on a CU at a time, and take twice as long as four of half
-  // the size, or somewhat less: the larger ones where that halves the rounds (192 x
-  // 100000 x 1024, 2 rounds against 3: 61.9 us, smaller 54.0; 256 rows, 2 against 4: 63.5 and 65.9).
-  // fp16 and fp32 rows have no registers for them.
+  // the size, or somewhat less: the larger ones where that halves the rounds (69 x 100000 x
+  // 1024, one round against two: 29.6 us, smaller 35.4; 130 rows, two and three: 57.4 and
+  // 46.8; 1024 x 32768 x 1024, two and four: 62 and 69).  fp16 and fp32 rows have no registers
+  // for them (fp16, spilled: 1024 x 32768 x 1024 121 us, smaller 75).
   if constexpr (kPieces<T> == 1)
     if (2 * kad_cdiv(count(128, 256), 512) <= kad_cdiv(count(64, 256), 512))
       return launch_tile<T, HALF, GATED, 8, 4, 64, 4, 2>(a, s);

@@ -153,7 +153,7 @@ def test_linear(device, M, N, K, dtype):
 
 # one shape for each tile of the kernel of many rows, and for rows that it splits first
 LARGE = [(700, 1900, 256), (1100, 3000, 300), (1100, 5000, 128), (4000, 8192, 130),
-         (2000, 1030, 640)]
+         (2000, 1030, 640), (25, 43000, 200)]
 
 
 def _assert_large(out, x, dense, residual=None):
