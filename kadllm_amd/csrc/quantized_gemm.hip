@@ -8,7 +8,8 @@
 // bf16 pieces, two for fp16 (11 bits) and three for fp32 (24 bits), each the leading
 // bits of what is left, so the sum is x itself.  With scales from 2^-15 to 1 the weight's
 // values are exact in fp16 too, and rows of fp16 go to v_mfma_f32_16x16x32_f16 as they are,
-// in pieces only where a block of 128 columns has another scale.  Sums are fp32 and
+// in pieces where one is another: in that block of 128 columns alone (the kernel of few
+// rows), or with all of the rows of the weight that a wave has (of many).  Sums are fp32 and
 // are rounded once, with the residual added.  The gated product h is rounded to one
 // bf16 piece for bf16 x (2^-8, as the model's own activation), else to as many
 // pieces as x has: 2^-15 for fp16, whose range h may leave, and 2^-22 for fp32.
@@ -52,7 +53,9 @@ __device__ __forceinline__ void split(float f, bf16_t (&p)[P]) {
 }
 
 // Rows of x as P bf16 pieces [P][M][KP], or (P = 1) rows of 16 bits as they are; zeros past
-// column K.  8 elements a thread.
+// column K.  8 elements a thread.  (1024 x 4096 fp32, 42 MB: 8.6 us, 4.9 TB/s; 1726 x 4560 bf16,
+// 31 MB: 9.5 us.  Split in the products' kernel instead, they would be split by each column
+// tile again.)
 template <typename T, int P>
 __global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ x, int64_t ldx,
                                                          uint16_t* __restrict__ out, int M, int K,
@@ -293,6 +296,13 @@ __device__ __forceinline__ void pieces_of(const u32x4 (&v)[sizeof(T) / 2],
 // rows themselves, whatever their type, alignment and length; else their pieces, padded to
 // whole blocks.  R: rows of a tile that are loaded, 16, or 4 where x has no more (the
 // product's other columns repeat them).
+// One row takes what the codes take to arrive (1 x 248320 x 1024, 135 MB: 24 us, 5.6 TB/s),
+// or, where they are few, a launch and a wave's walk over its blocks (1 x 1024 x 3584: 3.9 us,
+// 0.4 of it the codes at 5 TB/s; 10 x 8192 x 1024 4.3).  More rows take what comes through
+// the L2 caches: each workgroup reads its rows and codes itself (64 x 8192 x 8192, 256
+// workgroups of 32 x 64: 17.5 us, 0.13 GB of rows and 0.07 GB of codes, 12 TB/s).  fp32 rows
+// are three times the products, and their pieces are made in each workgroup: 300 x 1024 x 2048
+// 13.4 us, 0.28 PFLOP/s of the three.
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R>
 __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NW = W * NT;
@@ -478,6 +488,13 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 // BK columns, and each of the waves NW row blocks of the weight (gated: half of them the
 // gate's), whose codes it reads by itself, D - 1 blocks of 128 ahead.  A ring of SLOTS slices
 // is filled by direct loads.
+// The matrix unit bounds the largest tile, for about half its time: a workgroup's four waves
+// wait for a slice together, and what converts codes shares the issue slots (8192 x 8192 x
+// 8192 bf16 728 us, 1.51 PFLOP/s; 32768 x 1024 x 3584 192 us, 1.25; the unit alone, 2.37).  Smaller
+// calls are bound by what the tiles load through the L2 caches: 50 x 248320 x 1024 in tiles of
+// 64 x 256 42 us, 3.2 TB/s of codes, as much of rows, and 50 MB of y and the residual.  fp16 2048 x 8192 x 4096
+// 115 us, 1.19 PFLOP/s; fp32 1024 x 4096 x 4096 79 us and 8.6 for the pieces, 1.3 PFLOP/s of
+// its three products.
 // HALF: x is rows of fp16, else pieces.
 template <typename T, bool HALF, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int ntiles) {

@@ -40,8 +40,9 @@ class QuantizedWeight:
     """A weight [rows, cols] in 4 bits, as quantized_linear reads it: codes uint8
     [rows/16, cols/128, 64, 16] (sizes rounded up), of which bytes 4 j to 4 j + 3 of
     entry l of a block are row l % 16, columns 32 j + 8 (l // 16) to + 7, and scales
-    torch.float8_e8m0fnu [rows/16, cols/128, 16 rows, 4 groups].  Checked when it is made,
-    and not changed afterwards."""
+    torch.float8_e8m0fnu [rows/16, cols/128, 16 rows, 4 groups].  Types and sizes are
+    checked when it is made, and it is not changed afterwards; scales outside 2**-100 to
+    2**125 (which ``pack`` refuses) give undefined values."""
 
     __slots__ = ("codes", "scales", "rows", "cols")
 
@@ -153,8 +154,8 @@ def quantize_weight(weight):
     """``weight`` [N, K] (bf16, fp16 or fp32, any strides) in 4 bits.
 
     A group's scale is the smallest power of two s, from 2**-100 to 2**125, with amax <=
-    7 s (1 for a group of zeros); its codes are w / s to the nearest e2m1 value, ties to the even code, at
-    most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s and s above.
+    7 s (1 for a group of zeros); its codes are w / s to the nearest e2m1 value, ties to
+    the even code, at most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s and s above.
     A group that holds an infinity or NaN reads as NaN.  Columns past K and rows past N
     of the padded arrays are zeros.  Returns a QuantizedWeight."""
     if weight.ndim != 2 or 0 in weight.shape:
