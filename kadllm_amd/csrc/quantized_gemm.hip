@@ -484,6 +484,9 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
 
 typedef __attribute__((address_space(3))) void lds_void_t;
 
+// what is loaded in place of columns past the rows' end
+__device__ __attribute__((aligned(16))) const bf16_t kZeros[8] = {};
+
 // Many rows: a workgroup has 16 MT rows of x, which 4 waves share through LDS in slices of
 // BK columns, and each of the waves NW row blocks of the weight (gated: half of them the
 // gate's), whose codes it reads by itself, D - 1 blocks of 128 ahead.  A ring of SLOTS slices
@@ -492,11 +495,13 @@ typedef __attribute__((address_space(3))) void lds_void_t;
 // wait for a slice together, and what converts codes shares the issue slots (8192 x 8192 x
 // 8192 bf16 728 us, 1.51 PFLOP/s; 32768 x 1024 x 3584 192 us, 1.25; the unit alone, 2.37).  Smaller
 // calls are bound by what the tiles load through the L2 caches: 50 x 248320 x 1024 in tiles of
-// 64 x 256 42 us, 3.2 TB/s of codes, as much of rows, and 50 MB of y and the residual.  fp16 2048 x 8192 x 4096
-// 115 us, 1.19 PFLOP/s; fp32 1024 x 4096 x 4096 79 us and 8.6 for the pieces, 1.3 PFLOP/s of
-// its three products.
-// HALF: x is rows of fp16, else pieces.
-template <typename T, bool HALF, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+// 64 x 256 42 us, 3.2 TB/s of codes, as much of rows, and 50 MB of y and the residual.  fp16
+// 2048 x 8192 x 4096 115 us, 1.19 PFLOP/s; fp32 1024 x 4096 x 4096 79 us and 8.6 for the
+// pieces, 1.3 PFLOP/s of its three products.
+// HALF: x is rows of fp16, else pieces.  RAGGED: rows that end inside a block of columns, at
+// whole 16 bytes (1726 x 960 x 4560 25.5 us, copied and padded first 33; where all kernels
+// looked for an end the others took 2 % longer, the largest tile twice as long for registers).
+template <typename T, bool HALF, bool RAGGED, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int ntiles) {
   constexpr int P = HALF ? 1 : kPieces<T>, W = GATED ? 2 : 1, NT = NW / W;
   constexpr int BM = 16 * MT, GROUP = 8;
@@ -531,15 +536,18 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
     src[i] = (const bf16_t*)a.x + (int64_t)min(m0 + r, a.M - 1) * a.ldx +
              ((lane % CPR) ^ swizzle(r)) * 8;
   }
+  const int col = ((lane % CPR) ^ swizzle(wave * RPI + lane / CPR)) * 8;  // (of every load)
   // slice t (counted from a block kb's first) to its slot; past the last block, that one's
   // again (never multiplied)
   auto issue = [&](int kb, int t) {
     const int p = t % P, h = t / P % HALVES;
-    const int64_t from = (int64_t)min(kb + t / (P * HALVES), a.KB - 1) * 128 + h * BK + p * a.xp;
+    const int64_t k = (int64_t)min(kb + t / (P * HALVES), a.KB - 1) * 128 + h * BK;
+    const int64_t from = k + p * a.xp;
+    const bool in = !RAGGED || (int)k + col < a.K;
 #pragma unroll
     for (int i = 0; i < LPW; ++i)
       __builtin_amdgcn_global_load_lds(
-          (__attribute__((address_space(1))) void*)(src[i] + from),
+          (__attribute__((address_space(1))) void*)(in ? src[i] + from : kZeros),
           (lds_void_t*)(ring[t % SLOTS] + (wave + 4 * i) * RPI * BK), 16, 0, 0);
   };
   const Source<NW> w = source<NW, W>(a, nt);
@@ -676,7 +684,7 @@ int64_t pad128(int64_t k) { return kad_cdiv(k, 128) * 128; }
 
 template <typename T>
 bool in_place(const void* x, int64_t ldx, int K) {
-  return sizeof(T) == 2 && K % 128 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0;
+  return sizeof(T) == 2 && K % 8 == 0 && (uintptr_t)x % 16 == 0 && ldx % 8 == 0;
 }
 
 // Which kernel and tile.  n: rows of the weights in all (gated: the gate's and the up's).
@@ -719,11 +727,11 @@ void launch_stream(const Args& a, hipStream_t s) {
                      s, a);
 }
 
-template <typename T, bool HALF, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
+template <typename T, bool HALF, bool RAGGED, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 void launch_tile(const Args& a, hipStream_t s) {
   const int64_t mtiles = kad_cdiv(a.M, 16 * MT);
   const int64_t ntiles = kad_cdiv(a.cols, 64 * NW / (GATED ? 2 : 1));
-  hipLaunchKernelGGL((q4_tile_kernel<T, HALF, GATED, MT, NW, BK, SLOTS, D>),
+  hipLaunchKernelGGL((q4_tile_kernel<T, HALF, RAGGED, GATED, MT, NW, BK, SLOTS, D>),
                      dim3((unsigned)(mtiles * ntiles)), dim3(256), 0, s, a, (int)mtiles,
                      (int)ntiles);
 }
@@ -769,7 +777,7 @@ void stream(const Args& a, hipStream_t s) {
   return launch_stream<T, RAW, GATED, 2, 4 / W, 4, P == 1 ? 2 : 1>(a, s);
 }
 
-template <typename T, bool HALF, bool GATED>
+template <typename T, bool HALF, bool RAGGED, bool GATED>
 void tiles(const Args& a, hipStream_t s) {
   constexpr int P = HALF ? 1 : kPieces<T>;
   const int64_t n = (int64_t)a.cols * (GATED ? 2 : 1);
@@ -777,22 +785,23 @@ void tiles(const Args& a, hipStream_t s) {
   // up to two workgroups a CU, and up to 32 rows (32 x 248320 x 1024: bf16 35.3 us, 64 x 128
   // 45.9, 64 x 256 36.9; fp32 61, 83 and 72)
   if (count(32, 128) <= 512 || a.M <= 32)
-    return launch_tile<T, HALF, GATED, 2, 2, 128, 4, 4>(a, s);
+    return launch_tile<T, HALF, RAGGED, GATED, 2, 2, 128, 4, 4>(a, s);
   // slices of 64 columns and fewer codes ahead where the pieces of fp16 rows leave no
   // registers for more
   if (count(64, 128) <= 512) {
     constexpr int BK = HALF ? 64 : 128, D = HALF || P == 2 ? 2 : 4;
-    return launch_tile<T, HALF, GATED, 4, 2, BK, 4, D>(a, s);
+    return launch_tile<T, HALF, RAGGED, GATED, 4, 2, BK, 4, D>(a, s);
   }
   // Two of the largest tiles run on a CU at a time, and take twice as long as four of half
   // the size, or somewhat less: the larger ones where that halves the rounds (69 x 100000 x
   // 1024, one round against two: 29.6 us, smaller 35.4; 130 rows, two and three: 57.4 and
   // 46.8; 1024 x 32768 x 1024, two and four: 62 and 69).  fp16 and fp32 rows have no registers
-  // for them (fp16, spilled: 1024 x 32768 x 1024 121 us, smaller 75).
-  if constexpr (kPieces<T> == 1)
+  // for them (fp16, spilled: 1024 x 32768 x 1024 121 us, smaller 75), nor have ragged ones (4000 x
+  // 2880 x 2880: 150 us, smaller 72).
+  if constexpr (kPieces<T> == 1 && !RAGGED)
     if (2 * kad_cdiv(count(128, 256), 512) <= kad_cdiv(count(64, 256), 512))
-      return launch_tile<T, HALF, GATED, 8, 4, 64, 4, 2>(a, s);
-  return launch_tile<T, HALF, GATED, 4, 4, 64, 4, 2>(a, s);
+      return launch_tile<T, HALF, RAGGED, GATED, 8, 4, 64, 4, 2>(a, s);
+  return launch_tile<T, HALF, RAGGED, GATED, 4, 4, 64, 4, 2>(a, s);
 }
 
 // a product of the rows x as they are, or of their pieces in `ws`
@@ -807,7 +816,10 @@ void multiply(Args a, const void* x, int64_t ldx, void* ws, hipStream_t s) {
                        dim3((unsigned)kad_cdiv((int64_t)a.M * (KP / 8), 256)), dim3(256), 0, s,
                        (const T*)x, ldx, (uint16_t*)ws, a.M, a.K, KP);
   }
-  tiles<T, std::is_same_v<T, _Float16>, GATED>(a, s);
+  constexpr bool HALF = std::is_same_v<T, _Float16>;
+  if constexpr (sizeof(T) == 2)
+    if (a.x == x && a.K % 128) return tiles<T, HALF, true, GATED>(a, s);
+  tiles<T, HALF, false, GATED>(a, s);
 }
 
 // the same of rows that are pieces already, padded to whole blocks
@@ -815,7 +827,7 @@ template <typename T>
 void multiply_pieces(Args a, const bf16_t* x, hipStream_t s) {
   a.x = x, a.ldx = pad128(a.K), a.xp = a.M * a.ldx, a.K = (int)a.ldx;
   if (few(a.M, a.cols)) return stream<T, kPieces<T> == 1, false>(a, s);
-  tiles<T, false, false>(a, s);
+  tiles<T, false, false, false>(a, s);
 }
 
 struct Weight {

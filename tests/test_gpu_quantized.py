@@ -153,7 +153,7 @@ def test_linear(device, M, N, K, dtype):
 
 # one shape for each tile of the kernel of many rows, and for rows that it splits first
 LARGE = [(700, 1900, 256), (1100, 3000, 300), (1100, 5000, 128), (4000, 8192, 130),
-         (2000, 1030, 640), (25, 43000, 200)]
+         (2000, 1030, 640), (25, 43000, 200), (1300, 2100, 328)]
 
 
 def _assert_large(out, x, dense, residual=None):
@@ -200,6 +200,18 @@ def test_many_rows_exactly(device, M, N, K, dtype):
     assert not out[M // 2].isfinite().any() and out[M - 1].isnan().all()
     rest = [m for m in range(M) if m not in (M // 2, M - 1)]
     assert torch.equal(out[rest], got[rest])
+
+
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, N, K", [(9, 100, 200), (700, 1900, 264), (1100, 3000, 8),
+                                     (1100, 5000, 392), (4000, 8192, 72)])
+def test_what_is_beside_the_rows_is_not_read(device, M, N, K, dtype):
+    # rows at whole 16 bytes, which end inside a block of columns, in a buffer of NaN
+    q, dense = _weight(N, K, M + N)
+    wide = torch.full((M, K + 128), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 8:8 + K] = _values((M, K), K, dtype)
+    x = wide[:, 8:8 + K]
+    _assert_large(quantized_linear(x, q), x, dense)
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
