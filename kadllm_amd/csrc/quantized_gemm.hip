@@ -860,7 +860,8 @@ int check_sizes(int64_t M, int64_t N, int K) {
   // (a grid holds fewer than 2^32 work-items a dimension, and 65535 rows of tiles)
   KAD_REQUIRE(M <= 16 * 65535 && kad_cdiv(M, 32) * kad_cdiv(2 * N, 128) < (1ll << 32) / 256,
               "a product of %lld x %lld outputs", (long long)M, (long long)N);
-  KAD_REQUIRE(M * pad128(K) < (1ll << 35), "%lld rows of %d columns", (long long)M, K);
+  // (a thread of the pieces' kernel takes 8 elements; workgroups of 256)
+  KAD_REQUIRE(M * pad128(K) <= (1ll << 35) - 2048, "%lld rows of %d columns", (long long)M, K);
   return KAD_OK;
 }
 

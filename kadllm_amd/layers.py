@@ -15,13 +15,15 @@ EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 def gemm(a, w, out=None, *, epilogue=EPI_STORE, residual=None):
     """out[M, N'] = epilogue(a[M, K] @ w[N, K]^T) (bf16, fp32 accumulate).
 
-    w may be a QuantizedWeight (without the SwiGLU epilogue; rounded once, with the
+    w may be a QuantizedWeight (but for the SwiGLU epilogue; rounded once, with the
     residual added).  a, w, out may be row-strided 2-D views (last dim contiguous).  For the
     SwiGLU epilogue N' = N/2; for the residual epilogue ``residual`` [M, N]
     is added (it may be ``out`` itself).
     """
     M, K = a.shape
     if type(w) is QuantizedWeight:
+        if epilogue == EPI_SWIGLU:
+            raise ValueError("the SwiGLU epilogue takes no 4-bit weight; use quantized_gated_ffn")
         if out is None:
             out = torch.empty(M, w.rows, dtype=torch.bfloat16, device=a.device)
         return _linear(a, w, out, residual)

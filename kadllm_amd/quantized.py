@@ -155,7 +155,8 @@ def quantize_weight(weight):
 
     A group's scale is the smallest power of two s, from 2**-100 to 2**125, with amax <=
     7 s (1 for a group of zeros); its codes are w / s to the nearest e2m1 value, ties to
-    the even code, at most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s and s above.
+    the even code, at most 6.  An element is off by up to s / 4 below 2 s, s / 2 below 4 s
+    and s above.
     A group that holds an infinity or NaN reads as NaN.  Columns past K and rows past N
     of the padded arrays are zeros.  Returns a QuantizedWeight."""
     if weight.ndim != 2 or 0 in weight.shape:

@@ -200,7 +200,8 @@ class Qwen35Runner:
                 if cfg.linear_conv_kernel_dim != 4:
                     raise ValueError("the conv kernels are specialised for width 4")
                 self.layers.append(_GdnLayer(
-                    w_in=pack(w_in), w_ab=w_ab, conv_w=get(a + "conv1d.weight").reshape(self.conv_dim, 4).contiguous(),
+                    w_in=pack(w_in), w_ab=w_ab,
+                    conv_w=get(a + "conv1d.weight").reshape(self.conv_dim, 4).contiguous(),
                     A_log=get(a + "A_log"), dt_bias=get(a + "dt_bias"), norm_w=get(a + "norm.weight"),
                     w_out=pack(get(a + "out_proj.weight")), **common))
             else:
@@ -260,7 +261,8 @@ class Qwen35Runner:
     def conv_fuses(self, rows, L, lyr):
         """Whether kad_gemm_bf16_conv takes a prefill's projection."""
         C = self.conv_dim
-        return (self.weights is None and L % 128 == 0 and rows % 256 == 0 and (C + self.vd) % 256 == 0 and C % 256 == 0
+        return (self.weights is None and L % 128 == 0 and rows % 256 == 0
+                and (C + self.vd) % 256 == 0 and C % 256 == 0
                 and self.cfg.hidden_size % 64 == 0 and lyr.conv_w.is_contiguous()
                 and lyr.conv_w.data_ptr() % 16 == 0)
 

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import kadllm
-from kadllm_amd import _lib
+from kadllm_amd import _lib, layers
 from kadllm_amd.ops import (QuantizedWeight, dequantize_weight, quantize_weight,
                             quantized_gated_ffn, quantized_linear)
 from oracle import quantized_ref as ref
@@ -212,14 +212,35 @@ def test_c_quantize_refusals():
                    a["N"], a["K"], None) < 0, change
 
 
+def test_a_swiglu_product_takes_no_4_bit_weight():
+    x = torch.zeros(2, 40, dtype=BF)
+    with pytest.raises(ValueError):
+        layers.gemm(x, _weight(), epilogue=layers.EPI_SWIGLU)
+
+
+def test_c_product_of_as_many_rows_as_a_grid_takes():
+    bytes = ctypes.c_int64(0)
+    # 2^28 - 1 pieces of 128 columns: 16 of them a workgroup, 2^24 workgroups of 256
+    M, K = 617093, 435 * 128
+    args = (3, K + 3, 0, M, 20000, K - 3)
+    assert _rc("kad_quantized_linear_workspace_bytes", *args, ctypes.byref(bytes)) < 0
+    args = (3, K + 3, 0, M - 1, 20000, K - 3)
+    assert _rc("kad_quantized_linear_workspace_bytes", *args, ctypes.byref(bytes)) == 0
+    assert bytes.value == (M - 1) * K * 2
+
+
 def test_c_product_refusals():
     n = ctypes.c_int64(0)
     good = dict(x=P, ldx=64, dtype=1, codes=P, scales=P, r=None, ldr=0, y=P, ldy=32, ws=P,
                 bytes=1 << 30, M=3, N=32, K=64)
+    many = dict(M=3000, N=20000, ldy=20000, K=60)  # rows that are padded first
+    assert _rc("kad_quantized_linear_workspace_bytes", P, 64, 1, 3000, 20000, 60,
+               ctypes.byref(n)) == 0 and n.value == 3000 * 256
     for change in (dict(x=None), dict(codes=None), dict(scales=None), dict(y=None), dict(ldx=63),
-                   dict(ldy=31), dict(r=P, ldr=31), dict(ws=None), dict(ws=P + 8), dict(bytes=10),
-                   dict(M=0), dict(M=16 * 65535 + 1), dict(N=0), dict(K=0), dict(N=2**26 + 1, ldy=2**27), dict(dtype=7),
-                   dict(codes=P + 4), dict(K=2**20 + 1, ldx=2**21)):
+                   dict(ldy=31), dict(r=P, ldr=31), dict(many, ws=None), dict(many, ws=P + 8),
+                   dict(many, bytes=10), dict(M=0), dict(M=16 * 65535 + 1), dict(N=0), dict(K=0),
+                   dict(N=2**26 + 1, ldy=2**27), dict(dtype=7), dict(codes=P + 4),
+                   dict(K=2**20 + 1, ldx=2**21)):
         a = {**good, **change}
         assert _rc("kad_quantized_linear", a["x"], a["ldx"], a["dtype"], a["codes"], a["scales"],
                    a["r"], a["ldr"], a["y"], a["ldy"], a["ws"], a["bytes"], a["M"], a["N"], a["K"],
