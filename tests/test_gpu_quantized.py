@@ -522,3 +522,48 @@ def test_repeated_calls_give_the_same_bits(device):
         first = quantized_linear(x, q)
         for _ in range(3):
             assert torch.equal(quantized_linear(x, q), first)
+
+
+def test_quantised_in_a_graph(device):
+    w = _values((200, 1000), 1, BF)
+    x = _values((30, 1000), 2, BF)
+    quantize_weight(w)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q = quantize_weight(w)
+        back, y = dequantize_weight(q), quantized_linear(x, q)
+    for step in range(3):
+        w.copy_(_values((200, 1000), 5 + step, BF))
+        want = quantize_weight(w)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q.codes, want.codes)
+        assert torch.equal(q.scales.view(U8), want.scales.view(U8))
+        assert torch.equal(back, dequantize_weight(want))
+        assert torch.equal(y, quantized_linear(x, want))
+
+
+def test_offsets_past_32_bits(device):
+    # a weight of 2^33 and more elements: 16384 times the same 128 rows
+    n, N, K = 128, 2**21, 4224
+    part = _values((n, K), 1, BF)
+    q1 = quantize_weight(part)
+    w = part.expand(N // n, n, K).reshape(N, K)
+    q = quantize_weight(w)
+    del w
+    codes = q.codes.view(N // n, -1)
+    assert torch.equal(codes, q1.codes.view(1, -1).expand_as(codes))
+    scales = q.scales.view(U8).view(N // n, -1)
+    assert torch.equal(scales, q1.scales.view(U8).view(1, -1).expand_as(scales))
+    back = dequantize_weight(q).view(N // n, n, K)
+    assert torch.equal(back, dequantize_weight(q1).expand_as(back))
+    del back
+    for M in (2, 2100):  # and 2^32 outputs and residuals
+        x = torch.randint(-2, 3, (M, K), device="cuda").to(BF)
+        r = torch.randint(-2, 3, (M, n), device="cuda").to(BF)
+        y = quantized_linear(x, q, residual=r.repeat(1, N // n)).view(M, N // n, n)
+        assert torch.equal(y, y[:, -1:].expand_as(y))
+        _assert_large(y[:, -1], x, dequantize_weight(q1, F32).double(), r)
+    del y, q, codes, scales
+    torch.cuda.empty_cache()
