@@ -100,7 +100,14 @@ struct Args {
   int64_t ldy, yp;
   int M, N, K, KB;           // KB blocks of 128 columns
   int cols;                  // columns that are written: N, or (gated) N padded to 128
+  int by_rows;               // few rows: an XCD has all columns of a share of the row tiles
 };
+
+// Workgroup b of n in 8 runs, each of an XCD (which workgroups b, b + 8, .. are on).
+__device__ __forceinline__ int xcd_run(int b, int n) {
+  const int x = b % 8;
+  return x * (n / 8) + min(x, n % 8) + b / 8;
+}
 
 // a word of 8 codes times its group's scale, as an MFMA operand
 __device__ __forceinline__ bf16x8 operand(uint32_t codes, float scale) {
@@ -316,7 +323,13 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   __shared__ __attribute__((aligned(1024))) char lds[KS * kWave];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt = blockIdx.x * NT, m0 = blockIdx.y * (16 * MT);
+  int nt = blockIdx.x, mt = blockIdx.y;
+  if (a.by_rows) {
+    const int lid = xcd_run(mt * gridDim.x + nt, gridDim.x * gridDim.y);
+    mt = lid / (int)gridDim.x, nt = lid - mt * (int)gridDim.x;
+  }
+  const int m0 = mt * (16 * MT);
+  nt *= NT;
   char* own = lds + wave * kWave;
   f32x4 acc[NW][MT];
 #pragma unroll
@@ -520,7 +533,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
   __shared__ __attribute__((aligned(1024))) bf16_t ring[SLOTS][BM * BK];
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lid = xcd_logical_id(blockIdx.x, gridDim.x);
+  const int lid = xcd_run(blockIdx.x, gridDim.x);
   // runs of 8 row tiles a column tile, so that an XCD's L2 holds what its run shares
   const int g0 = lid / (GROUP * ntiles) * GROUP, in_group = lid - g0 * ntiles;
   const int gm = min(GROUP, mtiles - g0);
@@ -721,7 +734,14 @@ int64_t piece_bytes(const void* x, int64_t ldx, int64_t M, int64_t n, int K) {
 }
 
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R = 16>
-void launch_stream(const Args& a, hipStream_t s) {
+void launch_stream(Args a, hipStream_t s) {
+  // In the grid's order an XCD has an eighth of the columns, or a few of them, and reads all
+  // rows; where those pass its L2 (4 MB) and the codes in bytes, it has an eighth of the rows
+  // and reads all codes: bf16 2048 x 512 x 4096 15.7 us, in the grid's order 23.6; 1951 x 368 x
+  // 8912 26.9 and 38.1; fp32 300 x 1024 x 2048, 2.4 MB of rows: 13.5 and 12.2; bf16 32 x 8192 x
+  // 8192, 36 MB of codes: 13.4 and 10.5.
+  const int64_t rows = (int64_t)a.M * a.K * (RAW ? sizeof(T) : 2 * kPieces<T>);
+  a.by_rows = rows > (4 << 20) && rows > (int64_t)a.KB * 68 * a.cols * (GATED ? 2 : 1);
   const dim3 grid((unsigned)kad_cdiv(a.cols, 16 * NT), (unsigned)kad_cdiv(a.M, 16 * MT));
   hipLaunchKernelGGL((q4_stream_kernel<T, RAW, GATED, MT, NT, KS, D, R>), grid, dim3(64 * KS), 0,
                      s, a);

@@ -151,6 +151,16 @@ def test_linear(device, M, N, K, dtype):
     _assert_linear(quantized_linear(x, q, residual=r), x, dense, r)
 
 
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M, N, K", [(1000, 130, 3000), (1100, 200, 2048), (530, 70, 5001)])
+def test_linear_of_more_rows_than_columns(device, M, N, K, dtype):
+    # rows of more bytes than an L2 holds, and than the weight: another order of workgroups
+    q, dense = _weight(N, K, M + N)
+    x = _values((M, K), K, dtype)
+    r = _values((M, N), 7, dtype)
+    _assert_large(quantized_linear(x, q, residual=r), x, dense, r)
+
+
 # one shape for each tile of the kernel of many rows, and for rows that it splits first
 LARGE = [(700, 1900, 256), (1100, 3000, 300), (1100, 5000, 128), (4000, 8192, 130),
          (2000, 1030, 640), (25, 43000, 200), (1300, 2100, 328)]
