@@ -170,8 +170,8 @@ def quantize_weight(weight):
     device = _device_of(weight)
     weight, ld = _rows(weight)
     shapes = _padded(N, K)
-    codes = torch.empty(shapes[0], dtype=torch.uint8, device=weight.device)
-    scales = torch.empty(shapes[1], dtype=_SCALES, device=weight.device)
+    codes = weight.new_empty(*shapes[0], dtype=torch.uint8)
+    scales = weight.new_empty(*shapes[1], dtype=_SCALES)
     _launch(device, "kad_quantize_weight", weight.data_ptr(), ld, _lib.dtype_code(weight.dtype),
             codes.data_ptr(), scales.data_ptr(), N, K)
     return QuantizedWeight.__new__(QuantizedWeight)._set(codes, scales, N, K)
@@ -183,7 +183,7 @@ def dequantize_weight(weight, dtype=torch.bfloat16):
     if dtype not in _TYPES:
         raise TypeError("weights must be bf16, fp16 or fp32")
     device = _device_of(weight.codes, weight.scales)
-    out = torch.empty(weight.rows, weight.cols, dtype=dtype, device=weight.codes.device)
+    out = weight.codes.new_empty(weight.rows, weight.cols, dtype=dtype)
     _launch(device, "kad_dequantize_weight", weight.codes.data_ptr(), weight.scales.data_ptr(),
             out.data_ptr(), weight.cols, _lib.dtype_code(dtype), weight.rows, weight.cols)
     return out
@@ -231,7 +231,7 @@ def quantized_linear(x, weight, *, residual=None):
     _check_weight(weight)
     rows, r = _check_rows(x, weight.cols, weight.rows, residual)
     _device_of(x, weight.codes, residual)
-    out = _linear(rows, weight, rows.new_empty((rows.shape[0], weight.rows)), r)
+    out = _linear(rows, weight, rows.new_empty(rows.shape[0], weight.rows), r)
     return out if rows is x else out.view(*x.shape[:-1], weight.rows)
 
 
@@ -243,7 +243,7 @@ def _linear(x, weight, out, residual=None):
     r, ldr = (None, 0) if residual is None else _rows(residual)
     code, at = _lib.DTYPE_CODES[x.dtype], x.data_ptr()
     need = _workspace_bytes("kad_quantized_linear_workspace_bytes", at & 15, ldx, code, M, N, K)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     _launch(x.get_device(), "kad_quantized_linear", at, ldx, code, weight.codes.data_ptr(),
             weight.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(), max(out.stride(0), N),
             _lib.ptr(ws), need, M, N, K)
@@ -265,7 +265,7 @@ def quantized_gated_ffn(x, gate, up, down, *, residual=None):
         raise ValueError("gate and up must be [F, H] and down [H, F]")
     rows, r = _check_rows(x, H, H, residual)
     _device_of(x, gate.codes, up.codes, down.codes, residual)
-    out = _gated_ffn(rows, gate, up, down, rows.new_empty(rows.shape), r)
+    out = _gated_ffn(rows, gate, up, down, rows.new_empty(*rows.shape), r)
     return out if rows is x else out.view(x.shape)
 
 
@@ -277,7 +277,7 @@ def _gated_ffn(x, gate, up, down, out, residual=None):
     r, ldr = (None, 0) if residual is None else _rows(residual)
     code, at = _lib.DTYPE_CODES[x.dtype], x.data_ptr()
     need = _workspace_bytes("kad_quantized_gated_ffn_workspace_bytes", at & 15, ldx, code, M, H, F)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(need, dtype=torch.uint8)
     _launch(x.get_device(), "kad_quantized_gated_ffn", at, ldx, code, gate.codes.data_ptr(),
             gate.scales.data_ptr(), up.codes.data_ptr(), up.scales.data_ptr(),
             down.codes.data_ptr(), down.scales.data_ptr(), _lib.ptr(r), ldr, out.data_ptr(),
