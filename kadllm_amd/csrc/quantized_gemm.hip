@@ -285,8 +285,13 @@ __device__ __forceinline__ void pieces_of(const u32x4 (&v)[sizeof(T) / 2],
       for (int i = 0; i < 4; ++i) {
         const uint32_t lo = __float_as_uint(f[2 * i]), hi = __float_as_uint(f[2 * i + 1]);
         w[q][i] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
-        f[2 * i] = rest(f[2 * i], lo);
-        f[2 * i + 1] = rest(f[2 * i + 1], hi);
+        if (q == 0) {
+          f[2 * i] = rest(f[2 * i], lo);
+          f[2 * i + 1] = rest(f[2 * i + 1], hi);
+        } else {  // (finite by now)
+          f[2 * i] -= __uint_as_float(lo & 0xffff0000u);
+          f[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
+        }
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[P - 1][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
