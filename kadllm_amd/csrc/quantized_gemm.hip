@@ -100,7 +100,8 @@ struct Args {
   int64_t ldy, yp;
   int M, N, K, KB;           // KB blocks of 128 columns
   int cols;                  // columns that are written: N, or (gated) N padded to 128
-  int by_rows;               // few rows: an XCD has all columns of a share of the row tiles
+  int order;                 // few rows: 1 where an XCD has all columns of a share of the row
+                             // tiles, 2 all rows of a share of the columns, 0 the grid's order
 };
 
 // Workgroup b of n in 8 runs, each of an XCD (which workgroups b, b + 8, .. are on).
@@ -329,9 +330,10 @@ __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int nt = blockIdx.x, mt = blockIdx.y;
-  if (a.by_rows) {
+  if (a.order) {
     const int lid = xcd_run(mt * gridDim.x + nt, gridDim.x * gridDim.y);
-    mt = lid / (int)gridDim.x, nt = lid - mt * (int)gridDim.x;
+    const int n = a.order == 1 ? gridDim.x : gridDim.y, q = lid / n, r = lid - q * n;
+    mt = a.order == 1 ? q : r, nt = a.order == 1 ? r : q;
   }
   const int m0 = mt * (16 * MT);
   nt *= NT;
@@ -740,14 +742,20 @@ int64_t piece_bytes(const void* x, int64_t ldx, int64_t M, int64_t n, int K) {
 
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R = 16>
 void launch_stream(Args a, hipStream_t s) {
+  const dim3 grid((unsigned)kad_cdiv(a.cols, 16 * NT), (unsigned)kad_cdiv(a.M, 16 * MT));
   // In the grid's order an XCD has an eighth of the columns, or a few of them, and reads all
   // rows; where those pass its L2 (4 MB) and the codes in bytes, it has an eighth of the rows
   // and reads all codes: bf16 2048 x 512 x 4096 15.7 us, in the grid's order 23.6; 1951 x 368 x
   // 8912 26.9 and 38.1; fp32 300 x 1024 x 2048, 2.4 MB of rows: 13.5 and 12.2; bf16 32 x 8192 x
   // 8192, 36 MB of codes: 13.4 and 10.5.
   const int64_t rows = (int64_t)a.M * a.K * (RAW ? sizeof(T) : 2 * kPieces<T>);
-  a.by_rows = rows > (4 << 20) && rows > (int64_t)a.KB * 68 * a.cols * (GATED ? 2 : 1);
-  const dim3 grid((unsigned)kad_cdiv(a.cols, 16 * NT), (unsigned)kad_cdiv(a.M, 16 * MT));
+  const bool by_rows = rows > (4 << 20) && rows > (int64_t)a.KB * 68 * a.cols * (GATED ? 2 : 1);
+  // Else the row tiles of a column tile share an XCD by themselves where a row of the grid is
+  // whole rounds of 8; elsewhere they are numbered so, for the widest tiles (fp16 37 x 5001 x
+  // 2007, 79 column tiles: 6.0 us, in the grid's order 6.7; bf16 100 x 5000 x 2048 9.3 and 10.0;
+  // narrower ones gain nothing: 64 x 1400 x 8192 7.6 and 7.6).
+  const bool by_columns = NT * (GATED ? 2 : 1) == 4 && grid.y > 1 && grid.x % 8;
+  a.order = by_rows ? 1 : by_columns ? 2 : 0;
   hipLaunchKernelGGL((q4_stream_kernel<T, RAW, GATED, MT, NT, KS, D, R>), grid, dim3(64 * KS), 0,
                      s, a);
 }

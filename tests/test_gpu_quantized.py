@@ -152,9 +152,11 @@ def test_linear(device, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
-@pytest.mark.parametrize("M, N, K", [(1000, 130, 3000), (1100, 200, 2048), (530, 70, 5001)])
-def test_linear_of_more_rows_than_columns(device, M, N, K, dtype):
-    # rows of more bytes than an L2 holds, and than the weight: another order of workgroups
+@pytest.mark.parametrize("M, N, K", [(1000, 130, 3000), (1100, 200, 2048), (530, 70, 5001),
+                                     (37, 5001, 300), (100, 5000, 200), (200, 2700, 140)])
+def test_linear_in_other_orders_of_workgroups(device, M, N, K, dtype):
+    # rows of more bytes than an L2 holds, and than the weight; column tiles that are no
+    # whole rounds of the 8 XCDs
     q, dense = _weight(N, K, M + N)
     x = _values((M, K), K, dtype)
     r = _values((M, N), 7, dtype)
