@@ -516,7 +516,8 @@ int kad_cache_prefetch(const void* p0, int64_t bytes0, const void* p1, int64_t b
  *   hidden]; conv_dim = 2 kd + vd; rows of gdn_cols hold [q|k|v | z | a|b | pad].
  *   A layer with scales s_* has its weights but w_ab in 4 bits (kad_quantize_weight's
  *   codes, w_gu the gate's and w_up the up's): hidden, ffn, vd and q_heads head_dim
- *   multiples of 128 and fuse_conv 0.
+ *   multiples of 128, n, h and mixed 16-byte aligned, and fuse_conv 0; other calls are
+ *   refused before anything is enqueued.
  * kad_qwen_prefill  layers 0 .. layers - 1 over x [B*L, hidden] (updated in
  *   place).  state0/1[i]: a linear layer's conv state [B, conv_dim, 4] and fp32
  *   state [B, v_heads, k_dim, v_dim], an attention layer's K and V

@@ -11,6 +11,8 @@
 // arguments, hence bits, as the Python sequence, and every buffer is the
 // caller's.
 
+#include <climits>
+
 #include "kad_common.h"
 
 namespace {
@@ -28,6 +30,45 @@ int check_model(const kad_qwen_model* m) {
   KAD_REQUIRE(m && m->layers && m->n_layers > 0, "null model");
   KAD_REQUIRE(m->hidden > 0 && m->ffn > 0 && m->gdn_cols >= m->conv_dim + m->vd + m->ab_rows,
               "bad model dimensions");
+  return KAD_OK;
+}
+
+// The weights in 4 bits of the first `layers` layers, before anything is enqueued: whole
+// blocks of 128 columns, as the products get no workspace for others, no convolution fused
+// into their projection, sizes that they take, and everything at whole 16 bytes.
+int check_quantized(const kad_qwen_model& m, int layers, int64_t rows, bool fuse_conv,
+                    const void* n, const void* mixed, const void* h) {
+  const int H = m.hidden, qkv = (2 * m.q_heads + 2 * m.kv_heads) * m.head_dim;
+  for (int i = 0; i < layers; ++i) {
+    const kad_qwen_layer& l = m.layers[i];
+    const bool ffn = l.s_down != nullptr;
+    KAD_REQUIRE(ffn == (l.s_gate != nullptr) && ffn == (l.s_up != nullptr),
+                "layer %d: gate, up and down are in 4 bits together", i);
+    KAD_REQUIRE(!(fuse_conv && l.linear && l.s_in),
+                "layer %d: no convolution is fused into a projection in 4 bits", i);
+    const struct {
+      const void *w, *s, *x;
+      int N, K;
+    } weights[] = {
+        {l.w_gu, l.s_gate, n, m.ffn, H},
+        {l.w_up, l.s_up, n, m.ffn, H},
+        {l.w_down, l.s_down, h, H, m.ffn},
+        {l.linear ? l.w_in : l.w_qkv, l.linear ? l.s_in : l.s_qkv, n,
+         l.linear ? m.conv_dim + m.vd : qkv, H},
+        {l.linear ? l.w_out : l.w_o, l.linear ? l.s_out : l.s_o, mixed, H,
+         l.linear ? m.vd : m.q_heads * m.head_dim},
+    };
+    for (const auto& w : weights) {
+      if (!w.s) continue;
+      KAD_REQUIRE(w.w, "null pointer argument");
+      KAD_REQUIRE(w.K % 128 == 0, "layer %d: a weight in 4 bits of %d columns", i, w.K);
+      KAD_REQUIRE((((uintptr_t)w.w | (uintptr_t)w.s | (uintptr_t)w.x) % 16) == 0,
+                  "layer %d: a weight in 4 bits and its rows must be 16-byte aligned", i);
+      KAD_REQUIRE(rows <= INT_MAX, "%lld rows", (long long)rows);
+      int64_t need = 0;
+      KAD_TRY(kad_quantized_linear_workspace_bytes(w.x, w.K, kBf, (int)rows, w.N, w.K, &need));
+    }
+  }
   return KAD_OK;
 }
 
@@ -73,6 +114,8 @@ extern "C" int kad_qwen_prefill(const kad_qwen_model* m, const kad_qwen_prefill_
               "null pointer argument");
   KAD_REQUIRE(a->layers >= 0 && a->layers <= m->n_layers && a->B > 0 && a->L > 0,
               "bad dimensions");
+  KAD_TRY(check_quantized(*m, a->layers, (int64_t)a->B * a->L, a->fuse_conv != 0, a->n, a->mixed,
+                          a->h));
   const int B = a->B, L = a->L, rows = B * L, H = m->hidden, C = m->conv_dim, c = C + m->vd;
   const int cols = m->gdn_cols, HV = m->v_heads, nh = m->q_heads, nkv = m->kv_heads;
   const int hd = m->head_dim;
@@ -133,6 +176,7 @@ extern "C" int kad_qwen_decode_step(const kad_qwen_model* m, const kad_qwen_step
   KAD_REQUIRE(a->T == 1 || (a->prev0 && a->prev1 && a->parents && a->Wp > 0),
               "no parent rows for a second token");
   KAD_REQUIRE(a->keep ? a->next0 && a->next1 : a->k_ws && a->v_ws, "null pointer argument");
+  KAD_TRY(check_quantized(*m, m->n_layers, (int64_t)a->B * a->W, false, a->n, a->mixed, a->h));
   const int B = a->B, W = a->W, T = a->T, BW = B * W, H = m->hidden, C = m->conv_dim;
   const int c = C + m->vd, cols = m->gdn_cols, HV = m->v_heads, nab = m->ab_rows;
   const int nh = m->q_heads, nkv = m->kv_heads, hd = m->head_dim;
