@@ -8,9 +8,26 @@ checked by the C ABI, which raises KadLibraryError on a violation.
 import torch
 
 from . import _lib
+from .prefix_cache import _device_of
 from .quantized import QuantizedWeight, _linear
 
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
+
+
+def _check_gemm(a, w, out, residual, epilogue):
+    """What the C entry point, which is not given the weight's size, cannot see."""
+    M, K = a.shape
+    if K != w.cols or out.shape != (M, w.rows) or K == 0 or M == 0:
+        raise ValueError(f"a must be [M, {w.cols}] and out [M, {w.rows}]")
+    if out.stride(1) != 1 and w.rows > 1 or out.stride(0) < w.rows and M > 1:
+        raise ValueError("out must have whole rows that do not overlap")
+    if epilogue == EPI_RESIDUAL and (residual is None or residual.shape != out.shape):
+        raise ValueError("the residual epilogue adds a residual of out's shape")
+    if a.dtype != torch.bfloat16 or out.dtype != a.dtype or residual is not None and \
+            residual.dtype != a.dtype:
+        raise TypeError("products are bf16")
+    _device_of(a, w.codes, out, residual)
+
 
 def gemm(a, w, out=None, *, epilogue=EPI_STORE, residual=None):
     """out[M, N'] = epilogue(a[M, K] @ w[N, K]^T) (bf16, fp32 accumulate).
@@ -26,7 +43,9 @@ def gemm(a, w, out=None, *, epilogue=EPI_STORE, residual=None):
             raise ValueError("the SwiGLU epilogue takes no 4-bit weight; use quantized_gated_ffn")
         if out is None:
             out = torch.empty(M, w.rows, dtype=torch.bfloat16, device=a.device)
-        return _linear(a, w, out, residual)
+        r = residual if epilogue == EPI_RESIDUAL else None
+        _check_gemm(a, w, out, r, epilogue)
+        return _linear(a, w, out, r)
     N = w.shape[0]
     n_out = N // 2 if epilogue == EPI_SWIGLU else N
     if out is None:
