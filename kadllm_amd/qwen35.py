@@ -142,7 +142,6 @@ class Qwen35Runner:
                  weights=None):
         self.cfg = cfg
         self.weights = weights
-        pack = (lambda w: w) if weights is None else quantize_weight
         self.device = torch.device(device) if device is not None else \
             state_dict["embed_tokens.weight"].device
         if self.device.type != "cuda":
@@ -151,6 +150,13 @@ class Qwen35Runner:
 
         def get(name):
             return state_dict[name].detach().to(device=self.device, dtype=bf).contiguous()
+
+        def pack(w, rows, cols):
+            if weights is None:
+                return w
+            if w.shape != (rows, cols):  # (the products take the sizes from elsewhere)
+                raise ValueError(f"a weight of {tuple(w.shape)} where the model has {(rows, cols)}")
+            return quantize_weight(w)
 
         H = cfg.hidden_size
         if H % 64:
@@ -168,7 +174,7 @@ class Qwen35Runner:
                 raise ValueError("head_tokens must be a nonempty 1-D list of vocabulary ids")
             self.head_ids = ids.contiguous()
             self.lm_head = self.lm_head.index_select(0, self.head_ids).contiguous()
-        self.lm_head = pack(self.lm_head)
+        self.lm_head = pack(self.lm_head, self.lm_head.shape[0], H)
         self.norm_w = get("norm.weight")
         self.kd = cfg.linear_num_key_heads * cfg.linear_key_head_dim
         self.vd = cfg.linear_num_value_heads * cfg.linear_value_head_dim
@@ -183,7 +189,8 @@ class Qwen35Runner:
             if weights is None:
                 w_gu, w_down = pack_mlp(gate, up, down)
             else:
-                w_gu, w_down = (pack(gate), pack(up)), pack(down)
+                F_ = gate.shape[0]
+                w_gu, w_down = (pack(gate, F_, H), pack(up, F_, H)), pack(down, H, F_)
             common = dict(input_norm=get(p + "input_layernorm.weight"),
                           post_norm=get(p + "post_attention_layernorm.weight"),
                           w_gu=w_gu, w_down=w_down)
@@ -200,17 +207,19 @@ class Qwen35Runner:
                 if cfg.linear_conv_kernel_dim != 4:
                     raise ValueError("the conv kernels are specialised for width 4")
                 self.layers.append(_GdnLayer(
-                    w_in=pack(w_in), w_ab=w_ab,
+                    w_in=pack(w_in, self.conv_dim + self.vd, H), w_ab=w_ab,
                     conv_w=get(a + "conv1d.weight").reshape(self.conv_dim, 4).contiguous(),
                     A_log=get(a + "A_log"), dt_bias=get(a + "dt_bias"), norm_w=get(a + "norm.weight"),
-                    w_out=pack(get(a + "out_proj.weight")), **common))
+                    w_out=pack(get(a + "out_proj.weight"), H, self.vd), **common))
             else:
                 a = p + "self_attn."
                 w_qkv = torch.cat((get(a + "q_proj.weight"), get(a + "k_proj.weight"),
                                    get(a + "v_proj.weight")), 0).contiguous()
-                self.layers.append(_AttnLayer(w_qkv=pack(w_qkv), q_norm=get(a + "q_norm.weight"),
-                                              k_norm=get(a + "k_norm.weight"),
-                                              w_o=pack(get(a + "o_proj.weight")), **common))
+                self.layers.append(_AttnLayer(
+                    w_qkv=pack(w_qkv, self.attn_cols, H), q_norm=get(a + "q_norm.weight"),
+                    k_norm=get(a + "k_norm.weight"),
+                    w_o=pack(get(a + "o_proj.weight"), H, cfg.num_attention_heads * cfg.head_dim),
+                    **common))
         self._native = None
         # optional observer: trace(phase, layer, x) after each layer with a copy
         # of the residual stream rows (the last position only past a pruned
