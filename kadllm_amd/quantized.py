@@ -88,7 +88,8 @@ class QuantizedWeight:
         """From row-major parts: codes [N, ceil(K / 2)] (uint8, or
         torch.float4_e2m1fn_x2, the even column in a byte's low half) and scales
         [N, ceil(K / 32)] (torch.float8_e8m0fnu or its bytes as uint8), from 2**-100
-        to 2**125 or NaN.  ``cols`` is K (default: two for each byte)."""
+        to 2**125 or NaN; a group of zeros may have 2**-127 (byte 0) too, as it is
+        commonly stored, and gets 1.  ``cols`` is K (default: two for each byte)."""
         if codes.dtype is torch.float4_e2m1fn_x2:
             codes = codes.view(torch.uint8)
         if scales.dtype is _SCALES:
@@ -104,12 +105,17 @@ class QuantizedWeight:
             raise ValueError("codes must be [N, K / 2] and scales [N, K / 32]")
         if codes.device != scales.device:
             raise ValueError("all tensors must be on the same device")
-        if bool(((scales < 27) | ((scales > 252) & (scales < 255))).any()):
-            raise ValueError("scales must be from 2**-100 to 2**125, or NaN")
         if K % 2:
             codes = torch.cat((codes[:, :-1], codes[:, -1:] & 15), 1)
-        nb, kb = _padded(N, K)[0][:2]
         pad = torch.nn.functional.pad
+        bad = (scales < 27) | ((scales > 252) & (scales < 255))
+        if bool(bad.any()):
+            nonzero = (pad(codes, (0, -half % 16)).view(N, -1, 16) & 0x77).ne(0).any(2)
+            unused = (scales == 0) & ~nonzero
+            if bool((bad & ~unused).any()):
+                raise ValueError("scales must be from 2**-100 to 2**125, or NaN")
+            scales = scales.masked_fill(unused, 127)
+        nb, kb = _padded(N, K)[0][:2]
         codes = pad(codes, (0, kb * 64 - half, 0, nb * 16 - N))
         codes = codes.view(nb, 16, kb, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
         scales = pad(scales, (0, kb * 4 - scales.shape[1], 0, nb * 16 - N), value=127)
