@@ -656,7 +656,7 @@ int kad_block_prefix_attention(const void* q, int64_t sq_n, int64_t sq_t, int64_
  * [N/16][K/128][64][4 words]: word j of entry l of a block holds row l % 16, columns 32 j +
  * 8 (l / 16) .. +7, the first in the lowest bits; scales [N/16][K/128][16 rows][4 groups].
  * Scales are from 2^-100 to 2^125, or NaN (255).  Both arrays 16-byte aligned.  K up to 2^20,
- * N up to 2^26, fewer than 2^26 blocks of 16 x 128 to quantise or read back; fewer than 2^35
+ * N up to 2^26, up to 2^26 - 4 blocks of 16 x 128 to quantise or read back; fewer than 2^35
  * elements of x, padded to 128 columns.
  *
  * kad_quantize_weight: w [N, K] (bf16, fp16 or fp32, rows at stride ldw); a group's

@@ -145,11 +145,11 @@ int check(const void* w, const void* codes, const void* scales, int N, int K, in
   KAD_REQUIRE(N > 0 && K > 0, "empty dimensions");
   KAD_REQUIRE(w && codes && scales, "null pointer argument");
   KAD_REQUIRE(ld >= K, "rows of %d columns at stride %lld", K, (long long)ld);
-  KAD_REQUIRE(K <= kMaxK, "rows of %d columns", K);
+  KAD_REQUIRE(K <= kMaxK && N <= kMaxN, "a weight of %d rows of %d columns", N, K);
   KAD_REQUIRE((uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 16 == 0,
               "codes and scales must be 16-byte aligned");
-  // (a grid holds fewer than 2^32 work-items a dimension)
-  KAD_REQUIRE(kad_cdiv(N, 16) * kad_cdiv(K, 128) < (1ll << 26), "too large a weight");
+  // (a grid holds fewer than 2^32 work-items a dimension: 256 for 4 blocks)
+  KAD_REQUIRE(kad_cdiv(N, 16) * kad_cdiv(K, 128) <= (1ll << 26) - 4, "too large a weight");
   return KAD_OK;
 }
 

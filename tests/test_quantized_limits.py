@@ -4,7 +4,7 @@ launch is reached)."""
 import pytest
 import torch
 
-from kadllm_amd import layers
+from kadllm_amd import _lib, layers
 from kadllm_amd.ops import QuantizedWeight
 from oracle import quantized_ref as ref
 
@@ -73,3 +73,12 @@ def test_other_scales_are_refused(code, scale):
     codes[2, 39], scales[2, 2] = code, scale
     with pytest.raises(ValueError):
         QuantizedWeight.pack(codes, scales)
+
+
+@pytest.mark.parametrize("N, K", [(8193 * 16, 8191 * 128),  # 2^26 - 1 blocks: 2^24 workgroups
+                                  (2 ** 26 + 1, 128), (2 ** 26, 2048)])
+def test_weights_past_a_grid_are_refused(N, K):
+    P = 1 << 20  # an aligned address, which is not read
+    lib = _lib.load()
+    assert lib.kad_quantize_weight(P, K, 0, P, P, N, K, None) == -1
+    assert lib.kad_dequantize_weight(P, P, P, K, 0, N, K, None) == -1
