@@ -668,7 +668,8 @@ int kad_quantize_weight(const void* w, int64_t ldw, int dtype, void* codes, void
 int kad_dequantize_weight(const void* codes, const void* scales, void* out, int64_t ldo, int dtype,
                           int N, int K, kad_stream_t stream);
 /* y[M, N] = x[M, K] W^T + residual[M, N] (may be null, may be y), all of one dtype
- * (bf16, fp16, fp32) with rows at strides ldx, ldy, ldr; fp32 sums, rounded once.  The
+ * (bf16, fp16, fp32) with rows at strides ldx, ldy, ldr; fp32 sums, rounded once (fp32
+ * values of x below 2^-110 to within 2^-134).  The
  * workspace (16-byte aligned) has the size that kad_quantized_linear_workspace_bytes
  * gives for the same x, ldx and sizes (0: none); calls that overlap need one each. */
 int kad_quantized_linear_workspace_bytes(const void* x, int64_t ldx, int dtype, int M, int N,
@@ -679,7 +680,7 @@ int kad_quantized_linear(const void* x, int64_t ldx, int dtype, const void* code
                          int K, kad_stream_t stream);
 /* y[M, H] = (silu(x G^T) * (x U^T)) D^T + residual, x [M, H], G and U [F, H], D [H, F];
  * strides, types and workspace as above.  The product in the middle is held in
- * bf16 for bf16 rows (2^-8 of itself), to 2^-15 for fp16 and 2^-22 for fp32. */
+ * bf16 for bf16 rows (2^-8 of itself), to 2^-15 for fp16 and 2^-22 for fp32, or 2^-134. */
 int kad_quantized_gated_ffn_workspace_bytes(const void* x, int64_t ldx, int dtype, int M, int H,
                                             int F, int64_t* bytes);
 int kad_quantized_gated_ffn(const void* x, int64_t ldx, int dtype, const void* gate_codes,

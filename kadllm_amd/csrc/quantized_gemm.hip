@@ -6,13 +6,15 @@
 // The weight's values are exact in bf16 and go to v_mfma_f32_16x16x32_bf16 as they
 // are; what x has more bits than bf16 goes as further products: x is the sum of
 // bf16 pieces, two for fp16 (11 bits) and three for fp32 (24 bits), each the leading
-// bits of what is left, so the sum is x itself.  With scales from 2^-15 to 1 the weight's
-// values are exact in fp16 too, and rows of fp16 go to v_mfma_f32_16x16x32_f16 as they are,
-// in pieces where one is another: in that block of 128 columns alone (the kernel of few
-// rows), or with all of the rows of the weight that a wave has (of many).  Sums are fp32 and
-// are rounded once, with the residual added.  The gated product h is rounded to one
-// bf16 piece for bf16 x (2^-8, as the model's own activation), else to as many
-// pieces as x has: 2^-15 for fp16, whose range h may leave, and 2^-22 for fp32.
+// bits of what is left, so the sum is x itself (fp32 below 2^-110: to the nearest 2^-133,
+// bf16's lowest step; pieces held at other scales would take a conversion of the weight for
+// each).  With scales from 2^-15 to 1 the weight's values are exact in fp16 too, and rows of
+// fp16 go to v_mfma_f32_16x16x32_f16 as they are, in pieces where one is another: in that
+// block of 128 columns alone (the kernel of few rows), or with all of the rows of the weight
+// that a wave has (of many).  Sums are fp32 and are rounded once, with the residual added.
+// The gated product h is rounded to one bf16 piece for bf16 x (2^-8, as the model's own
+// activation), else to as many pieces as x has: 2^-15 for fp16, whose range h may leave, and
+// 2^-22 for fp32.
 
 #include <type_traits>
 

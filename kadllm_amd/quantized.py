@@ -232,8 +232,9 @@ def quantized_linear(x, weight, *, residual=None):
 
     x [..., K] bf16, fp16 or fp32 (any strides); residual [..., N] of x's type.
     Returns [..., N] in x's type.  Products are exact, sums are fp32 and are rounded
-    once, with the residual added.  fp16 rows take half as long where all scales are from
-    2**-15 to 1."""
+    once, with the residual added; of fp32 rows, values below 2**-110 count to within
+    2**-134 (they are taken in bf16 pieces, which end there).  fp16 rows take half as long
+    where all scales are from 2**-15 to 1."""
     _check_weight(weight)
     rows, r = _check_rows(x, weight.cols, weight.rows, residual)
     _device_of(x, weight.codes, residual)
@@ -263,7 +264,7 @@ def quantized_gated_ffn(x, gate, up, down, *, residual=None):
     x [..., H] bf16, fp16 or fp32 (any strides); residual [..., H] of x's type.
     Returns [..., H] in x's type.  Sums are fp32.  The product of the two
     projections, whose SiLU is computed in fp32, is held in bf16 for bf16 rows (off
-    by up to 2**-8 of itself), to 2**-15 for fp16 and 2**-22 for fp32."""
+    by up to 2**-8 of itself), to 2**-15 for fp16 and 2**-22 for fp32, or 2**-134."""
     for name, w in (("gate", gate), ("up", up), ("down", down)):
         _check_weight(w, name)
     F, H = gate.rows, gate.cols

@@ -101,3 +101,25 @@ def test_signalling_nan(device, M, N, K, dtype):
     assert out[rows].isnan().all()
     rest = [m for m in range(M) if m not in rows]
     assert bool((out[rest] == K).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, N", [(1, 64), (40, 64), (300, 64), (3000, 512), (9000, 512)])
+def test_rows_far_below_one(device, M, N, dtype):
+    # one weight of 2^100 in a row: y is x times it.  The pieces of fp32 rows end at 2^-133, the
+    # lowest step of bf16: values from 2^-110 are whole, others off by up to 2^-134
+    K = 512
+    g = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=g).double()
+    order = torch.randperm(K, generator=g)[:N]
+    q = quantize_weight((torch.eye(K)[order] * (1.0 if dtype is F16 else 2.0 ** 100)).cuda())
+    for e in (-14, -20) if dtype is F16 else (-60, -100, -109, -118, -126):
+        y = (x * 2.0 ** e).to(dtype)
+        out = quantized_linear(y.cuda(), q).double().cpu()
+        want = y[:, order].double() * (1.0 if dtype is F16 else 2.0 ** 100)
+        if dtype is not F32:
+            assert torch.equal(out, want), e
+        else:
+            whole = want.abs() >= 2.0 ** -10
+            assert torch.equal(out[whole], want[whole]), e
+            assert bool(((out - want).abs() <= 2.0 ** -34).all()), e
