@@ -535,6 +535,11 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
   // PIPE: a slice goes to registers while the one before multiplies
   constexpr bool PIPE = MT <= 4;
   constexpr int AHEAD = PIPE ? SLOTS : SLOTS - 1;  // slices loaded ahead
+  // Rows of fp16 in pieces: whether a row block's operand is made anew for each row tile.  Held
+  // for all of them it takes registers from the rows' addresses, which then come from scratch
+  // memory in either walk (fp16 4000 x 2880 x 2880: 109 us, made anew 78; in pieces 249 and 197).
+  // Rows of whole blocks need fewer addresses (in pieces 2048 x 8192 x 4096 329 us, anew 339).
+  constexpr bool ANEW = HALF && RAGGED && MT * NW >= 16;
   // loads that a wave issues after a slice's own before it waits for that slice: those of
   // SLOTS - 2 later ones, and the codes' and scales' of the blocks that begin meanwhile
   constexpr int LATER = LPW * (SLOTS - 2) + 2 * NW * ((SLOTS - 2) / (HALVES * P));
@@ -637,10 +642,13 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int
                   bf16x8 xf[kPieces<T>];
                   pieces_of<T>({__builtin_bit_cast(u32x4, frags[set][j][i])}, xf);
 #pragma unroll
-                  for (int n = 0; n < NW; ++n)
+                  for (int n = 0; n < NW; ++n) {
+                    if constexpr (ANEW) asm volatile("" : "+v"(codes[d].s[n]));
 #pragma unroll
                     for (int q = 0; q < kPieces<T>; ++q)
                       acc[n][i] = mfma16x16x32(made(codes[d], h * STEPS + j, n), xf[q], acc[n][i]);
+                    if constexpr (ANEW) __builtin_amdgcn_sched_barrier(0);
+                  }
                   __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
                 }
             } else {
