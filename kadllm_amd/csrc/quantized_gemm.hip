@@ -13,7 +13,9 @@
 // block of 128 columns alone (the kernel of few rows), or with all of the rows of the weight
 // that a wave has (of many).  Sums are fp32 and are rounded once, with the residual added.
 // The gated product h is rounded to one bf16 piece for bf16 x (2^-8, as the model's own
-// activation), else to as many pieces as x has: 2^-15 for fp16, whose range h may leave, and
+// activation: y is off by sqrt(2) times its own rounding, 0.0023 of its norm for 0.0017, and a
+// second piece is the second half's products again, 193 of 605 us with 32768 rows of 1024 and a
+// width of 3584), else to as many pieces as x has: 2^-15 for fp16, whose range h may leave, and
 // 2^-22 for fp32.
 
 #include <type_traits>
@@ -314,12 +316,13 @@ __device__ __forceinline__ void pieces_of(const u32x4 (&v)[sizeof(T) / 2],
 // whole blocks.  R: rows of a tile that are loaded, 16, or 4 where x has no more (the
 // product's other columns repeat them).
 // One row takes what the codes take to arrive (1 x 248320 x 1024, 135 MB: 24 us, 5.6 TB/s),
-// or, where they are few, a launch and a wave's walk over its blocks (1 x 1024 x 3584: 3.9 us,
-// 0.4 of it the codes at 5 TB/s; 10 x 8192 x 1024 4.3).  More rows take what comes through
+// or, where they are few, a launch and a wave's walk over its blocks (1 x 1024 x 3584: 3.8 us,
+// 0.4 of it the codes at 5 TB/s; 10 x 8192 x 1024 4.2).  More rows take what comes through
 // the L2 caches: each workgroup reads its rows and codes itself (64 x 8192 x 8192, 256
-// workgroups of 32 x 64: 17.5 us, 0.13 GB of rows and 0.07 GB of codes, 12 TB/s).  fp32 rows
-// are three times the products, and their pieces are made in each workgroup: 300 x 1024 x 2048
-// 13.4 us, 0.28 PFLOP/s of the three.
+// workgroups of 32 x 64: 20 us, from the caches 17.6, 0.13 GB of rows and 0.07 GB of codes,
+// 11 TB/s).  fp32 rows are three times the products, and their pieces are made in each
+// workgroup: 300 x 1024 x 2048 12.6 us, 0.30 PFLOP/s of the three.  (Traced kernels, with a
+// residual and, where nothing else is said, weights from beyond the caches.)
 template <typename T, bool RAW, bool GATED, int MT, int NT, int KS, int D, int R>
 __global__ __launch_bounds__(64 * KS) void q4_stream_kernel(Args a) {
   constexpr int P = kPieces<T>, W = GATED ? 2 : 1, NW = W * NT;
@@ -517,13 +520,14 @@ __device__ __attribute__((aligned(16))) const bf16_t kZeros[8] = {};
 // is filled by direct loads.
 // The matrix unit bounds the largest tile, for about half its time: a workgroup's four waves
 // wait for a slice together, and what converts codes shares the issue slots (8192 x 8192 x
-// 8192 bf16 728 us, 1.51 PFLOP/s; 32768 x 1024 x 3584 192 us, 1.25; the unit alone, 2.37).  Smaller
+// 8192 bf16 741 us, 1.48 PFLOP/s; 32768 x 1024 x 3584 192 us, 1.25; the unit alone, 2.37).  Smaller
 // calls are bound by what the tiles load through the L2 caches: 50 x 248320 x 1024 in tiles of
 // 64 x 256 42 us, 3.2 TB/s of codes, as much of rows, and 50 MB of y and the residual.  fp16
-// 2048 x 8192 x 4096 115 us, 1.19 PFLOP/s; fp32 1024 x 4096 x 4096 79 us and 8.6 for the
-// pieces, 1.3 PFLOP/s of its three products.
+// 2048 x 8192 x 4096 114 us, 1.2 PFLOP/s; fp32 1024 x 4096 x 4096 77 us and 8.4 for the
+// pieces, 1.3 PFLOP/s of its three products.  (Traced kernels, with a residual, weights in the
+// caches; from beyond them 1.01 to 1.1 times as long.)
 // HALF: x is rows of fp16, else pieces.  RAGGED: rows that end inside a block of columns, at
-// whole 16 bytes (1726 x 960 x 4560 25.5 us, copied and padded first 33; where all kernels
+// whole 16 bytes (1726 x 960 x 4560 25 us, copied and padded first 33; where all kernels
 // looked for an end the others took 2 % longer, the largest tile twice as long for registers).
 template <typename T, bool HALF, bool RAGGED, bool GATED, int MT, int NW, int BK, int SLOTS, int D>
 __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Args a, int mtiles, int ntiles) {
@@ -727,8 +731,9 @@ bool in_place(const void* x, int64_t ldx, int K) {
 // kernel 42, fp16 38 and 45, fp32 72 and 68; 300 x 4096 x 2048, 640: 12.5 and 12.7, 12.4 and
 // 13.3, 29 and 27; 32 x 50000 x 1024, 782: 12.8 and 11.1, 12.6 and 11.5, 24 and 18), and up
 // to 16 rows its tile of 16 x 64 whatever the weight (16 x 248320 x 1024: 33.4 us, of the
-// other kernel's 32.1 at best; fp16 33.6 and 36.4, fp32 46 and 54).  bf16, us, weights from
-// beyond the caches:
+// other kernel's 32.1 at best; fp16 33.6 and 36.4, fp32 46 and 54: one rule for all types).
+// These figures and those beside the rules below are of calls behind one another in a graph,
+// without a residual, weights from beyond the caches; bf16, us:
 //   M x N x K            16x16  16x32  16x64  32x64 | 32x128 64x128 64x256 128x256
 //   16 x 1024 x 3584       5.0    5.6    6.9    8.4 |  17     21     30      45
 //   128 x 1024 x 3584      7.5    5.4    6.4    8.9 |  17     22     31      47
@@ -758,7 +763,7 @@ void launch_stream(Args a, hipStream_t s) {
   // In the grid's order an XCD has an eighth of the columns, or a few of them, and reads all
   // rows; where those pass its L2 (4 MB) and the codes in bytes, it has an eighth of the rows
   // and reads all codes: bf16 2048 x 512 x 4096 15.7 us, in the grid's order 23.6; 1951 x 368 x
-  // 8912 26.9 and 38.1; fp32 300 x 1024 x 2048, 2.4 MB of rows: 13.5 and 12.2; bf16 32 x 8192 x
+  // 8912 26.9 and 38.1; fp32 300 x 1024 x 2048, 2.4 MB of rows: 12.4 and 11.4; bf16 32 x 8192 x
   // 8192, 36 MB of codes: 13.4 and 10.5.
   const int64_t rows = (int64_t)a.M * a.K * (RAW ? sizeof(T) : 2 * kPieces<T>);
   const bool by_rows = rows > (4 << 20) && rows > (int64_t)a.KB * 68 * a.cols * (GATED ? 2 : 1);
@@ -790,7 +795,7 @@ void stream(const Args& a, hipStream_t s) {
   // 8 waves share K from 12 blocks of it on (16 x 1024 x 1536 fp32: 4.9 us, 4 waves 5.5;
   // 16 x 2048 x 16384: 12.9 and 14.3; 1 x 1024 x 1024, 8 blocks: 2.9 and 2.2)
   const bool wide = a.KB >= 12;
-  // 4 rows or fewer load no more (1 x 1024 x 3584: 3.2 us, all 16 of the tile 3.9)
+  // 4 rows or fewer load no more (1 x 1024 x 3584: 3.5 us, all 16 of the tile 4.3)
   auto rows = [&](auto r) {
     constexpr int R = decltype(r)::value;
     if constexpr (!GATED)
@@ -807,7 +812,7 @@ void stream(const Args& a, hipStream_t s) {
     }
     // (fp32 rows, one block ahead, have too few in flight: 128 x 2048 x 16384 45 us, two ahead
     // 39; and with two ahead no registers for a second workgroup: 300 x 1024 x 2048, 304 of
-    // them, 14.6 us, of 4 waves 12)
+    // them, 12.9 us, of 4 waves 11.4)
     if (wide && (P < 3 || tiles * kad_cdiv(n, 64) <= 256))
       return launch_stream<T, RAW, GATED, 1, 4 / W, 8, P == 3 ? 2 : 1, R>(a, s);
     return launch_stream<T, RAW, GATED, 1, 4 / W, 4, 2, R>(a, s);
@@ -841,8 +846,9 @@ void tiles(const Args& a, hipStream_t s) {
   // the size, or somewhat less: the larger ones where that halves the rounds (69 x 100000 x
   // 1024, one round against two: 29.6 us, smaller 35.4; 130 rows, two and three: 57.4 and
   // 46.8; 1024 x 32768 x 1024, two and four: 62 and 69).  fp16 and fp32 rows have no registers
-  // for them (fp16, spilled: 1024 x 32768 x 1024 121 us, smaller 75), nor have ragged ones (4000 x
-  // 2880 x 2880: 150 us, smaller 72).
+  // for them (fp16, spilled: 1024 x 32768 x 1024 121 us, smaller 75, which itself keeps 9 to 30
+  // registers of its walk in pieces in scratch memory), nor have ragged ones (4000 x 2880 x
+  // 2880: 150 us, smaller 72).
   if constexpr (kPieces<T> == 1 && !RAGGED)
     if (2 * kad_cdiv(count(128, 256), 512) <= kad_cdiv(count(64, 256), 512))
       return launch_tile<T, HALF, RAGGED, GATED, 8, 4, 64, 4, 2>(a, s);
