@@ -29,6 +29,12 @@ int kad_launch_status(const char* what);
     }                                          \
   } while (0)
 
+// the status of a call that did not succeed is the caller's
+#define KAD_TRY(call)                          \
+  do {                                         \
+    if (const int rc = (call)) return rc;      \
+  } while (0)
+
 #define KAD_UNSUPPORTED(...)                   \
   do {                                         \
     kad_set_error(__VA_ARGS__);                \

@@ -923,11 +923,6 @@ int check_weight(Weight w) {
   return KAD_OK;
 }
 
-#define KAD_TRY(call)                    \
-  do {                                   \
-    if (const int rc = (call)) return rc; \
-  } while (0)
-
 // f.template operator()<T>() for the type of a dtype code
 template <typename F>
 int for_dtype(int dtype, F f) {

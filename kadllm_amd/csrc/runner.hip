@@ -19,11 +19,6 @@ namespace {
 
 constexpr int kBf = KAD_DTYPE_BF16, kF32 = KAD_DTYPE_F32;
 
-#define KAD_TRY(call)                    \
-  do {                                   \
-    if (const int rc = (call)) return rc; \
-  } while (0)
-
 uint16_t* at(const void* p, int64_t elements) { return (uint16_t*)const_cast<void*>(p) + elements; }
 
 int check_model(const kad_qwen_model* m) {
