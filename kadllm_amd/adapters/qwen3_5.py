@@ -64,7 +64,8 @@ class Qwen35GRBeamAdapter:
     weights="e2m1" (bf16 models) holds the projections, the FFN and the LM head
     in 4 bits (kadllm_amd.quantized), quantised once, here; the embedding stays in
     bf16.  Sums are in an order that depends on the rows of a call:
-    decode_incremental's logits equal decode's to rounding here too.
+    decode_incremental's logits equal decode's to rounding here too.  A call has at most
+    16 * 65535 rows (tokens of its prompts, or of its beams).
     """
 
     def __init__(self, text_model, lm_head, *, gdn_backend="torch", conv_backend="torch",

@@ -110,7 +110,7 @@ class QuantizedWeight:
         pad = torch.nn.functional.pad
         bad = (scales < 27) | ((scales > 252) & (scales < 255))
         if bool(bad.any()):
-            nonzero = (pad(codes, (0, -half % 16)).view(N, -1, 16) & 0x77).ne(0).any(2)
+            nonzero = (pad(codes, (0, -half % 16)).reshape(N, -1, 16) & 0x77).ne(0).any(2)
             unused = (scales == 0) & ~nonzero
             if bool((bad & ~unused).any()):
                 raise ValueError("scales must be from 2**-100 to 2**125, or NaN")

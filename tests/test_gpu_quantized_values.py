@@ -7,8 +7,8 @@ bit with the definition in 64 bits."""
 import pytest
 import torch
 
-from kadllm_amd.ops import (dequantize_weight, quantize_weight, quantized_gated_ffn,
-                            quantized_linear)
+from kadllm_amd.ops import (QuantizedWeight, dequantize_weight, quantize_weight,
+                            quantized_gated_ffn, quantized_linear)
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,21 @@ def test_rows_far_below_one(device, M, N, dtype):
             whole = want.abs() >= 2.0 ** -10
             assert torch.equal(out[whole], want[whole]), e
             assert bool(((out - want).abs() <= 2.0 ** -34).all()), e
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 40, 3000])
+def test_stored_groups_of_zeros(device, M, dtype):
+    # a weight with padding, as one is stored whose groups of zeros have the smallest scale
+    N, K = 520, 300
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(M))
+    w[500:], w[:, 256:], w[::3, 32:64] = 0.0, 0.0, 0.0
+    q = quantize_weight(w.cuda())
+    codes, scales = q.unpack()
+    groups = torch.nn.functional.pad(w, (0, -K % 32)).view(N, -1, 32)
+    stored = scales.view(torch.uint8).masked_fill((groups == 0).all(2).cuda(), 0)
+    p = QuantizedWeight.pack(codes, stored, cols=K)
+    assert torch.equal(p.codes, q.codes)
+    assert torch.equal(p.scales.view(torch.uint8), q.scales.view(torch.uint8))
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    assert torch.equal(quantized_linear(x, p), quantized_linear(x, q))

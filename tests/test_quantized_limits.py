@@ -61,6 +61,10 @@ def test_groups_of_zeros_may_have_the_smallest_scale(N, K):
     assert torch.equal(q.codes, want.codes)
     assert torch.equal(q.scales.view(U8), want.scales.view(U8))
     assert bool((stored == 0).any()) and torch.equal(q.unpack()[1].view(U8), scales)
+    # parts that are not contiguous
+    q = QuantizedWeight.pack(parts.T.contiguous().T, stored.T.contiguous().T, cols=K)
+    assert torch.equal(q.codes, want.codes)
+    assert torch.equal(q.scales.view(U8), want.scales.view(U8))
     # NaN stays NaN
     nan = QuantizedWeight.pack(parts, scales.masked_fill(zeros, 255), cols=K).unpack()[1].view(U8)
     assert bool((nan[zeros] == 255).all())
