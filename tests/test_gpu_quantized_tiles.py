@@ -214,6 +214,25 @@ def test_ffn_groups_that_are_not_numbers(device, M, H, F, dtype):
         bad[F // 2, 3] = kept
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M, H, F", [(1, 1024, 3584), (19, 2048, 5503), (256, 1024, 3584),
+                                     (9000, 500, 300), (32768, 1024, 3584)])
+def test_repeated_blocks_give_the_same_bits(device, M, H, F, dtype):
+    weights = [quantize_weight(_values(s, i) * s[1] ** -0.5)
+               for i, s in enumerate(((F, H), (F, H), (H, F)))]
+    x = _values((M, H), 4, dtype)
+    want = quantized_gated_ffn(x, *weights, residual=x)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        outs = [quantized_gated_ffn(x, *weights, residual=x)]
+        for stream in streams:  # at the same time
+            with torch.cuda.stream(stream):
+                outs.append(quantized_gated_ffn(x, *weights, residual=x))
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for out in outs)
+
+
 @pytest.mark.parametrize("dtype, first", [(BF, 8), (F16, 3), (F32, 8)])
 def test_rows_past_32_bits(device, dtype, first):
     # 2^32 and more elements of x: the same 1024 rows again and again, the last of them fewer
